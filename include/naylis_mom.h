@@ -24,7 +24,7 @@
 extern "C" {
 #endif
 
-#define NAYLIS_MOM_ABI_VERSION 21
+#define NAYLIS_MOM_ABI_VERSION 22
 
 #define NAYLIS_OK 0
 #define NAYLIS_ERR_ARG 1       /* invalid shape / argument (the reference raises RuntimeError) */
@@ -33,6 +33,7 @@ extern "C" {
 
 #define NAYLIS_DTYPE_F32 0
 #define NAYLIS_DTYPE_BF16 1
+#define NAYLIS_DTYPE_E4M3 2 /* OCP fp8 codes with one fp32 scale per row (caches) */
 
 /* noise_kind of naylis_mom_router_fwd */
 #define NAYLIS_NOISE_ADDITIVE 0        /* noise holds the perturbation itself */
@@ -475,6 +476,100 @@ int naylis_mom_decode_step(const double* state_in, double* state_out, const int3
                            const uint8_t* v8, const float* k_scale, const float* v_scale, void* out, int32_t* top_idx,
                            float* top_gates, int64_t B, int64_t D, int64_t H, int64_t R, int64_t E, int64_t block_size,
                            int64_t top_k, void* stream);
+
+/* ---------------------------------------------------- packed attention ---
+ * Causal attention over sequences of different lengths packed in one batch,
+ * with grouped heads (the reference runs one length and equal heads,
+ * model.py:279-345): out_i = softmax_j(scale q_i . k_j) v_j over the keys
+ * j <= i + lk - lq of the same sequence (the last query sees the last key; a
+ * query that sees none gets 0).  Query head h reads key head h / (H / Hkv).
+ *   q, out (T, H, head_dim), k, v (Tk, Hkv, head_dim) bf16; out dense
+ *   cu_q, cu_k (n_seqs + 1) int32 on the device: sequence i holds query rows
+ *   cu_q[i] .. cu_q[i + 1] - 1 and key rows cu_k[i] .. cu_k[i + 1] - 1.  Rows
+ *   before the first offset and from the last one on belong to no sequence:
+ *   their results and gradients are 0.  Offsets outside the tensors are
+ *   clamped to them; descending ones leave the rows that they span unspecified.
+ *   strides: host array, the token and head strides (elements) of q, k, v and,
+ *   for the backward, dout: 8 values there, 6 in the forward
+ *   lse (H, T) fp32, log2 domain, +inf for a query that sees no key; NULL in
+ *   the forward where no backward follows
+ *   delta (H, T) fp32: scratch of the backward
+ * The backward writes dense dq, dk, dv; the gradients of a key head are summed
+ * over its query heads in one fixed order in fp32.  No workspace.
+ * Constraints: head_dim 64 or 128, H a multiple of Hkv, scale > 0, pointers
+ * 16-byte aligned, strides multiples of 8, token strides under 2^23. */
+int naylis_mom_packed_attn_fwd(const void* q, const void* k, const void* v, const int32_t* cu_q, const int32_t* cu_k,
+                               void* out, float* lse, const int64_t* strides, float scale, int64_t n_seqs, int64_t T,
+                               int64_t Tk, int64_t H, int64_t Hkv, int64_t head_dim, void* stream);
+int naylis_mom_packed_attn_bwd(const void* q, const void* k, const void* v, const int32_t* cu_q, const int32_t* cu_k,
+                               const void* out, const float* lse, const void* dout, void* dq, void* dk, void* dv,
+                               float* delta, const int64_t* strides, float scale, int64_t n_seqs, int64_t T,
+                               int64_t Tk, int64_t H, int64_t Hkv, int64_t head_dim, void* stream);
+
+/* --------------------------------------------------------- paged cache ---
+ * Keys and values of earlier tokens in pages, and the attention of one new
+ * token per sequence over them (the reference keeps no cache: use_cache=False,
+ * pretrain.py:198).
+ *   k_pages, v_pages (pages, Hkv, page_size, head_dim), cache_dtype bf16, or
+ *   e4m3 codes with k_scale, v_scale (pages, Hkv, page_size) fp32: scale =
+ *   max|row| / 448 (1 for a row of zeros), code = e4m3(x / scale) rounded to
+ *   nearest even; scales NULL for bf16
+ *   table (B, W) int32: the pages of each sequence's tokens 0 .., in order
+ *
+ * naylis_mom_paged_append: k, v (T, Hkv, head_dim) bf16 with the token and
+ * head strides of the host array `strides` (k's, then v's): token t becomes
+ * token positions[t] of sequence rows[t] (of sequence t where rows is NULL).
+ * A token whose row, position or page lies outside the table or the cache
+ * (padding: position -1) is left out, and nothing else is written.  No two
+ * tokens of a call may have the same place.
+ *
+ * naylis_mom_paged_attn: out (B, H, head_dim) bf16 dense = softmax_n(scale
+ * q . k_n) v_n over the tokens n < lens[b] (int32); 0 where lens[b] <= 0; NaN
+ * for a sequence longer than its table row, or with a page outside the cache.
+ * Table entries and page rows past the sequence's end are not used, whatever
+ * they hold.  q (B, H, head_dim) bf16, q_strides: host array, its batch and
+ * head strides.
+ * Constraints: head_dim 64 or 128, page_size a power of two in [16, 256], H a
+ * multiple of Hkv, B <= 65535, scale > 0, pointers (tables and lengths apart)
+ * 16-byte aligned, strides multiples of 8, the first of a pair under 2^23. */
+int naylis_mom_paged_append(void* k_pages, void* v_pages, float* k_scale, float* v_scale, int cache_dtype,
+                            const void* k, const void* v, const int64_t* strides, const int32_t* table,
+                            const int32_t* positions, const int32_t* rows, int64_t T, int64_t pages, int64_t Hkv,
+                            int64_t page_size, int64_t head_dim, int64_t B, int64_t W, void* stream);
+size_t naylis_mom_paged_attn_workspace_bytes(int cache_dtype, int64_t B, int64_t H, int64_t Hkv, int64_t page_size,
+                                             int64_t head_dim, int64_t W);
+int naylis_mom_paged_attn(const void* q, const void* k_pages, const void* v_pages, const float* k_scale,
+                          const float* v_scale, int cache_dtype, const int32_t* table, const int32_t* lens, void* out,
+                          void* workspace, size_t workspace_bytes, const int64_t* q_strides, float scale, int64_t B,
+                          int64_t H, int64_t pages, int64_t Hkv, int64_t page_size, int64_t head_dim, int64_t W,
+                          void* stream);
+
+/* --------------------------------------------------- log probabilities ---
+ * Of given tokens under rows of logits (the reference keeps the summed loss of
+ * such rows, model.py:536-545), with each row's entropy and likeliest tokens:
+ *   lp = logits - logsumexp(logits), p = exp(lp)
+ *   logp (N) fp32 = lp[tokens]; 0 where the token is ignore_index, NaN where
+ *   it is neither that nor a column
+ *   entropy (N) fp32 = -sum_j p_j lp_j
+ *   top_ids (N, top) int64, top_logp (N, top) fp32: the `top` largest logits,
+ *   descending, equal ones by the lowest index, NaN before all numbers
+ *   stat (N, 3) fp32 for the backward: maximum, log of the sum of exponentials
+ *   less the maximum, entropy; may be NULL
+ * Columns of -inf have p = 0 and add nothing; a row without a finite logit is NaN.
+ * The backward writes, for the gradients of logp and entropy (either may be
+ * NULL; strides in elements, 0 for one value for all rows),
+ *   dlogits_j = g_logp (1[j = token] - p_j) - g_entropy p_j (lp_j + entropy)
+ * dense (N, V), in the logits' type; g_logp counts as 0 where the token is
+ * ignore_index.
+ * logits (N, V) in dtype (bf16 or fp32), row stride row_stride elements, any V
+ * and any address that its elements allow; top <= min(64, V). */
+int naylis_mom_logprobs_fwd(const void* logits, int dtype, int64_t row_stride, const int64_t* tokens, float* logp,
+                            float* entropy, float* stat, int64_t* top_ids, float* top_logp, int64_t N, int64_t V,
+                            int64_t top, int64_t ignore_index, void* stream);
+int naylis_mom_logprobs_bwd(const void* logits, int dtype, int64_t row_stride, const int64_t* tokens,
+                            const float* stat, const float* g_logp, int64_t g_logp_stride, const float* g_entropy,
+                            int64_t g_entropy_stride, void* dlogits, int64_t N, int64_t V, int64_t ignore_index,
+                            void* stream);
 
 /* -------------------------------------------------------------- timing ---
  * Optional instrumentation (no counterpart in the reference; for benchmarks):

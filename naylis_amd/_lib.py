@@ -14,7 +14,7 @@ import threading
 
 LIB_DIR = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib")
 LIB_PATH = os.path.join(LIB_DIR, "libnaylis_mom.so")
-ABI_VERSION = 21
+ABI_VERSION = 22
 
 NAYLIS_OK = 0
 NAYLIS_ERR_ARG = 1
@@ -84,6 +84,15 @@ SIGNATURES = {
                                        + [_int, _c_void_p, _size_t] + [_i64] * 4 + [_c_void_p]),
     "naylis_mom_bank_quant_fp8": (_int, [_c_void_p] * 6 + [_i64] * 2 + [_c_void_p]),
     "naylis_mom_decode_step": (_int, [_c_void_p] * 4 + [_int] + [_c_void_p] * 10 + [_i64] * 7 + [_c_void_p]),
+    "naylis_mom_packed_attn_fwd": (_int, [_c_void_p] * 8 + [_float] + [_i64] * 6 + [_c_void_p]),
+    "naylis_mom_packed_attn_bwd": (_int, [_c_void_p] * 13 + [_float] + [_i64] * 6 + [_c_void_p]),
+    "naylis_mom_paged_append": (_int, [_c_void_p] * 4 + [_int] + [_c_void_p] * 6 + [_i64] * 7 + [_c_void_p]),
+    "naylis_mom_paged_attn_workspace_bytes": (_size_t, [_int] + [_i64] * 6),
+    "naylis_mom_paged_attn": (_int, [_c_void_p] * 5 + [_int] + [_c_void_p] * 4 + [_size_t, _c_void_p, _float]
+                              + [_i64] * 7 + [_c_void_p]),
+    "naylis_mom_logprobs_fwd": (_int, [_c_void_p, _int, _i64] + [_c_void_p] * 6 + [_i64] * 4 + [_c_void_p]),
+    "naylis_mom_logprobs_bwd": (_int, [_c_void_p, _int, _i64] + [_c_void_p] * 3 + [_i64, _c_void_p, _i64, _c_void_p]
+                                + [_i64] * 3 + [_c_void_p]),
     "naylis_mom_timing_enable": (None, [_int]),
     "naylis_mom_timing_reset": (None, []),
     "naylis_mom_timing_get": (_int, [ctypes.c_char_p, ctypes.POINTER(ctypes.c_double),

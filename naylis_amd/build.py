@@ -65,7 +65,7 @@ def build_torch_ext(verbose=False):
     # the library, loaded here with global visibility as naylis_amd._lib does
     ctypes.CDLL(LIB, mode=ctypes.RTLD_GLOBAL)
     rocm = ce.ROCM_HOME or "/opt/rocm"  # headers of torch's stream type
-    ce.load(name=EXT_NAME, sources=[os.path.join(CSRC, f) for f in ("torch_layer.cpp", "torch_nodes.cpp")],
+    ce.load(name=EXT_NAME, sources=[os.path.join(CSRC, f) for f in ("torch_layer.cpp", "torch_nodes.cpp", "torch_serving.cpp")],
             build_directory=EXT_DIR, extra_include_paths=[INCLUDE, os.path.join(rocm, "include")],
             extra_cflags=["-O2", "-D__HIP_PLATFORM_AMD__=1"], extra_ldflags=["-lc10_hip"], verbose=verbose)
     if not os.path.exists(EXT):

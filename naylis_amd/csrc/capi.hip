@@ -1089,6 +1089,228 @@ int naylis_mom_rezero_bwd(const void* dy, int dy_dtype, const void* z, int z_dty
 
 }  // extern "C"
 
+// ------------------------------------------- packed attention, paged cache, log probabilities
+
+extern "C" {
+
+// token and head strides of a bf16 (rows, heads, hd) operand whose rows the kernels read in
+// 16-byte pieces; 64 rows' 32-bit byte offsets bound the token stride
+static int check_strides(const int64_t* s, const char* name, const char* who) {
+  if (s[0] < 0 || s[1] < 0 || s[0] % 8 != 0 || s[1] % 8 != 0 || s[0] >= ((int64_t)1 << 23) ||
+      s[1] >= ((int64_t)1 << 40))
+    return fail(NAYLIS_ERR_ARG, "%s: strides %lld, %lld of %s must be multiples of 8, the first under 2^23", who,
+                (long long)s[0], (long long)s[1], name);
+  return NAYLIS_OK;
+}
+
+static int check_pointers(std::initializer_list<const void*> ptrs, const char* who) {
+  for (const void* p : ptrs) {
+    if (!p) return fail(NAYLIS_ERR_ARG, "%s: null pointer argument", who);
+    if (!aligned16(p)) return fail(NAYLIS_ERR_ARG, "%s: all tensors must be 16-byte aligned", who);
+  }
+  return NAYLIS_OK;
+}
+
+static int check_scale(float scale, const char* who) {
+  if (!(scale > 0.f) || !std::isfinite(scale)) return fail(NAYLIS_ERR_ARG, "%s: scale must be positive", who);
+  return NAYLIS_OK;
+}
+
+static int check_packed(int64_t n, int64_t T, int64_t Tk, int64_t H, int64_t Hkv, int64_t head_dim, float scale,
+                        const int32_t* cu_q, const int32_t* cu_k, const char* who) {
+  if (n < 1 || T < 0 || Tk < 0 || H < 1 || Hkv < 1 || H % Hkv != 0)
+    return fail(NAYLIS_ERR_ARG, "%s: bad shape n_seqs=%lld T=%lld Tk=%lld H=%lld Hkv=%lld", who, (long long)n,
+                (long long)T, (long long)Tk, (long long)H, (long long)Hkv);
+  if (head_dim != 64 && head_dim != 128)
+    return fail(NAYLIS_ERR_ARG, "%s: head_dim %lld must be 64 or 128", who, (long long)head_dim);
+  int rc = check_scale(scale, who);
+  if (rc) return rc;
+  if (H > (1 << 20) || !packed_supported((long)n, (long)T, (long)Tk, (long)H, (long)Hkv))
+    return fail(NAYLIS_ERR_ARG, "%s: n_seqs=%lld T=%lld Tk=%lld H=%lld is too large", who, (long long)n,
+                (long long)T, (long long)Tk, (long long)H);
+  if (!cu_q || !cu_k) return fail(NAYLIS_ERR_ARG, "%s: null pointer argument", who);
+  return NAYLIS_OK;
+}
+
+int naylis_mom_packed_attn_fwd(const void* q, const void* k, const void* v, const int32_t* cu_q, const int32_t* cu_k,
+                               void* out, float* lse, const int64_t* strides, float scale, int64_t n_seqs, int64_t T,
+                               int64_t Tk, int64_t H, int64_t Hkv, int64_t head_dim, void* stream) {
+  const char* who = "mom_packed_attn_fwd";
+  int rc = check_packed(n_seqs, T, Tk, H, Hkv, head_dim, scale, cu_q, cu_k, who);
+  if (rc || T == 0) return rc;
+  if (!strides) return fail(NAYLIS_ERR_ARG, "%s: null pointer argument", who);
+  if ((rc = check_pointers({q, out}, who)) || (Tk > 0 && (rc = check_pointers({k, v}, who)))) return rc;
+  if ((rc = check_strides(strides, "q", who)) || (rc = check_strides(strides + 2, "k", who)) ||
+      (rc = check_strides(strides + 4, "v", who)))
+    return rc;
+  const PackedSeqs s{cu_q, cu_k, (int)n_seqs, (int)T, (int)Tk};
+  const PackedHeads d{(int)H, (int)Hkv, strides[0], strides[1], strides[2], strides[3], strides[4], strides[5], 0, 0};
+  return hip_status(launch_packed_fwd(q, k, v, out, lse, s, d, (int)head_dim, scale, (hipStream_t)stream), who);
+}
+
+int naylis_mom_packed_attn_bwd(const void* q, const void* k, const void* v, const int32_t* cu_q, const int32_t* cu_k,
+                               const void* out, const float* lse, const void* dout, void* dq, void* dk, void* dv,
+                               float* delta, const int64_t* strides, float scale, int64_t n_seqs, int64_t T,
+                               int64_t Tk, int64_t H, int64_t Hkv, int64_t head_dim, void* stream) {
+  const char* who = "mom_packed_attn_bwd";
+  int rc = check_packed(n_seqs, T, Tk, H, Hkv, head_dim, scale, cu_q, cu_k, who);
+  if (rc || (T == 0 && Tk == 0)) return rc;
+  if (!strides) return fail(NAYLIS_ERR_ARG, "%s: null pointer argument", who);
+  if (T > 0 && ((rc = check_pointers({q, out, dout, dq}, who)) || !lse || !delta))
+    return rc ? rc : fail(NAYLIS_ERR_ARG, "%s: null pointer argument", who);
+  if (Tk > 0 && (rc = check_pointers({k, v, dk, dv}, who))) return rc;
+  if ((rc = check_strides(strides, "q", who)) || (rc = check_strides(strides + 2, "k", who)) ||
+      (rc = check_strides(strides + 4, "v", who)) || (rc = check_strides(strides + 6, "dout", who)))
+    return rc;
+  const PackedSeqs s{cu_q, cu_k, (int)n_seqs, (int)T, (int)Tk};
+  const PackedHeads d{(int)H,     (int)Hkv,   strides[0], strides[1], strides[2],
+                      strides[3], strides[4], strides[5], strides[6], strides[7]};
+  return hip_status(
+      launch_packed_bwd(q, k, v, out, lse, dout, dq, dk, dv, delta, s, d, (int)head_dim, scale, (hipStream_t)stream),
+      who);
+}
+
+static int check_paged(int64_t pages, int64_t Hkv, int64_t page_size, int64_t B, int64_t W, int64_t G,
+                       int64_t head_dim, int dtype, const char* who) {
+  if (dtype != NAYLIS_DTYPE_BF16 && dtype != NAYLIS_DTYPE_E4M3)
+    return fail(NAYLIS_ERR_ARG, "%s: cache dtype %d must be bf16 or e4m3", who, dtype);
+  if (head_dim != 64 && head_dim != 128)
+    return fail(NAYLIS_ERR_ARG, "%s: head_dim %lld must be 64 or 128", who, (long long)head_dim);
+  if (page_size < 16 || page_size > 256 || (page_size & (page_size - 1)) != 0)
+    return fail(NAYLIS_ERR_ARG, "%s: page_size %lld must be a power of two in [16, 256]", who, (long long)page_size);
+  if (pages < 1 || pages >= ((int64_t)1 << 31) || Hkv < 1 || Hkv > 4096 || G < 1 || G > 4096 || B < 0 || W < 1 ||
+      B > 65535 || W * page_size >= ((int64_t)1 << 31) || B * ((W * page_size + 31) / 32) >= ((int64_t)1 << 30))
+    return fail(NAYLIS_ERR_ARG, "%s: bad shape pages=%lld Hkv=%lld group=%lld B=%lld table width %lld", who,
+                (long long)pages, (long long)Hkv, (long long)G, (long long)B, (long long)W);
+  return NAYLIS_OK;
+}
+
+static int check_cache(const PagedCacheDims& c, int dtype, const char* who) {
+  int rc = check_pointers({c.k, c.v}, who);
+  if (rc) return rc;
+  if (dtype == NAYLIS_DTYPE_E4M3 && (!c.k_scale || !c.v_scale))
+    return fail(NAYLIS_ERR_ARG, "%s: an e4m3 cache needs its scales", who);
+  return NAYLIS_OK;
+}
+
+int naylis_mom_paged_append(void* k_pages, void* v_pages, float* k_scale, float* v_scale, int cache_dtype,
+                            const void* k, const void* v, const int64_t* strides, const int32_t* table,
+                            const int32_t* positions, const int32_t* rows, int64_t T, int64_t pages, int64_t Hkv,
+                            int64_t page_size, int64_t head_dim, int64_t B, int64_t W, void* stream) {
+  const char* who = "mom_paged_append";
+  const PagedCacheDims c{k_pages, v_pages, k_scale, v_scale, (int)pages, (int)Hkv, (int)page_size, (int)B, (int)W, 1};
+  int rc = check_paged(pages, Hkv, page_size, B, W, 1, head_dim, cache_dtype, who);
+  if (rc || (rc = check_cache(c, cache_dtype, who))) return rc;
+  if (T < 0 || T >= ((int64_t)1 << 31) || T * Hkv * 2 * (head_dim / 8) / 256 >= ((int64_t)1 << 31) - 1)
+    return fail(NAYLIS_ERR_ARG, "%s: bad token count %lld", who, (long long)T);
+  if (!rows && T > B)
+    return fail(NAYLIS_ERR_ARG, "%s: %lld tokens without rows for a table of %lld sequences", who, (long long)T,
+                (long long)B);
+  if (T == 0 || B == 0) return NAYLIS_OK;
+  if (!strides || !table || !positions) return fail(NAYLIS_ERR_ARG, "%s: null pointer argument", who);
+  if ((rc = check_pointers({k, v}, who)) || (rc = check_strides(strides, "k", who)) ||
+      (rc = check_strides(strides + 2, "v", who)))
+    return rc;
+  const PagedNew src{(long)T, strides[0], strides[1], strides[2], strides[3]};
+  return hip_status(launch_paged_append(c, (int)head_dim, cache_dtype == NAYLIS_DTYPE_E4M3, k, v, table, positions,
+                                        rows, src, (hipStream_t)stream),
+                    who);
+}
+
+static PagedCacheDims paged_dims(int64_t H, int64_t pages, int64_t Hkv, int64_t page_size, int64_t B, int64_t W) {
+  return PagedCacheDims{nullptr, nullptr, nullptr, nullptr, (int)pages, (int)Hkv, (int)page_size,
+                        (int)B,  (int)W,  (int)(H / Hkv)};
+}
+
+static int check_paged_attn(int cache_dtype, int64_t B, int64_t H, int64_t pages, int64_t Hkv, int64_t page_size,
+                            int64_t head_dim, int64_t W, const char* who) {
+  if (Hkv < 1 || H < 1 || H % Hkv != 0)
+    return fail(NAYLIS_ERR_ARG, "%s: %lld query heads for %lld key heads", who, (long long)H, (long long)Hkv);
+  return check_paged(pages, Hkv, page_size, B, W, H / Hkv, head_dim, cache_dtype, who);
+}
+
+size_t naylis_mom_paged_attn_workspace_bytes(int cache_dtype, int64_t B, int64_t H, int64_t Hkv, int64_t page_size,
+                                             int64_t head_dim, int64_t W) {
+  if (check_paged_attn(cache_dtype, B, H, 1, Hkv, page_size, head_dim, W, "mom_paged_attn")) return 0;
+  const PagedCacheDims c = paged_dims(H, 1, Hkv, page_size, B, W);
+  return paged_ws_bytes(c, (int)head_dim, cache_dtype == NAYLIS_DTYPE_E4M3);
+}
+
+int naylis_mom_paged_attn(const void* q, const void* k_pages, const void* v_pages, const float* k_scale,
+                          const float* v_scale, int cache_dtype, const int32_t* table, const int32_t* lens, void* out,
+                          void* workspace, size_t workspace_bytes, const int64_t* q_strides, float scale, int64_t B,
+                          int64_t H, int64_t pages, int64_t Hkv, int64_t page_size, int64_t head_dim, int64_t W,
+                          void* stream) {
+  const char* who = "mom_paged_attn";
+  int rc = check_paged_attn(cache_dtype, B, H, pages, Hkv, page_size, head_dim, W, who);
+  if (rc || (rc = check_scale(scale, who)) || B == 0) return rc;
+  PagedCacheDims c = paged_dims(H, pages, Hkv, page_size, B, W);
+  c.k = const_cast<void*>(k_pages);
+  c.v = const_cast<void*>(v_pages);
+  c.k_scale = const_cast<float*>(k_scale);
+  c.v_scale = const_cast<float*>(v_scale);
+  if ((rc = check_cache(c, cache_dtype, who))) return rc;
+  if (!table || !lens || !q_strides) return fail(NAYLIS_ERR_ARG, "%s: null pointer argument", who);
+  if ((rc = check_pointers({q, out, workspace}, who)) || (rc = check_strides(q_strides, "q", who))) return rc;
+  const size_t need = paged_ws_bytes(c, (int)head_dim, cache_dtype == NAYLIS_DTYPE_E4M3);
+  if (workspace_bytes < need)
+    return fail(NAYLIS_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", who, workspace_bytes, need);
+  return hip_status(launch_paged_attn(c, (int)head_dim, cache_dtype == NAYLIS_DTYPE_E4M3, q, q_strides[0],
+                                      q_strides[1], table, lens, out, workspace, scale, (hipStream_t)stream),
+                    who);
+}
+
+static int check_logprobs(const void* logits, int dtype, int64_t ld, const int64_t* tokens, int64_t N, int64_t V,
+                          const char* who) {
+  int rc = check_dtype(dtype, who);
+  if (rc) return rc;
+  if (N < 0 || N >= ((int64_t)1 << 31) || V < 1 || V > (1 << 30))
+    return fail(NAYLIS_ERR_ARG, "%s: bad shape N=%lld V=%lld", who, (long long)N, (long long)V);
+  if (ld < 0) return fail(NAYLIS_ERR_ARG, "%s: row stride %lld must not be negative", who, (long long)ld);
+  if (N == 0) return NAYLIS_OK;
+  if (!logits || !tokens) return fail(NAYLIS_ERR_ARG, "%s: null pointer argument", who);
+  if ((uintptr_t)logits % (dtype == NAYLIS_DTYPE_BF16 ? 2 : 4) != 0)
+    return fail(NAYLIS_ERR_ARG, "%s: logits must be aligned to their elements", who);
+  return NAYLIS_OK;
+}
+
+int naylis_mom_logprobs_fwd(const void* logits, int dtype, int64_t row_stride, const int64_t* tokens, float* logp,
+                            float* entropy, float* stat, int64_t* top_ids, float* top_logp, int64_t N, int64_t V,
+                            int64_t top, int64_t ignore_index, void* stream) {
+  const char* who = "mom_logprobs_fwd";
+  int rc = check_logprobs(logits, dtype, row_stride, tokens, N, V, who);
+  if (rc) return rc;
+  if (top < 0 || top > kLogprobsMaxTop || top > V)
+    return fail(NAYLIS_ERR_ARG, "%s: top %lld must be in [0, min(%d, V)]", who, (long long)top, kLogprobsMaxTop);
+  if (N == 0) return NAYLIS_OK;
+  if (!logp || !entropy || (top > 0 && (!top_ids || !top_logp)))
+    return fail(NAYLIS_ERR_ARG, "%s: null pointer argument", who);
+  return hip_status(launch_logprobs_fwd(logits, dtype == NAYLIS_DTYPE_BF16, (long)row_stride, tokens, logp, entropy,
+                                        stat, top_ids, top_logp, (long)N, (int)V, (int)top, (long)ignore_index,
+                                        (hipStream_t)stream),
+                    who);
+}
+
+int naylis_mom_logprobs_bwd(const void* logits, int dtype, int64_t row_stride, const int64_t* tokens,
+                            const float* stat, const float* g_logp, int64_t g_logp_stride, const float* g_entropy,
+                            int64_t g_entropy_stride, void* dlogits, int64_t N, int64_t V, int64_t ignore_index,
+                            void* stream) {
+  const char* who = "mom_logprobs_bwd";
+  int rc = check_logprobs(logits, dtype, row_stride, tokens, N, V, who);
+  if (rc || N == 0) return rc;
+  if (g_logp_stride < 0 || g_entropy_stride < 0)
+    return fail(NAYLIS_ERR_ARG, "%s: gradient strides must not be negative", who);
+  if (!stat || !dlogits) return fail(NAYLIS_ERR_ARG, "%s: null pointer argument", who);
+  if ((uintptr_t)dlogits % (dtype == NAYLIS_DTYPE_BF16 ? 2 : 4) != 0)
+    return fail(NAYLIS_ERR_ARG, "%s: dlogits must be aligned to their elements", who);
+  return hip_status(launch_logprobs_bwd(logits, dtype == NAYLIS_DTYPE_BF16, (long)row_stride, tokens, stat, g_logp,
+                                        (long)g_logp_stride, g_entropy, (long)g_entropy_stride, dlogits, (long)N,
+                                        (int)V, (long)ignore_index, (hipStream_t)stream),
+                    who);
+}
+
+}  // extern "C"
+
 // ---------------------------------------------------------------- decode step
 namespace {
 

@@ -121,6 +121,60 @@ hipError_t launch_attn_bwd(const void* q, const void* k, const void* v, const vo
                            const void* dout, void* dq, void* dk, void* dv, float* delta, float scale, long B, long S,
                            long H, hipStream_t st);
 
+// Causal attention over packed sequences (packed.hip): q, o (T, H, hd) and k, v
+// (Tk, Hkv, hd) bf16, hd 64 or 128; sequence i holds query rows cu_q[i] ..
+// cu_q[i + 1] - 1 and key rows cu_k[i] .. (device arrays of n + 1 offsets).
+// lse (log2 domain, may be null in the forward) and delta (H, T) fp32.
+struct PackedSeqs {
+  const int32_t* cu_q;
+  const int32_t* cu_k;
+  int n, T, Tk;
+};
+struct PackedHeads {
+  int H, Hkv;
+  long ldq, hsq, ldk, hsk, ldv, hsv, ldd, hsd;  // token and head strides of q, k, v, dO (elements)
+};
+bool packed_supported(long n, long T, long Tk, long H, long Hkv);
+hipError_t launch_packed_fwd(const void* q, const void* k, const void* v, void* o, float* lse, const PackedSeqs& s,
+                             const PackedHeads& d, int hd, float scale, hipStream_t st);
+hipError_t launch_packed_bwd(const void* q, const void* k, const void* v, const void* o, const float* lse,
+                             const void* dout, void* dq, void* dk, void* dv, float* delta, const PackedSeqs& s,
+                             const PackedHeads& d, int hd, float scale, hipStream_t st);
+
+// Paged key / value cache (paged.hip): pages (P, Hkv, page, hd) bf16 or e4m3
+// codes with scales (P, Hkv, page); table (B, W) page ids; G query heads for a
+// key head.
+struct PagedCacheDims {
+  void* k;
+  void* v;
+  float* k_scale;
+  float* v_scale;
+  int P, Hkv, page, B, W, G;
+};
+struct PagedNew {
+  long T, ldk, hsk, ldv, hsv;  // new tokens, token and head strides of their k and v
+};
+struct PagedSplit {
+  int waves, rows, head_tiles;  // waves of a slice, its live query heads, slices of a key head
+};
+size_t paged_ws_bytes(const PagedCacheDims& c, int hd, bool fp8);
+hipError_t launch_paged_append(const PagedCacheDims& c, int hd, bool fp8, const void* k, const void* v,
+                               const int32_t* table, const int32_t* positions, const int32_t* rows,
+                               const PagedNew& src, hipStream_t st);
+hipError_t launch_paged_attn(const PagedCacheDims& c, int hd, bool fp8, const void* q, long ldq, long hsq,
+                             const int32_t* table, const int32_t* lens, void* out, void* ws, float scale,
+                             hipStream_t st);
+
+// Log probabilities of tokens (logprobs.hip): logits (N, V) bf16 or fp32 with
+// row stride ld; stat (N, 3) fp32, top_ids / top_logp (N, top).
+constexpr int kLogprobsMaxTop = 64;
+hipError_t launch_logprobs_fwd(const void* logits, bool bf16, long ld, const int64_t* tokens, float* logp,
+                               float* entropy, float* stat, int64_t* top_ids, float* top_logp, long N, int V, int top,
+                               long ignore_index, hipStream_t st);
+hipError_t launch_logprobs_bwd(const void* logits, bool bf16, long ld, const int64_t* tokens, const float* stat,
+                               const float* g_logp, long gl_stride, const float* g_entropy, long ge_stride,
+                               void* dlogits, long N, int V, long ignore_index, hipStream_t st);
+
 // SwiGLU of the decoder MLP (swiglu.hip): h = silu(g) * u forward; backward
 // writes dg and du from dh; n elements, a multiple of 8.
 hipError_t launch_swiglu(const void* g, const void* u, const void* dh, void* h_or_dg, void* du, bool bf16, bool bwd,

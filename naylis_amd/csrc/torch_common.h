@@ -79,5 +79,6 @@ struct ProbsGrad {
 ProbsGrad probs_grad(const at::Tensor& g, int64_t E);
 
 void bind_nodes(pybind11::module_& m);
+void bind_serving(pybind11::module_& m);
 
 }  // namespace naylis_ext

@@ -340,6 +340,7 @@ std::vector<at::Tensor> mom_layer_node(at::Tensor x, c10::optional<at::Tensor> m
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "Autograd nodes over the C ABI of libnaylis_mom.so";
   bind_nodes(m);
+  bind_serving(m);
   m.def("layer_fwd", &layer_fwd, "MoM layer forward (router, bank K/V, q projection, read, o projection)");
   m.def("layer_bwd", &layer_bwd, "MoM layer backward (the forward's gradients in one fixed order)");
   m.def("mom_layer", &mom_layer_node,

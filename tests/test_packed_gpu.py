@@ -1,0 +1,276 @@
+"""packed_attention (naylis_mom_packed_attn_*) against fp64 attention of each
+sequence on the same bf16 inputs: lengths around the tiles (32-row products,
+64-row stages, 128-row workgroups), empty sequences, queries without keys, keys
+of earlier tokens, grouped heads, heads of 64 and 128, rows outside every
+sequence, more sequences than one wave's lanes."""
+import math
+import random
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+# query lengths, key lengths (None: the same), H, Hkv, hd, rows outside before and behind
+CASES = [
+    ([1], None, 1, 1, 64, 0, 0),
+    ([1], [1], 2, 1, 128, 0, 0),
+    ([31, 1, 0, 33], None, 2, 1, 64, 0, 0),
+    ([64, 65, 127, 129], None, 4, 2, 128, 3, 200),
+    ([5, 200, 40], [0, 131, 40], 4, 1, 64, 0, 5),       # no keys at all; queries before the first key
+    ([150, 0, 7], [20, 90, 7], 4, 4, 128, 1, 1),
+    ([257, 3, 300], [700, 3, 513], 8, 8, 128, 0, 0),
+    ([1, 1, 1, 64], [1000, 64, 65, 128], 8, 2, 64, 0, 0),  # single new tokens after a cached prompt
+    ([1021], None, 6, 3, 64, 0, 0),
+    ([700], [2100], 6, 3, 128, 0, 0),
+    ([2048, 999], None, 32, 8, 64, 0, 0),
+    ([1537, 130], None, 16, 2, 128, 0, 130),
+    ([(7 * i) % 150 for i in range(70)], None, 4, 2, 64, 10, 10),
+    ([(11 * i) % 40 for i in range(130)], [(11 * i) % 40 + (i % 3) * 50 for i in range(130)], 2, 1, 128, 0, 0),
+]
+
+
+def _inputs(lq, lk, H, Hkv, hd, head, tail, dev, seed=0):
+    g = torch.Generator(device=dev).manual_seed(seed + len(lq) + H)
+    lk = lq if lk is None else lk
+    T, Tk = head + sum(lq) + tail, tail + sum(lk) + head
+    q, d = (torch.randn(T, H, hd, generator=g, device=dev) for _ in range(2))
+    k, v = (torch.randn(Tk, Hkv, hd, generator=g, device=dev) for _ in range(2))
+    q[T // 2:] *= 5  # sharp rows: the running maximum has to move
+    cq = torch.tensor([head] + [head + sum(lq[:i + 1]) for i in range(len(lq))], dtype=torch.int32, device=dev)
+    ck = torch.tensor([tail] + [tail + sum(lk[:i + 1]) for i in range(len(lk))], dtype=torch.int32, device=dev)
+    return [t.bfloat16() for t in (q, k, v, d)] + [cq, ck]
+
+
+def _reference(q, k, v, d, cq, ck, scale):
+    """fp64 results and, for each, what bounds its error: a bf16 rounding is at
+    most 2^-8 relative, P (or dS) and the result are rounded once each, which
+    is 2^-7 of the sum of the terms' magnitudes; delta reads the rounded output,
+    whose error is 2^-8 of sum |dO| |o|, inside the 2^-7 too.  fp32 sums of at
+    most 4096 terms and exponents of scores under 2^9 add less than 2^-10."""
+    H, Hkv = q.shape[1], k.shape[1]
+    G = H // Hkv
+    shapes = {"o": q, "dq": q, "dk": k, "dv": v}
+    res = {n: (torch.zeros(t.shape, dtype=torch.float64, device=q.device),
+               torch.zeros(t.shape, dtype=torch.float64, device=q.device)) for n, t in shapes.items()}
+    cq, ck = cq.tolist(), ck.tolist()
+    for a, b, e, f in zip(cq, cq[1:], ck, ck[1:]):
+        lq, lk = b - a, f - e
+        if lq == 0 or lk == 0:
+            continue
+        see = torch.ones(lq, lk, dtype=torch.bool, device=q.device).tril(lk - lq)
+        for h in range(H):
+            x, dx = q[a:b, h].double(), d[a:b, h].double()
+            y, z = k[e:f, h // G].double(), v[e:f, h // G].double()
+            p = torch.softmax((x @ y.T * scale).masked_fill(~see, -math.inf), -1).nan_to_num(0.0)
+            o = p @ z
+            dp = dx @ z.T
+            delta = (dx * o).sum(-1, keepdim=True)
+            ds = p * (dp - delta) * scale
+            ads = p * (dp.abs() + delta.abs() + (dx.abs() * o.abs()).sum(-1, keepdim=True)) * scale
+            for n, at, want, size in (("o", (slice(a, b), h), o, p @ z.abs()), ("dq", (slice(a, b), h), ds @ y, ads @ y.abs()),
+                                      ("dk", (slice(e, f), h // G), ds.T @ x, ads.T @ x.abs()),
+                                      ("dv", (slice(e, f), h // G), p.T @ dx, p.T @ dx.abs())):
+                res[n][0][at] += want
+                res[n][1][at] += size
+    return {n: (w, s * (2.0 ** -7 + 2.0 ** -10)) for n, (w, s) in res.items()}
+
+
+def _run(q, k, v, d, cq, ck, scale):
+    from naylis_amd.mom_kernels import packed_attention
+    q, k, v = (t.detach().requires_grad_() for t in (q, k, v))
+    o = packed_attention(q, k, v, cq, ck, scale=scale)
+    grads = torch.autograd.grad(o, (q, k, v), d)
+    return dict(zip(("o", "dq", "dk", "dv"), (o.detach(), *grads)))
+
+
+def _check(got, want):
+    for n, (w, bound) in want.items():
+        err = (got[n].double() - w).abs()
+        assert bool((err <= bound + 1e-30).all()), (n, float((err / (bound + 1e-30)).max()))
+
+
+@pytest.mark.parametrize("case", CASES, ids=lambda c: f"{len(c[0])}seqs-{sum(c[0])}-H{c[2]}/{c[3]}x{c[4]}")
+def test_packed_matches_fp64(case, dev):
+    x = _inputs(*case, dev)
+    scale = case[4] ** -0.5
+    got = _run(*x, scale)
+    _check(got, _reference(*x, scale))
+    from naylis_amd.mom_kernels import packed_attention
+    with torch.no_grad():  # the call without a gradient gives the same
+        assert torch.equal(packed_attention(*x[:3], *x[4:]), got["o"])
+
+
+def test_packed_gradient_matches_differences(dev):
+    """The gradient along a direction against a difference quotient of the fp64
+    formula at the kernel's own inputs."""
+    x = _inputs([40, 17], [55, 17], 4, 2, 64, 0, 0, dev)
+    q, k, v, d, cq, ck = x
+    got = _run(*x, 0.125)
+    g = torch.Generator(device=dev).manual_seed(5)
+
+    def value(q, k, v):
+        total = 0.0
+        for a, b, e, f in zip(cq.tolist(), cq.tolist()[1:], ck.tolist(), ck.tolist()[1:]):
+            see = torch.ones(b - a, f - e, dtype=torch.bool, device=dev).tril(f - e - b + a)
+            for h in range(4):
+                s = (q[a:b, h] @ k[e:f, h // 2].T * 0.125).masked_fill(~see, -math.inf)
+                total = total + ((torch.softmax(s, -1) @ v[e:f, h // 2]) * d[a:b, h].double()).sum()
+        return total
+
+    for i, n in enumerate(("dq", "dk", "dv")):
+        u = torch.randn(x[i].shape, generator=g, device=dev, dtype=torch.float64)
+        lo, hi = ([t.double() + (s * 1e-4 * u if j == i else 0) for j, t in enumerate((q, k, v))] for s in (-1, 1))
+        slope = float(value(*hi) - value(*lo)) / 2e-4
+        w, bound = _reference(*x, 0.125)[n]
+        assert abs(float((got[n].double() * u).sum()) - slope) <= float((bound * u.abs()).sum()) + 1e-5 * abs(slope)
+
+
+def test_packed_sequences_do_not_see_each_other(dev):
+    """Garbage in one sequence reaches no other, bit for bit, and neither does
+    what stands outside the sequences; runs repeat bit for bit."""
+    x = _inputs([70, 130, 45], [70, 190, 45], 4, 2, 128, 5, 9, dev)
+    a = _run(*x, 0.1)
+    b = _run(*x, 0.1)
+    assert all(torch.equal(a[n], b[n]) for n in a)
+    y = [t.clone() for t in x]
+    cq, ck = x[4].tolist(), x[5].tolist()
+    for t, c in ((y[0], cq), (y[3], cq), (y[1], ck), (y[2], ck)):
+        t[c[1]:c[2]] = math.nan
+        t[:c[0]] = math.inf
+        t[c[3]:] = math.nan
+    c = _run(*y, 0.1)
+    for n, off in (("o", cq), ("dq", cq), ("dk", ck), ("dv", ck)):
+        for s in (slice(0, off[1]), slice(off[2], None)):
+            assert torch.equal(a[n][s], c[n][s]), n
+    assert bool((a["o"][:5] == 0).all() and (a["dk"][ck[3]:] == 0).all() and (a["dv"][:ck[0]] == 0).all())
+
+
+def test_packed_is_causal(dev):
+    x = _inputs([333], [400], 4, 4, 64, 0, 0, dev)
+    y = [t.clone() for t in x]
+    for t in y[1:3]:
+        t[267:] *= 7  # keys behind query 199's last
+    assert torch.equal(_run(*x, 0.125)["o"][:200], _run(*y, 0.125)["o"][:200])
+
+
+def test_packed_equals_the_batch_kernel(dev):
+    """Equal lengths and heads of 64: the framework's batch attention within
+    both kernels' bounds."""
+    from naylis_amd.mom_kernels import packed_attention
+    from naylis_amd.mom_kernels.hip_attention import causal_attention
+    g = torch.Generator(device=dev).manual_seed(3)
+    q, k, v = (torch.randn(3, 200, 4, 64, generator=g, device=dev).bfloat16() for _ in range(3))
+    cu = torch.arange(0, 601, 200, dtype=torch.int32, device=dev)
+    got = packed_attention(*(t.view(600, 4, 64) for t in (q, k, v)), cu).view(3, 200, 4, 64)
+    want = causal_attention(q, k, v, 0.125)
+    assert float((got.float() - want.float()).norm() / want.float().norm()) < 2.0 ** -7
+
+
+def test_packed_takes_views(dev):
+    """q, k, v as slices of one projection, gradients of strided and expanded
+    outputs, int64 offsets, and unaligned or feature-strided operands (copied)."""
+    from naylis_amd.mom_kernels import packed_attention
+    q, k, v, d, cq, ck = _inputs([90, 41], None, 4, 2, 64, 0, 0, dev)
+    want = _run(q, k, v, d, cq, ck, 0.125)
+    qkv = torch.cat([t.flatten(1) for t in (q, k, v)], 1).requires_grad_()
+    a, b, c = (t.view(131, -1, 64) for t in qkv.split([256, 128, 128], 1))
+    o = packed_attention(a, b, c, cq.long())
+    assert torch.equal(o, want["o"])
+    dd = torch.cat([d, d], 2)[..., 64:]  # strided gradient
+    grad, = torch.autograd.grad(o, qkv, dd)
+    assert torch.equal(grad, torch.cat([want[n].flatten(1) for n in ("dq", "dk", "dv")], 1))
+    ones = _run(q, k, v, torch.ones_like(d), cq, ck, 0.125)
+    x, y, z = (t.clone().requires_grad_() for t in (q, k, v))
+    packed_attention(x, y, z, cq).sum().backward()  # an expanded gradient
+    assert all(torch.equal(t.grad, ones[n]) for t, n in ((x, "dq"), (y, "dk"), (z, "dv")))
+    for make in (lambda t: torch.cat([t.new_zeros(1), t.flatten()])[1:].view(t.shape),  # not 16-byte aligned
+                 lambda t: t.permute(2, 0, 1).contiguous().permute(1, 2, 0),   # features not dense
+                 lambda t: t.transpose(0, 1).contiguous().transpose(0, 1)):    # heads outermost
+        assert torch.equal(packed_attention(make(q), make(k), make(v), cq), want["o"])
+
+
+def test_packed_empty_tensors(dev):
+    from naylis_amd.mom_kernels import packed_attention
+    z = lambda n, h: torch.zeros(n, h, 64, dtype=torch.bfloat16, device=dev, requires_grad=True)  # noqa: E731
+    none, some = (torch.tensor(c, dtype=torch.int32, device=dev) for c in ([0, 0], [0, 9]))
+    o = packed_attention(z(0, 4), z(0, 2), z(0, 2), none)
+    assert o.shape == (0, 4, 64)
+    q, k, v = z(9, 4), z(0, 2), z(0, 2)
+    o = packed_attention(q, k, v, some, none)
+    o.sum().backward()
+    assert bool((o == 0).all() and (q.grad == 0).all()) and k.grad.shape == (0, 2, 64)
+    q, k, v = z(0, 4), z(9, 2), z(9, 2)
+    packed_attention(q, k, v, none, some).sum().backward()
+    assert bool((k.grad == 0).all() and (v.grad == 0).all())
+
+
+def test_packed_offsets_out_of_range_stay_inside(dev):
+    """Offsets outside the tensors are clamped to them; descending ones leave
+    rows unspecified and nothing else."""
+    from naylis_amd.mom_kernels import packed_attention
+    q, k, v, d, _, _ = _inputs([200], None, 2, 2, 64, 0, 0, dev)
+    c = lambda *x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    want = packed_attention(q, k, v, c(0, 200))
+    assert torch.equal(packed_attention(q, k, v, c(-5, 1 << 30)), want)
+    rnd = random.Random(0)
+    for _ in range(5):
+        packed_attention(q, k, v, c(*(rnd.randint(-300, 500) for _ in range(6))),
+                         c(*(rnd.randint(-300, 500) for _ in range(6))))
+    torch.cuda.synchronize()
+    assert torch.equal(packed_attention(q, k, v, c(0, 200)), want)
+
+
+def test_packed_streams_and_graph(dev):
+    """Another stream than the current one at creation, and a captured forward
+    and backward replayed on new inputs and new offsets."""
+    x = _inputs([100, 156], [130, 300], 4, 2, 128, 0, 0, dev)
+    want = _run(*x, 0.1)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = _run(*x, 0.1)
+    s.synchronize()
+    assert all(torch.equal(got[n], want[n]) for n in want)
+    held = [t.clone() for t in x]
+    with torch.cuda.stream(s):
+        _run(*held, 0.1)
+    s.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        outs = _run(*held, 0.1)
+    for lens in ([100, 156], [1, 255], [256, 0]):
+        y = _inputs(lens, [130, 300], 4, 2, 128, 0, 0, dev, seed=lens[0])
+        for a, b in zip(held, y):
+            a.copy_(b)
+        eager = _run(*y, 0.1)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(outs[n], eager[n]) for n in eager), lens
+
+
+def test_packed_second_derivative_raises(dev):
+    from naylis_amd.mom_kernels import packed_attention
+    q, k, v, d, cq, ck = _inputs([70], None, 2, 1, 64, 0, 0, dev)
+    want = _run(q, k, v, d, cq, ck, 0.125)
+    q, k, v, d = (t.requires_grad_() for t in (q, k, v, d))
+    got = torch.autograd.grad(packed_attention(q, k, v, cq), (q, k, v), d, create_graph=True)
+    assert all(torch.equal(a, want[n]) for a, n in zip(got, ("dq", "dk", "dv")))
+    with pytest.raises(RuntimeError, match="not implemented"):
+        torch.autograd.grad(got[0].float().sum(), k)
+
+
+def test_packed_refusals(dev):
+    from naylis_amd.mom_kernels import packed_attention
+    q, k, v, d, cq, ck = _inputs([20], None, 4, 2, 64, 0, 0, dev)
+    bad = [(q.float(), k, v, cq), (q[:, :3], k, v, cq), (q, k, v[:, :1], cq), (q[..., :32], k[..., :32], v[..., :32], cq),
+           (q, k.cpu(), v, cq), (q, k, v, cq.cpu()), (q, k, v, cq.float()), (q, k, v, cq[:1]), (q[0], k, v, cq),
+           (q, k[:, :0], v[:, :0], cq)]
+    for args in bad:
+        with pytest.raises(RuntimeError, match="packed_attention"):
+            packed_attention(*args)
+    for scale in (0.0, -1.0, math.inf, math.nan):
+        with pytest.raises(RuntimeError, match="scale"):
+            packed_attention(q, k, v, cq, scale=scale)
+    with pytest.raises(RuntimeError, match="packed_attention"):
+        packed_attention(q, k, v, cq, torch.cat([ck, ck]))
