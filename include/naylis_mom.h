@@ -553,8 +553,8 @@ int naylis_mom_paged_attn(const void* q, const void* k_pages, const void* v_page
  *   entropy (N) fp32 = -sum_j p_j lp_j
  *   top_ids (N, top) int64, top_logp (N, top) fp32: the `top` largest logits,
  *   descending, equal ones by the lowest index, NaN before all numbers
- *   stat (N, 3) fp32 for the backward: maximum, log of the sum of exponentials
- *   less the maximum, entropy; may be NULL
+ *   stat (N, 3) fp32 for the backward (reference and log2 of the sum in powers
+ *   of two, entropy); may be NULL
  * Columns of -inf have p = 0 and add nothing; a row without a finite logit is NaN.
  * The backward writes, for the gradients of logp and entropy (either may be
  * NULL; strides in elements, 0 for one value for all rows),
@@ -562,10 +562,14 @@ int naylis_mom_paged_attn(const void* q, const void* k_pages, const void* v_page
  * dense (N, V), in the logits' type; g_logp counts as 0 where the token is
  * ignore_index.
  * logits (N, V) in dtype (bf16 or fp32), row stride row_stride elements, any V
- * and any address that its elements allow; top <= min(64, V). */
+ * and any address that its elements allow; top <= min(64, V).  Workspace of the
+ * forward: naylis_mom_logprobs_workspace_bytes, 8-byte aligned (0 bytes for
+ * many rows, or narrow ones: then it may be NULL). */
+size_t naylis_mom_logprobs_workspace_bytes(int64_t N, int64_t V, int64_t top);
 int naylis_mom_logprobs_fwd(const void* logits, int dtype, int64_t row_stride, const int64_t* tokens, float* logp,
-                            float* entropy, float* stat, int64_t* top_ids, float* top_logp, int64_t N, int64_t V,
-                            int64_t top, int64_t ignore_index, void* stream);
+                            float* entropy, float* stat, int64_t* top_ids, float* top_logp, void* workspace,
+                            size_t workspace_bytes, int64_t N, int64_t V, int64_t top, int64_t ignore_index,
+                            void* stream);
 int naylis_mom_logprobs_bwd(const void* logits, int dtype, int64_t row_stride, const int64_t* tokens,
                             const float* stat, const float* g_logp, int64_t g_logp_stride, const float* g_entropy,
                             int64_t g_entropy_stride, void* dlogits, int64_t N, int64_t V, int64_t ignore_index,

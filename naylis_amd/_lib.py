@@ -90,7 +90,9 @@ SIGNATURES = {
     "naylis_mom_paged_attn_workspace_bytes": (_size_t, [_int] + [_i64] * 6),
     "naylis_mom_paged_attn": (_int, [_c_void_p] * 5 + [_int] + [_c_void_p] * 4 + [_size_t, _c_void_p, _float]
                               + [_i64] * 7 + [_c_void_p]),
-    "naylis_mom_logprobs_fwd": (_int, [_c_void_p, _int, _i64] + [_c_void_p] * 6 + [_i64] * 4 + [_c_void_p]),
+    "naylis_mom_logprobs_workspace_bytes": (_size_t, [_i64] * 3),
+    "naylis_mom_logprobs_fwd": (_int, [_c_void_p, _int, _i64] + [_c_void_p] * 7 + [_size_t] + [_i64] * 4
+                                + [_c_void_p]),
     "naylis_mom_logprobs_bwd": (_int, [_c_void_p, _int, _i64] + [_c_void_p] * 3 + [_i64, _c_void_p, _i64, _c_void_p]
                                 + [_i64] * 3 + [_c_void_p]),
     "naylis_mom_timing_enable": (None, [_int]),

@@ -1274,9 +1274,15 @@ static int check_logprobs(const void* logits, int dtype, int64_t ld, const int64
   return NAYLIS_OK;
 }
 
+size_t naylis_mom_logprobs_workspace_bytes(int64_t N, int64_t V, int64_t top) {
+  if (N < 0 || N >= ((int64_t)1 << 31) || V < 1 || V > (1 << 30) || top < 0 || top > kLogprobsMaxTop) return 0;
+  return logprobs_ws_bytes((long)N, (int)V, (int)top);
+}
+
 int naylis_mom_logprobs_fwd(const void* logits, int dtype, int64_t row_stride, const int64_t* tokens, float* logp,
-                            float* entropy, float* stat, int64_t* top_ids, float* top_logp, int64_t N, int64_t V,
-                            int64_t top, int64_t ignore_index, void* stream) {
+                            float* entropy, float* stat, int64_t* top_ids, float* top_logp, void* workspace,
+                            size_t workspace_bytes, int64_t N, int64_t V, int64_t top, int64_t ignore_index,
+                            void* stream) {
   const char* who = "mom_logprobs_fwd";
   int rc = check_logprobs(logits, dtype, row_stride, tokens, N, V, who);
   if (rc) return rc;
@@ -1285,9 +1291,14 @@ int naylis_mom_logprobs_fwd(const void* logits, int dtype, int64_t row_stride, c
   if (N == 0) return NAYLIS_OK;
   if (!logp || !entropy || (top > 0 && (!top_ids || !top_logp)))
     return fail(NAYLIS_ERR_ARG, "%s: null pointer argument", who);
+  const size_t need = logprobs_ws_bytes((long)N, (int)V, (int)top);
+  if (workspace_bytes < need)
+    return fail(NAYLIS_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", who, workspace_bytes, need);
+  if (need && (!workspace || (uintptr_t)workspace % 8 != 0))
+    return fail(NAYLIS_ERR_ARG, "%s: the workspace must be 8-byte aligned", who);
   return hip_status(launch_logprobs_fwd(logits, dtype == NAYLIS_DTYPE_BF16, (long)row_stride, tokens, logp, entropy,
-                                        stat, top_ids, top_logp, (long)N, (int)V, (int)top, (long)ignore_index,
-                                        (hipStream_t)stream),
+                                        stat, top_ids, top_logp, workspace, (long)N, (int)V, (int)top,
+                                        (long)ignore_index, (hipStream_t)stream),
                     who);
 }
 

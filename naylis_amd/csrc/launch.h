@@ -168,9 +168,10 @@ hipError_t launch_paged_attn(const PagedCacheDims& c, int hd, bool fp8, const vo
 // Log probabilities of tokens (logprobs.hip): logits (N, V) bf16 or fp32 with
 // row stride ld; stat (N, 3) fp32, top_ids / top_logp (N, top).
 constexpr int kLogprobsMaxTop = 64;
+size_t logprobs_ws_bytes(long N, int V, int top);
 hipError_t launch_logprobs_fwd(const void* logits, bool bf16, long ld, const int64_t* tokens, float* logp,
-                               float* entropy, float* stat, int64_t* top_ids, float* top_logp, long N, int V, int top,
-                               long ignore_index, hipStream_t st);
+                               float* entropy, float* stat, int64_t* top_ids, float* top_logp, void* ws, long N,
+                               int V, int top, long ignore_index, hipStream_t st);
 hipError_t launch_logprobs_bwd(const void* logits, bool bf16, long ld, const int64_t* tokens, const float* stat,
                                const float* g_logp, long gl_stride, const float* g_entropy, long ge_stride,
                                void* dlogits, long N, int V, long ignore_index, hipStream_t st);

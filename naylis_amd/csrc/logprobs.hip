@@ -5,28 +5,42 @@
 //   dx_j = g_logp (1[j = token] - p_j) - g_H p_j (lp_j + H).
 // The reference keeps the summed loss of such rows (model.py:536-545).
 //
-// One workgroup per row, any V, any row stride and address: 16-byte chunks at
-// the row's own alignment, its two ragged ends element by element.  Forward:
-// one pass with a running maximum m, sum of e^{x - m} and sum of
-// e^{x - m} (x - m) per thread, joined at the end; H = log s - t / s.  Bound by
-// HBM (the logits once).  Statistics are fp32, saved as (m, log s, H): x - m is
-// nearly exact where their sum would lose the last bits of small lp.
+// One workgroup per row (a few wide rows: one per part of a row, and a second
+// launch that joins them), any V, any row stride and address: 16-byte chunks
+// from the row's first 16-byte boundary, the few elements beside them one a
+// thread.  Forward: one pass with a running reference c (log2 of the largest
+// e^x so far), s = sum 2^z and t = sum 2^z z, z = x log2 e - c, per thread;
+// H = (log2 s - t / s) ln 2.  All statistics are fp32, saved as (c, log2 s, H):
+// lp = (x log2 e - c - log2 s) ln 2 keeps the last bits that a single
+// log-sum-exp would lose.
 //
-// The top k come from a second look at the row, out of the caches: the k-th
-// largest of the threads' maxima is a value that at least k logits reach, and
-// few others; those are collected in LDS and ranked (value, then lowest index).
-// Where too many reach it (a row of equal logits) k passes take one each.
+// The top k come from a second look at the row (registers, or the caches): the
+// k-th largest of the threads' maxima is a value that at least k logits reach,
+// and few others; those are collected in LDS and ranked (value, then lowest
+// index).  Where too many reach it (a row of equal logits) k passes take one each.
+//
+// Many rows are bound by HBM: 4096 x 50001 bf16 69 us (5.9 TB/s; fp32 127 us, 6.5
+// TB/s), with the top 20, read twice, 122; a thread that keeps values as fp32
+// between maximum and sum, 8 chunks at a time, takes 200 registers and 105 us.
+// The gradient 180 us (4.6 TB/s read and written; a copy reaches 4.95).  Few rows
+// are bound by the steps within a workgroup: 64 x 32768 with the top 20 8.9 us
+// (1024 threads; 19.6 with 512 and a second read), of which 3 are launch and
+// first load.  One row of 151999 in 8 parts 13.7 us, in one 21.9; 64 of them 17.4
+// and 22.9.  Parts of 4096 columns of a 32768 row cost more than they save (9 + 6 us).
 #include "common.h"
 #include "launch.h"
 #include "timing.h"
 
+#include <algorithm>
 #include <type_traits>
 
 namespace naylis {
 
 namespace {
 
-constexpr int kCand = 1024;  // candidates ranked at once
+constexpr int kCand = 1024;     // candidates ranked at once
+constexpr int kMaxParts = 8;    // parts of a row
+constexpr float kLn2 = 0.6931471805599453f;
 
 // order of torch's descending sort as an unsigned key: NaN first, -0 equal to 0
 __device__ __forceinline__ uint32_t sort_key(float x) {
@@ -42,222 +56,379 @@ __device__ __forceinline__ float value(T x) {
     return x;
 }
 
-// A row of V values in 16-byte chunks of E, counted from the 16-byte boundary
-// at or before it: chunk i holds elements E i - skip .. E i - skip + E - 1.
+// A row of V values: whole 16-byte chunks of E from the first 16-byte boundary
+// on, and the few elements before and behind them, one for each of the first
+// threads (`extra`).
 template <typename T>
 struct Row {
   static constexpr int E = 16 / sizeof(T);
   const T* x;
-  int V, skip, chunks;
+  int V, head, chunks;
   __device__ __forceinline__ Row(const T* p, int V_) : x(p), V(V_) {
-    skip = (int)((uintptr_t)p % 16 / sizeof(T));
-    chunks = (V + skip + E - 1) / E;
+    head = min((int)((16 - (uintptr_t)p % 16) % 16 / sizeof(T)), V);
+    chunks = (V - head) / E;
   }
-  // chunk i as fp32; elements outside the row (and chunks past it) are -inf
-  __device__ __forceinline__ void get(int i, float (&f)[E]) const {
-    const int j0 = E * i - skip;
-    if (j0 >= 0 && j0 + E <= V) {
-      const uint4 u = __builtin_bit_cast(uint4, *reinterpret_cast<const f32x4*>(x + j0));
-      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  __device__ __forceinline__ int first(int i) const { return head + E * i; }
+  // the element outside the chunks that thread tid holds, or -1
+  __device__ __forceinline__ int extra(int tid) const {
+    const int j = tid < head ? tid : tid + E * chunks;
+    return j < V && (tid < head || j >= head + E * chunks) ? j : -1;
+  }
+  template <bool ONCE>  // not read again: kept out of the caches' way
+  __device__ __forceinline__ uint4 get(int i) const {
+    const f32x4* p = reinterpret_cast<const f32x4*>(x + first(i));
+    return __builtin_bit_cast(uint4, ONCE ? __builtin_nontemporal_load(p) : *p);
+  }
+  // U chunks i0, i0 + step, ..; those past the last are -inf
+  template <int U, bool ONCE>
+  __device__ __forceinline__ void get(uint4 (&u)[U], int i0, int step, bool all) const {
+    if (all) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if constexpr (E == 8) {
-          f[2 * e] = __uint_as_float(w[e] << 16);
-          f[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
-        } else {
-          f[e] = __uint_as_float(w[e]);
-        }
-      }
+      for (int i = 0; i < U; ++i) u[i] = get<ONCE>(i0 + i * step);
     } else {
+      const uint32_t none = E == 8 ? 0xff80ff80u : 0xff800000u;
 #pragma unroll
-      for (int e = 0; e < E; ++e) f[e] = j0 + e >= 0 && j0 + e < V ? value(x[j0 + e]) : -INFINITY;
+      for (int i = 0; i < U; ++i)
+        u[i] = i0 + i * step < chunks ? get<ONCE>(i0 + i * step) : make_uint4(none, none, none, none);
     }
   }
 };
 
-// (m, s, t) of two parts of a row
+// element e of a chunk
+template <int E>
+__device__ __forceinline__ float element(const uint4& u, int e) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  if constexpr (E == 4) return __uint_as_float(w[e]);
+  return __uint_as_float((e & 1) ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
+}
+
+// max(a, b, c), NaN left out; written out because fmaxf of bits from memory
+// costs a second instruction that quiets NaN
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+
+// Sums of a part of a row in powers of two, against a reference c (the log2 of
+// its largest e^x, rounded once: all terms of a sum use the same number, so its
+// rounding drops out): s = sum 2^z, t = sum 2^z z with z = x log2 e - c.
+// m is the largest x itself.
 struct Sums {
-  float m, s, t;
-  __device__ __forceinline__ void join(const Sums& o) {
-    const float mn = fmaxf(m, o.m);
-    const float da = m - mn, db = o.m - mn;  // -inf parts are empty: weight 0
-    const float a = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(da * kLog2e);
-    const float b = o.m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(db * kLog2e);
-    t = (m == -INFINITY ? 0.f : a * fmaf(da, s, t)) + (o.m == -INFINITY ? 0.f : b * fmaf(db, o.s, o.t));
-    s = a * s + b * o.s;
-    m = mn;
+  float m, c, s, t;
+  // against the reference of a whole; an empty part (m = -inf) weighs nothing
+  __device__ __forceinline__ void rescale(float cw) {
+    const float d = c - cw, a = __builtin_amdgcn_exp2f(d);
+    t = m == -INFINITY ? 0.f : a * fmaf(d, s, t);
+    s = m == -INFINITY ? 0.f : a * s;
+    c = cw;
   }
 };
+
+// U chunks of a thread into its sums: per value a shift or mask, half a maximum,
+// two fused multiply-adds, an exponential, a maximum and a sum
+template <int E, int U>
+__device__ __forceinline__ void add_chunks(Sums& a, const uint4 (&u)[U], bool& nan) {
+  float m = a.m;
+#pragma unroll
+  for (int i = 0; i < U; ++i)
+#pragma unroll
+    for (int e = 0; e < E; e += 2) m = max3(m, element<E>(u[i], e), element<E>(u[i], e + 1));
+  if (m == -INFINITY) {  // nothing but -inf (or NaN) so far
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+#pragma unroll
+      for (int e = 0; e < E; ++e) nan |= element<E>(u[i], e) != element<E>(u[i], e);
+    return;
+  }
+  const float c = m * kLog2e;
+  if (a.m == -INFINITY)
+    a.c = c;
+  else if (m > a.m)
+    a.rescale(c);
+  a.m = m;
+  float s[2] = {a.s, 0.f}, t[2] = {a.t, 0.f};  // two chains
+#pragma unroll
+  for (int i = 0; i < U; ++i)
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const float z = fmaf(element<E>(u[i], e), kLog2e, -a.c), p = __builtin_amdgcn_exp2f(z);
+      s[e & 1] += p;
+      t[e & 1] = fmaf(p, fmaxf(z, -1e30f), t[e & 1]);  // 0 log 0 = 0
+    }
+  a.s = s[0] + s[1];
+  a.t = t[0] + t[1];
+}
+
+// one value more
+__device__ __forceinline__ void add_one(Sums& a, float x, bool& nan) {
+  nan |= x != x;
+  if (!(x > -INFINITY)) return;
+  if (a.m == -INFINITY) {
+    a.m = x;
+    a.c = x * kLog2e;
+  } else if (x > a.m) {
+    a.m = x;
+    a.rescale(x * kLog2e);
+  }
+  const float z = fmaf(x, kLog2e, -a.c), p = __builtin_amdgcn_exp2f(z);
+  a.s += p;
+  a.t = fmaf(p, fmaxf(z, -1e30f), a.t);
+}
+
+// The order of the top: a logit's sort key, then the lowest column.
+__device__ __forceinline__ unsigned long long rank_key(float f, int j) {
+  return ((unsigned long long)sort_key(f) << 32) | (uint32_t)~j;
+}
+__device__ __forceinline__ int column(unsigned long long k) { return (int)~(uint32_t)k; }
+__device__ __forceinline__ float logit(unsigned long long k) {
+  const uint32_t u = (uint32_t)(k >> 32);
+  return __uint_as_float((u >> 31) ? u & 0x7fffffffu : ~u);
+}
+
+// log p of a logit from its row's reference and log2 of its sum
+__device__ __forceinline__ float log_prob(float x, float c, float ls) {
+  return (fmaf(x, kLog2e, -c) - ls) * kLn2;
+}
+
+// Joins the sums of `count` <= 64 parts that stand in LDS; every lane gets them.
+__device__ __forceinline__ Sums join_parts(const float* c, const float* s, const float* t, int count) {
+  const int lane = threadIdx.x & 63, i = min(lane, count - 1);
+  Sums a{c[i], c[i], s[i], t[i]};
+  a.rescale(wave_allmax(a.c));
+  a.s = wave_allsum(lane < count ? a.s : 0.f);
+  a.t = wave_allsum(lane < count ? a.t : 0.f);
+  return a;
+}
+
+struct LogprobsOut {
+  float* logp;
+  float* entropy;
+  float* stat;
+  int64_t* top_ids;
+  float* top_logp;
+};
+
+// A row's numbers from its sums (one thread); returns log2 s.  A row without a
+// finite logit: c = -inf, NaN throughout.
+__device__ __forceinline__ void write_row(const LogprobsOut& o, long r, const Sums& a, float ls, float xt, bool ignored,
+                                          bool in_range) {
+  const float ent = (ls - a.t / a.s) * kLn2;
+  o.logp[r] = ignored ? 0.f : in_range ? log_prob(xt, a.c, ls) : __builtin_nanf("");
+  o.entropy[r] = ent;
+  if (o.stat) {
+    o.stat[3 * r] = a.c;
+    o.stat[3 * r + 1] = ls;
+    o.stat[3 * r + 2] = ent;
+  }
+}
 
 }  // namespace
 
-template <typename T, int NT>
+// One row, or (parts > 1) one of its parts of `width` columns: then the sums
+// and the part's `top` rank keys (0 behind its last) go to `part_sums` and
+// `part_keys` for logprobs_join_kernel.
+// HELD: a thread's U chunks are all there are and stay in registers, so that
+// the second look (TOP) reads no memory; else they pass U at a time.
+template <typename T, int NT, int U, bool HELD, bool TOP>
 __global__ __launch_bounds__(NT) void logprobs_fwd_kernel(const T* __restrict__ logits, long ld,
-                                                          const int64_t* __restrict__ tokens,
-                                                          float* __restrict__ logp, float* __restrict__ entropy,
-                                                          float* __restrict__ stat, int64_t* __restrict__ top_ids,
-                                                          float* __restrict__ top_logp, int V, int top,
-                                                          long ignore_index) {
-  constexpr int E = Row<T>::E, W = NT / 64, U = 4;
-  __shared__ Sums red[W];
-  __shared__ float maxima[NT];
-  __shared__ uint32_t cand_key[kCand];
-  __shared__ int cand_id[kCand];
-  __shared__ int count;
-  __shared__ uint32_t bound_s;
-  __shared__ unsigned long long best_s[W];
+                                                          const int64_t* __restrict__ tokens, LogprobsOut o, int V,
+                                                          int top, long ignore_index, int parts, int width,
+                                                          float* __restrict__ part_sums,
+                                                          unsigned long long* __restrict__ part_keys) {
+  constexpr int E = Row<T>::E, W = NT / 64;
+  constexpr int RB = 4;       // key bits found in a round
+  constexpr int VW = 16 / W;  // their values that a wave looks at
+  constexpr int KEYBITS = sizeof(T) == 2 ? 16 : 32;
+  static_assert(W == 16 || W == 4, "a power of four waves");
+  __shared__ float red[3][W];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const long r = blockIdx.x;
-  const Row<T> row(logits + r * ld, V);
-  const long tok = tokens[r];
+  const int col0 = blockIdx.y * width;  // the first column of this part
+  const T* x = logits + r * ld;
+  const Row<T> row(x + col0, min(width, V - col0));
+  const long tok = parts == 1 ? tokens[r] : 0;
   const bool in_range = tok >= 0 && tok < V;
-  const float xt = value(row.x[in_range ? tok : 0]);
+  const float xt = parts == 1 ? value(x[in_range ? tok : 0]) : 0.f;
+  const int je = row.extra(tid);
+  const float xe = je >= 0 ? value(row.x[je]) : -INFINITY;
 
-  Sums a{-INFINITY, 0.f, 0.f};
+  Sums a{-INFINITY, -INFINITY, 0.f, 0.f};
   bool nan = false;
-  for (int c0 = tid; c0 < row.chunks; c0 += NT * U) {
-    float f[U][E];
-#pragma unroll
-    for (int u = 0; u < U; ++u) row.get(c0 + u * NT, f[u]);
-    float m = a.m;
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int e = 0; e < E; ++e) m = fmaxf(m, f[u][e]);
-    if (m == -INFINITY) {  // nothing but -inf (or NaN) so far
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int e = 0; e < E; ++e) nan |= f[u][e] != f[u][e];
-      continue;
+  uint4 u[U];
+  if constexpr (HELD) {
+    row.template get<U, !TOP>(u, tid, NT, NT * U <= row.chunks);
+    add_chunks<E, U>(a, u, nan);
+  } else {
+    for (int c0 = 0; c0 < row.chunks; c0 += NT * U) {
+      row.template get<U, !TOP>(u, c0 + tid, NT, c0 + NT * U <= row.chunks);
+      add_chunks<E, U>(a, u, nan);
     }
-    if (a.m != -INFINITY) {
-      const float da = a.m - m, al = __builtin_amdgcn_exp2f(da * kLog2e);
-      a.t = al * fmaf(da, a.s, a.t);
-      a.s *= al;
-    }
-    a.m = m;
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const float d = f[u][e] - m, p = __builtin_amdgcn_exp2f(d * kLog2e);
-        a.s += p;
-        a.t = fmaf(p, fmaxf(d, -1e30f), a.t);  // 0 log 0 = 0
-      }
   }
-  if (top > 0) maxima[tid] = a.m;  // a logit of the row, or -inf
-  if (nan) {
-    a.s = __builtin_nanf("");
-    if (a.m == -INFINITY) a.m = 0.f;
+  add_one(a, xe, nan);
+  const float mine = a.m;  // one of the logits, or -inf
+  if (nan) a = Sums{0.f, 0.f, __builtin_nanf(""), 0.f};
+  a.rescale(wave_allmax(a.c));
+  a.s = wave_allsum(a.s);
+  a.t = wave_allsum(a.t);
+  if (lane == 0) {
+    red[0][wave] = a.c;
+    red[1][wave] = a.s;
+    red[2][wave] = a.t;
   }
-  // the wave's lanes, then the waves
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    Sums b{__shfl_xor(a.m, o, 64), __shfl_xor(a.s, o, 64), __shfl_xor(a.t, o, 64)};
-    a.join(b);
-  }
-  if (lane == 0) red[wave] = a;
-  if (tid == 0) count = 0;
   __syncthreads();
-  a = red[0];
-#pragma unroll
-  for (int i = 1; i < W; ++i) a.join(red[i]);
-  const float ls = logf(a.s);  // a row without a finite logit: m = -inf, log 0, NaN below
+  a = join_parts(red[0], red[1], red[2], W);
+  const float ls = log2f(a.s);
+  const long part = r * parts + blockIdx.y;
   if (tid == 0) {
-    const float ent = ls - a.t / a.s;
-    logp[r] = tok == ignore_index ? 0.f : in_range ? (xt - a.m) - ls : __builtin_nanf("");
-    entropy[r] = ent;
-    if (stat) {
-      stat[3 * r] = a.m;
-      stat[3 * r + 1] = ls;
-      stat[3 * r + 2] = ent;
+    if (parts == 1) {
+      write_row(o, r, a, ls, xt, tok == ignore_index, in_range);
+    } else {
+      part_sums[3 * part] = a.c;
+      part_sums[3 * part + 1] = a.s;
+      part_sums[3 * part + 2] = a.t;
     }
   }
-  if (top == 0) return;
-
-  // the k-th largest of the threads' maxima, bit by bit from the top
-  if (wave == 0) {
-    uint32_t key[NT / 64];
+  if constexpr (TOP) {
+    __shared__ uint32_t maxima[NT];
+    __shared__ int counts[2][16];
+    __shared__ unsigned long long cand[kCand];
+    __shared__ int count;
+    __shared__ unsigned long long best_s[W];
+    maxima[tid] = sort_key(mine) >> (32 - KEYBITS);
+    if (tid == 0) count = 0;
+    __syncthreads();
+    // the top-th largest of the threads' maxima, four bits of its key a round: the
+    // waves count the maxima that reach the bits found so far and each next four
+    uint32_t key[NT / 64], bound = 0;
 #pragma unroll
-    for (int i = 0; i < NT / 64; ++i) key[i] = sort_key(maxima[64 * i + lane]);
-    uint32_t bound = 0;
-    for (int bit = 31; bit >= 0; --bit) {
-      const uint32_t next = bound | (1u << bit);
-      int n = 0;
+    for (int i = 0; i < NT / 64; ++i) key[i] = maxima[64 * i + lane];
 #pragma unroll
-      for (int i = 0; i < NT / 64; ++i) n += __popcll(__ballot(key[i] >= next));
-      if (n >= top) bound = next;
+    for (int shift = KEYBITS - RB, round = 0; shift >= 0; shift -= RB, ++round) {
+#pragma unroll
+      for (int v = 0; v < VW; ++v) {
+        const uint32_t next = bound | ((uint32_t)(wave * VW + v) << shift);
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < NT / 64; ++i) n += __popcll(__ballot(key[i] >= next));
+        if (lane == 0) counts[round & 1][wave * VW + v] = n;
+      }
+      __syncthreads();
+      // the counts fall, so the last value that `top` maxima reach is how many such there are, less one
+      const int w = __popcll(__ballot(lane < 16 && counts[round & 1][lane & 15] >= top)) - 1;
+      bound |= (uint32_t)max(w, 0) << shift;
     }
-    if (lane == 0) bound_s = bound;
-  }
-  __syncthreads();
-  const uint32_t bound = bound_s;
-  for (int c0 = tid; c0 < row.chunks; c0 += NT * U) {
-    float f[U][E];
+    // (bound 0: fewer threads than `top` have a logit)
+    const float least = bound == 0 ? -INFINITY : logit((unsigned long long)bound << (64 - KEYBITS));
+    const bool plain = a.s == a.s;  // no NaN, which a maximum leaves out
+    auto collect = [&](float f, int j) {
+      if (f < least) return;
+      const int at = atomicAdd(&count, 1);
+      if (at < kCand) cand[at] = rank_key(f, col0 + j);
+    };
+    if (je >= 0) collect(xe, je);
+    auto look = [&](int c0) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) row.get(c0 + u * NT, f[u]);
+      for (int i = 0; i < U; ++i) {
+        const int c = c0 + tid + i * NT;
+        float most = -INFINITY;
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+        for (int e = 0; e < E; e += 2) most = max3(most, element<E>(u[i], e), element<E>(u[i], e + 1));
+        if (c < row.chunks && !(plain && most < least)) {
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const int j = E * (c0 + u * NT) - row.skip + e;
-        if (sort_key(f[u][e]) >= bound && j >= 0 && j < V) {
-          const int at = atomicAdd(&count, 1);
-          if (at < kCand) {
-            cand_key[at] = sort_key(f[u][e]);
-            cand_id[at] = j;
-          }
+          for (int e = 0; e < E; ++e) collect(element<E>(u[i], e), row.first(c) + e);
         }
       }
-  }
-  __syncthreads();
-  int64_t* ids = top_ids + r * top;
-  float* lps = top_logp + r * top;
-  const int n = count;
-  if (n <= kCand) {
-    for (int i = tid; i < n; i += NT) {
-      const uint32_t k = cand_key[i];
-      const int id = cand_id[i];
-      int rank = 0;
-      for (int j = 0; j < n; ++j) rank += cand_key[j] > k || (cand_key[j] == k && cand_id[j] < id);
-      if (rank < top) {
-        ids[rank] = id;
-        lps[rank] = (value(row.x[id]) - a.m) - ls;
+    };
+    if constexpr (HELD) {
+      look(0);
+    } else {
+      for (int c0 = 0; c0 < row.chunks; c0 += NT * U) {
+        row.template get<U, false>(u, c0 + tid, NT, c0 + NT * U <= row.chunks);
+        look(c0);
       }
     }
-    return;
-  }
-  // one pass for each: the best logit behind the last one taken
-  unsigned long long last = ~0ull;  // key, then the lowest index first
-  for (int i = 0; i < top; ++i) {
-    unsigned long long best = 0;
-    for (int c = tid; c < row.chunks; c += NT) {
-      float f[E];
-      row.get(c, f);
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const int j = E * c - row.skip + e;
-        if (j < 0 || j >= V) continue;
-        const unsigned long long k = ((unsigned long long)sort_key(f[e]) << 32) | (uint32_t)~j;
+    __syncthreads();
+    const int n = count;
+    auto write = [&](int rank, unsigned long long k) {
+      if (parts == 1) {
+        o.top_ids[r * top + rank] = column(k);
+        o.top_logp[r * top + rank] = log_prob(logit(k), a.c, ls);
+      } else {
+        part_keys[part * top + rank] = k;
+      }
+    };
+    if (parts > 1 && tid >= n && tid < top) write(tid, 0);
+    if (n <= kCand) {
+      for (int i = tid; i < n; i += NT) {
+        const unsigned long long k = cand[i];
+        int rank = 0;
+#pragma unroll 8
+        for (int j = 0; j < n; ++j) rank += cand[j] > k;
+        if (rank < top) write(rank, k);
+      }
+      return;
+    }
+    // one pass for each: the best logit behind the last one taken
+    unsigned long long last = ~0ull;
+    for (int i = 0; i < top; ++i) {
+      unsigned long long best = 0;
+      const auto see = [&](float f, int j) {
+        const unsigned long long k = rank_key(f, col0 + j);
         if (k < last && k > best) best = k;
+      };
+      if (je >= 0) see(xe, je);
+      for (int c = tid; c < row.chunks; c += NT) {
+        const uint4 v = row.template get<false>(c);
+#pragma unroll
+        for (int e = 0; e < E; ++e) see(element<E>(v, e), row.first(c) + e);
       }
-    }
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const unsigned long long k = __shfl_xor(best, o, 64);
-      best = k > best ? k : best;
-    }
-    __syncthreads();
-    if (lane == 0) best_s[wave] = best;
-    __syncthreads();
+      for (int o = 1; o < 64; o <<= 1) {
+        const unsigned long long k = __shfl_xor(best, o, 64);
+        best = k > best ? k : best;
+      }
+      __syncthreads();
+      if (lane == 0) best_s[wave] = best;
+      __syncthreads();
 #pragma unroll
-    for (int w = 0; w < W; ++w) best = best_s[w] > best ? best_s[w] : best;
-    last = best;
-    if (tid == 0) {
-      const int id = (int)~(uint32_t)best;
-      ids[i] = id;
-      lps[i] = (value(row.x[id]) - a.m) - ls;
+      for (int w = 0; w < W; ++w) best = best_s[w] > best ? best_s[w] : best;
+      last = best;
+      if (tid == 0) write(i, best);
+    }
+  }
+}
+
+// A row from its parts.
+template <typename T>
+__global__ __launch_bounds__(256) void logprobs_join_kernel(const T* __restrict__ logits, long ld,
+                                                            const int64_t* __restrict__ tokens, LogprobsOut o, int V,
+                                                            int top, long ignore_index, int parts,
+                                                            const float* __restrict__ part_sums,
+                                                            const unsigned long long* __restrict__ part_keys) {
+  __shared__ float red[3][kMaxParts];
+  __shared__ unsigned long long cand[kMaxParts * kLogprobsMaxTop];
+  const int tid = threadIdx.x;
+  const long r = blockIdx.x;
+  const long tok = tokens[r];
+  const bool in_range = tok >= 0 && tok < V;
+  const float xt = value(logits[r * ld + (in_range ? tok : 0)]);
+  if (tid < 3 * parts) red[tid % 3][tid / 3] = part_sums[3 * r * parts + tid];
+  const int n = parts * top;
+  for (int i = tid; i < n; i += 256) cand[i] = part_keys[r * n + i];
+  __syncthreads();
+  const Sums a = join_parts(red[0], red[1], red[2], parts);
+  const float ls = log2f(a.s);
+  if (tid == 0) write_row(o, r, a, ls, xt, tok == ignore_index, in_range);
+  for (int i = tid; i < n; i += 256) {
+    const unsigned long long k = cand[i];
+    if (k == 0) continue;  // behind a part's last logit
+    int rank = 0;
+#pragma unroll 8
+    for (int j = 0; j < n; ++j) rank += cand[j] > k;
+    if (rank < top) {
+      o.top_ids[r * top + rank] = column(k);
+      o.top_logp[r * top + rank] = log_prob(logit(k), a.c, ls);
     }
   }
 }
@@ -277,75 +448,104 @@ __global__ __launch_bounds__(256) void logprobs_bwd_kernel(const T* __restrict__
   const T* x = logits + r * ld;
   const bool same = (uintptr_t)x % 16 == (uintptr_t)out.x % 16;
   const long tok = tokens[r];
-  const float m = stat[3 * r], ls = stat[3 * r + 1], ent = stat[3 * r + 2];
+  const float ref = stat[3 * r], ls = stat[3 * r + 1], ent = stat[3 * r + 2];
   const float gl = !g_logp || tok == ignore_index ? 0.f
                    : tok >= 0 && tok < V          ? g_logp[r * gl_stride]
                                                   : __builtin_nanf("");
   const float ge = g_entropy ? g_entropy[r * ge_stride] : 0.f;
-  for (int c = threadIdx.x; c < out.chunks; c += 256) {
-    const int j0 = E * c - out.skip;
-    const bool whole = j0 >= 0 && j0 + E <= V;
-    float f[E], d[E];
-    if (whole && same) {
-      const uint4 u = __builtin_bit_cast(uint4, *reinterpret_cast<const f32x4*>(x + j0));
-      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  // z ln 2 = log p; 0 log 0 = 0 (the comparison keeps NaN)
+  const auto grad = [&](float f, int j) {
+    const float z = fmaf(f, kLog2e, -ref) - ls, p = __builtin_amdgcn_exp2f(z);
+    return (j == tok ? gl : 0.f) - p * fmaf(ge, fmaf(z < -1e30f ? -1e30f : z, kLn2, ent), gl);
+  };
+  T* dx = dlogits + r * (long)V;
+  constexpr int U = 4;
+  for (int c0 = threadIdx.x; c0 < out.chunks; c0 += 256 * U) {
+    uint4 u[U];
+    if (same) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if constexpr (E == 8) {
-          f[2 * e] = __uint_as_float(w[e] << 16);
-          f[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
-        } else {
-          f[e] = __uint_as_float(w[e]);
-        }
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < E; ++e) f[e] = j0 + e >= 0 && j0 + e < V ? value(x[j0 + e]) : -INFINITY;
+      for (int i = 0; i < U; ++i)
+        u[i] = *reinterpret_cast<const uint4*>(x + out.first(min(c0 + 256 * i, out.chunks - 1)));
     }
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const float lp = (f[e] - m) - ls, p = expf(lp);
-      // 0 log 0 = 0 (the comparison keeps NaN)
-      d[e] = (j0 + e == tok ? gl : 0.f) - p * fmaf(ge, (lp < -1e30f ? -1e30f : lp) + ent, gl);
-    }
-    if (whole) {
-      if constexpr (E == 8) {
-        bf16x8 o;
+    for (int i = 0; i < U; ++i) {
+      const int j0 = out.first(c0 + 256 * i);
+      if (c0 + 256 * i >= out.chunks) break;
+      float d[E];
+      if (same) {
 #pragma unroll
-        for (int e = 0; e < E; ++e) o[e] = (__bf16)d[e];
-        __builtin_nontemporal_store(__builtin_bit_cast(f32x4, o), reinterpret_cast<f32x4*>(dlogits + r * (long)V + j0));
+        for (int e = 0; e < E; ++e) d[e] = grad(element<E>(u[i], e), j0 + e);
       } else {
-        f32x4 o;
+#pragma unroll
+        for (int e = 0; e < E; ++e) d[e] = grad(value(x[j0 + e]), j0 + e);
+      }
+      f32x4 o;
+      if constexpr (E == 8) {
+        bf16x8 h;
+#pragma unroll
+        for (int e = 0; e < E; ++e) h[e] = (__bf16)d[e];
+        o = __builtin_bit_cast(f32x4, h);
+      } else {
 #pragma unroll
         for (int e = 0; e < E; ++e) o[e] = d[e];
-        __builtin_nontemporal_store(o, reinterpret_cast<f32x4*>(dlogits + r * (long)V + j0));
       }
-    } else {
-#pragma unroll
-      for (int e = 0; e < E; ++e)
-        if (j0 + e >= 0 && j0 + e < V) {
-          if constexpr (E == 8)
-            dlogits[r * (long)V + j0 + e] = f32_to_bf16(d[e]);
-          else
-            dlogits[r * (long)V + j0 + e] = d[e];
-        }
+      __builtin_nontemporal_store(o, reinterpret_cast<f32x4*>(dx + j0));
     }
+  }
+  const int je = out.extra(threadIdx.x);
+  if (je >= 0) {
+    const float d = grad(value(x[je]), je);
+    if constexpr (E == 8)
+      dx[je] = f32_to_bf16(d);
+    else
+      dx[je] = d;
   }
 }
 
+// A few wide rows are cut into parts, up to two workgroups a CU, and joined by
+// a second launch.
+static int logprobs_parts(long N, int V) {
+  return V < 65536 ? 1 : (int)std::max(1L, std::min(512 / std::max(N, 1L), (long)kMaxParts));
+}
+
+size_t logprobs_ws_bytes(long N, int V, int top) {
+  const int parts = logprobs_parts(N, V);
+  return parts == 1 ? 0 : (size_t)N * parts * (8 * (size_t)top + 12);
+}
+
 hipError_t launch_logprobs_fwd(const void* logits, bool bf16, long ld, const int64_t* tokens, float* logp,
-                               float* entropy, float* stat, int64_t* top_ids, float* top_logp, long N, int V, int top,
-                               long ignore_index, hipStream_t st) {
+                               float* entropy, float* stat, int64_t* top_ids, float* top_logp, void* ws, long N,
+                               int V, int top, long ignore_index, hipStream_t st) {
+  const LogprobsOut o{logp, entropy, stat, top_ids, top_logp};
+  const int parts = logprobs_parts(N, V);
+  const int width = parts == 1 ? V : ((V + parts - 1) / parts + 63) / 64 * 64;
+  auto* keys = (unsigned long long*)ws;
+  auto* sums = (float*)(keys + (size_t)N * parts * top);
   auto run = [&](auto kernel, auto* x, int threads) {
     NAYLIS_TIMED("logprobs_fwd", st,
-                 hipLaunchKernelGGL(kernel, dim3((unsigned)N), dim3(threads), 0, st, x, ld, tokens, logp, entropy,
-                                    stat, top_ids, top_logp, V, top, ignore_index));
+                 hipLaunchKernelGGL(kernel, dim3((unsigned)N, parts), dim3(threads), 0, st, x, ld, tokens, o, V, top,
+                                    ignore_index, parts, width, sums, keys));
+    return hipGetLastError();
   };
-  if (bf16)
-    run(logprobs_fwd_kernel<bf16_t, 512>, (const bf16_t*)logits, 512);
-  else
-    run(logprobs_fwd_kernel<float, 512>, (const float*)logits, 512);
-  return hipGetLastError();
+  auto pick = [&](auto* x, auto want) {
+    typedef std::remove_const_t<std::remove_pointer_t<decltype(x)>> T;
+    constexpr bool TOP = decltype(want)::value;
+    const long chunks = (long)width * sizeof(T) / 16;
+    if (chunks <= 256 * 4) return run(logprobs_fwd_kernel<T, 256, 4, true, TOP>, x, 256);
+    if (N > 512) return run(logprobs_fwd_kernel<T, 256, 4, false, TOP>, x, 256);
+    if (chunks <= 1024 * 4) return run(logprobs_fwd_kernel<T, 1024, 4, true, TOP>, x, 1024);
+    return run(logprobs_fwd_kernel<T, 1024, 4, false, TOP>, x, 1024);
+  };
+  auto all = [&](auto* x) {
+    typedef std::remove_const_t<std::remove_pointer_t<decltype(x)>> T;
+    const hipError_t e = top > 0 ? pick(x, std::true_type{}) : pick(x, std::false_type{});
+    if (e != hipSuccess || parts == 1) return e;
+    NAYLIS_TIMED("logprobs_join", st,
+                 hipLaunchKernelGGL(logprobs_join_kernel<T>, dim3((unsigned)N), dim3(256), 0, st, x, ld, tokens, o, V,
+                                    top, ignore_index, parts, (const float*)sums, (const unsigned long long*)keys));
+    return hipGetLastError();
+  };
+  return bf16 ? all((const bf16_t*)logits) : all((const float*)logits);
 }
 
 hipError_t launch_logprobs_bwd(const void* logits, bool bf16, long ld, const int64_t* tokens, const float* stat,

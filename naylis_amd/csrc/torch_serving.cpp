@@ -251,10 +251,12 @@ variable_list logprobs_forward(const at::Tensor& x, const at::Tensor& tokens, in
   at::Tensor logp = at::empty({N}, f32_like(x)), entropy = at::empty({N}, f32_like(x));
   at::Tensor ids = at::empty({N, top}, x.options().dtype(at::kLong)), lps = at::empty({N, top}, f32_like(x));
   if (stat) *stat = at::empty({N, 3}, f32_like(x));
+  const size_t bytes = naylis_mom_logprobs_workspace_bytes(N, V, top);
+  const at::Tensor ws = bytes ? workspace(bytes, x) : at::Tensor();
   check(naylis_mom_logprobs_fwd(x.data_ptr(), dtype_code(x), x.stride(0), tokens.data_ptr<int64_t>(),
                                 logp.data_ptr<float>(), entropy.data_ptr<float>(),
                                 stat ? stat->data_ptr<float>() : nullptr, ids.data_ptr<int64_t>(),
-                                lps.data_ptr<float>(), N, V, top, ignore_index, st));
+                                lps.data_ptr<float>(), ptr(ws), bytes, N, V, top, ignore_index, st));
   return {logp, entropy, ids, lps};
 }
 

@@ -93,17 +93,24 @@ def test_paged_attention_workspace(lib):
     assert _attn(lib, B=0) == _lib.NAYLIS_OK
 
 
-def _logprobs(lib, dtype=1, ld=100, N=3, V=100, top=0, x=P, tok=P, ids=P):
-    return lib.naylis_mom_logprobs_fwd(x, dtype, ld, tok, P, P, P, ids, ids, N, V, top, -100, None)
+def _logprobs(lib, dtype=1, ld=100, N=3, V=100, top=0, x=P, tok=P, ids=P, ws=P, ws_bytes=1 << 40):
+    return lib.naylis_mom_logprobs_fwd(x, dtype, ld, tok, P, P, P, ids, ids, ws, ws_bytes, N, V, top, -100, None)
 
 
 @pytest.mark.parametrize("bad,text", [
     (dict(dtype=2), "dtype"), (dict(N=-1), "bad shape"), (dict(V=0), "bad shape"), (dict(ld=-1), "row stride"),
     (dict(top=-1), "top"), (dict(top=65), "top"), (dict(V=10, top=11), "top"), (dict(x=None), "null"),
     (dict(tok=None), "null"), (dict(top=1, ids=None), "null"), (dict(x=ctypes.c_void_p(4097)), "aligned"),
-    (dict(dtype=0, x=ODD), "aligned")])
+    (dict(dtype=0, x=ODD), "aligned"), (dict(V=70000, ld=70000, ws=None), "workspace"), (dict(V=70000, ws=ODD), "workspace")])
 def test_logprobs_refusals(lib, bad, text):
     _refused(lib, _logprobs(lib, **bad), text)
+
+
+def test_logprobs_workspace(lib):
+    need = lib.naylis_mom_logprobs_workspace_bytes(3, 70000, 20)
+    assert need > 0 and lib.naylis_mom_logprobs_workspace_bytes(3, 1000, 20) == 0
+    assert lib.naylis_mom_logprobs_workspace_bytes(4096, 70000, 20) == 0
+    assert _logprobs(lib, V=70000, top=20, ws_bytes=need - 1) == _lib.NAYLIS_ERR_WORKSPACE
 
 
 def test_logprobs_backward_refusals(lib):
