@@ -1233,7 +1233,7 @@ size_t naylis_mom_paged_attn_workspace_bytes(int cache_dtype, int64_t B, int64_t
                                              int64_t head_dim, int64_t W) {
   if (check_paged_attn(cache_dtype, B, H, 1, Hkv, page_size, head_dim, W, "mom_paged_attn")) return 0;
   const PagedCacheDims c = paged_dims(H, 1, Hkv, page_size, B, W);
-  return paged_ws_bytes(c, (int)head_dim, cache_dtype == NAYLIS_DTYPE_E4M3);
+  return paged_ws_bytes(c, (int)head_dim);
 }
 
 int naylis_mom_paged_attn(const void* q, const void* k_pages, const void* v_pages, const float* k_scale,
@@ -1252,7 +1252,7 @@ int naylis_mom_paged_attn(const void* q, const void* k_pages, const void* v_page
   if ((rc = check_cache(c, cache_dtype, who))) return rc;
   if (!table || !lens || !q_strides) return fail(NAYLIS_ERR_ARG, "%s: null pointer argument", who);
   if ((rc = check_pointers({q, out, workspace}, who)) || (rc = check_strides(q_strides, "q", who))) return rc;
-  const size_t need = paged_ws_bytes(c, (int)head_dim, cache_dtype == NAYLIS_DTYPE_E4M3);
+  const size_t need = paged_ws_bytes(c, (int)head_dim);
   if (workspace_bytes < need)
     return fail(NAYLIS_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", who, workspace_bytes, need);
   return hip_status(launch_paged_attn(c, (int)head_dim, cache_dtype == NAYLIS_DTYPE_E4M3, q, q_strides[0],

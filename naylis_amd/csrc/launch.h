@@ -155,9 +155,10 @@ struct PagedNew {
   long T, ldk, hsk, ldv, hsv;  // new tokens, token and head strides of their k and v
 };
 struct PagedSplit {
-  int waves, rows, head_tiles;  // waves of a slice, its live query heads, slices of a key head
+  int wgs, rows, head_tiles;  // workgroups of a slice, its most query heads, slices of a key head
+  bool whole;                 // a workgroup takes a sequence
 };
-size_t paged_ws_bytes(const PagedCacheDims& c, int hd, bool fp8);
+size_t paged_ws_bytes(const PagedCacheDims& c, int hd);
 hipError_t launch_paged_append(const PagedCacheDims& c, int hd, bool fp8, const void* k, const void* v,
                                const int32_t* table, const int32_t* positions, const int32_t* rows,
                                const PagedNew& src, hipStream_t st);

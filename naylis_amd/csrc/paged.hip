@@ -7,32 +7,42 @@
 //
 // Attention: o[b, h] = softmax_n(scale q[b, h] . k[n]) v[n] over the sequence's
 // tokens n < lens[b].  Bound by memory: every live K and V byte is read once
-// (from L2 again when more than 16 query heads share a key head).
+// (again for each further 16 query heads of a key head), past the caches.
 //
-// Work is dealt in steps of 32 (bf16) or 64 (e4m3) tokens: each key head's
-// steps of all sequences form one list, cut into equal ranges for its waves,
-// so a long sequence among short ones keeps no wave waiting.  A wave that holds
-// a whole sequence writes its result; the others leave (max, sum, o) partials
-// that a second kernel joins.  Lengths stay on the device: each wave finds its
-// range's first sequence by a scan over them.
+// Work is dealt in steps of 32 tokens: each slice's (key head's) steps of all
+// sequences form one list, cut into equal ranges for its workgroups and those
+// into quarters for their waves, so a long sequence among short ones keeps no
+// wave waiting.  The waves of a workgroup join what they hold of one sequence
+// in LDS; what several workgroups hold of it goes to a second kernel as (max,
+// sum, o) partials.  Lengths stay on the device: each wave finds its range's
+// first sequence by a scan over them.
 //
 // Per step a wave forms S^T = K Q^T (v_mfma_f32_16x16x32_bf16: 16 tokens x up
 // to 16 query heads of the key head, zeros for missing ones) with K straight
 // from memory, and O^T += V^T P^T with V through the wave's own piece of LDS,
-// which transposes it; P leaves the accumulators as the B operand.  The next
-// step's K and V are in flight meanwhile, and no barrier is needed.
+// which transposes it; P leaves the accumulators as the B operand, rounded to
+// bf16 (with e4m3 pages, times V's scale).  The next step's K is loaded as soon
+// as the products have read this one's, V as soon as LDS has, and no barrier is
+// needed.  Loads bypass the caches: 64 sequences of up to 4096 tokens, 8 key
+// heads of 128, 588 MB: 113 -> 103 us (5.7 TB/s; the kernel 97 us, the join and
+// its launch 6).  Three contexts of 65537 .. 131072 tokens, e4m3, 747 MB: 151 ->
+// 124 us (6.0 TB/s); in steps of 64 tokens 134 us (256 registers).  One sequence of
+// 500 tokens, 16 heads of 64: 7.9 us, of which 5 are launch and dependent loads.
 #include "common.h"
 #include "launch.h"
 #include "packed_tiles.h"
 #include "timing.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace naylis {
 
 namespace {
 
-constexpr int kRowsMfma = 16;  // query heads of a product
+constexpr int kRowsMfma = 16;       // query heads of a product
+constexpr int kPagedStep = 32;         // tokens of a step
+constexpr int kPagedMaxWgs = 512;   // workgroups that share a slice's steps
 
 __device__ __forceinline__ f32x4 mfma16(const bf16x8& a, const bf16x8& b, const f32x4& c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
@@ -120,13 +130,12 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedCacheDims c, con
 namespace {
 
 // Steps of the sequences before b, of all of them, and the steps of a wave's range.
-template <int TOK>
 struct StepList {
   const int32_t* lens;
   int B, cap;  // sequences, tokens that a table row holds
 
   __device__ __forceinline__ int len(int b) const { return b < B ? min(max(lens[b], 0), cap) : 0; }
-  __device__ __forceinline__ int steps(int b) const { return (len(b) + TOK - 1) / TOK; }
+  __device__ __forceinline__ int steps(int b) const { return (len(b) + kPagedStep - 1) / kPagedStep; }
 
   // sum of steps over sequences [0, b)
   __device__ __forceinline__ int before(int b) const {
@@ -162,22 +171,50 @@ struct StepList {
   }
 };
 
-}  // namespace
+// What the waves of a workgroup hand each other: up to two partials each (the
+// first and the last sequence of a wave's range), in order.
+struct PartSeq {
+  int b, first, steps;  // sequence (-1: none), its first step in the list, its steps
+};
 
-// partials of (key head slice, wave, 0: the range's first sequence / 1: its last)
+// LDS of a wave: its V tile (32 tokens), where its last partial goes too (16
+// rows of fp32, once the tile is no longer needed), then its first partial.
+template <int HD, int ROWS>
+constexpr int kWaveLds = 32 * 2 * HD + ROWS * HD * 4;
 template <int HD>
-__device__ __forceinline__ long part_row(const PagedSplit& p, int slice, int w, int slot) {
-  return (((long)slice * p.waves + w) * 2 + slot) * p.rows;
+__device__ __forceinline__ int part_offset(int slot) {
+  static_assert(kRowsMfma * 4 == 32 * 2, "a partial fits the V tile");
+  return slot == 0 ? 32 * 2 * HD : 0;
 }
 
-// grid (waves / 4, slices): slice = (key head, 16 of its query heads)
-template <int HD, bool FP8>
+template <int HD>
+__device__ __forceinline__ int v_slot(int row, int chunk) {  // byte of a 16-byte chunk in the V tile
+  const int f = HD == 128 ? 2 * (row & 7) : 2 * ((row >> 1) & 3);
+  return row * 2 * HD + ((chunk ^ f) << 4);
+}
+
+__device__ __forceinline__ uint4 load_once16(const uint8_t* p) {
+  return __builtin_bit_cast(uint4, __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(p)));
+}
+
+}  // namespace
+
+// partials of (slice, workgroup, 0: the first sequence of its range / 1: the last)
+__device__ __forceinline__ long part_row(const PagedSplit& p, int slice, int wg, int slot) {
+  return (((long)slice * p.wgs + wg) * 2 + slot) * p.rows;
+}
+
+// grid (workgroups of a slice, slices): slice = (key head, 16 of its query heads).
+// A workgroup takes a range of the step list, or (p.whole) the sequence of its
+// number, its four waves a quarter each.
+// ROWS: partials' rows, at least the query heads of a slice.
+template <int HD, bool FP8, int ROWS>
 __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedCacheDims c, const bf16_t* __restrict__ q, long ldq,
                                                             long hsq, const int32_t* __restrict__ table,
                                                             const int32_t* __restrict__ lens,
                                                             bf16_t* __restrict__ out, float* __restrict__ part,
                                                             float2* __restrict__ stat, PagedSplit p, float sc) {
-  constexpr int TOK = FP8 ? 64 : 32;     // tokens of a step
+  constexpr int TOK = kPagedStep;        // tokens of a step
   constexpr int NS = TOK / 16;           // its 16-token products
   constexpr int KS = HD / 32;            // products along the features
   constexpr int NT = HD / 16;            // 16-feature tiles of the output
@@ -185,29 +222,40 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedCacheDims c, co
   constexpr int KL = RB / 64;            // 16-byte loads of a lane for 16 tokens of K
   constexpr int VR = 1024 / RB;          // rows of V that a load of 64 lanes covers
   constexpr int VL = TOK / VR;           // such loads
-  __shared__ __align__(16) uint8_t vt_all[4][TOK * 2 * HD];
+  __shared__ __align__(16) uint8_t lds[4 * kWaveLds<HD, ROWS>];
+  __shared__ PartSeq seqs[8];
+  __shared__ float2 stats[8][ROWS];
   const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  uint8_t* vt = vt_all[wave];
-  const int w = blockIdx.x * 4 + wave, slice = blockIdx.y;
+  uint8_t* vt = lds + wave * kWaveLds<HD, ROWS>;
+  const int wg = blockIdx.x, slice = blockIdx.y;
   const int kvh = slice / p.head_tiles, h0 = kRowsMfma * (slice % p.head_tiles);
   const int nh = min(kRowsMfma, c.G - h0);  // live query heads of the slice
-  const StepList<TOK> list{lens, c.B, c.W * c.page};
+  const int H = c.Hkv * c.G, hbase = kvh * c.G + h0;
+  const StepList list{lens, c.B, c.W * c.page};
 
-  const int total = list.before(c.B);
-  const int range = max((total + p.waves - 1) / p.waves, 1);
-  int at = w * range;
-  const int end = min(at + range, total);
-  if (at >= end) return;
-  int b, first;
-  list.find(at, b, first);
+  int wg0, wg1, at, end, b = wg, first = 0;
+  if (p.whole) {
+    wg0 = 0;
+    wg1 = list.steps(wg);
+  } else {
+    const int total = list.before(c.B), range = max((total + p.wgs - 1) / p.wgs, 1);
+    wg0 = min(wg * range, total);
+    wg1 = min(wg0 + range, total);
+  }
+  {
+    const int quarter = (wg1 - wg0 + 3) / 4;
+    at = min(wg0 + wave * quarter, wg1);
+    end = min(at + quarter, wg1);
+  }
+  if (!p.whole && at < end) list.find(at, b, first);
+  if (lane < 2) seqs[2 * wave + lane].b = -1;
 
-  const long page_bytes = (long)c.Hkv * c.page * RB;
-  const long head_off = (long)kvh * c.page * RB;
   const int shift = 31 - __clz(c.page);
-  const int voff = lane * 16;                     // V: row lane / (RB / 16), piece lane % (RB / 16)
-  const int koff = r16 * RB + g * 16;             // K: row r16, pieces g, g + 4, ..
+  const int voff = lane * 16;          // V: row lane / (RB / 16), piece lane % (RB / 16)
+  const int koff = r16 * RB + g * 16;  // K: row r16, pieces g, g + 4, ..
   const int vrow = lane / (RB / 16), vpc = lane % (RB / 16);
+  const int begin = at;
 
   while (at < end && b < c.B) {
     const int n = list.len(b), nsteps = (n + TOK - 1) / TOK;
@@ -216,7 +264,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedCacheDims c, co
 
     bf16x8 qf[KS];
     {
-      const bf16_t* qp = q + (long)b * ldq + (long)(kvh * c.G + h0 + min(r16, nh - 1)) * hsq;
+      const bf16_t* qp = q + (long)b * ldq + (long)(hbase + min(r16, nh - 1)) * hsq;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
         // feature order of the products: as the lane's 16-byte pieces of K hold them
@@ -233,8 +281,9 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedCacheDims c, co
     // pages of the next 64 products' tokens, one a lane
     int ids = 0, ids_at = -64;
     uint4 kx[NS][KL], vx[VL];
-    float ksc[NS], vsc[NS];  // scales of token 16 i + r16
-    auto load = [&](int step) {
+    f32x4 ksc[NS], vsc[NS];  // scales of tokens 16 i + 4 g ..
+    long row16[NS];          // cache row of each 16-token group of the step being loaded
+    auto find_pages = [&](int step) {
 #pragma unroll
       for (int i = 0; i < NS; ++i) {
         const int t16 = step * NS + i;  // 16-token group of the sequence
@@ -248,25 +297,33 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedCacheDims c, co
           bad = true;
           id = 0;
         }
-        const int off = (t16 << 4) & (c.page - 1);
-        const uint8_t* kp = (const uint8_t*)c.k + id * page_bytes + head_off + (long)off * RB;
-        const uint8_t* vp = (const uint8_t*)c.v + id * page_bytes + head_off + (long)off * RB;
+        row16[i] = ((long)id * c.Hkv + kvh) * c.page + ((t16 << 4) & (c.page - 1));
+      }
+    };
+    auto load_k = [&]() {
 #pragma unroll
-        for (int j = 0; j < KL; ++j) kx[i][j] = *reinterpret_cast<const uint4*>(kp + koff + 64 * j);
+      for (int i = 0; i < NS; ++i) {
 #pragma unroll
-        for (int j = 0; j < VL / NS; ++j)
-          vx[i * (VL / NS) + j] = *reinterpret_cast<const uint4*>(vp + voff + 1024 * j);
+        for (int j = 0; j < KL; ++j) kx[i][j] = load_once16((const uint8_t*)c.k + row16[i] * RB + koff + 64 * j);
         if constexpr (FP8) {
-          const long srow = ((long)id * c.Hkv + kvh) * c.page + off + r16;
-          ksc[i] = c.k_scale[srow];
-          vsc[i] = c.v_scale[srow];
+          ksc[i] = *reinterpret_cast<const f32x4*>(c.k_scale + row16[i] + 4 * g);
+          vsc[i] = *reinterpret_cast<const f32x4*>(c.v_scale + row16[i] + 4 * g);
         }
       }
     };
-    load(s0);
+    auto load_v = [&]() {
+#pragma unroll
+      for (int i = 0; i < NS; ++i)
+#pragma unroll
+        for (int j = 0; j < VL / NS; ++j)
+          vx[i * (VL / NS) + j] = load_once16((const uint8_t*)c.v + row16[i] * RB + voff + 1024 * j);
+    };
+    find_pages(s0);
+    load_k();
+    load_v();
     for (int s = s0; s < s1; ++s) {
       const int tok0 = s * TOK;
-      // K fragments, then S^T: lane = query head r16, registers = tokens 16 i + 4 g + v
+      // S^T: lane = query head r16, registers = tokens 16 i + 4 g + v
       f32x4 x[NS];
 #pragma unroll
       for (int i = 0; i < NS; ++i) {
@@ -285,40 +342,43 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedCacheDims c, co
       }
       const bool tail = tok0 + TOK > n;
       // V rows to LDS as bf16; rows past the sequence as zeros, whatever the page holds there
+      auto store_v = [&]() {
 #pragma unroll
-      for (int j = 0; j < VL; ++j) {
-        const int row = j * VR + vrow;
-        uint4 u = vx[j];
-        if (tail && tok0 + row >= n) u = make_uint4(0, 0, 0, 0);
-        if constexpr (FP8) {
-          const int ch = 2 * vpc;
-          const int fx = HD == 128 ? 2 * (row & 7) : 2 * ((row >> 1) & 3);
-          *reinterpret_cast<bf16x8*>(vt + row * 2 * HD + ((ch ^ fx) << 4)) = widen8(u.x, u.y);
-          *reinterpret_cast<bf16x8*>(vt + row * 2 * HD + (((ch + 1) ^ fx) << 4)) = widen8(u.z, u.w);
-        } else {
-          const int fx = HD == 128 ? 2 * (row & 7) : 2 * ((row >> 1) & 3);
-          *reinterpret_cast<uint4*>(vt + row * 2 * HD + ((vpc ^ fx) << 4)) = u;
+        for (int j = 0; j < VL; ++j) {
+          const int row = j * VR + vrow;
+          uint4 u = vx[j];
+          if (tail && tok0 + row >= n) u = make_uint4(0, 0, 0, 0);
+          if constexpr (FP8) {
+            *reinterpret_cast<bf16x8*>(vt + v_slot<HD>(row, 2 * vpc)) = widen8(u.x, u.y);
+            *reinterpret_cast<bf16x8*>(vt + v_slot<HD>(row, 2 * vpc + 1)) = widen8(u.z, u.w);
+          } else {
+            *reinterpret_cast<uint4*>(vt + v_slot<HD>(row, vpc)) = u;
+          }
         }
-      }
-      float kss[NS][4], vss[NS][4];
+        lds_order();
+      };
+      f32x4 kss[NS], vss[NS];
       if constexpr (FP8) {
 #pragma unroll
-        for (int i = 0; i < NS; ++i)
-#pragma unroll
-          for (int v = 0; v < 4; ++v) {
-            kss[i][v] = __shfl(ksc[i], 4 * g + v, 64);
-            vss[i][v] = __shfl(vsc[i], 4 * g + v, 64);
-          }
+        for (int i = 0; i < NS; ++i) {
+          kss[i] = ksc[i] * sc;
+          vss[i] = vsc[i];
+        }
       }
-      lds_order();
-      if (s + 1 < s1) load(s + 1);
+      // registers go to the next step's loads as soon as they are read
+      const bool more = s + 1 < s1;
+      if (more) {
+        find_pages(s + 1);
+        load_k();
+      }
+      store_v();
+      if (more) load_v();
       float mx = -INFINITY;
 #pragma unroll
       for (int i = 0; i < NS; ++i)
 #pragma unroll
         for (int v = 0; v < 4; ++v) {
-          if constexpr (FP8) x[i][v] *= kss[i][v];
-          x[i][v] *= sc;
+          x[i][v] *= FP8 ? kss[i][v] : sc;
           if (tail && tok0 + 16 * i + 4 * g + v >= n) {
             x[i][v] = -INFINITY;
             if constexpr (FP8) vss[i][v] = 0.f;
@@ -340,127 +400,187 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedCacheDims c, co
           l += x[i][v];
           if constexpr (FP8) x[i][v] *= vss[i][v];
         }
-      // O^T += V^T P^T over 32 tokens: registers of two products are the B operand
+      // O^T += V^T P^T: registers of the two products are the B operand
+      bf16x8 pf;
 #pragma unroll
-      for (int i = 0; i < NS; i += 2) {
-        bf16x8 pf;
+      for (int e = 0; e < 4; ++e) {
+        pf[e] = (__bf16)x[0][e];
+        pf[4 + e] = (__bf16)x[1][e];
+      }
+      const int rlo = 4 * g + (r16 >> 2), rhi = rlo + 16;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          pf[e] = (__bf16)x[i][e];
-          pf[4 + e] = (__bf16)x[i + 1][e];
-        }
-        const int rlo = 16 * i + 4 * g + (r16 >> 2), rhi = rlo + 16;
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          const int ch = 2 * t + ((r16 & 3) >> 1), b8 = 8 * (r16 & 1);
-          const int flo = HD == 128 ? 2 * (rlo & 7) : 2 * ((rlo >> 1) & 3);
-          const int fhi = HD == 128 ? 2 * (rhi & 7) : 2 * ((rhi >> 1) & 3);
-          const v4i16 lo = lds_read_tr16(reinterpret_cast<const bf16_t*>(vt + rlo * 2 * HD + ((ch ^ flo) << 4) + b8));
-          const v4i16 hi = lds_read_tr16(reinterpret_cast<const bf16_t*>(vt + rhi * 2 * HD + ((ch ^ fhi) << 4) + b8));
-          typedef short v8i16 __attribute__((ext_vector_type(8)));
-          const v8i16 vf = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-          acc[t] = mfma16(__builtin_bit_cast(bf16x8, vf), pf, acc[t]);
-        }
+      for (int t = 0; t < NT; ++t) {
+        const int ch = 2 * t + ((r16 & 3) >> 1), b8 = 8 * (r16 & 1);
+        const v4i16 lo = lds_read_tr16(reinterpret_cast<const bf16_t*>(vt + v_slot<HD>(rlo, ch) + b8));
+        const v4i16 hi = lds_read_tr16(reinterpret_cast<const bf16_t*>(vt + v_slot<HD>(rhi, ch) + b8));
+        typedef short v8i16 __attribute__((ext_vector_type(8)));
+        const v8i16 vf = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        acc[t] = mfma16(__builtin_bit_cast(bf16x8, vf), pf, acc[t]);
       }
       lds_order();
     }
     const auto add = [](float a, float b2) { return a + b2; };
     l = xor32_f32(xor16_f32(l, add), add);
     if (bad) l = __builtin_nanf("");  // a page that is none: the sequence's result is NaN
-    if (r16 < nh) {
-      const int h = kvh * c.G + h0 + r16;
-      if (s0 == 0 && s1 == nsteps) {
+    if (s0 == 0 && s1 == nsteps) {
+      if (r16 < nh) {
         const float inv = 1.f / l;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
           bf16x4 o;
 #pragma unroll
           for (int v = 0; v < 4; ++v) o[v] = (__bf16)(acc[t][v] * inv);
-          *reinterpret_cast<bf16x4*>(out + ((long)b * c.Hkv * c.G + h) * HD + 16 * t + 4 * g) = o;
+          *reinterpret_cast<bf16x4*>(out + ((long)b * H + hbase + r16) * HD + 16 * t + 4 * g) = o;
         }
-      } else {
-        const long row = part_row<HD>(p, slice, w, at == w * range ? 0 : 1) + r16;
-#pragma unroll
-        for (int t = 0; t < NT; ++t) *reinterpret_cast<f32x4*>(part + row * HD + 16 * t + 4 * g) = acc[t];
-        if (g == 0) stat[row] = make_float2(m, l);
       }
+    } else {
+      const int slot = at == begin ? 0 : 1;
+      if (r16 < nh) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+          *reinterpret_cast<f32x4*>(reinterpret_cast<float*>(vt + part_offset<HD>(slot)) + r16 * HD + 16 * t + 4 * g) =
+              acc[t];
+        if (g == 0) stats[2 * wave + slot][r16] = make_float2(m, l);
+      }
+      if (lane == 0) seqs[2 * wave + slot] = PartSeq{b, first, nsteps};
     }
     at = first + s1;
     first += nsteps;
     ++b;
     while (b < c.B && list.steps(b) == 0) ++b;  // sequences without tokens hold no step
   }
+  __syncthreads();
+
+  // the waves' partials of one sequence, joined: its result where the workgroup
+  // held all of it, else the workgroup's partial
+  for (int i = tid; i < nh * (HD / 4); i += 256) {
+    const int r = i / (HD / 4), f = 4 * (i % (HD / 4));
+    float m = kNegBig, l = 0.f;
+    f32x4 a = f32x4{};
+    for (int e = 0; e < 8; ++e) {
+      const PartSeq cur = seqs[e];
+      if (cur.b < 0) continue;
+      const float2 st = stats[e][r];
+      const float* px =
+          reinterpret_cast<const float*>(lds + (e >> 1) * kWaveLds<HD, ROWS> + part_offset<HD>(e & 1)) + r * HD + f;
+      const float mn = fmaxf(m, st.x), wa = __builtin_amdgcn_exp2f(m - mn), wb = __builtin_amdgcn_exp2f(st.x - mn);
+      a = a * wa + *reinterpret_cast<const f32x4*>(px) * wb;
+      l = l * wa + st.y * wb;
+      m = mn;
+      int nb = -1;  // the next partial's sequence
+      for (int e2 = e + 1; e2 < 8 && nb < 0; ++e2) nb = seqs[e2].b;
+      if (nb == cur.b) continue;
+      if (cur.first >= wg0 && cur.first + cur.steps <= wg1) {
+        const float inv = 1.f / l;
+        bf16x4 o;
+#pragma unroll
+        for (int v = 0; v < 4; ++v) o[v] = (__bf16)(a[v] * inv);
+        *reinterpret_cast<bf16x4*>(out + ((long)cur.b * H + hbase + r) * HD + f) = o;
+      } else {
+        const long row = part_row(p, slice, wg, cur.first <= wg0 ? 0 : 1) + r;
+        *reinterpret_cast<f32x4*>(part + row * HD + f) = a;
+        if (f == 0) stat[row] = make_float2(m, l);
+      }
+      m = kNegBig;
+      l = 0.f;
+      a = f32x4{};
+    }
+  }
+  // zeros for the sequences without tokens
+  if (p.whole ? wg1 == 0 : wg == 0) {
+    for (int z = p.whole ? wg : 0; z < (p.whole ? wg + 1 : c.B); ++z)
+      if (list.len(z) == 0)
+        for (int i = tid; i < nh * (HD / 4); i += 256)
+          *reinterpret_cast<bf16x4*>(out + ((long)z * H + hbase) * HD + 4 * i) = bf16x4{};
+  }
 }
 
-// Joins a sequence's partials, or writes zeros for a sequence without tokens;
-// nothing where one wave held it whole.  Grid (H, B), HD threads a range of waves.
-template <int HD, int TOK>
+// Joins the workgroups' partials of a sequence; nothing where one of them held
+// it whole.  Grid (H, B).
+template <int HD>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedCacheDims c, const int32_t* __restrict__ lens,
                                                          bf16_t* __restrict__ out, const float* __restrict__ part,
                                                          const float2* __restrict__ stat, PagedSplit p) {
-  constexpr int NG = 256 / HD;  // groups of threads, each over every NG-th wave's partial
-  __shared__ float red[NG][HD];
-  __shared__ float2 reds[NG];
-  const int h = blockIdx.x, b = blockIdx.y, f = threadIdx.x % HD, gi = threadIdx.x / HD;
-  const StepList<TOK> list{lens, c.B, c.W * c.page};
+  constexpr int TR = HD / 4, NG = 256 / TR;  // threads of a partial; partials read at once
+  __shared__ float weight[kPagedMaxWgs];
+  __shared__ float red[4];
+  __shared__ f32x4 sums[NG][TR];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int h = blockIdx.x, b = blockIdx.y;
+  const StepList list{lens, c.B, c.W * c.page};
   const int n = list.steps(b);
-  bf16_t* o = out + ((long)b * c.Hkv * c.G + h) * HD;
-  if (n == 0) {
-    if (gi == 0) o[f] = 0;
-    return;
-  }
-  const int total = list.before(c.B), range = max((total + p.waves - 1) / p.waves, 1);
+  if (n == 0) return;
+  const int total = list.before(c.B), range = max((total + p.wgs - 1) / p.wgs, 1);
   const int first = list.before(b), w0 = first / range, w1 = (first + n - 1) / range;
   if (w0 == w1) return;
   const int kvh = h / c.G, hr = h % c.G, slice = kvh * p.head_tiles + hr / kRowsMfma;
-  float m = kNegBig, l = 0.f, a = 0.f;
-  for (int w = w0 + gi; w <= w1; w += NG) {
-    // the wave's first sequence, unless its range begins before this one
-    const long row = part_row<HD>(p, slice, w, w * range >= first ? 0 : 1) + hr % kRowsMfma;
-    const float2 st = stat[row];
-    const float mn = fmaxf(m, st.x), x = __builtin_amdgcn_exp2f(m - mn), y = __builtin_amdgcn_exp2f(st.x - mn);
-    a = a * x + part[row * HD + f] * y;
-    l = l * x + st.y * y;
-    m = mn;
+  const int count = w1 - w0 + 1;
+  // a workgroup's first sequence, unless its range begins before this one
+  const auto row = [&](int i) {
+    const int w = w0 + i;
+    return part_row(p, slice, w, w * range >= first ? 0 : 1) + hr % kRowsMfma;
+  };
+  const auto block = [&](float x, auto op) {
+    x = wave_allreduce_f32(x, op);
+    if (lane == 0) red[wave] = x;
+    __syncthreads();
+    x = op(op(red[0], red[1]), op(red[2], red[3]));
+    __syncthreads();
+    return x;
+  };
+  float m = kNegBig, l = 0.f;
+  for (int i = tid; i < count; i += 256) {
+    weight[i] = stat[row(i)].x;
+    m = fmaxf(m, weight[i]);
   }
-  red[gi][f] = a;
-  if (f == 0) reds[gi] = make_float2(m, l);
+  m = block(m, [](float a, float b) { return fmaxf(a, b); });
+  for (int i = tid; i < count; i += 256) {
+    weight[i] = __builtin_amdgcn_exp2f(weight[i] - m);
+    l += weight[i] * stat[row(i)].y;
+  }
+  l = block(l, [](float a, float b) { return a + b; });  // (its barriers are the weights' too)
+  f32x4 a = f32x4{};
+  const int gi = tid / TR, f = tid % TR;
+#pragma unroll 4
+  for (int i = gi; i < count; i += NG)
+    a += *reinterpret_cast<const f32x4*>(part + row(i) * HD + 4 * f) * weight[i];
+  sums[gi][f] = a;
   __syncthreads();
   if (gi) return;
-  float mn = kNegBig;
 #pragma unroll
-  for (int i = 0; i < NG; ++i) mn = fmaxf(mn, reds[i].x);
-  a = l = 0.f;
+  for (int i = 1; i < NG; ++i) a += sums[i][f];
+  const float inv = 1.f / l;
+  bf16x4 o;
 #pragma unroll
-  for (int i = 0; i < NG; ++i) {
-    const float y = __builtin_amdgcn_exp2f(reds[i].x - mn);
-    a += red[i][f] * y;
-    l += reds[i].y * y;
-  }
-  o[f] = f32_to_bf16(a / l);
+  for (int v = 0; v < 4; ++v) o[v] = (__bf16)(a[v] * inv);
+  *reinterpret_cast<bf16x4*>(out + ((long)b * c.Hkv * c.G + h) * HD + 4 * f) = o;
 }
 
-// Waves for each slice: 8 a CU over all slices, a whole number of workgroups,
-// and no more than the tables' steps (rounded up).
-PagedSplit paged_split(const PagedCacheDims& c, int hd, bool fp8) {
+// A workgroup for each sequence where tables hold at most 16 steps, four for each
+// wave, and no second launch (128 sequences of up to 500 tokens, 8 key heads of
+// 128: 38 us against 50).  Else the list is cut for two workgroups a CU over all
+// slices, and no finer than a step a wave.
+// Three or four a CU take longer (three contexts of 65537 .. 131072 tokens, e4m3:
+// 124 us with 512 workgroups, 147 with 768, 130 with 1024).
+PagedSplit paged_split(const PagedCacheDims& c) {
   PagedSplit p;
   p.head_tiles = (c.G + kRowsMfma - 1) / kRowsMfma;
-  p.rows = std::min(c.G, kRowsMfma);
+  p.rows = c.G <= 4 ? 4 : kRowsMfma;
   const long slices = (long)c.Hkv * p.head_tiles;
-  const int tok = fp8 ? 64 : 32;
-  const long cap = (long)c.B * (((long)c.W * c.page + tok - 1) / tok);
-  const long waves = std::min(std::max(2048 / slices, 4L), std::max(cap, 1L));
-  p.waves = (int)((waves + 3) / 4 * 4);
+  const long cap = ((long)c.W * c.page + kPagedStep - 1) / kPagedStep;
+  p.whole = cap <= 16;
+  p.wgs = (int)(p.whole ? std::max(c.B, 1)
+                        : std::max(1L, std::min({512 / slices, (c.B * cap + 3) / 4, (long)kPagedMaxWgs})));
   return p;
 }
 
 size_t paged_part_floats(const PagedCacheDims& c, const PagedSplit& p, int hd) {
-  return (size_t)c.Hkv * p.head_tiles * p.waves * 2 * p.rows * hd;
+  return p.whole ? 0 : (size_t)c.Hkv * p.head_tiles * p.wgs * 2 * p.rows * hd;
 }
 
-size_t paged_ws_bytes(const PagedCacheDims& c, int hd, bool fp8) {
-  const PagedSplit p = paged_split(c, hd, fp8);
-  return paged_part_floats(c, p, hd) * 4 + (size_t)c.Hkv * p.head_tiles * p.waves * 2 * p.rows * 8;
+size_t paged_ws_bytes(const PagedCacheDims& c, int hd) {
+  const size_t n = paged_part_floats(c, paged_split(c), hd);
+  return std::max(n * 4 + n / hd * 8, (size_t)16);  // (0 would mean a refusal)
 }
 
 hipError_t launch_paged_append(const PagedCacheDims& c, int hd, bool fp8, const void* k, const void* v,
@@ -482,30 +602,31 @@ hipError_t launch_paged_append(const PagedCacheDims& c, int hd, bool fp8, const 
 hipError_t launch_paged_attn(const PagedCacheDims& c, int hd, bool fp8, const void* q, long ldq, long hsq,
                              const int32_t* table, const int32_t* lens, void* out, void* ws, float scale,
                              hipStream_t st) {
-  const PagedSplit p = paged_split(c, hd, fp8);
+  const PagedSplit p = paged_split(c);
   float* part = (float*)ws;
   float2* stat = (float2*)(part + paged_part_floats(c, p, hd));
   auto run = [&](auto kernel) {
     NAYLIS_TIMED("paged_attn", st,
-                 hipLaunchKernelGGL(kernel, dim3(p.waves / 4, c.Hkv * p.head_tiles), dim3(256), 0, st, c,
+                 hipLaunchKernelGGL(kernel, dim3(p.wgs, c.Hkv * p.head_tiles), dim3(256), 0, st, c,
                                     (const bf16_t*)q, ldq, hsq, table, lens, (bf16_t*)out, part, stat, p,
                                     scale * kLog2e));
   };
-  if (hd == 64)
-    fp8 ? run(paged_attn_kernel<64, true>) : run(paged_attn_kernel<64, false>);
-  else
-    fp8 ? run(paged_attn_kernel<128, true>) : run(paged_attn_kernel<128, false>);
+  auto pick = [&](auto rows) {
+    constexpr int R = decltype(rows)::value;
+    if (hd == 64)
+      fp8 ? run(paged_attn_kernel<64, true, R>) : run(paged_attn_kernel<64, false, R>);
+    else
+      fp8 ? run(paged_attn_kernel<128, true, R>) : run(paged_attn_kernel<128, false, R>);
+  };
+  p.rows == 4 ? pick(std::integral_constant<int, 4>{}) : pick(std::integral_constant<int, 16>{});
   const hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return e;
+  if (e != hipSuccess || p.whole || p.wgs == 1) return e;
   auto join = [&](auto kernel) {
     NAYLIS_TIMED("paged_join", st,
                  hipLaunchKernelGGL(kernel, dim3(c.Hkv * c.G, c.B), dim3(256), 0, st, c, lens, (bf16_t*)out,
                                     (const float*)part, (const float2*)stat, p));
   };
-  if (hd == 64)
-    fp8 ? join(paged_join_kernel<64, 64>) : join(paged_join_kernel<64, 32>);
-  else
-    fp8 ? join(paged_join_kernel<128, 64>) : join(paged_join_kernel<128, 32>);
+  hd == 64 ? join(paged_join_kernel<64>) : join(paged_join_kernel<128>);
   return hipGetLastError();
 }
 
