@@ -493,7 +493,7 @@ int naylis_mom_decode_step(const double* state_in, double* state_out, const int3
  *   for the backward, dout: 8 values there, 6 in the forward
  *   lse (H, T) fp32, log2 domain, +inf for a query that sees no key; NULL in
  *   the forward where no backward follows
- *   delta (H, T) fp32: scratch of the backward
+ *   stats (2, H, T) fp32: scratch of the backward
  * The backward writes dense dq, dk, dv; the gradients of a key head are summed
  * over its query heads in one fixed order in fp32.  No workspace.
  * Constraints: head_dim 64 or 128, H a multiple of Hkv, scale > 0, pointers
@@ -503,7 +503,7 @@ int naylis_mom_packed_attn_fwd(const void* q, const void* k, const void* v, cons
                                int64_t Tk, int64_t H, int64_t Hkv, int64_t head_dim, void* stream);
 int naylis_mom_packed_attn_bwd(const void* q, const void* k, const void* v, const int32_t* cu_q, const int32_t* cu_k,
                                const void* out, const float* lse, const void* dout, void* dq, void* dk, void* dv,
-                               float* delta, const int64_t* strides, float scale, int64_t n_seqs, int64_t T,
+                               float* stats, const int64_t* strides, float scale, int64_t n_seqs, int64_t T,
                                int64_t Tk, int64_t H, int64_t Hkv, int64_t head_dim, void* stream);
 
 /* --------------------------------------------------------- paged cache ---

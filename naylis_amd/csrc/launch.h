@@ -124,7 +124,7 @@ hipError_t launch_attn_bwd(const void* q, const void* k, const void* v, const vo
 // Causal attention over packed sequences (packed.hip): q, o (T, H, hd) and k, v
 // (Tk, Hkv, hd) bf16, hd 64 or 128; sequence i holds query rows cu_q[i] ..
 // cu_q[i + 1] - 1 and key rows cu_k[i] .. (device arrays of n + 1 offsets).
-// lse (log2 domain, may be null in the forward) and delta (H, T) fp32.
+// lse (H, T; log2 domain, may be null in the forward) and stats (2, H, T) fp32.
 struct PackedSeqs {
   const int32_t* cu_q;
   const int32_t* cu_k;
@@ -138,7 +138,7 @@ bool packed_supported(long n, long T, long Tk, long H, long Hkv);
 hipError_t launch_packed_fwd(const void* q, const void* k, const void* v, void* o, float* lse, const PackedSeqs& s,
                              const PackedHeads& d, int hd, float scale, hipStream_t st);
 hipError_t launch_packed_bwd(const void* q, const void* k, const void* v, const void* o, const float* lse,
-                             const void* dout, void* dq, void* dk, void* dv, float* delta, const PackedSeqs& s,
+                             const void* dout, void* dq, void* dk, void* dv, float* stats, const PackedSeqs& s,
                              const PackedHeads& d, int hd, float scale, hipStream_t st);
 
 // Paged key / value cache (paged.hip): pages (P, Hkv, page, hd) bf16 or e4m3

@@ -20,6 +20,8 @@
 #include "packed_tiles.h"
 #include "timing.h"
 
+#include <type_traits>
+
 namespace naylis {
 
 namespace {
@@ -48,6 +50,11 @@ struct RowFrag {
   __device__ __forceinline__ bf16x8 get(const uint8_t* tile, int row0, int ks) const {
     return *reinterpret_cast<const bf16x8*>(tile + row0 * 2 * HD + off[ks]);
   }
+  // to a buffer that lies `bit` bytes (a power of two past the tile) off
+  __device__ __forceinline__ void move(int bit) {
+#pragma unroll
+    for (int ks = 0; ks < HD / 16; ++ks) off[ks] ^= bit;
+  }
 };
 
 // A fragment of X^T, features 32 t .. 32 t + 31, over rows k0 .. k0 + 15 (k0
@@ -71,6 +78,54 @@ struct TransFrag {
     const v8i16 v = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
     return __builtin_bit_cast(bf16x8, v);
   }
+  __device__ __forceinline__ void move(int bit) {
+#pragma unroll
+    for (int t = 0; t < HD / 32; ++t) {
+      lo[t] ^= bit;
+      hi[t] ^= bit;
+    }
+  }
+};
+
+// The same two with one offset each, the others from it by XOR where they are
+// used: an instruction for each read, and 14 registers fewer (heads of 128).
+struct LeanFrag {
+  int rows, trans;
+  __device__ __forceinline__ explicit LeanFrag(int lane) {
+    rows = RowFrag<128>(lane).off[0];
+    trans = TransFrag<128>(lane).lo[0];
+  }
+  // not computed ahead and kept
+  __device__ __forceinline__ void renew() { asm volatile("" : "+v"(rows), "+v"(trans)); }
+  __device__ __forceinline__ void move(int bit) {
+    rows ^= bit;
+    trans ^= bit;
+  }
+  __device__ __forceinline__ bf16x8 get(const uint8_t* tile, int row0, int ks) const {
+    return *reinterpret_cast<const bf16x8*>(tile + row0 * 256 + (rows ^ (ks << 5)));
+  }
+  __device__ __forceinline__ bf16x8 get_t(const uint8_t* tile, int k0, int t) const {
+    const int lo = trans ^ (t << 6);  // 8 rows on, the swizzle differs in one bit
+    const v4i16 a = lds_read_tr16(reinterpret_cast<const bf16_t*>(tile + k0 * 256 + lo));
+    const v4i16 b = lds_read_tr16(reinterpret_cast<const bf16_t*>(tile + k0 * 256 + (lo ^ 0x820)));
+    typedef short v8i16 __attribute__((ext_vector_type(8)));
+    const v8i16 v = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+    return __builtin_bit_cast(bf16x8, v);
+  }
+};
+struct FullFrag : RowFrag<64>, TransFrag<64> {
+  __device__ __forceinline__ explicit FullFrag(int lane) : RowFrag<64>(lane), TransFrag<64>(lane) {}
+  __device__ __forceinline__ void renew() {}
+  __device__ __forceinline__ void move(int bit) {
+    RowFrag<64>::move(bit);
+    TransFrag<64>::move(bit);
+  }
+  __device__ __forceinline__ bf16x8 get(const uint8_t* tile, int row0, int ks) const {
+    return RowFrag<64>::get(tile, row0, ks);
+  }
+  __device__ __forceinline__ bf16x8 get_t(const uint8_t* tile, int k0, int t) const {
+    return TransFrag<64>::get(tile, k0, t);
+  }
 };
 
 // Rows [row, row + rows) of one head, up to the sequence's end: a resource
@@ -82,29 +137,78 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const bf16_t* base, 
   return make_rsrc(base + (long)row * ld, live > 0 ? ((uint32_t)(live - 1) * (uint32_t)ld + hd) * 2 : 0);
 }
 
-// A thread's share of a 64-row stage of one operand.
+// A wave's share of the stages of one operand, 64 rows each, from memory to LDS
+// directly: 64 lanes x 16 bytes land in lane order, so the swizzle is on the
+// source side.  Rows past the sequence are zeros; a stage past it loads nothing
+// but counts as loads in flight.  The load is written in assembly because the
+// compiler would wait for every such load before the next transposing LDS read;
+// it has no register output, and the waits in wait_loads are those that its
+// readers need.
+typedef int i32x4 __attribute__((ext_vector_type(4)));
 template <int HD>
-struct StageCopy {
-  static constexpr int N = kStageRows * HD / 8 / 256;  // 16-byte chunks
-  int voff[N], lds[N];
-  __device__ __forceinline__ StageCopy(int tid, int ld) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int r = (i * 256 + tid) / (HD / 8), c = tid % (HD / 8);
-      voff[i] = (r * ld + c * 8) * 2;
-      lds[i] = r * 2 * HD + ((c ^ swz<HD>(r)) << 4);
-    }
+struct StageLoad {
+  static constexpr int N = kStageRows * 2 * HD / 1024 / 4;  // loads of a wave
+  const bf16_t* base;
+  long ld;
+  int len, wave, voff;  // (pieces lie 16 or 32 rows apart, where the swizzle is the same)
+  __device__ __forceinline__ StageLoad(const bf16_t* p, long ld_, int len_, int wave_, int lane)
+      : base(p), ld(ld_), len(len_), wave(wave_) {
+    const int at = wave * 1024 + lane * 16, r = at / (2 * HD), ch = at % (2 * HD) / 16;
+    voff = (r * (int)ld + (ch ^ swz<HD>(r)) * 8) * 2;
   }
-  __device__ __forceinline__ void load(uint4 (&x)[N], __amdgpu_buffer_rsrc_t rs) const {
+  __device__ __forceinline__ void load(uint32_t lds, int stage) const {
+    const int row = stage * kStageRows, live = min(len - row, kStageRows);
+    const uint64_t a = (uint64_t)(base + (long)row * ld);
+    const uint32_t bytes = live > 0 ? ((uint32_t)(live - 1) * (uint32_t)ld + HD) * 2 : 0;
+    const i32x4 rs{(int)(uint32_t)a, (int)((a >> 32) & 0xffff), (int)bytes, 0x00020000};
 #pragma unroll
     for (int i = 0; i < N; ++i)
-      x[i] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rs, voff[i], 0, 0));
-  }
-  __device__ __forceinline__ void store(const uint4 (&x)[N], uint8_t* tile) const {
-#pragma unroll
-    for (int i = 0; i < N; ++i) *reinterpret_cast<uint4*>(tile + lds[i]) = x[i];
+      asm volatile(
+          "s_mov_b32 m0, %0\n\t"
+          "s_nop 0\n\t"
+          "buffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds + (i * 4 + wave) * 1024),
+          "v"(voff), "s"(rs), "s"(i * (4096 / HD) * (int)ld)
+          : "memory", "m0");
   }
 };
+
+// 64 floats p[first ..] of len (zeros past it) to LDS, 4 bytes a lane.
+__device__ __forceinline__ void load_floats(const float* p, int len, int first, int lane, uint32_t lds) {
+  const uint64_t a = (uint64_t)(p + first);
+  const i32x4 rs{(int)(uint32_t)a, (int)((a >> 32) & 0xffff), max(len - first, 0) * 4, 0x00020000};
+  asm volatile(
+      "s_mov_b32 m0, %0\n\t"
+      "s_nop 0\n\t"
+      "buffer_load_dword %1, %2, 0 offen lds" ::"s"(lds),
+      "v"(lane * 4), "s"(rs)
+      : "memory", "m0");
+}
+
+// All but the newest n loads of every wave are in LDS, and what the waves have
+// read from LDS so far may be overwritten.
+template <int n>
+__device__ __forceinline__ void wait_loads() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(n) : "memory");
+}
+
+// max(m, x0 .. x15) of a product's results.  In assembly because fmaxf quiets
+// NaN first, an instruction more for each; m has to come from an instruction
+// that reads one of the results and that the compiler places, because it counts
+// the wait states after a matrix instruction, and not for assembly.
+__device__ __forceinline__ float max_of(float m, const f32x16& x) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3\n\t"
+      "v_max3_f32 %0, %0, %4, %5\n\t"
+      "v_max3_f32 %0, %0, %6, %7\n\t"
+      "v_max3_f32 %0, %0, %8, %9\n\t"
+      "v_max3_f32 %0, %0, %10, %11\n\t"
+      "v_max3_f32 %0, %0, %12, %13\n\t"
+      "v_max3_f32 %0, %0, %14, %15"
+      : "=&v"(r)
+      : "v"(m), "v"(x[2]), "v"(x[3]), "v"(x[4]), "v"(x[5]), "v"(x[6]), "v"(x[7]), "v"(x[8]), "v"(x[9]), "v"(x[10]),
+        "v"(x[11]), "v"(x[12]), "v"(x[13]), "v"(x[14]), "v"(x[15]));
+  return r;
+}
 
 // B operand fragments of 32 rows straight from memory: lane l gets row l % 32
 // of the resource, features 16 ks + 8 (l / 32) + e.
@@ -148,91 +252,121 @@ struct Head {
 
 }  // namespace
 
-// Forward: 4 waves of 32 queries.
+// Forward: 4 waves of 32 queries.  The walk over 32-key tiles is pipelined by
+// one: while the vector units take the exponentials of tile t, the matrix units
+// form the scores of tile t + 1, and while those add P V of tile t, the maximum
+// of tile t + 1 is found.  K and V stages go from memory to LDS directly, K a
+// stage further ahead than V, each into the buffer that the barrier before has
+// freed: barrier 1 of a stage stands after the last use of its K, barrier 2
+// after that of its V.
 template <int HD>
-__global__ __launch_bounds__(256, HD == 64 ? 4 : 2) void packed_fwd_kernel(
+__global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void packed_fwd_kernel(
     const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, const bf16_t* __restrict__ v, bf16_t* __restrict__ o,
     float* __restrict__ lse, PackedSeqs s, PackedHeads d, float c) {
-  constexpr int NT = HD / 32;
-  __shared__ __align__(16) uint8_t kt[2][kStageRows * 2 * HD];
-  __shared__ __align__(16) uint8_t vt[2][kStageRows * 2 * HD];
+  constexpr int NT = HD / 32, NK = HD / 16, STAGE = kStageRows * 2 * HD;
+  __shared__ __align__(1024) uint8_t ring[4 * STAGE];  // K even, K odd, V even, V odd
   const PackedTile tile = find_tile<false>(s, blockIdx.x / d.H);
   if (!tile.live) return;
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5, col = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const Head hd(blockIdx.x % d.H, d);
   const bf16_t* qb = q + (long)tile.q0 * d.ldq + (long)hd.h * d.hsq;
-  const bf16_t* kb = k + (long)tile.k0 * d.ldk + (long)hd.kvh * d.hsk;
-  const bf16_t* vb = v + (long)tile.k0 * d.ldv + (long)hd.kvh * d.hsv;
   const int shift = tile.lk - tile.lq;  // query i sees keys up to i + shift
   const int q0 = tile.block * kTileRows + wave * 32, row = q0 + col;
 
-  bf16x8 qf[HD / 16];
+  bf16x8 qf[NK];
   load_rows<HD>(qf, rows_rsrc(qb, d.ldq, q0, tile.lq, 32, HD), (int)d.ldq, lane);
-  const StageCopy<HD> ck(tid, (int)d.ldk), cv(tid, (int)d.ldv);
-  const RowFrag<HD> rf(lane);
-  const TransFrag<HD> tf(lane);
-  f32x16 acc[NT];
-  clear(acc);
-  float m = kNegBig, l = 0.f;
+  const StageLoad<HD> lk(k + (long)tile.k0 * d.ldk + (long)hd.kvh * d.hsk, d.ldk, tile.lk, wave, lane);
+  const StageLoad<HD> lv(v + (long)tile.k0 * d.ldv + (long)hd.kvh * d.hsv, d.ldv, tile.lk, wave, lane);
+  RowFrag<HD> rf(lane);
+  TransFrag<HD> tf(lane);
+  tf.move(2 * STAGE);
+  const uint32_t ring0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)ring;  // LDS byte address
   const int keys = min(tile.lq, (tile.block + 1) * kTileRows) + shift;  // seen by the tile's last query
   const int nst = (max(keys, 0) + kStageRows - 1) / kStageRows;
-  uint4 xk[StageCopy<HD>::N], xv[StageCopy<HD>::N];
-  ck.load(xk, rows_rsrc(kb, d.ldk, 0, tile.lk, kStageRows, HD));
-  cv.load(xv, rows_rsrc(vb, d.ldv, 0, tile.lk, kStageRows, HD));
-  ck.store(xk, kt[0]);
-  cv.store(xv, vt[0]);
-  lds_barrier();
-  for (int st = 0; st < nst; ++st) {
-    const int nx = min(st + 1, nst - 1) * kStageRows;  // past the last stage: loaded again, not read
-    ck.load(xk, rows_rsrc(kb, d.ldk, nx, tile.lk, kStageRows, HD));
-    cv.load(xv, rows_rsrc(vb, d.ldv, nx, tile.lk, kStageRows, HD));
-    const uint8_t* ks_ = kt[st & 1];
-    const uint8_t* vs_ = vt[st & 1];
+  const int nt = min(max(q0 + 32 + shift + 31, 0) / 32, 2 * nst);  // key tiles that the wave's queries see
+
+  f32x16 acc[NT], x;  // x: scores, then weights, of the tile at hand
+  clear(acc);
+  float m = kNegBig, l = 0.f;
+  // mask of tile t, its maximum, and the sums rescaled where that is a new one
+  auto settle = [&](f32x16& z, int t) {
+    if (32 * t + 31 > q0 + shift) {
+      asm volatile("");  // a branch, not 16 selects for every tile
 #pragma unroll
-    for (int sub = 0; sub < 2; ++sub) {
-      const int kv0 = st * kStageRows + 32 * sub;
-      if (kv0 > q0 + 31 + shift) continue;  // above the diagonal (wave-uniform)
-      f32x16 x = f32x16{};
+      for (int i = 0; i < 16; ++i)
+        if (32 * t + acc_row(g, i) > row + shift) z[i] = -INFINITY;
+    }
+    const float mx = max_of(fmaxf(z[0], z[1]), z) * c;
+    if (__builtin_expect(__any(mx > m), 0)) {
+      // per query, so that a row's result does not depend on its neighbours'
+      const float mn = fmaxf(m, xor32_f32(mx, [](float a, float b) { return fmaxf(a, b); }));
+      const float al = __builtin_amdgcn_exp2f(m - mn);
+      m = mn;
+      l *= al;
 #pragma unroll
-      for (int ks = 0; ks < HD / 16; ++ks) x = mfma32(rf.get(ks_, 32 * sub, ks), qf[ks], x);
-      if (kv0 + 31 > q0 + shift) {
+      for (int u = 0; u < NT; ++u)
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (kv0 + acc_row(g, i) > row + shift) x[i] = -INFINITY;
-      }
-      float mx = x[0];
-#pragma unroll
-      for (int i = 1; i < 16; ++i) mx = fmaxf(mx, x[i]);
-      if (__any(mx * c > m)) {
-        // per query, so that a row's result does not depend on its neighbours'
-        const float mr = xor32_f32(mx, [](float a, float b) { return fmaxf(a, b); }) * c;
-        const float mn = fmaxf(m, mr);
-        const float al = __builtin_amdgcn_exp2f(m - mn);
-        m = mn;
-        l *= al;
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) acc[t][i] *= al;
-      }
-      float ls = 0.f;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        x[i] = __builtin_amdgcn_exp2f(fmaf(x[i], c, -m));
-        ls += x[i];
-      }
-      l += ls;
+        for (int i = 0; i < 16; ++i) acc[u][i] *= al;
+    }
+  };
+  auto weigh = [&](int i) {
+    x[i] = __builtin_amdgcn_exp2f(fmaf(x[i], c, -m));
+    l += x[i];
+  };
+  // Tile t (the first or second of its stage) with its scores in x; leaves
+  // those of t + 1 there.  The lanes' LDS offsets move to the other buffer a
+  // stage at a time, so that tiles differ by constants.
+  auto step = [&](auto second, int t) {
+    constexpr int HALF = 32 * 2 * HD, SECOND = decltype(second)::value;
+    const uint8_t* vb = ring + SECOND * HALF;
+    const uint8_t* kb = ring + (SECOND ? 0 : HALF);
+    auto add_pv = [&]() {
       const bf16x8 pf[2] = {pack8(x, 0), pack8(x, 8)};
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int t = 0; t < NT; ++t) acc[t] = mfma32(tf.get(vs_, 32 * sub + 16 * h, t), pf[h], acc[t]);
+        for (int u = 0; u < NT; ++u) acc[u] = mfma32(tf.get(vb, 16 * h, u), pf[h], acc[u]);
+    };
+    if (t + 1 < nt) {
+      f32x16 y = f32x16{};
+#pragma unroll
+      for (int ks = 0; ks < NK; ++ks) {
+        y = mfma32(rf.get(kb, 0, ks), qf[ks], y);
+#pragma unroll
+        for (int i = 0; i < 16 / NK; ++i) weigh(ks * (16 / NK) + i);
+      }
+      add_pv();
+      settle(y, t + 1);
+      x = y;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) weigh(i);
+      add_pv();
     }
-    ck.store(xk, kt[(st + 1) & 1]);
-    cv.store(xv, vt[(st + 1) & 1]);
-    lds_barrier();
+  };
+
+  lk.load(ring0, 0);
+  lv.load(ring0 + 2 * STAGE, 0);
+  lk.load(ring0 + STAGE, 1);
+  wait_loads<StageLoad<HD>::N>();
+  if (nt > 0) {
+    x = f32x16{};
+#pragma unroll
+    for (int ks = 0; ks < NK; ++ks) x = mfma32(rf.get(ring, 0, ks), qf[ks], x);
+    settle(x, 0);
   }
+  for (int st = 0; st < nst; ++st) {
+    lv.load(ring0 + (2 + ((st + 1) & 1)) * STAGE, st + 1);
+    if (2 * st < nt) step(std::false_type{}, 2 * st);
+    wait_loads<StageLoad<HD>::N>();  // K of stage st + 1 is in LDS, that of st no longer needed
+    lk.load(ring0 + (st & 1) * STAGE, st + 2);
+    rf.move(STAGE);
+    if (2 * st + 1 < nt) step(std::true_type{}, 2 * st + 1);
+    wait_loads<StageLoad<HD>::N>();  // V likewise
+    tf.move(STAGE);
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the late loads (zeros) land before LDS goes to another workgroup
   const float ls = xor32_f32(l, [](float a, float b) { return a + b; });
   if (row < tile.lq) {
     // a query without keys: zeros, and a log-sum-exp under which every backward weight is 0
@@ -243,16 +377,15 @@ __global__ __launch_bounds__(256, HD == 64 ? 4 : 2) void packed_fwd_kernel(
   }
 }
 
-// dQ (and delta = rowsum(dO o), which the dK/dV kernel reads): the forward's
-// walk with P from the log-sum-exp.
+// dQ: the forward's walk with P from the log-sum-exp.  Leaves (2, H, T) for the
+// dK/dV kernel: -lse / c and -delta, delta = rowsum(dO o).
 template <int HD>
 __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void packed_bwd_dq_kernel(
     const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, const bf16_t* __restrict__ v,
     const bf16_t* __restrict__ o, const float* __restrict__ lse, const bf16_t* __restrict__ dout,
-    bf16_t* __restrict__ dq, float* __restrict__ delta, PackedSeqs s, PackedHeads d, float scale) {
-  constexpr int NT = HD / 32;
-  __shared__ __align__(16) uint8_t kt[2][kStageRows * 2 * HD];
-  __shared__ __align__(16) uint8_t vt[2][kStageRows * 2 * HD];
+    bf16_t* __restrict__ dq, float* __restrict__ stats, PackedSeqs s, PackedHeads d, float scale) {
+  constexpr int NT = HD / 32, STAGE = kStageRows * 2 * HD;
+  __shared__ __align__(1024) uint8_t ring[4 * STAGE];  // K even, K odd, V even, V odd
   const PackedTile tile = find_tile<false>(s, blockIdx.x / d.H);
   if (!tile.live) return;
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5, col = lane & 31;
@@ -281,27 +414,25 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void packed_bwd_dq_kernel(
 #pragma unroll
       for (int e = 0; e < 8; ++e) md = fmaf(-(float)df[ks][e], (float)of[ks][e], md);
     md = xor32_f32(md, [](float a, float b) { return a + b; });
-    if (g == 0 && row < tile.lq) delta[stat] = -md;
+    if (g == 0 && row < tile.lq) {
+      stats[stat] = ml / c;
+      stats[(long)d.H * s.T + stat] = md;
+    }
   }
-  const StageCopy<HD> ck(tid, (int)d.ldk), cv(tid, (int)d.ldv);
-  const RowFrag<HD> rf(lane);
-  const TransFrag<HD> tf(lane);
+  const StageLoad<HD> lk(kb, d.ldk, tile.lk, wave, lane), lv(vb, d.ldv, tile.lk, wave, lane);
+  RowFrag<HD> rf(lane);
+  TransFrag<HD> tf(lane);
+  const uint32_t ring0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)ring;
   f32x16 acc[NT];
   clear(acc);
   const int keys = min(tile.lq, (tile.block + 1) * kTileRows) + shift;
   const int nst = (max(keys, 0) + kStageRows - 1) / kStageRows;
-  uint4 xk[StageCopy<HD>::N], xv[StageCopy<HD>::N];
-  ck.load(xk, rows_rsrc(kb, d.ldk, 0, tile.lk, kStageRows, HD));
-  cv.load(xv, rows_rsrc(vb, d.ldv, 0, tile.lk, kStageRows, HD));
-  ck.store(xk, kt[0]);
-  cv.store(xv, vt[0]);
-  lds_barrier();
+  lk.load(ring0, 0);
+  lv.load(ring0 + 2 * STAGE, 0);
   for (int st = 0; st < nst; ++st) {
-    const int nx = min(st + 1, nst - 1) * kStageRows;
-    ck.load(xk, rows_rsrc(kb, d.ldk, nx, tile.lk, kStageRows, HD));
-    cv.load(xv, rows_rsrc(vb, d.ldv, nx, tile.lk, kStageRows, HD));
-    const uint8_t* ks_ = kt[st & 1];
-    const uint8_t* vs_ = vt[st & 1];
+    wait_loads<0>();  // stage st is in LDS, st - 1 read by every wave
+    lk.load(ring0 + ((st + 1) & 1) * STAGE, st + 1);
+    lv.load(ring0 + (2 + ((st + 1) & 1)) * STAGE, st + 1);
 #pragma unroll
     for (int sub = 0; sub < 2; ++sub) {
       const int kv0 = st * kStageRows + 32 * sub;
@@ -311,10 +442,11 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void packed_bwd_dq_kernel(
       for (int i = 0; i < 16; ++i) dp[i] = md;
 #pragma unroll
       for (int ks = 0; ks < HD / 16; ++ks) {
-        x = mfma32(rf.get(ks_, 32 * sub, ks), qf[ks], x);
-        dp = mfma32(rf.get(vs_, 32 * sub, ks), df[ks], dp);
+        x = mfma32(rf.get(ring, 32 * sub, ks), qf[ks], x);
+        dp = mfma32(rf.get(ring + 2 * STAGE, 32 * sub, ks), df[ks], dp);
       }
       if (kv0 + 31 > q0 + shift) {
+        asm volatile("");  // a branch, not 16 selects for every tile
 #pragma unroll
         for (int i = 0; i < 16; ++i)
           if (kv0 + acc_row(g, i) > row + shift) x[i] = -INFINITY;
@@ -325,29 +457,29 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void packed_bwd_dq_kernel(
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int t = 0; t < NT; ++t) acc[t] = mfma32(tf.get(ks_, 32 * sub + 16 * h, t), sf[h], acc[t]);
+        for (int t = 0; t < NT; ++t) acc[t] = mfma32(tf.get(ring, 32 * sub + 16 * h, t), sf[h], acc[t]);
     }
-    ck.store(xk, kt[(st + 1) & 1]);
-    cv.store(xv, vt[(st + 1) & 1]);
-    lds_barrier();
+    rf.move(STAGE);
+    tf.move(STAGE);
   }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the late loads (zeros) land before LDS goes to another workgroup
   if (row < tile.lq) store_row<HD>(dq + (((long)tile.q0 + row) * d.H + hd.h) * HD, acc, scale, g);
 }
 
-// dK, dV: 4 waves of 32 keys, whose K and V rows stay in registers; for each
-// query head of the group, the queries from the diagonal to the end pass
-// through LDS with their -lse / c and -delta, which start the accumulators of
-// S and dP.  Queries past the sequence get -inf there, so their P is 0.
-template <int HD>
-__global__ __launch_bounds__(256, HD == 64 ? 2 : 1) void packed_bwd_dkdv_kernel(
+// dK, dV: waves of 32 keys, whose K and V rows stay in registers; for each query
+// head of the group, the queries from the diagonal to the end pass through LDS with their -lse / c and -delta, which start the accumulators of
+// S and dP.  Queries past the sequence are zeros throughout: their P is 1, their
+// dO and dS 0.
+template <int HD, int KB>
+__global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void packed_bwd_dkdv_kernel(
     const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, const bf16_t* __restrict__ v,
-    const float* __restrict__ lse, const bf16_t* __restrict__ dout, const float* __restrict__ delta,
+    const bf16_t* __restrict__ dout, const float* __restrict__ stats,
     bf16_t* __restrict__ dk, bf16_t* __restrict__ dv, PackedSeqs s, PackedHeads d, float scale) {
-  constexpr int NT = HD / 32;
-  __shared__ __align__(16) uint8_t qt[2][kStageRows * 2 * HD];
-  __shared__ __align__(16) uint8_t dt[2][kStageRows * 2 * HD];
-  __shared__ __align__(16) float rows[2][2][kStageRows];  // [buffer][-lse / c, -delta][query]
-  const PackedTile tile = find_tile<true>(s, blockIdx.x / d.Hkv);
+  constexpr int NT = HD / 32, STAGE = kStageRows * 2 * HD;
+  __shared__ __align__(1024) uint8_t ring[4 * STAGE];      // Q even, Q odd, dO even, dO odd
+  __shared__ __align__(1024) float rows[2][2][kStageRows];  // [buffer][-lse / c, -delta][query]
+  constexpr int SPLIT = 128 / KB;  // waves that share 32 keys, each with a part of every stage's queries
+  const PackedTile tile = find_tile<true, KB>(s, blockIdx.x / d.Hkv);
   if (!tile.live) return;
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5, col = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -358,59 +490,47 @@ __global__ __launch_bounds__(256, HD == 64 ? 2 : 1) void packed_bwd_dkdv_kernel(
   const bf16_t* db = dout + (long)tile.q0 * d.ldd + (long)kvh * group * d.hsd;
   const long sb = (long)kvh * group * s.T + tile.q0;
   const int shift = tile.lk - tile.lq;
-  const int kv0 = tile.block * kTileRows + wave * 32, row = kv0 + col;
-  const float c = scale * kLog2e, rc = 1.f / c;
+  const int kv0 = tile.block * KB + wave / SPLIT * 32, row = kv0 + col, share = wave % SPLIT;
+  const float c = scale * kLog2e;
 
   bf16x8 kf[HD / 16], vf[HD / 16];
   load_rows<HD>(kf, rows_rsrc(kb, d.ldk, kv0, tile.lk, 32, HD), (int)d.ldk, lane);
   load_rows<HD>(vf, rows_rsrc(vb, d.ldv, kv0, tile.lk, 32, HD), (int)d.ldv, lane);
-  const StageCopy<HD> cq(tid, (int)d.ldq), cd(tid, (int)d.ldd);
-  const RowFrag<HD> rf(lane);
-  const TransFrag<HD> tf(lane);
+  std::conditional_t<HD == 64, FullFrag, LeanFrag> fr(lane);
+  const uint32_t ring0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)ring;
+  const uint32_t rows0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)rows;
   f32x16 ak[NT], av[NT];
   clear(ak);
   clear(av);
-  const int first = max(tile.block * kTileRows - shift, 0);  // the first query that sees a key of the tile
+  const int first = max(tile.block * KB - shift, 0);  // the first query that sees a key of the tile
   const int st0 = first / kStageRows;
   const int nst = max((tile.lq + kStageRows - 1) / kStageRows - st0, 0), steps = nst * group;
-  // threads 0 .. 63 carry -lse / c, 64 .. 127 -delta of the stage's queries
-  auto load_stat = [&](int head, int st) {
-    const int r = st * kStageRows + (tid & 63);
-    const long i = sb + (long)head * s.T + min(r, tile.lq - 1);
-    if (tid < 64) return r < tile.lq ? -lse[i] * rc : -INFINITY;
-    return tid < 128 && r < tile.lq ? -delta[i] : 0.f;
-  };
-  uint4 xq[StageCopy<HD>::N], xd[StageCopy<HD>::N];
-  float xs = 0.f;
-  auto load = [&](int head, int st) {
-    cq.load(xq, rows_rsrc(qb + (long)head * d.hsq, d.ldq, st * kStageRows, tile.lq, kStageRows, HD));
-    cd.load(xd, rows_rsrc(db + (long)head * d.hsd, d.ldd, st * kStageRows, tile.lq, kStageRows, HD));
-    xs = load_stat(head, st);
-  };
-  auto store = [&](int buf) {
-    cq.store(xq, qt[buf]);
-    cd.store(xd, dt[buf]);
-    if (tid < 128) rows[buf][tid >> 6][tid & 63] = xs;
+  StageLoad<HD> lq(qb, d.ldq, tile.lq, wave, lane), ld(db, d.ldd, tile.lq, wave, lane);
+  // stage st of head `head` into buffer buf; past the last head nothing
+  auto load = [&](int head, int st, int buf) {
+    lq.base = qb + (long)head * d.hsq;
+    ld.base = db + (long)head * d.hsd;
+    lq.len = ld.len = head < group ? tile.lq : 0;
+    lq.load(ring0 + buf * STAGE, st);
+    ld.load(ring0 + (2 + buf) * STAGE, st);
+    if (wave < 2) load_floats(stats + (long)wave * d.H * s.T + sb + (long)head * s.T, lq.len, st * kStageRows, lane,
+                              rows0 + (buf * 2 + wave) * kStageRows * 4);
   };
   int head = 0, st = st0;
-  if (steps > 0) {
-    load(head, st);
-    store(0);
-  }
-  lds_barrier();
+  load(steps > 0 ? 0 : group, st, 0);
   for (int step = 0; step < steps; ++step) {
     const int buf = step & 1, cur = st;
-    if (step + 1 < steps) {  // the next stage, or the next head's first (past the last: loaded again, not read)
-      if (++st == st0 + nst) {
-        st = st0;
-        ++head;
-      }
+    if (++st == st0 + nst) {  // the next stage, or the next head's first
+      st = st0;
+      ++head;
     }
-    load(head, st);
+    wait_loads<0>();  // this step's stage is in LDS, the one before read by every wave
+    load(head, st, buf ^ 1);
 #pragma unroll
-    for (int sub = 0; sub < 2; ++sub) {
-      const int q0 = cur * kStageRows + 32 * sub;
+    for (int i2 = 0; i2 < 2 / SPLIT; ++i2) {
+      const int sub = SPLIT == 1 ? i2 : share, q0 = cur * kStageRows + 32 * sub;
       if (kv0 > q0 + 31 + shift) continue;  // above the diagonal
+      fr.renew();
       f32x16 x, dp;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -424,12 +544,13 @@ __global__ __launch_bounds__(256, HD == 64 ? 2 : 1) void packed_bwd_dkdv_kernel(
       }
 #pragma unroll
       for (int ks = 0; ks < HD / 16; ++ks) {
-        x = mfma32(rf.get(qt[buf], 32 * sub, ks), kf[ks], x);
-        dp = mfma32(rf.get(dt[buf], 32 * sub, ks), vf[ks], dp);
+        x = mfma32(fr.get(ring, 32 * sub, ks), kf[ks], x);
+        dp = mfma32(fr.get(ring + 2 * STAGE, 32 * sub, ks), vf[ks], dp);
       }
 #pragma unroll
       for (int i = 0; i < 16; ++i) x[i] = __builtin_amdgcn_exp2f(x[i] * c);
       if (kv0 + 31 > q0 + shift) {
+        asm volatile("");  // a branch, not 16 selects for every tile
 #pragma unroll
         for (int i = 0; i < 16; ++i)
           if (row > q0 + acc_row(g, i) + shift) x[i] = 0.f;
@@ -442,12 +563,39 @@ __global__ __launch_bounds__(256, HD == 64 ? 2 : 1) void packed_bwd_dkdv_kernel(
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-          av[t] = mfma32(tf.get(dt[buf], 32 * sub + 16 * h, t), pf[h], av[t]);
-          ak[t] = mfma32(tf.get(qt[buf], 32 * sub + 16 * h, t), sf[h], ak[t]);
+          av[t] = mfma32(fr.get_t(ring + 2 * STAGE, 32 * sub + 16 * h, t), pf[h], av[t]);
+          ak[t] = mfma32(fr.get_t(ring, 32 * sub + 16 * h, t), sf[h], ak[t]);
         }
     }
-    store(buf ^ 1);
+    fr.move(STAGE);
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the late loads (zeros) land before LDS goes to another workgroup
+  if constexpr (SPLIT == 2) {  // the second half's sums to the first's, in this order
+    static_assert(2 * (HD / 4) * 64 * 16 == 4 * STAGE, "");
+    f32x4* sums = reinterpret_cast<f32x4*>(ring) + wave / 2 * (HD / 4) * 64 + lane;  // 64 x 2 HD fp32 a pair: the ring, exactly
     lds_barrier();
+    if (share == 1) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          sums[(8 * t + i) * 64] = f32x4{ak[t][4 * i], ak[t][4 * i + 1], ak[t][4 * i + 2], ak[t][4 * i + 3]};
+          sums[(8 * t + 4 + i) * 64] = f32x4{av[t][4 * i], av[t][4 * i + 1], av[t][4 * i + 2], av[t][4 * i + 3]};
+        }
+    }
+    lds_barrier();
+    if (share == 1) return;
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const f32x4 a = sums[(8 * t + i) * 64], b = sums[(8 * t + 4 + i) * 64];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          ak[t][4 * i + e] += a[e];
+          av[t][4 * i + e] += b[e];
+        }
+      }
   }
   if (row < tile.lk) {
     const long at = (((long)tile.k0 + row) * d.Hkv + kvh) * HD;
@@ -459,7 +607,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 2 : 1) void packed_bwd_dkdv_kernel(
 // The grid has one workgroup per (tile, head).
 bool packed_supported(long n, long T, long Tk, long H, long Hkv) {
   return n > 0 && H > 0 && Hkv > 0 && n < (1 << 20) && T < (1L << 30) && Tk < (1L << 30) &&
-         packed_tiles(T, n) * H < (1L << 31) && packed_tiles(Tk, n) * Hkv < (1L << 31);
+         packed_tiles(T, n) * H < (1L << 31) && packed_tiles(Tk, n, 64) * Hkv < (1L << 31);
 }
 
 hipError_t launch_packed_fwd(const void* q, const void* k, const void* v, void* o, float* lse, const PackedSeqs& s,
@@ -478,20 +626,20 @@ hipError_t launch_packed_fwd(const void* q, const void* k, const void* v, void* 
 }
 
 hipError_t launch_packed_bwd(const void* q, const void* k, const void* v, const void* o, const float* lse,
-                             const void* dout, void* dq, void* dk, void* dv, float* delta, const PackedSeqs& s,
+                             const void* dout, void* dq, void* dk, void* dv, float* stats, const PackedSeqs& s,
                              const PackedHeads& d, int hd, float scale, hipStream_t st) {
-  const dim3 gq((unsigned)(packed_tiles(s.T, s.n) * d.H)), gk((unsigned)(packed_tiles(s.Tk, s.n) * d.Hkv));
+  const dim3 gq((unsigned)(packed_tiles(s.T, s.n) * d.H)), gk((unsigned)(packed_tiles(s.Tk, s.n, hd == 64 ? 128 : 64) * d.Hkv));
   auto run_dq = [&](auto kernel) {
     NAYLIS_TIMED("packed_bwd_dq", st,
                  hipLaunchKernelGGL(kernel, gq, dim3(256), 0, st, (const bf16_t*)q, (const bf16_t*)k,
-                                    (const bf16_t*)v, (const bf16_t*)o, lse, (const bf16_t*)dout, (bf16_t*)dq, delta,
+                                    (const bf16_t*)v, (const bf16_t*)o, lse, (const bf16_t*)dout, (bf16_t*)dq, stats,
                                     s, d, scale));
     return hipGetLastError();
   };
   auto run_dkdv = [&](auto kernel) {
     NAYLIS_TIMED("packed_bwd_dkdv", st,
                  hipLaunchKernelGGL(kernel, gk, dim3(256), 0, st, (const bf16_t*)q, (const bf16_t*)k,
-                                    (const bf16_t*)v, lse, (const bf16_t*)dout, delta, (bf16_t*)dk, (bf16_t*)dv, s, d,
+                                    (const bf16_t*)v, (const bf16_t*)dout, (const float*)stats, (bf16_t*)dk, (bf16_t*)dv, s, d,
                                     scale));
     return hipGetLastError();
   };
@@ -500,7 +648,7 @@ hipError_t launch_packed_bwd(const void* q, const void* k, const void* v, const 
     if (e != hipSuccess) return e;
   }
   if (s.Tk == 0) return hipSuccess;
-  return hd == 64 ? run_dkdv(packed_bwd_dkdv_kernel<64>) : run_dkdv(packed_bwd_dkdv_kernel<128>);
+  return hd == 64 ? run_dkdv(packed_bwd_dkdv_kernel<64, 128>) : run_dkdv(packed_bwd_dkdv_kernel<128, 64>);
 }
 
 }  // namespace naylis

@@ -22,8 +22,8 @@ namespace naylis {
 
 constexpr int kTileRows = 128;
 
-// most tiles of `rows` rows in n sequences, the two outer ranges included
-inline long packed_tiles(long rows, long n) { return (rows + (kTileRows - 1) * (n + 2)) / kTileRows; }
+// most tiles of `tile` rows that `rows` rows in n sequences have, the two outer ranges included
+inline long packed_tiles(long rows, long n, int tile = kTileRows) { return (rows + (tile - 1) * (n + 2)) / tile; }
 
 struct PackedTile {
   int q0, lq, k0, lk;  // the sequence: first rows and lengths
@@ -63,31 +63,37 @@ __device__ __forceinline__ PackedSpan packed_span(const PackedSeqs& s, int i) {
 // (KEYS false): work = keys that the tile's last query sees, growing with the
 // tile.  Key tiles: work = queries that see the tile's first key, falling with
 // the tile.  The outer ranges have no work.
-template <bool KEYS>
+template <bool KEYS, int TILE>
 __device__ __forceinline__ int tiles_over(const PackedSpan& p, bool outer, int x) {
-  const int rows = KEYS ? p.lk : p.lq, all = (rows + kTileRows - 1) / kTileRows;
+  const int rows = KEYS ? p.lk : p.lq, all = (rows + TILE - 1) / TILE;
   if (x < 0) return all;
   if (outer) return 0;
-  if (KEYS) return p.lq <= x ? 0 : min(all, max(0, (p.lk - x + kTileRows - 1) / kTileRows));
+  if (KEYS) return p.lq <= x ? 0 : min(all, max(0, (p.lk - x + TILE - 1) / TILE));
   const int y = x - p.lk + p.lq;  // tiles whose end min(lq, (j + 1) rows) lies over y
-  return y < 0 ? all : y >= p.lq ? 0 : all - y / kTileRows;
+  return y < 0 ? all : y >= p.lq ? 0 : all - y / TILE;
 }
 
-template <bool KEYS>
-__device__ __forceinline__ PackedTile find_tile(const PackedSeqs& s, int rank) {
+template <bool KEYS, int TILE>
+__device__ __forceinline__ PackedTile search_tile(const PackedSeqs& s, int rank) {
   const int lane = threadIdx.x & 63, count = s.n + 2;
   const PackedSpan mine = packed_span(s, lane);
   const auto outer = [&](int i) { return i == 0 || i == s.n + 1; };
   const auto total = [&](int x) {
-    int t = tiles_over<KEYS>(mine, outer(lane), x);
+    int t = tiles_over<KEYS, TILE>(mine, outer(lane), x);
     for (int base = 64; base < count; base += 64)
-      t += tiles_over<KEYS>(packed_span(s, base + lane), outer(base + lane), x);
+      t += tiles_over<KEYS, TILE>(packed_span(s, base + lane), outer(base + lane), x);
     return __builtin_amdgcn_readfirstlane(wave_allsum_i32(t));
   };
   PackedTile tile{0, 0, 0, 0, 0, false};
   if (rank >= total(-1)) return tile;
   // the first level whose work no tile before `rank` lies under: F(128 lo) <= rank
-  int lo = 0, hi = ((KEYS ? s.T : s.Tk) + kTileRows - 1) / kTileRows;
+  int most = KEYS ? mine.lq : mine.lk;
+  for (int base = 64; base < count; base += 64) {
+    const PackedSpan p = packed_span(s, base + lane);
+    most = max(most, KEYS ? p.lq : p.lk);
+  }
+  int lo = 0, hi = (-wave_allmin_i32(-most) + kTileRows - 1) / kTileRows;
+  hi = __builtin_amdgcn_readfirstlane(hi);
   while (lo < hi) {
     const int mid = (lo + hi) / 2;
     if (total(mid * kTileRows) <= rank)
@@ -99,8 +105,8 @@ __device__ __forceinline__ PackedTile find_tile(const PackedSeqs& s, int rank) {
   int left = rank - total(x);
   for (int base = 0; base < count; base += 64) {
     const PackedSpan p = base == 0 ? mine : packed_span(s, base + lane);
-    const int over = tiles_over<KEYS>(p, outer(base + lane), x);
-    const int here = tiles_over<KEYS>(p, outer(base + lane), above) - over;
+    const int over = tiles_over<KEYS, TILE>(p, outer(base + lane), x);
+    const int here = tiles_over<KEYS, TILE>(p, outer(base + lane), above) - over;
     int sum = here;  // inclusive scan
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -116,7 +122,7 @@ __device__ __forceinline__ PackedTile find_tile(const PackedSeqs& s, int rank) {
       tile.k0 = __builtin_amdgcn_readlane(p.k0, src);
       tile.lk = __builtin_amdgcn_readlane(p.lk, src);
       if (base + src == 0 || base + src == s.n + 1) (KEYS ? tile.lq : tile.lk) = 0;
-      const int all = ((KEYS ? tile.lk : tile.lq) + kTileRows - 1) / kTileRows;
+      const int all = ((KEYS ? tile.lk : tile.lq) + TILE - 1) / TILE;
       tile.block = KEYS ? o + nth : all - 1 - o - nth;
       tile.live = tile.block >= 0 && tile.block < all;
       return tile;
@@ -124,6 +130,26 @@ __device__ __forceinline__ PackedTile find_tile(const PackedSeqs& s, int rank) {
     left -= __builtin_amdgcn_readlane(sum, 63);
   }
   return tile;
+}
+
+// The workgroup's tile: searched by its first wave alone (the others' vector
+// units would do the same 300 instructions for nothing).
+template <bool KEYS, int TILE = kTileRows>
+__device__ __forceinline__ PackedTile find_tile(const PackedSeqs& s, int rank) {
+  __shared__ PackedTile found;
+  if (threadIdx.x < 64) {
+    const PackedTile t = search_tile<KEYS, TILE>(s, rank);
+    if (threadIdx.x == 0) found = t;
+  }
+  __syncthreads();
+  PackedTile t = found;
+  t.q0 = __builtin_amdgcn_readfirstlane(t.q0);
+  t.lq = __builtin_amdgcn_readfirstlane(t.lq);
+  t.k0 = __builtin_amdgcn_readfirstlane(t.k0);
+  t.lk = __builtin_amdgcn_readfirstlane(t.lk);
+  t.block = __builtin_amdgcn_readfirstlane(t.block);
+  t.live = __builtin_amdgcn_readfirstlane((int)t.live) != 0;
+  return t;
 }
 
 }  // namespace naylis
