@@ -491,20 +491,21 @@ int naylis_mom_decode_step(const double* state_in, double* state_out, const int3
  *   clamped to them; descending ones leave the rows that they span unspecified.
  *   strides: host array, the token and head strides (elements) of q, k, v and,
  *   for the backward, dout: 8 values there, 6 in the forward
- *   lse (H, T) fp32, log2 domain, +inf for a query that sees no key; NULL in
- *   the forward where no backward follows
+ *   lse (H, T) fp32, log2 domain, +inf for a query that sees no key, and rest
+ *   (T, H, head_dim) bf16, what out's rounding left: for the backward, both NULL
+ *   in a forward that none follows
  *   stats (2, H, T) fp32: scratch of the backward
  * The backward writes dense dq, dk, dv; the gradients of a key head are summed
  * over its query heads in one fixed order in fp32.  No workspace.
  * Constraints: head_dim 64 or 128, H a multiple of Hkv, scale > 0, pointers
  * 16-byte aligned, strides multiples of 8, token strides under 2^23. */
 int naylis_mom_packed_attn_fwd(const void* q, const void* k, const void* v, const int32_t* cu_q, const int32_t* cu_k,
-                               void* out, float* lse, const int64_t* strides, float scale, int64_t n_seqs, int64_t T,
-                               int64_t Tk, int64_t H, int64_t Hkv, int64_t head_dim, void* stream);
+                               void* out, void* rest, float* lse, const int64_t* strides, float scale, int64_t n_seqs,
+                               int64_t T, int64_t Tk, int64_t H, int64_t Hkv, int64_t head_dim, void* stream);
 int naylis_mom_packed_attn_bwd(const void* q, const void* k, const void* v, const int32_t* cu_q, const int32_t* cu_k,
-                               const void* out, const float* lse, const void* dout, void* dq, void* dk, void* dv,
-                               float* stats, const int64_t* strides, float scale, int64_t n_seqs, int64_t T,
-                               int64_t Tk, int64_t H, int64_t Hkv, int64_t head_dim, void* stream);
+                               const void* out, const void* rest, const float* lse, const void* dout, void* dq,
+                               void* dk, void* dv, float* stats, const int64_t* strides, float scale, int64_t n_seqs,
+                               int64_t T, int64_t Tk, int64_t H, int64_t Hkv, int64_t head_dim, void* stream);
 
 /* --------------------------------------------------------- paged cache ---
  * Keys and values of earlier tokens in pages, and the attention of one new

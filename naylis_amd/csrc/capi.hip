@@ -1133,30 +1133,31 @@ static int check_packed(int64_t n, int64_t T, int64_t Tk, int64_t H, int64_t Hkv
 }
 
 int naylis_mom_packed_attn_fwd(const void* q, const void* k, const void* v, const int32_t* cu_q, const int32_t* cu_k,
-                               void* out, float* lse, const int64_t* strides, float scale, int64_t n_seqs, int64_t T,
-                               int64_t Tk, int64_t H, int64_t Hkv, int64_t head_dim, void* stream) {
+                               void* out, void* rest, float* lse, const int64_t* strides, float scale, int64_t n_seqs,
+                               int64_t T, int64_t Tk, int64_t H, int64_t Hkv, int64_t head_dim, void* stream) {
   const char* who = "mom_packed_attn_fwd";
   int rc = check_packed(n_seqs, T, Tk, H, Hkv, head_dim, scale, cu_q, cu_k, who);
   if (rc || T == 0) return rc;
   if (!strides) return fail(NAYLIS_ERR_ARG, "%s: null pointer argument", who);
   if ((rc = check_pointers({q, out}, who)) || (Tk > 0 && (rc = check_pointers({k, v}, who)))) return rc;
+  if (lse && (rc = check_pointers({rest}, who))) return rc;
   if ((rc = check_strides(strides, "q", who)) || (rc = check_strides(strides + 2, "k", who)) ||
       (rc = check_strides(strides + 4, "v", who)))
     return rc;
   const PackedSeqs s{cu_q, cu_k, (int)n_seqs, (int)T, (int)Tk};
   const PackedHeads d{(int)H, (int)Hkv, strides[0], strides[1], strides[2], strides[3], strides[4], strides[5], 0, 0};
-  return hip_status(launch_packed_fwd(q, k, v, out, lse, s, d, (int)head_dim, scale, (hipStream_t)stream), who);
+  return hip_status(launch_packed_fwd(q, k, v, out, rest, lse, s, d, (int)head_dim, scale, (hipStream_t)stream), who);
 }
 
 int naylis_mom_packed_attn_bwd(const void* q, const void* k, const void* v, const int32_t* cu_q, const int32_t* cu_k,
-                               const void* out, const float* lse, const void* dout, void* dq, void* dk, void* dv,
-                               float* stats, const int64_t* strides, float scale, int64_t n_seqs, int64_t T,
-                               int64_t Tk, int64_t H, int64_t Hkv, int64_t head_dim, void* stream) {
+                               const void* out, const void* rest, const float* lse, const void* dout, void* dq,
+                               void* dk, void* dv, float* stats, const int64_t* strides, float scale, int64_t n_seqs,
+                               int64_t T, int64_t Tk, int64_t H, int64_t Hkv, int64_t head_dim, void* stream) {
   const char* who = "mom_packed_attn_bwd";
   int rc = check_packed(n_seqs, T, Tk, H, Hkv, head_dim, scale, cu_q, cu_k, who);
   if (rc || (T == 0 && Tk == 0)) return rc;
   if (!strides) return fail(NAYLIS_ERR_ARG, "%s: null pointer argument", who);
-  if (T > 0 && ((rc = check_pointers({q, out, dout, dq}, who)) || !lse || !stats))
+  if (T > 0 && ((rc = check_pointers({q, out, rest, dout, dq}, who)) || !lse || !stats))
     return rc ? rc : fail(NAYLIS_ERR_ARG, "%s: null pointer argument", who);
   if (Tk > 0 && (rc = check_pointers({k, v, dk, dv}, who))) return rc;
   if ((rc = check_strides(strides, "q", who)) || (rc = check_strides(strides + 2, "k", who)) ||
@@ -1166,7 +1167,8 @@ int naylis_mom_packed_attn_bwd(const void* q, const void* k, const void* v, cons
   const PackedHeads d{(int)H,     (int)Hkv,   strides[0], strides[1], strides[2],
                       strides[3], strides[4], strides[5], strides[6], strides[7]};
   return hip_status(
-      launch_packed_bwd(q, k, v, out, lse, dout, dq, dk, dv, stats, s, d, (int)head_dim, scale, (hipStream_t)stream),
+      launch_packed_bwd(q, k, v, out, rest, lse, dout, dq, dk, dv, stats, s, d, (int)head_dim, scale,
+                        (hipStream_t)stream),
       who);
 }
 

@@ -234,6 +234,24 @@ __device__ __forceinline__ void store_row(bf16_t* p, const f32x16 (&a)[HD / 32],
   }
 }
 
+// The same as two bf16 tensors: the rounded values, and what rounding left.
+template <int HD>
+__device__ __forceinline__ void store_row_hilo(bf16_t* p, bf16_t* rest, const f32x16 (&a)[HD / 32], float x, int g) {
+#pragma unroll
+  for (int t = 0; t < HD / 32; ++t) {
+    f32x16 s;
+#pragma unroll
+    for (int v = 0; v < 16; ++v) s[v] = a[t][v] * x;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      bf16x8 hi, lo;
+      pack8_hilo(s, 8 * h, hi, lo);
+      *reinterpret_cast<bf16x8*>(p + 32 * t + 16 * g + 8 * h) = hi;
+      *reinterpret_cast<bf16x8*>(rest + 32 * t + 16 * g + 8 * h) = lo;
+    }
+  }
+}
+
 template <int N>
 __device__ __forceinline__ void clear(f32x16 (&a)[N]) {
 #pragma unroll
@@ -262,7 +280,7 @@ struct Head {
 template <int HD>
 __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void packed_fwd_kernel(
     const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, const bf16_t* __restrict__ v, bf16_t* __restrict__ o,
-    float* __restrict__ lse, PackedSeqs s, PackedHeads d, float c) {
+    bf16_t* __restrict__ rest, float* __restrict__ lse, PackedSeqs s, PackedHeads d, float c) {
   constexpr int NT = HD / 32, NK = HD / 16, STAGE = kStageRows * 2 * HD;
   __shared__ __align__(1024) uint8_t ring[4 * STAGE];  // K even, K odd, V even, V odd
   const PackedTile tile = find_tile<false>(s, blockIdx.x / d.H);
@@ -372,18 +390,25 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void packed_fwd_kernel(
     // a query without keys: zeros, and a log-sum-exp under which every backward weight is 0
     const bool none = row + shift < 0;
     const long at = (long)tile.q0 + row;
-    store_row<HD>(o + (at * d.H + hd.h) * HD, acc, none ? 0.f : 1.f / ls, g);
+    const long off = (at * d.H + hd.h) * HD;
+    if (lse)
+      store_row_hilo<HD>(o + off, rest + off, acc, none ? 0.f : 1.f / ls, g);
+    else
+      store_row<HD>(o + off, acc, none ? 0.f : 1.f / ls, g);
     if (lse && g == 0) lse[(long)hd.h * s.T + at] = none ? INFINITY : m + log2f(ls);
   }
 }
 
 // dQ: the forward's walk with P from the log-sum-exp.  Leaves (2, H, T) for the
-// dK/dV kernel: -lse / c and -delta, delta = rowsum(dO o).
+// dK/dV kernel: -lse / c and -delta, delta = rowsum(dO o) of the forward's o
+// before its rounding (o + rest): with the rounded o alone the error of dQ and dK
+// (2-norm, against fp64) is 2.6e-3, with both 2.4e-3, of which each rounding that
+// remains, of dS and of the result, makes 1.7e-3.
 template <int HD>
 __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void packed_bwd_dq_kernel(
     const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, const bf16_t* __restrict__ v,
-    const bf16_t* __restrict__ o, const float* __restrict__ lse, const bf16_t* __restrict__ dout,
-    bf16_t* __restrict__ dq, float* __restrict__ stats, PackedSeqs s, PackedHeads d, float scale) {
+    const bf16_t* __restrict__ o, const bf16_t* __restrict__ rest, const float* __restrict__ lse,
+    const bf16_t* __restrict__ dout, bf16_t* __restrict__ dq, float* __restrict__ stats, PackedSeqs s, PackedHeads d, float scale) {
   constexpr int NT = HD / 32, STAGE = kStageRows * 2 * HD;
   __shared__ __align__(1024) uint8_t ring[4 * STAGE];  // K even, K odd, V even, V odd
   const PackedTile tile = find_tile<false>(s, blockIdx.x / d.H);
@@ -395,7 +420,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void packed_bwd_dq_kernel(
   const bf16_t* kb = k + (long)tile.k0 * d.ldk + (long)hd.kvh * d.hsk;
   const bf16_t* vb = v + (long)tile.k0 * d.ldv + (long)hd.kvh * d.hsv;
   const bf16_t* db = dout + (long)tile.q0 * d.ldd + (long)hd.h * d.hsd;
-  const bf16_t* ob = o + ((long)tile.q0 * d.H + hd.h) * HD;
+  const long ob = ((long)tile.q0 * d.H + hd.h) * HD;
   const int shift = tile.lk - tile.lq;
   const int q0 = tile.block * kTileRows + wave * 32, row = q0 + col;
   const float c = scale * kLog2e;
@@ -407,12 +432,13 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void packed_bwd_dq_kernel(
   const float ml = -lse[stat];
   float md = 0.f;  // -delta of the lane's query
   {
-    bf16x8 of[HD / 16];
-    load_rows<HD>(of, rows_rsrc(ob, (long)d.H * HD, q0, tile.lq, 32, HD), d.H * HD, lane);
+    bf16x8 of[HD / 16], lf[HD / 16];
+    load_rows<HD>(of, rows_rsrc(o + ob, (long)d.H * HD, q0, tile.lq, 32, HD), d.H * HD, lane);
+    load_rows<HD>(lf, rows_rsrc(rest + ob, (long)d.H * HD, q0, tile.lq, 32, HD), d.H * HD, lane);
 #pragma unroll
     for (int ks = 0; ks < HD / 16; ++ks)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) md = fmaf(-(float)df[ks][e], (float)of[ks][e], md);
+      for (int e = 0; e < 8; ++e) md = fmaf(-(float)df[ks][e], (float)of[ks][e] + (float)lf[ks][e], md);
     md = xor32_f32(md, [](float a, float b) { return a + b; });
     if (g == 0 && row < tile.lq) {
       stats[stat] = ml / c;
@@ -610,13 +636,13 @@ bool packed_supported(long n, long T, long Tk, long H, long Hkv) {
          packed_tiles(T, n) * H < (1L << 31) && packed_tiles(Tk, n, 64) * Hkv < (1L << 31);
 }
 
-hipError_t launch_packed_fwd(const void* q, const void* k, const void* v, void* o, float* lse, const PackedSeqs& s,
-                             const PackedHeads& d, int hd, float scale, hipStream_t st) {
+hipError_t launch_packed_fwd(const void* q, const void* k, const void* v, void* o, void* rest, float* lse,
+                             const PackedSeqs& s, const PackedHeads& d, int hd, float scale, hipStream_t st) {
   const dim3 grid((unsigned)(packed_tiles(s.T, s.n) * d.H));
   auto run = [&](auto kernel) {
     NAYLIS_TIMED("packed_fwd", st,
                  hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, (const bf16_t*)q, (const bf16_t*)k,
-                                    (const bf16_t*)v, (bf16_t*)o, lse, s, d, scale * kLog2e));
+                                    (const bf16_t*)v, (bf16_t*)o, (bf16_t*)rest, lse, s, d, scale * kLog2e));
   };
   if (hd == 64)
     run(packed_fwd_kernel<64>);
@@ -625,14 +651,14 @@ hipError_t launch_packed_fwd(const void* q, const void* k, const void* v, void* 
   return hipGetLastError();
 }
 
-hipError_t launch_packed_bwd(const void* q, const void* k, const void* v, const void* o, const float* lse,
-                             const void* dout, void* dq, void* dk, void* dv, float* stats, const PackedSeqs& s,
+hipError_t launch_packed_bwd(const void* q, const void* k, const void* v, const void* o, const void* rest,
+                             const float* lse, const void* dout, void* dq, void* dk, void* dv, float* stats, const PackedSeqs& s,
                              const PackedHeads& d, int hd, float scale, hipStream_t st) {
   const dim3 gq((unsigned)(packed_tiles(s.T, s.n) * d.H)), gk((unsigned)(packed_tiles(s.Tk, s.n, hd == 64 ? 128 : 64) * d.Hkv));
   auto run_dq = [&](auto kernel) {
     NAYLIS_TIMED("packed_bwd_dq", st,
                  hipLaunchKernelGGL(kernel, gq, dim3(256), 0, st, (const bf16_t*)q, (const bf16_t*)k,
-                                    (const bf16_t*)v, (const bf16_t*)o, lse, (const bf16_t*)dout, (bf16_t*)dq, stats,
+                                    (const bf16_t*)v, (const bf16_t*)o, (const bf16_t*)rest, lse, (const bf16_t*)dout, (bf16_t*)dq, stats,
                                     s, d, scale));
     return hipGetLastError();
   };

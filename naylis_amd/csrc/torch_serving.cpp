@@ -56,29 +56,37 @@ struct PackedArgs {
   int64_t n() const { return cu_q.size(0) - 1; }
 };
 
-at::Tensor packed_forward(const PackedArgs& a, at::Tensor* lse, void* st) {
+// What a backward needs beside the inputs and the result.
+struct PackedSaved {
+  at::Tensor rest, lse;
+};
+
+at::Tensor packed_forward(const PackedArgs& a, PackedSaved* saved, void* st) {
   const int64_t T = a.q.size(0), Tk = a.k.size(0), H = a.q.size(1), hd = a.q.size(2);
   at::Tensor out = at::empty({T, H, hd}, a.q.options());
   const int64_t strides[6] = {a.q.stride(0), a.q.stride(1), a.k.stride(0),
                               a.k.stride(1), a.v.stride(0), a.v.stride(1)};
-  if (lse) *lse = at::empty({H, T}, f32_like(a.q));
+  if (saved) *saved = {at::empty_like(out), at::empty({H, T}, f32_like(a.q))};
   check(naylis_mom_packed_attn_fwd(a.q.data_ptr(), a.k.data_ptr(), a.v.data_ptr(), a.cu_q.data_ptr<int32_t>(),
                                    a.cu_k.data_ptr<int32_t>(), out.data_ptr(),
-                                   lse ? lse->data_ptr<float>() : nullptr, strides, (float)a.scale, a.n(), T, Tk, H,
-                                   a.k.size(1), hd, st));
+                                   saved ? saved->rest.data_ptr() : nullptr,
+                                   saved ? saved->lse.data_ptr<float>() : nullptr, strides, (float)a.scale, a.n(), T,
+                                   Tk, H, a.k.size(1), hd, st));
   return out;
 }
 
-variable_list packed_grads(const PackedArgs& a, const at::Tensor& out, const at::Tensor& lse, const at::Tensor& grad) {
+variable_list packed_grads(const PackedArgs& a, const at::Tensor& out, const PackedSaved& saved,
+                           const at::Tensor& grad) {
   at::DeviceGuard guard(a.q.device());
   const at::Tensor dout = rows_of(grad.to(a.q.scalar_type()));
   const int64_t T = a.q.size(0), Tk = a.k.size(0), H = a.q.size(1), Hkv = a.k.size(1), hd = a.q.size(2);
   at::Tensor dq = at::empty({T, H, hd}, a.q.options()), dk = at::empty({Tk, Hkv, hd}, a.q.options());
-  at::Tensor dv = at::empty({Tk, Hkv, hd}, a.q.options()), stats = at::empty({2, H, T}, lse.options());
+  at::Tensor dv = at::empty({Tk, Hkv, hd}, a.q.options()), stats = at::empty({2, H, T}, saved.lse.options());
   const int64_t strides[8] = {a.q.stride(0), a.q.stride(1), a.k.stride(0), a.k.stride(1),
                               a.v.stride(0), a.v.stride(1), dout.stride(0), dout.stride(1)};
   check(naylis_mom_packed_attn_bwd(a.q.data_ptr(), a.k.data_ptr(), a.v.data_ptr(), a.cu_q.data_ptr<int32_t>(),
-                                   a.cu_k.data_ptr<int32_t>(), out.data_ptr(), lse.data_ptr<float>(), dout.data_ptr(),
+                                   a.cu_k.data_ptr<int32_t>(), out.data_ptr(), saved.rest.data_ptr(),
+                                   saved.lse.data_ptr<float>(), dout.data_ptr(),
                                    dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), stats.data_ptr<float>(), strides,
                                    (float)a.scale, a.n(), T, Tk, H, Hkv, hd, current_stream(a.q)));
   return {dq, dk, dv};
@@ -88,8 +96,9 @@ variable_list packed_grads(const PackedArgs& a, const at::Tensor& out, const at:
 // second derivative raises instead of leaving this part out.
 struct PackedAttentionGrad : public Function<PackedAttentionGrad> {
   static variable_list forward(AutogradContext*, at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor cu_q,
-                               at::Tensor cu_k, at::Tensor out, at::Tensor lse, at::Tensor dout, double scale) {
-    return packed_grads({q, k, v, cu_q, cu_k, scale}, out, lse, dout);
+                               at::Tensor cu_k, at::Tensor out, at::Tensor rest, at::Tensor lse, at::Tensor dout,
+                               double scale) {
+    return packed_grads({q, k, v, cu_q, cu_k, scale}, out, {rest, lse}, dout);
   }
   static variable_list backward(AutogradContext*, variable_list) {
     TORCH_CHECK(false, "packed_attention: the derivative of its backward is not implemented");
@@ -100,8 +109,9 @@ struct PackedAttention : public Function<PackedAttention> {
   static at::Tensor forward(AutogradContext* ctx, at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor cu_q,
                             at::Tensor cu_k, double scale, int64_t st) {
     const PackedArgs a{rows_of(q), rows_of(k), rows_of(v), cu_q, cu_k, scale};
-    at::Tensor lse, out = packed_forward(a, &lse, stream_ptr(st));
-    ctx->save_for_backward({a.q, a.k, a.v, cu_q, cu_k, out, lse});
+    PackedSaved saved;
+    at::Tensor out = packed_forward(a, &saved, stream_ptr(st));
+    ctx->save_for_backward({a.q, a.k, a.v, cu_q, cu_k, out, saved.rest, saved.lse});
     ctx->saved_data["scale"] = scale;
     return out;
   }
@@ -109,8 +119,8 @@ struct PackedAttention : public Function<PackedAttention> {
     const variable_list s = ctx->get_saved_variables();
     const double scale = ctx->saved_data["scale"].toDouble();
     variable_list g = at::GradMode::is_enabled()
-                          ? PackedAttentionGrad::apply(s[0], s[1], s[2], s[3], s[4], s[5], s[6], grads[0], scale)
-                          : packed_grads({s[0], s[1], s[2], s[3], s[4], scale}, s[5], s[6], grads[0]);
+                          ? PackedAttentionGrad::apply(s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7], grads[0], scale)
+                          : packed_grads({s[0], s[1], s[2], s[3], s[4], scale}, s[5], {s[6], s[7]}, grads[0]);
     g.resize(7);
     return g;
   }

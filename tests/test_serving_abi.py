@@ -28,9 +28,9 @@ def _refused(lib, rc, text):
 
 
 def _packed(lib, n=1, T=10, Tk=10, H=4, Hkv=2, hd=64, scale=0.1, q=P, cu=P, strides=(256, 64, 128, 64, 128, 64, 256, 64)):
-    fwd = lib.naylis_mom_packed_attn_fwd(q, P, P, cu, cu, P, P, _i64(*strides), scale, n, T, Tk, H, Hkv, hd, None)
+    fwd = lib.naylis_mom_packed_attn_fwd(q, P, P, cu, cu, P, P, P, _i64(*strides), scale, n, T, Tk, H, Hkv, hd, None)
     msg = lib.naylis_mom_last_error()
-    bwd = lib.naylis_mom_packed_attn_bwd(q, P, P, cu, cu, P, P, P, P, P, P, P, _i64(*strides), scale, n, T, Tk, H, Hkv,
+    bwd = lib.naylis_mom_packed_attn_bwd(q, P, P, cu, cu, P, P, P, P, P, P, P, P, _i64(*strides), scale, n, T, Tk, H, Hkv,
                                          hd, None)
     assert fwd == bwd and msg.split(b":")[1] == lib.naylis_mom_last_error().split(b":")[1]
     return fwd
