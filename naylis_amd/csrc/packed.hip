@@ -277,20 +277,22 @@ struct Head {
 // stage further ahead than V, each into the buffer that the barrier before has
 // freed: barrier 1 of a stage stands after the last use of its K, barrier 2
 // after that of its V.
-template <int HD>
+// SPLIT 2, for grids that leave CUs idle: 64 queries, each 32 of them with two waves, which take the even and the odd key tiles (one of each stage, so
+// that one barrier a stage does) and join their sums at the end.
+template <int HD, int SPLIT>
 __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void packed_fwd_kernel(
     const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, const bf16_t* __restrict__ v, bf16_t* __restrict__ o,
     bf16_t* __restrict__ rest, float* __restrict__ lse, PackedSeqs s, PackedHeads d, float c) {
-  constexpr int NT = HD / 32, NK = HD / 16, STAGE = kStageRows * 2 * HD;
+  constexpr int NT = HD / 32, NK = HD / 16, STAGE = kStageRows * 2 * HD, ROWS = kTileRows / SPLIT;
   __shared__ __align__(1024) uint8_t ring[4 * STAGE];  // K even, K odd, V even, V odd
-  const PackedTile tile = find_tile<false>(s, blockIdx.x / d.H);
+  const PackedTile tile = find_tile<false, ROWS>(s, blockIdx.x / d.H);
   if (!tile.live) return;
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5, col = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const Head hd(blockIdx.x % d.H, d);
   const bf16_t* qb = q + (long)tile.q0 * d.ldq + (long)hd.h * d.hsq;
   const int shift = tile.lk - tile.lq;  // query i sees keys up to i + shift
-  const int q0 = tile.block * kTileRows + wave * 32, row = q0 + col;
+  const int q0 = tile.block * ROWS + wave / SPLIT * 32, row = q0 + col, share = wave % SPLIT;
 
   bf16x8 qf[NK];
   load_rows<HD>(qf, rows_rsrc(qb, d.ldq, q0, tile.lq, 32, HD), (int)d.ldq, lane);
@@ -300,7 +302,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void packed_fwd_kernel(
   TransFrag<HD> tf(lane);
   tf.move(2 * STAGE);
   const uint32_t ring0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)ring;  // LDS byte address
-  const int keys = min(tile.lq, (tile.block + 1) * kTileRows) + shift;  // seen by the tile's last query
+  const int keys = min(tile.lq, (tile.block + 1) * ROWS) + shift;  // seen by the tile's last query
   const int nst = (max(keys, 0) + kStageRows - 1) / kStageRows;
   const int nt = min(max(q0 + 32 + shift + 31, 0) / 32, 2 * nst);  // key tiles that the wave's queries see
 
@@ -333,12 +335,12 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void packed_fwd_kernel(
     l += x[i];
   };
   // Tile t (the first or second of its stage) with its scores in x; leaves
-  // those of t + 1 there.  The lanes' LDS offsets move to the other buffer a
+  // those of the wave's next one, t + SPLIT, there.  The lanes' LDS offsets move to the other buffer a
   // stage at a time, so that tiles differ by constants.
   auto step = [&](auto second, int t) {
     constexpr int HALF = 32 * 2 * HD, SECOND = decltype(second)::value;
     const uint8_t* vb = ring + SECOND * HALF;
-    const uint8_t* kb = ring + (SECOND ? 0 : HALF);
+    const uint8_t* kb = ring + (SECOND != (SPLIT == 1) ? HALF : 0);
     auto add_pv = [&]() {
       const bf16x8 pf[2] = {pack8(x, 0), pack8(x, 8)};
 #pragma unroll
@@ -346,7 +348,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void packed_fwd_kernel(
 #pragma unroll
         for (int u = 0; u < NT; ++u) acc[u] = mfma32(tf.get(vb, 16 * h, u), pf[h], acc[u]);
     };
-    if (t + 1 < nt) {
+    if (t + SPLIT < nt) {
       f32x16 y = f32x16{};
 #pragma unroll
       for (int ks = 0; ks < NK; ++ks) {
@@ -355,7 +357,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void packed_fwd_kernel(
         for (int i = 0; i < 16 / NK; ++i) weigh(ks * (16 / NK) + i);
       }
       add_pv();
-      settle(y, t + 1);
+      settle(y, t + SPLIT);
       x = y;
     } else {
 #pragma unroll
@@ -368,23 +370,61 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void packed_fwd_kernel(
   lv.load(ring0 + 2 * STAGE, 0);
   lk.load(ring0 + STAGE, 1);
   wait_loads<StageLoad<HD>::N>();
-  if (nt > 0) {
+  if (share < nt) {
     x = f32x16{};
 #pragma unroll
-    for (int ks = 0; ks < NK; ++ks) x = mfma32(rf.get(ring, 0, ks), qf[ks], x);
-    settle(x, 0);
+    for (int ks = 0; ks < NK; ++ks) x = mfma32(rf.get(ring + share * 32 * 2 * HD, 0, ks), qf[ks], x);
+    settle(x, share);
   }
-  for (int st = 0; st < nst; ++st) {
-    lv.load(ring0 + (2 + ((st + 1) & 1)) * STAGE, st + 1);
-    if (2 * st < nt) step(std::false_type{}, 2 * st);
-    wait_loads<StageLoad<HD>::N>();  // K of stage st + 1 is in LDS, that of st no longer needed
-    lk.load(ring0 + (st & 1) * STAGE, st + 2);
-    rf.move(STAGE);
-    if (2 * st + 1 < nt) step(std::true_type{}, 2 * st + 1);
-    wait_loads<StageLoad<HD>::N>();  // V likewise
-    tf.move(STAGE);
+  if constexpr (SPLIT == 1) {
+    for (int st = 0; st < nst; ++st) {
+      lv.load(ring0 + (2 + ((st + 1) & 1)) * STAGE, st + 1);
+      if (2 * st < nt) step(std::false_type{}, 2 * st);
+      wait_loads<StageLoad<HD>::N>();  // K of stage st + 1 is in LDS, that of st no longer needed
+      lk.load(ring0 + (st & 1) * STAGE, st + 2);
+      rf.move(STAGE);
+      if (2 * st + 1 < nt) step(std::true_type{}, 2 * st + 1);
+      wait_loads<StageLoad<HD>::N>();  // V likewise
+      tf.move(STAGE);
+    }
+  } else {
+    for (int st = 0; st < nst; ++st) {
+      wait_loads<0>();  // K of stage st + 1 and V of st are in LDS, what stage st - 1 used is free
+      rf.move(STAGE);
+      lk.load(ring0 + (st & 1) * STAGE, st + 2);
+      lv.load(ring0 + (2 + ((st + 1) & 1)) * STAGE, st + 1);
+      if (2 * st + share < nt) {
+        if (share)
+          step(std::true_type{}, 2 * st + 1);
+        else
+          step(std::false_type{}, 2 * st);
+      }
+      tf.move(STAGE);
+    }
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the late loads (zeros) land before LDS goes to another workgroup
+  if constexpr (SPLIT == 2) {  // the odd tiles' sums to the even ones' (m is -1e30 and all else 0 where there were none)
+    float* sums = reinterpret_cast<float*>(ring) + wave / 2 * (HD / 2 + 2) * 64 + lane;
+    lds_barrier();
+    if (share == 1) {
+#pragma unroll
+      for (int u = 0; u < NT; ++u)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sums[(16 * u + i) * 64] = acc[u][i];
+      sums[HD / 2 * 64] = m;
+      sums[(HD / 2 + 1) * 64] = l;
+    }
+    lds_barrier();
+    if (share == 1) return;
+    const float mo = sums[HD / 2 * 64], mn = fmaxf(m, mo);
+    const float a = __builtin_amdgcn_exp2f(m - mn), b = __builtin_amdgcn_exp2f(mo - mn);
+    m = mn;
+    l = l * a + sums[(HD / 2 + 1) * 64] * b;
+#pragma unroll
+    for (int u = 0; u < NT; ++u)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[u][i] = acc[u][i] * a + sums[(16 * u + i) * 64] * b;
+  }
   const float ls = xor32_f32(l, [](float a, float b) { return a + b; });
   if (row < tile.lq) {
     // a query without keys: zeros, and a log-sum-exp under which every backward weight is 0
@@ -633,22 +673,24 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void packed_bwd_dkdv_kernel(
 // The grid has one workgroup per (tile, head).
 bool packed_supported(long n, long T, long Tk, long H, long Hkv) {
   return n > 0 && H > 0 && Hkv > 0 && n < (1 << 20) && T < (1L << 30) && Tk < (1L << 30) &&
-         packed_tiles(T, n) * H < (1L << 31) && packed_tiles(Tk, n, 64) * Hkv < (1L << 31);
+         packed_tiles(T, n, 64) * H < (1L << 31) && packed_tiles(Tk, n, 64) * Hkv < (1L << 31);
 }
 
 hipError_t launch_packed_fwd(const void* q, const void* k, const void* v, void* o, void* rest, float* lse,
                              const PackedSeqs& s, const PackedHeads& d, int hd, float scale, hipStream_t st) {
-  const dim3 grid((unsigned)(packed_tiles(s.T, s.n) * d.H));
-  auto run = [&](auto kernel) {
+  auto run = [&](auto kernel, int rows) {
     NAYLIS_TIMED("packed_fwd", st,
-                 hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, (const bf16_t*)q, (const bf16_t*)k,
-                                    (const bf16_t*)v, (bf16_t*)o, (bf16_t*)rest, lse, s, d, scale * kLog2e));
+                 hipLaunchKernelGGL(kernel, dim3((unsigned)(packed_tiles(s.T, s.n, rows) * d.H)), dim3(256), 0, st,
+                                    (const bf16_t*)q, (const bf16_t*)k, (const bf16_t*)v, (bf16_t*)o, (bf16_t*)rest,
+                                    lse, s, d, scale * kLog2e));
+    return hipGetLastError();
   };
-  if (hd == 64)
-    run(packed_fwd_kernel<64>);
-  else
-    run(packed_fwd_kernel<128>);
-  return hipGetLastError();
+  // under one and a half tiles a CU: 4000 queries of 8 heads of 128 (272 tiles)
+  // 95 -> 73 us, 2000 52 -> 39, 500 18 -> 15; from two a CU on level or slower
+  // (4000 queries of 16 heads 106 -> 112, of 32 171 -> 199)
+  const bool split = packed_tiles(s.T, s.n) * d.H < 384;
+  if (hd == 64) return split ? run(packed_fwd_kernel<64, 2>, 64) : run(packed_fwd_kernel<64, 1>, 128);
+  return split ? run(packed_fwd_kernel<128, 2>, 64) : run(packed_fwd_kernel<128, 1>, 128);
 }
 
 hipError_t launch_packed_bwd(const void* q, const void* k, const void* v, const void* o, const void* rest,
