@@ -494,18 +494,21 @@ int naylis_mom_decode_step(const double* state_in, double* state_out, const int3
  *   lse (H, T) fp32, log2 domain, +inf for a query that sees no key, and rest
  *   (T, H, head_dim) bf16, what out's rounding left: for the backward, both NULL
  *   in a forward that none follows
- *   stats (2, H, T) fp32: scratch of the backward
+ *   workspace: naylis_mom_packed_attn_bwd_workspace_bytes
  * The backward writes dense dq, dk, dv; the gradients of a key head are summed
- * over its query heads in one fixed order in fp32.  No workspace.
+ * over its query heads in one fixed order in fp32.
  * Constraints: head_dim 64 or 128, H a multiple of Hkv, scale > 0, pointers
  * 16-byte aligned, strides multiples of 8, token strides under 2^23. */
 int naylis_mom_packed_attn_fwd(const void* q, const void* k, const void* v, const int32_t* cu_q, const int32_t* cu_k,
                                void* out, void* rest, float* lse, const int64_t* strides, float scale, int64_t n_seqs,
                                int64_t T, int64_t Tk, int64_t H, int64_t Hkv, int64_t head_dim, void* stream);
+size_t naylis_mom_packed_attn_bwd_workspace_bytes(int64_t n_seqs, int64_t T, int64_t Tk, int64_t H, int64_t Hkv,
+                                                  int64_t head_dim);
 int naylis_mom_packed_attn_bwd(const void* q, const void* k, const void* v, const int32_t* cu_q, const int32_t* cu_k,
                                const void* out, const void* rest, const float* lse, const void* dout, void* dq,
-                               void* dk, void* dv, float* stats, const int64_t* strides, float scale, int64_t n_seqs,
-                               int64_t T, int64_t Tk, int64_t H, int64_t Hkv, int64_t head_dim, void* stream);
+                               void* dk, void* dv, void* workspace, size_t workspace_bytes, const int64_t* strides,
+                               float scale, int64_t n_seqs, int64_t T, int64_t Tk, int64_t H, int64_t Hkv,
+                               int64_t head_dim, void* stream);
 
 /* --------------------------------------------------------- paged cache ---
  * Keys and values of earlier tokens in pages, and the attention of one new

@@ -85,7 +85,8 @@ SIGNATURES = {
     "naylis_mom_bank_quant_fp8": (_int, [_c_void_p] * 6 + [_i64] * 2 + [_c_void_p]),
     "naylis_mom_decode_step": (_int, [_c_void_p] * 4 + [_int] + [_c_void_p] * 10 + [_i64] * 7 + [_c_void_p]),
     "naylis_mom_packed_attn_fwd": (_int, [_c_void_p] * 9 + [_float] + [_i64] * 6 + [_c_void_p]),
-    "naylis_mom_packed_attn_bwd": (_int, [_c_void_p] * 14 + [_float] + [_i64] * 6 + [_c_void_p]),
+    "naylis_mom_packed_attn_bwd_workspace_bytes": (_size_t, [_i64] * 6),
+    "naylis_mom_packed_attn_bwd": (_int, [_c_void_p] * 13 + [_size_t, _c_void_p, _float] + [_i64] * 6 + [_c_void_p]),
     "naylis_mom_paged_append": (_int, [_c_void_p] * 4 + [_int] + [_c_void_p] * 6 + [_i64] * 7 + [_c_void_p]),
     "naylis_mom_paged_attn_workspace_bytes": (_size_t, [_int] + [_i64] * 6),
     "naylis_mom_paged_attn": (_int, [_c_void_p] * 5 + [_int] + [_c_void_p] * 4 + [_size_t, _c_void_p, _float]

@@ -1149,15 +1149,25 @@ int naylis_mom_packed_attn_fwd(const void* q, const void* k, const void* v, cons
   return hip_status(launch_packed_fwd(q, k, v, out, rest, lse, s, d, (int)head_dim, scale, (hipStream_t)stream), who);
 }
 
+size_t naylis_mom_packed_attn_bwd_workspace_bytes(int64_t n_seqs, int64_t T, int64_t Tk, int64_t H, int64_t Hkv,
+                                                  int64_t head_dim) {
+  static const int32_t any = 0;  // (not read)
+  if (check_packed(n_seqs, T, Tk, H, Hkv, head_dim, 1.f, &any, &any, "mom_packed_attn_bwd")) return 0;
+  const PackedSeqs s{nullptr, nullptr, (int)n_seqs, (int)T, (int)Tk};
+  const PackedHeads d{(int)H, (int)Hkv, 0, 0, 0, 0, 0, 0, 0, 0};
+  return std::max(packed_bwd_ws_bytes(s, d, (int)head_dim), (size_t)16);  // (0 is a refusal)
+}
+
 int naylis_mom_packed_attn_bwd(const void* q, const void* k, const void* v, const int32_t* cu_q, const int32_t* cu_k,
                                const void* out, const void* rest, const float* lse, const void* dout, void* dq,
-                               void* dk, void* dv, float* stats, const int64_t* strides, float scale, int64_t n_seqs,
-                               int64_t T, int64_t Tk, int64_t H, int64_t Hkv, int64_t head_dim, void* stream) {
+                               void* dk, void* dv, void* workspace, size_t workspace_bytes, const int64_t* strides,
+                               float scale, int64_t n_seqs, int64_t T, int64_t Tk, int64_t H, int64_t Hkv,
+                               int64_t head_dim, void* stream) {
   const char* who = "mom_packed_attn_bwd";
   int rc = check_packed(n_seqs, T, Tk, H, Hkv, head_dim, scale, cu_q, cu_k, who);
   if (rc || (T == 0 && Tk == 0)) return rc;
-  if (!strides) return fail(NAYLIS_ERR_ARG, "%s: null pointer argument", who);
-  if (T > 0 && ((rc = check_pointers({q, out, rest, dout, dq}, who)) || !lse || !stats))
+  if (!strides || !workspace) return fail(NAYLIS_ERR_ARG, "%s: null pointer argument", who);
+  if (T > 0 && ((rc = check_pointers({q, out, rest, dout, dq}, who)) || !lse))
     return rc ? rc : fail(NAYLIS_ERR_ARG, "%s: null pointer argument", who);
   if (Tk > 0 && (rc = check_pointers({k, v, dk, dv}, who))) return rc;
   if ((rc = check_strides(strides, "q", who)) || (rc = check_strides(strides + 2, "k", who)) ||
@@ -1166,8 +1176,12 @@ int naylis_mom_packed_attn_bwd(const void* q, const void* k, const void* v, cons
   const PackedSeqs s{cu_q, cu_k, (int)n_seqs, (int)T, (int)Tk};
   const PackedHeads d{(int)H,     (int)Hkv,   strides[0], strides[1], strides[2],
                       strides[3], strides[4], strides[5], strides[6], strides[7]};
+  const size_t need = packed_bwd_ws_bytes(s, d, (int)head_dim);
+  if (workspace_bytes < need)
+    return fail(NAYLIS_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", who, workspace_bytes, need);
+  if (!aligned16(workspace)) return fail(NAYLIS_ERR_ARG, "%s: all tensors must be 16-byte aligned", who);
   return hip_status(
-      launch_packed_bwd(q, k, v, out, rest, lse, dout, dq, dk, dv, stats, s, d, (int)head_dim, scale,
+      launch_packed_bwd(q, k, v, out, rest, lse, dout, dq, dk, dv, workspace, s, d, (int)head_dim, scale,
                         (hipStream_t)stream),
       who);
 }

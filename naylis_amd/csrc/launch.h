@@ -124,8 +124,7 @@ hipError_t launch_attn_bwd(const void* q, const void* k, const void* v, const vo
 // Causal attention over packed sequences (packed.hip): q, o (T, H, hd) and k, v
 // (Tk, Hkv, hd) bf16, hd 64 or 128; sequence i holds query rows cu_q[i] ..
 // cu_q[i + 1] - 1 and key rows cu_k[i] .. (device arrays of n + 1 offsets).
-// lse (H, T; log2 domain) and stats (2, H, T) fp32; rest: o less its rounding
-// (bf16, o's shape).  lse and rest are null in a forward without a backward.
+// lse (H, T; log2 domain) fp32; rest: o less its rounding (bf16, o's shape).  lse and rest are null in a forward without a backward.
 struct PackedSeqs {
   const int32_t* cu_q;
   const int32_t* cu_k;
@@ -136,11 +135,12 @@ struct PackedHeads {
   long ldq, hsq, ldk, hsk, ldv, hsv, ldd, hsd;  // token and head strides of q, k, v, dO (elements)
 };
 bool packed_supported(long n, long T, long Tk, long H, long Hkv);
+size_t packed_bwd_ws_bytes(const PackedSeqs& s, const PackedHeads& d, int hd);
 hipError_t launch_packed_fwd(const void* q, const void* k, const void* v, void* o, void* rest, float* lse,
                              const PackedSeqs& s, const PackedHeads& d, int hd, float scale, hipStream_t st);
 hipError_t launch_packed_bwd(const void* q, const void* k, const void* v, const void* o, const void* rest,
-                             const float* lse, const void* dout, void* dq, void* dk, void* dv, float* stats, const PackedSeqs& s,
-                             const PackedHeads& d, int hd, float scale, hipStream_t st);
+                             const float* lse, const void* dout, void* dq, void* dk, void* dv, void* ws,
+                             const PackedSeqs& s, const PackedHeads& d, int hd, float scale, hipStream_t st);
 
 // Paged key / value cache (paged.hip): pages (P, Hkv, page, hd) bf16 or e4m3
 // codes with scales (P, Hkv, page); table (B, W) page ids; G query heads for a

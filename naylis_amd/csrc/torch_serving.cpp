@@ -81,13 +81,14 @@ variable_list packed_grads(const PackedArgs& a, const at::Tensor& out, const Pac
   const at::Tensor dout = rows_of(grad.to(a.q.scalar_type()));
   const int64_t T = a.q.size(0), Tk = a.k.size(0), H = a.q.size(1), Hkv = a.k.size(1), hd = a.q.size(2);
   at::Tensor dq = at::empty({T, H, hd}, a.q.options()), dk = at::empty({Tk, Hkv, hd}, a.q.options());
-  at::Tensor dv = at::empty({Tk, Hkv, hd}, a.q.options()), stats = at::empty({2, H, T}, saved.lse.options());
+  at::Tensor dv = at::empty({Tk, Hkv, hd}, a.q.options());
+  at::Tensor ws = workspace(need(naylis_mom_packed_attn_bwd_workspace_bytes(a.n(), T, Tk, H, Hkv, hd)), a.q);
   const int64_t strides[8] = {a.q.stride(0), a.q.stride(1), a.k.stride(0), a.k.stride(1),
                               a.v.stride(0), a.v.stride(1), dout.stride(0), dout.stride(1)};
   check(naylis_mom_packed_attn_bwd(a.q.data_ptr(), a.k.data_ptr(), a.v.data_ptr(), a.cu_q.data_ptr<int32_t>(),
                                    a.cu_k.data_ptr<int32_t>(), out.data_ptr(), saved.rest.data_ptr(),
                                    saved.lse.data_ptr<float>(), dout.data_ptr(),
-                                   dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), stats.data_ptr<float>(), strides,
+                                   dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), ws.numel(), strides,
                                    (float)a.scale, a.n(), T, Tk, H, Hkv, hd, current_stream(a.q)));
   return {dq, dk, dv};
 }

@@ -27,10 +27,10 @@ def _refused(lib, rc, text):
     assert text in lib.naylis_mom_last_error().decode(), lib.naylis_mom_last_error()
 
 
-def _packed(lib, n=1, T=10, Tk=10, H=4, Hkv=2, hd=64, scale=0.1, q=P, cu=P, strides=(256, 64, 128, 64, 128, 64, 256, 64)):
+def _packed(lib, n=1, T=10, Tk=10, H=4, Hkv=2, hd=64, scale=0.1, q=P, cu=P, strides=(256, 64, 128, 64, 128, 64, 256, 64), ws_bytes=1 << 40):
     fwd = lib.naylis_mom_packed_attn_fwd(q, P, P, cu, cu, P, P, P, _i64(*strides), scale, n, T, Tk, H, Hkv, hd, None)
     msg = lib.naylis_mom_last_error()
-    bwd = lib.naylis_mom_packed_attn_bwd(q, P, P, cu, cu, P, P, P, P, P, P, P, P, _i64(*strides), scale, n, T, Tk, H, Hkv,
+    bwd = lib.naylis_mom_packed_attn_bwd(q, P, P, cu, cu, P, P, P, P, P, P, P, P, ws_bytes, _i64(*strides), scale, n, T, Tk, H, Hkv,
                                          hd, None)
     assert fwd == bwd and msg.split(b":")[1] == lib.naylis_mom_last_error().split(b":")[1]
     return fwd
@@ -45,6 +45,16 @@ def _packed(lib, n=1, T=10, Tk=10, H=4, Hkv=2, hd=64, scale=0.1, q=P, cu=P, stri
     (dict(strides=(1 << 23, 64, 128, 64, 128, 64, 256, 64)), "strides")])
 def test_packed_refusals(lib, bad, text):
     _refused(lib, _packed(lib, **bad), text)
+
+
+def test_packed_workspace(lib):
+    need = lib.naylis_mom_packed_attn_bwd_workspace_bytes(1, 10, 10, 4, 2, 64)
+    args = (P, P, P, P, P, P, P, P, P, P, P, P, P, need - 1, _i64(256, 64, 128, 64, 128, 64, 256, 64), 0.1, 1, 10, 10, 4, 2, 64)
+    assert lib.naylis_mom_packed_attn_bwd(*args, None) == _lib.NAYLIS_ERR_WORKSPACE
+    # the group's heads in parts where few key tiles stand for many heads, not where they fill the chip
+    few, many = (lib.naylis_mom_packed_attn_bwd_workspace_bytes(1, n, n, 8, 2, 128) for n in (1000, 1000000))
+    assert few > 2 * 8 * 1000 * 4 + 2 * 2 * 1000 * 2 * 128 * 4 and many == 2 * 8 * 1000000 * 4
+    assert lib.naylis_mom_packed_attn_bwd_workspace_bytes(1, 10, 10, 3, 2, 64) == 0
 
 
 def test_packed_nothing_to_do(lib):
