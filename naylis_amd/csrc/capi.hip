@@ -1267,8 +1267,9 @@ int naylis_mom_paged_attn(const void* q, const void* k_pages, const void* v_page
   c.v_scale = const_cast<float*>(v_scale);
   if ((rc = check_cache(c, cache_dtype, who))) return rc;
   if (!table || !lens || !q_strides) return fail(NAYLIS_ERR_ARG, "%s: null pointer argument", who);
-  if ((rc = check_pointers({q, out, workspace}, who)) || (rc = check_strides(q_strides, "q", who))) return rc;
+  if ((rc = check_pointers({q, out}, who)) || (rc = check_strides(q_strides, "q", who))) return rc;
   const size_t need = paged_ws_bytes(c, (int)head_dim);
+  if (need && (rc = check_pointers({workspace}, who))) return rc;
   if (workspace_bytes < need)
     return fail(NAYLIS_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", who, workspace_bytes, need);
   return hip_status(launch_paged_attn(c, (int)head_dim, cache_dtype == NAYLIS_DTYPE_E4M3, q, q_strides[0],

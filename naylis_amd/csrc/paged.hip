@@ -206,7 +206,7 @@ __device__ __forceinline__ long part_row(const PagedSplit& p, int slice, int wg,
 
 // grid (workgroups of a slice, slices): slice = (key head, 16 of its query heads).
 // A workgroup takes a range of the step list, or (p.whole) the sequence of its
-// number, its four waves a quarter each.
+// number, its waves an equal share each.
 // ROWS: partials' rows, at least the query heads of a slice.
 template <int HD, bool FP8, int ROWS>
 __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedCacheDims c, const bf16_t* __restrict__ q, long ldq,
@@ -244,9 +244,9 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedCacheDims c, co
     wg1 = min(wg0 + range, total);
   }
   {
-    const int quarter = (wg1 - wg0 + 3) / 4;
-    at = min(wg0 + wave * quarter, wg1);
-    end = min(at + quarter, wg1);
+    const int share = (wg1 - wg0 + 3) / 4;
+    at = min(wg0 + wave * share, wg1);
+    end = min(at + share, wg1);
   }
   if (!p.whole && at < end) list.find(at, b, first);
   if (lane < 2) seqs[2 * wave + lane].b = -1;
@@ -452,24 +452,40 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedCacheDims c, co
   __syncthreads();
 
   // the waves' partials of one sequence, joined: its result where the workgroup
-  // held all of it, else the workgroup's partial
+  // held all of it, else the workgroup's partial.  Everything is read up front:
+  // one LDS latency, not one for each partial.
+  PartSeq ps[8];
+  int next[8];  // sequence of the partial behind
+#pragma unroll
+  for (int e = 0; e < 8; ++e) ps[e] = seqs[e];
+  int nb = -1;
+#pragma unroll
+  for (int e = 7; e >= 0; --e) {
+    next[e] = nb;
+    if (ps[e].b >= 0) nb = ps[e].b;
+  }
   for (int i = tid; i < nh * (HD / 4); i += 256) {
     const int r = i / (HD / 4), f = 4 * (i % (HD / 4));
+    float2 st[8];
+    f32x4 px[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      st[e] = stats[e][r];
+      px[e] = *reinterpret_cast<const f32x4*>(
+          reinterpret_cast<const float*>(lds + (e >> 1) * kWaveLds<HD, ROWS> + part_offset<HD>(e & 1)) + r * HD + f);
+    }
     float m = kNegBig, l = 0.f;
     f32x4 a = f32x4{};
+#pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const PartSeq cur = seqs[e];
+      const PartSeq& cur = ps[e];
       if (cur.b < 0) continue;
-      const float2 st = stats[e][r];
-      const float* px =
-          reinterpret_cast<const float*>(lds + (e >> 1) * kWaveLds<HD, ROWS> + part_offset<HD>(e & 1)) + r * HD + f;
-      const float mn = fmaxf(m, st.x), wa = __builtin_amdgcn_exp2f(m - mn), wb = __builtin_amdgcn_exp2f(st.x - mn);
-      a = a * wa + *reinterpret_cast<const f32x4*>(px) * wb;
-      l = l * wa + st.y * wb;
+      const float mn = fmaxf(m, st[e].x), wa = __builtin_amdgcn_exp2f(m - mn),
+                  wb = __builtin_amdgcn_exp2f(st[e].x - mn);
+      a = a * wa + px[e] * wb;
+      l = l * wa + st[e].y * wb;
       m = mn;
-      int nb = -1;  // the next partial's sequence
-      for (int e2 = e + 1; e2 < 8 && nb < 0; ++e2) nb = seqs[e2].b;
-      if (nb == cur.b) continue;
+      if (next[e] == cur.b) continue;
       if (cur.first >= wg0 && cur.first + cur.steps <= wg1) {
         const float inv = 1.f / l;
         bf16x4 o;
@@ -580,7 +596,7 @@ size_t paged_part_floats(const PagedCacheDims& c, const PagedSplit& p, int hd) {
 
 size_t paged_ws_bytes(const PagedCacheDims& c, int hd) {
   const size_t n = paged_part_floats(c, paged_split(c), hd);
-  return std::max(n * 4 + n / hd * 8, (size_t)16);  // (0 would mean a refusal)
+  return n * 4 + n / hd * 8;
 }
 
 hipError_t launch_paged_append(const PagedCacheDims& c, int hd, bool fp8, const void* k, const void* v,

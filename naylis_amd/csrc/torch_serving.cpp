@@ -35,7 +35,9 @@ at::Tensor indices(const at::Tensor& t, const at::Tensor& q, const char* who, co
   same_device(t, q, who, name);
   TORCH_CHECK(t.scalar_type() == at::kInt || t.scalar_type() == at::kLong, who, ": ", name,
               " must be int32 or int64, got ", t.scalar_type());
-  return t.to(at::kInt).contiguous();
+  // int64 beyond int32 stays out of range instead of wrapping into it
+  if (t.scalar_type() == at::kLong) return t.clamp(INT32_MIN, INT32_MAX).to(at::kInt).contiguous();
+  return t.contiguous();
 }
 
 // A (rows, heads, hd) operand as the kernels read it: whole 16-byte pieces at
@@ -197,6 +199,7 @@ void paged_append(const at::Tensor& kp, const at::Tensor& vp, const c10::optiona
   const char* who = "paged_append";
   const Cache c = cache_of(kp, vp, ks, vs, who);
   at::DeviceGuard guard(kp.device());
+  TORCH_CHECK(!wants_grad({k_in, v_in, kp, vp}), who, " has no backward: call it without gradients");
   at::NoGradGuard no_grad;
   TORCH_CHECK(k_in.dim() == 3 && v_in.sizes() == k_in.sizes() && k_in.size(1) == c.Hkv && k_in.size(2) == c.hd &&
                   k_in.scalar_type() == at::kBFloat16 && v_in.scalar_type() == at::kBFloat16,
@@ -238,12 +241,12 @@ at::Tensor paged_attention(const at::Tensor& q_in, const at::Tensor& kp, const a
               who, ": block_table must be (B, pages of a sequence) and seq_lens (B,) for the ", B, " rows of q");
   const at::Tensor q = rows_of(q_in);
   at::Tensor out = at::empty({B, H, c.hd}, q.options());
-  at::Tensor ws = workspace(
-      need(naylis_mom_paged_attn_workspace_bytes(c.dtype, B, H, c.Hkv, c.page, c.hd, table.size(1))), q);
+  const size_t bytes = naylis_mom_paged_attn_workspace_bytes(c.dtype, B, H, c.Hkv, c.page, c.hd, table.size(1));
+  const at::Tensor ws = bytes ? workspace(bytes, q) : at::Tensor();
   const int64_t strides[2] = {q.stride(0), q.stride(1)};
   check(naylis_mom_paged_attn(q.data_ptr(), kp.data_ptr(), vp.data_ptr(), c.k_scale(), c.v_scale(), c.dtype,
-                              table.data_ptr<int32_t>(), lens.data_ptr<int32_t>(), out.data_ptr(), ws.data_ptr(),
-                              ws.numel(), strides, (float)scale, B, H, c.pages, c.Hkv, c.page, c.hd, table.size(1),
+                              table.data_ptr<int32_t>(), lens.data_ptr<int32_t>(), out.data_ptr(), ptr(ws), bytes,
+                              strides, (float)scale, B, H, c.pages, c.Hkv, c.page, c.hd, table.size(1),
                               stream_ptr(st)));
   return out;
 }

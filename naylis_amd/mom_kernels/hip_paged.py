@@ -48,7 +48,8 @@ def paged_append(cache: PagedCache, k, v, block_table, positions, rows=None):
     block_table (B, W) int32: each sequence's pages in order.  Token t becomes
     token positions[t] of sequence rows[t]; without rows, of sequence t.  Tokens
     whose position, row or page is outside the table or the cache (position -1
-    for padding) are left out.  No two tokens may have the same place."""
+    for padding) are left out.  No two tokens of a call may have the same place.
+    No backward: raises where k or v want a gradient."""
     _torch_ext.load().paged_append(*cache, k, v, block_table, positions, rows,
                                    _lib.stream_of(cache.k.device) if cache.k.is_cuda else 0)
 

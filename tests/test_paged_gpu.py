@@ -120,8 +120,11 @@ def test_append_writes_its_rows_alone(fp8, hd, dev):
     rows = torch.tensor([i % 2 for i in range(T)], dtype=torch.int32, device=dev)
     pos = torch.tensor([i // 2 for i in range(T)], dtype=torch.int32, device=dev)
     pos[10], pos[11], pos[12], rows[13], rows[14] = -1, 48, 1 << 30, 2, -1
+    far = pos.long()
+    far[10] = (1 << 32) + 3  # beyond int32: out of range, not token 3
     pos[16], pos[18], pos[17] = 33, 47, 32  # row 0's last page; row 1's page 9
-    paged_append(cache, k, v, table, pos, rows)
+    far[16:19] = pos[16:19].long()
+    paged_append(cache, k, v, table, far, rows.long())
     for new, pages, old in ((k, cache.k, before[0]), (v, cache.v, before[1])):
         codes, scale = _quantized(new) if fp8 else (new, None)
         want = old.clone()
@@ -285,6 +288,8 @@ def test_paged_refusals(dev):
         paged_attention(q, cache, table, lens, scale=0.0)
     with pytest.raises(RuntimeError, match="no backward"):
         paged_attention(q.clone().requires_grad_(), cache, table, lens)
+    with pytest.raises(RuntimeError, match="no backward"):
+        paged_append(cache, c["k"][:2].clone().requires_grad_(), c["v"][:2], table, c["pos"][:2])
     k, v, pos = c["k"][:2], c["v"][:2], c["pos"][:2]
     bad = [(cache, k.float(), v.float(), table, pos), (cache, k, v[:1], table, pos), (cache, k[:, :1], v[:, :1], table, pos),
            (cache, k, v, table, pos[:1]), (cache, k, v, table, pos, pos[:1]), (cache, k, v, table[0], pos),

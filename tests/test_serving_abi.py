@@ -89,15 +89,15 @@ def _attn(lib, dtype=1, B=2, H=4, pages=8, Hkv=2, page=16, hd=64, W=3, scale=0.1
 @pytest.mark.parametrize("bad,text", [
     (dict(H=5), "query heads"), (dict(Hkv=0), "query heads"), (dict(H=0), "query heads"), (dict(page=24), "page_size"),
     (dict(hd=256), "head_dim"), (dict(scale=-1.0), "scale"), (dict(dtype=7), "dtype"), (dict(q=None), "null"),
-    (dict(ws=None), "null"), (dict(lens=None), "null"), (dict(q=ODD), "aligned"), (dict(B=1 << 20), "bad shape")])
+    (dict(W=100, ws=None), "null"), (dict(lens=None), "null"), (dict(q=ODD), "aligned"), (dict(B=1 << 20), "bad shape")])
 def test_paged_attention_refusals(lib, bad, text):
     _refused(lib, _attn(lib, **bad), text)
 
 
 def test_paged_attention_workspace(lib):
-    need = lib.naylis_mom_paged_attn_workspace_bytes(1, 2, 4, 2, 16, 64, 3)
-    assert need > 0
-    assert _attn(lib, ws_bytes=need - 1) == _lib.NAYLIS_ERR_WORKSPACE
+    need = lib.naylis_mom_paged_attn_workspace_bytes(1, 2, 4, 2, 16, 64, 100)
+    assert need > 0 and lib.naylis_mom_paged_attn_workspace_bytes(1, 2, 4, 2, 16, 64, 3) == 0
+    assert _attn(lib, W=100, ws_bytes=need - 1) == _lib.NAYLIS_ERR_WORKSPACE
     assert lib.naylis_mom_paged_attn_workspace_bytes(1, 2, 5, 2, 16, 64, 3) == 0
     assert "query heads" in lib.naylis_mom_last_error().decode()
     assert _attn(lib, B=0) == _lib.NAYLIS_OK
