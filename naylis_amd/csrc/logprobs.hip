@@ -110,6 +110,14 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return r;
 }
 
+// Logits over 2^24 either way count as 2^24, infinities stay: a row masked by the
+// type's lowest value is even, not NaN.  x log2 e - c below keeps what rounding c
+// left of the product, at most 1 for the largest x up to here and 2^102 at 2e38.
+constexpr float kMost = 16777216.f;
+__device__ __forceinline__ float tame(float x) {
+  return fabsf(x) > kMost && fabsf(x) != INFINITY ? copysignf(kMost, x) : x;
+}
+
 // Sums of a part of a row in powers of two, against a reference c (the log2 of
 // its largest e^x, rounded once: all terms of a sum use the same number, so its
 // rounding drops out): s = sum 2^z, t = sum 2^z z with z = x log2 e - c.
@@ -141,21 +149,28 @@ __device__ __forceinline__ void add_chunks(Sums& a, const uint4 (&u)[U], bool& n
       for (int e = 0; e < E; ++e) nan |= element<E>(u[i], e) != element<E>(u[i], e);
     return;
   }
-  const float c = m * kLog2e;
+  const float c = tame(m) * kLog2e;
   if (a.m == -INFINITY)
     a.c = c;
   else if (m > a.m)
     a.rescale(c);
   a.m = m;
   float s[2] = {a.s, 0.f}, t[2] = {a.t, 0.f};  // two chains
+  auto add = [&](auto cut) {
 #pragma unroll
-  for (int i = 0; i < U; ++i)
+    for (int i = 0; i < U; ++i)
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const float z = fmaf(element<E>(u[i], e), kLog2e, -a.c), p = __builtin_amdgcn_exp2f(z);
-      s[e & 1] += p;
-      t[e & 1] = fmaf(p, fmaxf(z, -1e30f), t[e & 1]);  // 0 log 0 = 0
-    }
+      for (int e = 0; e < E; ++e) {
+        const float z = fmaf(cut(element<E>(u[i], e)), kLog2e, -a.c), p = __builtin_amdgcn_exp2f(z);
+        s[e & 1] += p;
+        t[e & 1] = fmaf(p, fmaxf(z, -1e30f), t[e & 1]);  // 0 log 0 = 0
+      }
+  };
+  // beside a largest value within 2^24 a lower one weighs nothing, cut or not
+  if (__ballot(fabsf(m) > kMost) == 0)
+    add([](float x) { return x; });
+  else
+    add(tame);
   a.s = s[0] + s[1];
   a.t = t[0] + t[1];
 }
@@ -164,14 +179,15 @@ __device__ __forceinline__ void add_chunks(Sums& a, const uint4 (&u)[U], bool& n
 __device__ __forceinline__ void add_one(Sums& a, float x, bool& nan) {
   nan |= x != x;
   if (!(x > -INFINITY)) return;
+  const float y = tame(x);
   if (a.m == -INFINITY) {
     a.m = x;
-    a.c = x * kLog2e;
+    a.c = y * kLog2e;
   } else if (x > a.m) {
     a.m = x;
-    a.rescale(x * kLog2e);
+    a.rescale(y * kLog2e);
   }
-  const float z = fmaf(x, kLog2e, -a.c), p = __builtin_amdgcn_exp2f(z);
+  const float z = fmaf(y, kLog2e, -a.c), p = __builtin_amdgcn_exp2f(z);
   a.s += p;
   a.t = fmaf(p, fmaxf(z, -1e30f), a.t);
 }
@@ -188,7 +204,7 @@ __device__ __forceinline__ float logit(unsigned long long k) {
 
 // log p of a logit from its row's reference and log2 of its sum
 __device__ __forceinline__ float log_prob(float x, float c, float ls) {
-  return (fmaf(x, kLog2e, -c) - ls) * kLn2;
+  return (fmaf(tame(x), kLog2e, -c) - ls) * kLn2;
 }
 
 // Joins the sums of `count` <= 64 parts that stand in LDS; every lane gets them.
@@ -453,8 +469,11 @@ __global__ __launch_bounds__(256) void logprobs_bwd_kernel(const T* __restrict__
                    : tok >= 0 && tok < V          ? g_logp[r * gl_stride]
                                                   : __builtin_nanf("");
   const float ge = g_entropy ? g_entropy[r * ge_stride] : 0.f;
+  // beside a largest value within 2^24 a lower one weighs nothing, cut or not
+  const bool far = fabsf(ref) >= kMost * kLog2e;
   // z ln 2 = log p; 0 log 0 = 0 (the comparison keeps NaN)
   const auto grad = [&](float f, int j) {
+    if (far) f = tame(f);
     const float z = fmaf(f, kLog2e, -ref) - ls, p = __builtin_amdgcn_exp2f(z);
     return (j == tok ? gl : 0.f) - p * fmaf(ge, fmaf(z < -1e30f ? -1e30f : z, kLn2, ent), gl);
   };

@@ -137,6 +137,32 @@ def test_logprobs_ties_masks_and_nan(V, dev):
             assert abs(float(r.entropy[0]) - math.log(V)) < 1e-4  # V / 512 additions and more, each 2^-24
 
 
+@pytest.mark.parametrize("V", [1003, 70001])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+def test_logprobs_of_lowest_values(dtype, V, dev):
+    """Masks of the type's lowest value: nothing beside other logits, an even row
+    by themselves; large logits either way; gradients finite."""
+    from naylis_amd.mom_kernels import token_logprobs
+    low = torch.finfo(dtype).min
+    x = torch.full((5, V), low, dtype=dtype, device=dev)
+    x[1, 10:20] = 1.0
+    x[2] = -low
+    x[3] = -1e4
+    x[3, 5] = 1e4
+    x[4, ::2] = -math.inf
+    tok = torch.tensor([7, 12, V - 1, 5, 1], device=dev)
+    x.requires_grad_()
+    r = token_logprobs(x, tok, top=3)
+    want = [-math.log(V), -math.log(10), -math.log(V), 0.0, -math.log(V // 2)]
+    for i, w in enumerate(want):  # V / 512 + 80 fp32 additions in the sum, and log's own steps
+        bound = (V / 512 + 80) * 2.0 ** -23 + 12 * 2.0 ** -22
+        assert abs(float(r.logp[i].detach()) - w) < bound and abs(float(r.entropy[i].detach()) + w) < bound, i
+    assert r.top_ids.tolist() == [[0, 1, 2], [10, 11, 12], [0, 1, 2], [5, 0, 1], [1, 3, 5]]
+    d, = torch.autograd.grad(r.logp.sum() + r.entropy.sum(), x)
+    assert bool(d.isfinite().all()) and bool((d[1, 20:] == 0).all()) and bool((d[4, ::2] == 0).all())
+    assert abs(float(d[0, 7]) - (1 - 1 / V)) < 2.0 ** -8
+
+
 def test_logprobs_ignored_and_bad_tokens(dev):
     from naylis_amd.mom_kernels import token_logprobs
     x, _ = _rows(5, 300, torch.bfloat16, dev)
