@@ -342,7 +342,8 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void packed_fwd_kernel(
   const uint32_t ring0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)ring;  // LDS byte address
   const int keys = min(tile.lq, (tile.block + 1) * ROWS) + shift;  // seen by the tile's last query
   const int nst = (max(keys, 0) + kStageRows - 1) / kStageRows;
-  const int nt = min(max(q0 + 32 + shift + 31, 0) / 32, 2 * nst);  // key tiles that the wave's queries see
+  // key tiles that the wave's queries see (a wave behind the sequence has none)
+  const int nt = q0 < tile.lq ? min(max(q0 + 32 + shift + 31, 0) / 32, 2 * nst) : 0;
 
   f32x16 acc[NT], x;  // x: scores, then weights, of the tile at hand
   clear(acc);
@@ -541,7 +542,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void packed_bwd_dq_kernel(
 #pragma unroll
     for (int i2 = 0; i2 < 2 / SPLIT; ++i2) {
       const int sub = SPLIT == 1 ? i2 : share, kv0 = st * kStageRows + 32 * sub;
-      if (kv0 > q0 + 31 + shift) continue;
+      if (kv0 > q0 + 31 + shift || q0 >= tile.lq) continue;
       f32x16 x = f32x16{}, dp;
 #pragma unroll
       for (int i = 0; i < 16; ++i) dp[i] = md;
@@ -643,7 +644,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void packed_bwd_dkdv_kernel(
 #pragma unroll
     for (int i2 = 0; i2 < 2 / SPLIT; ++i2) {
       const int sub = SPLIT == 1 ? i2 : share, q0 = cur * kStageRows + 32 * sub;
-      if (kv0 > q0 + 31 + shift) continue;  // above the diagonal
+      if (kv0 > q0 + 31 + shift || q0 >= tile.lq || kv0 >= tile.lk) continue;  // above the diagonal, or outside
       fr.renew();
       f32x16 x, dp;
 #pragma unroll
