@@ -498,7 +498,8 @@ int naylis_mom_decode_step(const double* state_in, double* state_out, const int3
  * The backward writes dense dq, dk, dv; the gradients of a key head are summed
  * over its query heads in one fixed order in fp32.
  * Constraints: head_dim 64 or 128, H a multiple of Hkv, scale > 0, pointers
- * 16-byte aligned, strides multiples of 8, token strides under 2^23. */
+ * 16-byte aligned, strides multiples of 8, token strides and H head_dim under
+ * 2^23, 2^24 tiles of 64 rows and heads. */
 int naylis_mom_packed_attn_fwd(const void* q, const void* k, const void* v, const int32_t* cu_q, const int32_t* cu_k,
                                void* out, void* rest, float* lse, const int64_t* strides, float scale, int64_t n_seqs,
                                int64_t T, int64_t Tk, int64_t H, int64_t Hkv, int64_t head_dim, void* stream);
@@ -534,8 +535,9 @@ int naylis_mom_packed_attn_bwd(const void* q, const void* k, const void* v, cons
  * they hold.  q (B, H, head_dim) bf16, q_strides: host array, its batch and
  * head strides.
  * Constraints: head_dim 64 or 128, page_size a power of two in [16, 256], H a
- * multiple of Hkv, B <= 65535, scale > 0, pointers (tables and lengths apart)
- * 16-byte aligned, strides multiples of 8, the first of a pair under 2^23. */
+ * multiple of Hkv, Hkv ceil(H / Hkv / 16) and B <= 65535, scale > 0, pointers
+ * (tables and lengths apart) 16-byte aligned, strides multiples of 8, the first
+ * of a pair under 2^23. */
 int naylis_mom_paged_append(void* k_pages, void* v_pages, float* k_scale, float* v_scale, int cache_dtype,
                             const void* k, const void* v, const int64_t* strides, const int32_t* table,
                             const int32_t* positions, const int32_t* rows, int64_t T, int64_t pages, int64_t Hkv,
@@ -567,7 +569,7 @@ int naylis_mom_paged_attn(const void* q, const void* k_pages, const void* v_page
  * dense (N, V), in the logits' type; g_logp counts as 0 where the token is
  * ignore_index.
  * logits (N, V) in dtype (bf16 or fp32), row stride row_stride elements, any V
- * and any address that its elements allow; top <= min(64, V).  Workspace of the
+ * and any address that its elements allow; N < 2^24, top <= min(64, V).  Workspace of the
  * forward: naylis_mom_logprobs_workspace_bytes, 8-byte aligned (0 bytes for
  * many rows, or narrow ones: then it may be NULL). */
 size_t naylis_mom_logprobs_workspace_bytes(int64_t N, int64_t V, int64_t top);

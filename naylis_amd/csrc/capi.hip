@@ -1125,7 +1125,7 @@ static int check_packed(int64_t n, int64_t T, int64_t Tk, int64_t H, int64_t Hkv
     return fail(NAYLIS_ERR_ARG, "%s: head_dim %lld must be 64 or 128", who, (long long)head_dim);
   int rc = check_scale(scale, who);
   if (rc) return rc;
-  if (H > (1 << 20) || !packed_supported((long)n, (long)T, (long)Tk, (long)H, (long)Hkv))
+  if (H > (1 << 23) / head_dim || !packed_supported((long)n, (long)T, (long)Tk, (long)H, (long)Hkv))
     return fail(NAYLIS_ERR_ARG, "%s: n_seqs=%lld T=%lld Tk=%lld H=%lld is too large", who, (long long)n,
                 (long long)T, (long long)Tk, (long long)H);
   if (!cu_q || !cu_k) return fail(NAYLIS_ERR_ARG, "%s: null pointer argument", who);
@@ -1217,7 +1217,7 @@ int naylis_mom_paged_append(void* k_pages, void* v_pages, float* k_scale, float*
   const PagedCacheDims c{k_pages, v_pages, k_scale, v_scale, (int)pages, (int)Hkv, (int)page_size, (int)B, (int)W, 1};
   int rc = check_paged(pages, Hkv, page_size, B, W, 1, head_dim, cache_dtype, who);
   if (rc || (rc = check_cache(c, cache_dtype, who))) return rc;
-  if (T < 0 || T >= ((int64_t)1 << 31) || T * Hkv * 2 * (head_dim / 8) / 256 >= ((int64_t)1 << 31) - 1)
+  if (T < 0 || T >= ((int64_t)1 << 31) || T * Hkv * 2 * (head_dim / 8) >= ((int64_t)1 << 32) - 256)
     return fail(NAYLIS_ERR_ARG, "%s: bad token count %lld", who, (long long)T);
   if (!rows && T > B)
     return fail(NAYLIS_ERR_ARG, "%s: %lld tokens without rows for a table of %lld sequences", who, (long long)T,
@@ -1242,6 +1242,9 @@ static int check_paged_attn(int cache_dtype, int64_t B, int64_t H, int64_t pages
                             int64_t head_dim, int64_t W, const char* who) {
   if (Hkv < 1 || H < 1 || H % Hkv != 0)
     return fail(NAYLIS_ERR_ARG, "%s: %lld query heads for %lld key heads", who, (long long)H, (long long)Hkv);
+  if (Hkv * ((H / Hkv + 15) / 16) > 65535)  // one grid row for 16 query heads of a key head
+    return fail(NAYLIS_ERR_ARG, "%s: %lld query heads for %lld key heads are too many", who, (long long)H,
+                (long long)Hkv);
   return check_paged(pages, Hkv, page_size, B, W, H / Hkv, head_dim, cache_dtype, who);
 }
 
@@ -1281,7 +1284,7 @@ static int check_logprobs(const void* logits, int dtype, int64_t ld, const int64
                           const char* who) {
   int rc = check_dtype(dtype, who);
   if (rc) return rc;
-  if (N < 0 || N >= ((int64_t)1 << 31) || V < 1 || V > (1 << 30))
+  if (N < 0 || N >= (1 << 24) || V < 1 || V > (1 << 30))  // (a launch has under 2^32 threads)
     return fail(NAYLIS_ERR_ARG, "%s: bad shape N=%lld V=%lld", who, (long long)N, (long long)V);
   if (ld < 0) return fail(NAYLIS_ERR_ARG, "%s: row stride %lld must not be negative", who, (long long)ld);
   if (N == 0) return NAYLIS_OK;
@@ -1292,7 +1295,7 @@ static int check_logprobs(const void* logits, int dtype, int64_t ld, const int64
 }
 
 size_t naylis_mom_logprobs_workspace_bytes(int64_t N, int64_t V, int64_t top) {
-  if (N < 0 || N >= ((int64_t)1 << 31) || V < 1 || V > (1 << 30) || top < 0 || top > kLogprobsMaxTop) return 0;
+  if (N < 0 || N >= (1 << 24) || V < 1 || V > (1 << 30) || top < 0 || top > kLogprobsMaxTop) return 0;
   return logprobs_ws_bytes((long)N, (int)V, (int)top);
 }
 

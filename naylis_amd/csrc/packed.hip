@@ -717,10 +717,10 @@ __global__ __launch_bounds__(256) void packed_sum_kernel(const float* __restrict
   *reinterpret_cast<bf16x4*>((blockIdx.y ? dv : dk) + i) = o;
 }
 
-// The grid has one workgroup per (tile, head).
+// The grid has one workgroup per (tile, head), and a launch under 2^32 threads.
 bool packed_supported(long n, long T, long Tk, long H, long Hkv) {
   return n > 0 && H > 0 && Hkv > 0 && n < (1 << 20) && T < (1L << 30) && Tk < (1L << 30) &&
-         packed_tiles(T, n, 64) * H < (1L << 31) && packed_tiles(Tk, n, 64) * Hkv < (1L << 31);
+         packed_tiles(T, n, 64) * H < (1L << 24) && packed_tiles(Tk, n, 64) * Hkv < (1L << 24);
 }
 
 hipError_t launch_packed_fwd(const void* q, const void* k, const void* v, void* o, void* rest, float* lse,

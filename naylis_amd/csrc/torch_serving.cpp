@@ -40,11 +40,15 @@ at::Tensor indices(const at::Tensor& t, const at::Tensor& q, const char* who, co
   return t.contiguous();
 }
 
+// Strides of a (rows, heads, hd) operand; of a single row or head torch keeps any.
+int64_t head_stride(const at::Tensor& t) { return t.size(1) == 1 ? t.size(2) : t.stride(1); }
+int64_t row_stride(const at::Tensor& t) { return t.size(0) == 1 ? t.size(1) * t.size(2) : t.stride(0); }
+
 // A (rows, heads, hd) operand as the kernels read it: whole 16-byte pieces at
 // aligned addresses, features dense.  Anything else is copied.
 at::Tensor rows_of(const at::Tensor& t) {
-  const bool fits = t.stride(2) == 1 && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 && t.stride(0) < (1 << 23) &&
-                    (uintptr_t)t.data_ptr() % 16 == 0;
+  const bool fits = t.stride(2) == 1 && row_stride(t) % 8 == 0 && head_stride(t) % 8 == 0 &&
+                    row_stride(t) < (1 << 23) && (uintptr_t)t.data_ptr() % 16 == 0;
   if (fits) return t;
   const at::Tensor c = t.contiguous();
   return (uintptr_t)c.data_ptr() % 16 == 0 ? c : c.clone();
@@ -66,8 +70,8 @@ struct PackedSaved {
 at::Tensor packed_forward(const PackedArgs& a, PackedSaved* saved, void* st) {
   const int64_t T = a.q.size(0), Tk = a.k.size(0), H = a.q.size(1), hd = a.q.size(2);
   at::Tensor out = at::empty({T, H, hd}, a.q.options());
-  const int64_t strides[6] = {a.q.stride(0), a.q.stride(1), a.k.stride(0),
-                              a.k.stride(1), a.v.stride(0), a.v.stride(1)};
+  const int64_t strides[6] = {row_stride(a.q), head_stride(a.q), row_stride(a.k),
+                              head_stride(a.k), row_stride(a.v), head_stride(a.v)};
   if (saved) *saved = {at::empty_like(out), at::empty({H, T}, f32_like(a.q))};
   check(naylis_mom_packed_attn_fwd(a.q.data_ptr(), a.k.data_ptr(), a.v.data_ptr(), a.cu_q.data_ptr<int32_t>(),
                                    a.cu_k.data_ptr<int32_t>(), out.data_ptr(),
@@ -85,8 +89,8 @@ variable_list packed_grads(const PackedArgs& a, const at::Tensor& out, const Pac
   at::Tensor dq = at::empty({T, H, hd}, a.q.options()), dk = at::empty({Tk, Hkv, hd}, a.q.options());
   at::Tensor dv = at::empty({Tk, Hkv, hd}, a.q.options());
   at::Tensor ws = workspace(need(naylis_mom_packed_attn_bwd_workspace_bytes(a.n(), T, Tk, H, Hkv, hd)), a.q);
-  const int64_t strides[8] = {a.q.stride(0), a.q.stride(1), a.k.stride(0), a.k.stride(1),
-                              a.v.stride(0), a.v.stride(1), dout.stride(0), dout.stride(1)};
+  const int64_t strides[8] = {row_stride(a.q), head_stride(a.q), row_stride(a.k), head_stride(a.k),
+                              row_stride(a.v), head_stride(a.v), row_stride(dout), head_stride(dout)};
   check(naylis_mom_packed_attn_bwd(a.q.data_ptr(), a.k.data_ptr(), a.v.data_ptr(), a.cu_q.data_ptr<int32_t>(),
                                    a.cu_k.data_ptr<int32_t>(), out.data_ptr(), saved.rest.data_ptr(),
                                    saved.lse.data_ptr<float>(), dout.data_ptr(),
@@ -214,7 +218,7 @@ void paged_append(const at::Tensor& kp, const at::Tensor& vp, const c10::optiona
   TORCH_CHECK(pos.dim() == 1 && pos.size(0) == T && (!row.defined() || row.sizes() == pos.sizes()), who,
               ": positions and rows must hold one entry for each of the ", T, " tokens");
   const at::Tensor k = rows_of(k_in), v = rows_of(v_in);
-  const int64_t strides[4] = {k.stride(0), k.stride(1), v.stride(0), v.stride(1)};
+  const int64_t strides[4] = {row_stride(k), head_stride(k), row_stride(v), head_stride(v)};
   check(naylis_mom_paged_append(kp.data_ptr(), vp.data_ptr(), c.k_scale(), c.v_scale(), c.dtype, k.data_ptr(),
                                 v.data_ptr(), strides, table.data_ptr<int32_t>(), pos.data_ptr<int32_t>(),
                                 row.defined() ? row.data_ptr<int32_t>() : nullptr, T, c.pages, c.Hkv, c.page, c.hd,
@@ -243,7 +247,7 @@ at::Tensor paged_attention(const at::Tensor& q_in, const at::Tensor& kp, const a
   at::Tensor out = at::empty({B, H, c.hd}, q.options());
   const size_t bytes = naylis_mom_paged_attn_workspace_bytes(c.dtype, B, H, c.Hkv, c.page, c.hd, table.size(1));
   const at::Tensor ws = bytes ? workspace(bytes, q) : at::Tensor();
-  const int64_t strides[2] = {q.stride(0), q.stride(1)};
+  const int64_t strides[2] = {row_stride(q), head_stride(q)};
   check(naylis_mom_paged_attn(q.data_ptr(), kp.data_ptr(), vp.data_ptr(), c.k_scale(), c.v_scale(), c.dtype,
                               table.data_ptr<int32_t>(), lens.data_ptr<int32_t>(), out.data_ptr(), ptr(ws), bytes,
                               strides, (float)scale, B, H, c.pages, c.Hkv, c.page, c.hd, table.size(1),

@@ -219,6 +219,25 @@ def test_logprobs_views_and_shapes(dev):
     assert e.logp.shape == (0,) and e.top_ids.shape == (0, 5)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+def test_logprobs_far_rows(dtype, dev):
+    """Rows further than 2^31 elements and 2^32 bytes from the first."""
+    from naylis_amd.mom_kernels import token_logprobs
+    N, V, ld = 300, 1000, (1 << 23) - 5
+    x = torch.randn(N, V, generator=torch.Generator(device=dev).manual_seed(2), device=dev).to(dtype)
+    far = torch.as_strided(torch.empty(N * ld, dtype=dtype, device=dev), (N, V), (ld, 1)).copy_(x)
+    tok = torch.arange(N, device=dev)
+    y, z = x.requires_grad_(), far.requires_grad_()
+    a, b = token_logprobs(y, tok, top=5), token_logprobs(z, tok, top=5)
+    assert torch.equal(a.top_ids, b.top_ids)
+    for s, t in ((a.logp, b.logp), (a.entropy, b.entropy), (a.top_logp, b.top_logp)):
+        # the same values on other chunks: the sums' order differs (at most V / 256 + 16 additions)
+        assert float((s - t).detach().abs().max()) <= 2 * ((V / 256 + 16) * 2.0 ** -23 + 12 * 2.0 ** -22)
+    ga, = torch.autograd.grad(a.logp.sum(), y)
+    gb, = torch.autograd.grad(b.logp.sum(), z)
+    assert float((ga.float() - gb.float()).abs().max()) <= torch.finfo(dtype).eps + 2.0 ** -18
+
+
 def test_logprobs_graph(dev):
     from naylis_amd.mom_kernels import token_logprobs
     x, tok = _rows(8, 4099, torch.bfloat16, dev)

@@ -192,6 +192,40 @@ def test_packed_takes_views(dev):
         assert torch.equal(packed_attention(make(q), make(k), make(v), cq), want["o"])
 
 
+def test_packed_single_rows_and_heads(dev):
+    """One token, or one head, of a wider tensor whose strides are no whole
+    16-byte pieces (torch takes any stride of a single row for dense)."""
+    from naylis_amd.mom_kernels import packed_attention
+    g = torch.Generator(device=dev).manual_seed(8)
+    x = torch.randn(3, 643, generator=g, device=dev).bfloat16()
+    q, k, v = (torch.as_strided(x, (1, 2, 64), (643, 64, 1), 128 * i) for i in range(3))
+    assert q.is_contiguous() and q.stride(0) % 8 != 0
+    cu = torch.tensor([0, 1], dtype=torch.int32, device=dev)
+    assert torch.equal(packed_attention(q, k, v, cu), v)
+    y = torch.randn(5, 3, 64, generator=g, device=dev).bfloat16()
+    q, k, v = (torch.as_strided(y, (5, 1, 64), (192, 7, 1), 64 * i) for i in range(3))
+    cu = torch.tensor([0, 5], dtype=torch.int32, device=dev)
+    assert torch.equal(packed_attention(q, k, v, cu), packed_attention(*(t.clone() for t in (q, k, v)), cu))
+
+
+def test_packed_far_rows(dev):
+    """Rows and heads further than 2^32 bytes from the tensor's start."""
+    T, ld = 290, (1 << 23) - 8
+    q, k, v, d, cq, ck = _inputs([T], None, 4, 2, 64, 0, 0, dev)
+    want = _run(q, k, v, d, cq, ck, 0.125)
+    room = torch.empty(T * ld + 64, dtype=torch.bfloat16, device=dev)
+    far = [torch.as_strided(room, t.shape, (ld, 1 << 20, 1), at) for t, at in ((q, 0), (k, 64), (v, 128), (d, 192))]
+    for f, t in zip(far, (q, k, v, d)):
+        f.copy_(t)
+    got = _run(*far, cq, ck, 0.125)
+    assert all(torch.equal(got[n], want[n]) for n in got)
+    step = room.numel() // 4 // 192 * 192
+    for i, t in enumerate((q, k, v)):  # heads outermost
+        far[i] = torch.as_strided(room, t.shape, (192, 4 // t.size(1) * step, 1), 64 * i).copy_(t)
+    got = _run(*far[:3], d, cq, ck, 0.125)
+    assert all(torch.equal(got[n], want[n]) for n in got)
+
+
 def test_packed_empty_tensors(dev):
     from naylis_amd.mom_kernels import packed_attention
     z = lambda n, h: torch.zeros(n, h, 64, dtype=torch.bfloat16, device=dev, requires_grad=True)  # noqa: E731

@@ -257,6 +257,18 @@ def test_paged_views_streams_and_graph(dev):
             assert torch.equal(cache.k[table[b, n // 16], :, n % 16], held["k"][b])
 
 
+def test_paged_single_sequence_of_odd_rows(dev):
+    """One sequence's q, k, v out of a tensor whose rows are no whole 16-byte pieces."""
+    from naylis_amd.mom_kernels import new_paged_cache, paged_append, paged_attention
+    x = torch.randn(2, 389, generator=torch.Generator(device=dev).manual_seed(4), device=dev).bfloat16()
+    q, k, v = (torch.as_strided(x, (1, 2, 64), (389, 64, 1), 128 * i) for i in range(3))
+    cache = new_paged_cache(1, 2, 16, 64, dev)
+    table = torch.zeros(1, 1, dtype=torch.int32, device=dev)
+    paged_append(cache, k, v, table, torch.zeros(1, dtype=torch.int32, device=dev))
+    assert torch.equal(cache.k[0, :, 0], k[0]) and torch.equal(cache.v[0, :, 0], v[0])
+    assert torch.equal(paged_attention(q, cache, table, torch.ones(1, dtype=torch.int32, device=dev)), v)
+
+
 def test_paged_append_marks_the_cache_written(dev):
     """A graph that saved the cache notices the write."""
     from naylis_amd.mom_kernels import paged_append

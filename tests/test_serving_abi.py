@@ -42,7 +42,9 @@ def _packed(lib, n=1, T=10, Tk=10, H=4, Hkv=2, hd=64, scale=0.1, q=P, cu=P, stri
     (dict(T=1 << 30), "too large"), (dict(n=1 << 20), "too large"), (dict(q=None), "null"), (dict(cu=None), "null"),
     (dict(q=ODD), "aligned"), (dict(strides=(260, 64, 128, 64, 128, 64, 256, 64)), "strides"),
     (dict(strides=(256, 64, 128, 64, -128, 64, 256, 64)), "strides"),
-    (dict(strides=(1 << 23, 64, 128, 64, 128, 64, 256, 64)), "strides")])
+    (dict(strides=(1 << 23, 64, 128, 64, 128, 64, 256, 64)), "strides"),
+    # rows of the output over 2^23 features; more tiles than a launch has workgroups
+    (dict(H=1 << 18, Hkv=1 << 10), "too large"), (dict(T=1 << 29, H=4, Hkv=4), "too large")])
 def test_packed_refusals(lib, bad, text):
     _refused(lib, _packed(lib, **bad), text)
 
@@ -72,7 +74,8 @@ def _append(lib, dtype=1, T=4, pages=8, Hkv=2, page=16, hd=64, B=4, W=3, scale=P
     (dict(page=48), "page_size"), (dict(page=512), "page_size"), (dict(hd=32), "head_dim"), (dict(pages=0), "bad shape"),
     (dict(Hkv=0), "bad shape"), (dict(W=0), "bad shape"), (dict(B=70000), "bad shape"), (dict(W=1 << 28), "bad shape"),
     (dict(T=5), "without rows"), (dict(T=-1), "token count"), (dict(k=None), "null"), (dict(table=None), "null"),
-    (dict(k=ODD), "aligned"), (dict(strides=(4, 64, 128, 64)), "strides")])
+    (dict(k=ODD), "aligned"), (dict(strides=(4, 64, 128, 64)), "strides"),
+    (dict(T=1 << 28, rows=P), "token count")])
 def test_append_refusals(lib, bad, text):
     _refused(lib, _append(lib, **bad), text)
 
@@ -89,7 +92,8 @@ def _attn(lib, dtype=1, B=2, H=4, pages=8, Hkv=2, page=16, hd=64, W=3, scale=0.1
 @pytest.mark.parametrize("bad,text", [
     (dict(H=5), "query heads"), (dict(Hkv=0), "query heads"), (dict(H=0), "query heads"), (dict(page=24), "page_size"),
     (dict(hd=256), "head_dim"), (dict(scale=-1.0), "scale"), (dict(dtype=7), "dtype"), (dict(q=None), "null"),
-    (dict(W=100, ws=None), "null"), (dict(lens=None), "null"), (dict(q=ODD), "aligned"), (dict(B=1 << 20), "bad shape")])
+    (dict(W=100, ws=None), "null"), (dict(lens=None), "null"), (dict(q=ODD), "aligned"), (dict(B=1 << 20), "bad shape"),
+    (dict(H=4096 * 257, Hkv=4096), "too many")])
 def test_paged_attention_refusals(lib, bad, text):
     _refused(lib, _attn(lib, **bad), text)
 
@@ -108,7 +112,7 @@ def _logprobs(lib, dtype=1, ld=100, N=3, V=100, top=0, x=P, tok=P, ids=P, ws=P, 
 
 
 @pytest.mark.parametrize("bad,text", [
-    (dict(dtype=2), "dtype"), (dict(N=-1), "bad shape"), (dict(V=0), "bad shape"), (dict(ld=-1), "row stride"),
+    (dict(dtype=2), "dtype"), (dict(N=-1), "bad shape"), (dict(N=1 << 24), "bad shape"), (dict(V=0), "bad shape"), (dict(ld=-1), "row stride"),
     (dict(top=-1), "top"), (dict(top=65), "top"), (dict(V=10, top=11), "top"), (dict(x=None), "null"),
     (dict(tok=None), "null"), (dict(top=1, ids=None), "null"), (dict(x=ctypes.c_void_p(4097)), "aligned"),
     (dict(dtype=0, x=ODD), "aligned"), (dict(V=70000, ld=70000, ws=None), "workspace"), (dict(V=70000, ws=ODD), "workspace")])
