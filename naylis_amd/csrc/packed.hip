@@ -28,6 +28,10 @@ namespace naylis {
 namespace {
 
 constexpr int kStageRows = 64;
+// The forward's reference stays until a score (log2 domain) passes it by more:
+// weights reach 2^8, which costs fp32 sums and bf16 weights nothing, and few
+// tiles rescale the sums (of 32 queries one has a new maximum in most tiles).
+constexpr float kSlack = 8.f;
 
 // LDS rows of HD bf16 without padding; 16-byte chunk c of row r sits in slot
 // c ^ swz(r).  16 consecutive rows' chunk c then cover 256 bytes (row
@@ -348,7 +352,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void packed_fwd_kernel(
   f32x16 acc[NT], x;  // x: scores, then weights, of the tile at hand
   clear(acc);
   float m = kNegBig, l = 0.f;
-  // mask of tile t, its maximum, and the sums rescaled where that is a new one
+  // mask of tile t, its maximum, and the sums rescaled where that is far above the reference
   auto settle = [&](f32x16& z, int t) {
     if (32 * t + 31 > q0 + shift) {
       asm volatile("");  // a branch, not 16 selects for every tile
@@ -356,10 +360,11 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void packed_fwd_kernel(
       for (int i = 0; i < 16; ++i)
         if (32 * t + acc_row(g, i) > row + shift) z[i] = -INFINITY;
     }
-    const float mx = max_of(fmaxf(z[0], z[1]), z) * c;
-    if (__builtin_expect(__any(mx > m), 0)) {
+    const float over = fmaf(max_of(fmaxf(z[0], z[1]), z), c, -kSlack);
+    if (__builtin_expect(__any(over > m), 0)) {
       // per query, so that a row's result does not depend on its neighbours'
-      const float mn = fmaxf(m, xor32_f32(mx, [](float a, float b) { return fmaxf(a, b); }));
+      const float most = xor32_f32(over, [](float a, float b) { return fmaxf(a, b); });
+      const float mn = most > m ? most + kSlack : m;
       const float al = __builtin_amdgcn_exp2f(m - mn);
       m = mn;
       l *= al;

@@ -148,6 +148,19 @@ def test_packed_sequences_do_not_see_each_other(dev):
     assert bool((a["o"][:5] == 0).all() and (a["dk"][ck[3]:] == 0).all() and (a["dv"][:ck[0]] == 0).all())
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("top", [4.0, 30.0])
+def test_packed_rising_scores(top, hd, dev):
+    """Scores that grow or fall along the keys by a little or a lot a tile."""
+    q, k, v, d, cq, ck = _inputs([300, 300], [420, 420], 4, 2, hd, 0, 0, dev)
+    one = torch.ones(hd, device=dev)
+    ramp = torch.linspace(0, top, 420, device=dev)
+    k = (k.float() * 0.1 + torch.cat([ramp, ramp.flip(0)])[:, None, None] * one / hd ** 0.5).bfloat16()
+    q = (q.float() * 0.1 + one).bfloat16()
+    x = (q, k, v, d, cq, ck)
+    _check(_run(*x, 0.7), _reference(*x, 0.7))
+
+
 def test_packed_is_causal(dev):
     x = _inputs([333], [400], 4, 4, 64, 0, 0, dev)
     y = [t.clone() for t in x]
