@@ -544,22 +544,30 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedCacheDims c, const
     __syncthreads();
     return x;
   };
+  // all that most sequences have is under way at once: a partial a group of
+  // threads, a (maximum, sum) or two a thread
+  const int gi = tid / TR, f = tid % TR;
+  const auto piece = [&](int i) { return *reinterpret_cast<const f32x4*>(part + row(i) * HD + 4 * f); };
+  const f32x4 mine = piece(min(gi, count - 1));
+  float2 st[kPagedMaxWgs / 256];
   float m = kNegBig, l = 0.f;
-  for (int i = tid; i < count; i += 256) {
-    weight[i] = stat[row(i)].x;
-    m = fmaxf(m, weight[i]);
+#pragma unroll
+  for (int u = 0; u < kPagedMaxWgs / 256; ++u) {
+    const int i = tid + 256 * u;
+    st[u] = i < count ? stat[row(i)] : float2{kNegBig, 0.f};
+    m = fmaxf(m, st[u].x);
   }
   m = block(m, [](float a, float b) { return fmaxf(a, b); });
-  for (int i = tid; i < count; i += 256) {
-    weight[i] = __builtin_amdgcn_exp2f(weight[i] - m);
-    l += weight[i] * stat[row(i)].y;
+#pragma unroll
+  for (int u = 0; u < kPagedMaxWgs / 256; ++u) {
+    const float w = __builtin_amdgcn_exp2f(st[u].x - m);
+    weight[tid + 256 * u] = w;
+    l += w * st[u].y;
   }
   l = block(l, [](float a, float b) { return a + b; });  // (its barriers are the weights' too)
-  f32x4 a = f32x4{};
-  const int gi = tid / TR, f = tid % TR;
+  f32x4 a = gi < count ? mine * weight[gi] : f32x4{};
 #pragma unroll 4
-  for (int i = gi; i < count; i += NG)
-    a += *reinterpret_cast<const f32x4*>(part + row(i) * HD + 4 * f) * weight[i];
+  for (int i = gi + NG; i < count; i += NG) a += piece(i) * weight[i];
   sums[gi][f] = a;
   __syncthreads();
   if (gi) return;
