@@ -5,6 +5,8 @@
 // for one token costs little more than its host time.
 #include "torch_common.h"
 
+#include <cmath>
+
 namespace naylis_ext {
 
 using torch::autograd::AutogradContext;
@@ -39,6 +41,12 @@ at::Tensor indices(const at::Tensor& t, const at::Tensor& q, const char* who, co
   if (t.scalar_type() == at::kLong) return t.clamp(INT32_MIN, INT32_MAX).to(at::kInt).contiguous();
   return t.contiguous();
 }
+
+// Stream of a call: 0 is the current one, looked up here because that costs the
+// caller in Python a tenth of a call for one token.
+void* stream_of(int64_t st, const at::Tensor& t) { return st ? stream_ptr(st) : current_stream(t); }
+
+double scale_of(const c10::optional<double>& scale, int64_t hd) { return scale ? *scale : 1.0 / std::sqrt((double)hd); }
 
 // Strides of a (rows, heads, hd) operand; of a single row or head torch keeps any.
 int64_t head_stride(const at::Tensor& t) { return t.size(1) == 1 ? t.size(2) : t.stride(1); }
@@ -134,7 +142,7 @@ struct PackedAttention : public Function<PackedAttention> {
 };
 
 at::Tensor packed_attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& cu_q,
-                            const at::Tensor& cu_k, double scale, int64_t st) {
+                            const at::Tensor& cu_k, c10::optional<double> scale_in, int64_t stream) {
   const char* who = "packed_attention";
   on_gpu(q, who, "q");
   at::DeviceGuard guard(q.device());
@@ -151,9 +159,11 @@ at::Tensor packed_attention(const at::Tensor& q, const at::Tensor& k, const at::
   const at::Tensor ck = cu_k.is_same(cu_q) ? cq : indices(cu_k, q, who, "cu_seqlens_k");
   TORCH_CHECK(cq.dim() == 1 && cq.size(0) >= 2 && ck.sizes() == cq.sizes(), who,
               ": cu_seqlens and cu_seqlens_k must hold n + 1 offsets of the same n >= 1 sequences");
-  if (wants_grad({q, k, v})) return PackedAttention::apply(q, k, v, cq, ck, scale, st);
+  const double scale = scale_of(scale_in, q.size(2));
+  void* st = stream_of(stream, q);
+  if (wants_grad({q, k, v})) return PackedAttention::apply(q, k, v, cq, ck, scale, reinterpret_cast<int64_t>(st));
   at::NoGradGuard no_grad;
-  return packed_forward({rows_of(q), rows_of(k), rows_of(v), cq, ck, scale}, nullptr, stream_ptr(st));
+  return packed_forward({rows_of(q), rows_of(k), rows_of(v), cq, ck, scale}, nullptr, st);
 }
 
 // ---- paged cache ----------------------------------------------------------------
@@ -222,13 +232,14 @@ void paged_append(const at::Tensor& kp, const at::Tensor& vp, const c10::optiona
   check(naylis_mom_paged_append(kp.data_ptr(), vp.data_ptr(), c.k_scale(), c.v_scale(), c.dtype, k.data_ptr(),
                                 v.data_ptr(), strides, table.data_ptr<int32_t>(), pos.data_ptr<int32_t>(),
                                 row.defined() ? row.data_ptr<int32_t>() : nullptr, T, c.pages, c.Hkv, c.page, c.hd,
-                                table.size(0), table.size(1), stream_ptr(st)));
+                                table.size(0), table.size(1), stream_of(st, kp)));
   for (const at::Tensor& t : {c.k, c.v, c.ks, c.vs}) written(t);
 }
 
 at::Tensor paged_attention(const at::Tensor& q_in, const at::Tensor& kp, const at::Tensor& vp,
                            const c10::optional<at::Tensor>& ks, const c10::optional<at::Tensor>& vs,
-                           const at::Tensor& table_in, const at::Tensor& lens_in, double scale, int64_t st) {
+                           const at::Tensor& table_in, const at::Tensor& lens_in, c10::optional<double> scale,
+                           int64_t st) {
   const char* who = "paged_attention";
   const Cache c = cache_of(kp, vp, ks, vs, who);
   at::DeviceGuard guard(kp.device());
@@ -250,8 +261,8 @@ at::Tensor paged_attention(const at::Tensor& q_in, const at::Tensor& kp, const a
   const int64_t strides[2] = {row_stride(q), head_stride(q)};
   check(naylis_mom_paged_attn(q.data_ptr(), kp.data_ptr(), vp.data_ptr(), c.k_scale(), c.v_scale(), c.dtype,
                               table.data_ptr<int32_t>(), lens.data_ptr<int32_t>(), out.data_ptr(), ptr(ws), bytes,
-                              strides, (float)scale, B, H, c.pages, c.Hkv, c.page, c.hd, table.size(1),
-                              stream_ptr(st)));
+                              strides, (float)scale_of(scale, c.hd), B, H, c.pages, c.Hkv, c.page, c.hd,
+                              table.size(1), stream_of(st, kp)));
   return out;
 }
 
@@ -338,7 +349,7 @@ struct Logprobs : public Function<Logprobs> {
 };
 
 variable_list token_logprobs(const at::Tensor& logits, const at::Tensor& tokens_in, int64_t top, int64_t ignore_index,
-                             int64_t st) {
+                             int64_t stream) {
   const char* who = "token_logprobs";
   on_gpu(logits, who, "logits");
   at::DeviceGuard guard(logits.device());
@@ -352,12 +363,13 @@ variable_list token_logprobs(const at::Tensor& logits, const at::Tensor& tokens_
               ": tokens must be int64 or int32");
   const at::Tensor tokens = tokens_in.reshape({-1}).to(at::kLong).contiguous();
   const at::Tensor x = logit_rows(logits);  // part of the graph where it copies
+  void* st = stream_of(stream, logits);
   variable_list out;
   if (wants_grad({logits})) {
-    out = Logprobs::apply(x, tokens, top, ignore_index, st);
+    out = Logprobs::apply(x, tokens, top, ignore_index, reinterpret_cast<int64_t>(st));
   } else {
     at::NoGradGuard no_grad;
-    out = logprobs_forward(x, tokens, top, ignore_index, nullptr, stream_ptr(st));
+    out = logprobs_forward(x, tokens, top, ignore_index, nullptr, st);
   }
   if (logits.dim() == 2) return out;
   std::vector<int64_t> lead = tokens_in.sizes().vec(), tops = lead;

@@ -8,7 +8,7 @@ pass or a packed training batch has them, with grouped heads, heads of 64 or
 """
 from __future__ import annotations
 
-from .. import _lib, _torch_ext
+from .. import _torch_ext
 
 
 def packed_attention(q, k, v, cu_seqlens, cu_seqlens_k=None, scale=None):
@@ -27,6 +27,5 @@ def packed_attention(q, k, v, cu_seqlens, cu_seqlens_k=None, scale=None):
     in a row of v reaches queries up to 31 rows before it too.  A forward with
     gradients keeps, beside its inputs and the output, what the output's rounding
     left (as much again) and (H, T) fp32.  The derivative of the backward raises."""
-    return _torch_ext.load().packed_attention(
-        q, k, v, cu_seqlens, cu_seqlens if cu_seqlens_k is None else cu_seqlens_k,
-        q.shape[-1] ** -0.5 if scale is None else float(scale), _lib.stream_of(q.device) if q.is_cuda else 0)
+    return _torch_ext.load().packed_attention(q, k, v, cu_seqlens,
+                                              cu_seqlens if cu_seqlens_k is None else cu_seqlens_k, scale, 0)

@@ -13,7 +13,7 @@ from typing import NamedTuple, Optional
 
 import torch
 
-from .. import _lib, _torch_ext
+from .. import _torch_ext
 
 
 class PagedCache(NamedTuple):
@@ -50,8 +50,9 @@ def paged_append(cache: PagedCache, k, v, block_table, positions, rows=None):
     whose position, row or page is outside the table or the cache (position -1
     for padding) are left out.  No two tokens of a call may have the same place.
     No backward: raises where k or v want a gradient."""
-    _torch_ext.load().paged_append(*cache, k, v, block_table, positions, rows,
-                                   _lib.stream_of(cache.k.device) if cache.k.is_cuda else 0)
+    if torch._C._get_tracing_state() is not None:
+        raise RuntimeError("paged_append writes in place, which torch.jit.trace does not record")
+    _torch_ext.load().paged_append(*cache, k, v, block_table, positions, rows, 0)
 
 
 def paged_attention(q, cache: PagedCache, block_table, seq_lens, scale=None):
@@ -62,6 +63,4 @@ def paged_attention(q, cache: PagedCache, block_table, seq_lens, scale=None):
     q k^T) v over the first seq_lens[b] tokens of sequence b (append the new
     token first), zeros for length 0, NaN for a length past the table's row or a
     page outside the cache.  scale defaults to head_dim ** -0.5.  No backward."""
-    return _torch_ext.load().paged_attention(
-        q, *cache, block_table, seq_lens, q.shape[-1] ** -0.5 if scale is None else float(scale),
-        _lib.stream_of(q.device) if q.is_cuda else 0)
+    return _torch_ext.load().paged_attention(q, *cache, block_table, seq_lens, scale, 0)

@@ -121,3 +121,28 @@ def test_policy_gradient_matches_fp64(dev):
     for n, a, b in zip(names, got, want):
         # about eight bf16 roundings (2^-8 each) lie between the loss and a weight
         assert float((a.double() - b).norm() / b.norm()) < 8 * 2.0 ** -8, n
+
+
+def test_operators_under_trace(dev):
+    """Traced calls run again on new inputs; the append, whose result is what it
+    writes, refuses to be traced."""
+    from naylis_amd import mom_kernels as mk
+    g = torch.Generator(device=dev).manual_seed(6)
+    rand = lambda *s: torch.randn(*s, generator=g, device=dev).bfloat16()  # noqa: E731
+    cu, tok = torch.tensor([0, 5, 20], dtype=torch.int32, device=dev), torch.arange(4, device=dev)
+    cache = mk.new_paged_cache(4, 2, 16, 64, dev, fp8=True)
+    table = torch.arange(4, dtype=torch.int32, device=dev).view(2, 2)
+    lens = torch.tensor([20, 3], dtype=torch.int32, device=dev)
+    for row in range(2):
+        mk.paged_append(cache, rand(32, 2, 64), rand(32, 2, 64), table, torch.arange(32, device=dev),
+                        torch.full((32,), row, device=dev))
+    calls = [(lambda q, k, v: mk.packed_attention(q, k, v, cu), lambda: (rand(20, 4, 64), rand(20, 2, 64), rand(20, 2, 64))),
+             (lambda x: tuple(mk.token_logprobs(x, tok, top=3)), lambda: (rand(4, 100),)),
+             (lambda q: mk.paged_attention(q, cache, table, lens), lambda: (rand(2, 4, 64),))]
+    for call, inputs in calls:
+        traced, x = torch.jit.trace(call, inputs(), check_trace=False), inputs()
+        got, want = traced(*x), call(*x)
+        pairs = zip(got, want) if isinstance(want, tuple) else [(got, want)]
+        assert all(torch.equal(a, b) for a, b in pairs)
+    with pytest.raises(RuntimeError, match="in place"):
+        torch.jit.trace(lambda k: mk.paged_append(cache, k, k, table, lens), (rand(2, 2, 64),))
