@@ -15,6 +15,15 @@
 // shared heads' gradients are summed in one workgroup in a fixed order, in
 // fp32, with no atomics.  Probabilities and dS enter their products as bf16
 // (at most half a step, 2^-9 of a value's binade); all sums are fp32.
+//
+// Bound by power and by the softmax's vector work beside the matrix units.  Over
+// 16k tokens, with the products that each gradient kernel forms again counted, the
+// forward runs at 1.07 PFLOP/s with 16 heads of 128 (a large matrix product at 1.14
+// for as long) and 0.94 of 64, dQ at 1.24 and 1.0, dK/dV at 1.05 and 1.0; on tensors
+// of zeros, which take less power, all at 1.2 to 1.6.  Nine sequences of 48 .. 3885
+// tokens, 16 heads of 64: 107 us forward, 423 with the gradients; four of 499 .. 4093,
+// 32 / 8 heads of 128: 213 and 960.  The first loads of a tile and the last tiles'
+// tail are a quarter of such batches.
 #include "common.h"
 #include "launch.h"
 #include "packed_tiles.h"
@@ -319,8 +328,9 @@ struct Head {
 // stage further ahead than V, each into the buffer that the barrier before has
 // freed: barrier 1 of a stage stands after the last use of its K, barrier 2
 // after that of its V.
-// SPLIT 2, for grids that leave CUs idle: 64 queries, each 32 of them with two waves, which take the even and the odd key tiles (one of each stage, so
-// that one barrier a stage does) and join their sums at the end.
+// SPLIT 2, for grids that leave CUs idle: 64 queries, each 32 of them with two
+// waves, which take the even and the odd key tiles (one of each stage, so that one
+// barrier a stage does) and join their sums at the end.
 template <int HD, int SPLIT>
 __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void packed_fwd_kernel(
     const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, const bf16_t* __restrict__ v, bf16_t* __restrict__ o,
@@ -378,9 +388,9 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void packed_fwd_kernel(
     x[i] = __builtin_amdgcn_exp2f(fmaf(x[i], c, -m));
     l += x[i];
   };
-  // Tile t (the first or second of its stage) with its scores in x; leaves
-  // those of the wave's next one, t + SPLIT, there.  The lanes' LDS offsets move to the other buffer a
-  // stage at a time, so that tiles differ by constants.
+  // Tile t (the first or second of its stage) with its scores in x; leaves those of
+  // the wave's next one, t + SPLIT, there.  The lanes' LDS offsets move to the other
+  // buffer a stage at a time, so that tiles differ by constants.
   auto step = [&](auto second, int t) {
     constexpr int HALF = 32 * 2 * HD, SECOND = decltype(second)::value;
     const uint8_t* vb = ring + SECOND * HALF;
@@ -493,7 +503,8 @@ template <int HD, int SPLIT>
 __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void packed_bwd_dq_kernel(
     const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, const bf16_t* __restrict__ v,
     const bf16_t* __restrict__ o, const bf16_t* __restrict__ rest, const float* __restrict__ lse,
-    const bf16_t* __restrict__ dout, bf16_t* __restrict__ dq, float* __restrict__ stats, PackedSeqs s, PackedHeads d, float scale) {
+    const bf16_t* __restrict__ dout, bf16_t* __restrict__ dq, float* __restrict__ stats, PackedSeqs s, PackedHeads d,
+    float scale) {
   constexpr int NT = HD / 32, STAGE = kStageRows * 2 * HD, ROWS = kTileRows / SPLIT;
   __shared__ __align__(1024) uint8_t ring[4 * STAGE];  // K even, K odd, V even, V odd
   const PackedTile tile = find_tile<false, ROWS>(s, blockIdx.x / d.H);
@@ -582,9 +593,11 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void packed_bwd_dq_kernel(
 }
 
 // dK, dV: waves of 32 keys, whose K and V rows stay in registers; for each query
-// head of the group, the queries from the diagonal to the end pass through LDS with their -lse / c and -delta, which start the accumulators of
-// S and dP.  Queries past the sequence are zeros throughout: their P is 1, their
-// dO and dS 0.
+// head of the group, the queries from the diagonal to the end pass through LDS with
+// their -lse / c and -delta, which start the accumulators of S and dP.  Queries past
+// the sequence are zeros throughout: their P is 1, their dO and dS 0.  Eight waves
+// on stages of 128 queries take longer than two workgroups of four (472 -> 510 us
+// for four sequences of 499 .. 4093, 32 / 8 heads of 128).
 // parts > 1, for grids that leave CUs idle: a workgroup walks a part of the
 // group's heads and leaves fp32 sums (parts, Tk, Hkv, HD) for packed_sum_kernel.
 template <int HD, int KB>
@@ -728,6 +741,16 @@ bool packed_supported(long n, long T, long Tk, long H, long Hkv) {
          packed_tiles(T, n, 64) * H < (1L << 24) && packed_tiles(Tk, n, 64) * Hkv < (1L << 24);
 }
 
+// Two waves for 32 queries where the grid is under three quarters of the
+// workgroups that run at once (two a CU with heads of 128, three of 64).
+// Forward / dQ, us: 4000 queries of 8 heads of 128 92 -> 75 / 102 -> 78, 500 17 -> 14
+// / 20 -> 17, of 16 heads of 64 75 -> 56 / 72 -> 65; beyond it 10 x 500 queries of 8
+// heads of 128 20 -> 25 / 23 -> 33, 4000 of 32 150 -> 189 / 197 -> 220, of 24 heads
+// of 64 82 -> 87 / 88 -> 93.
+static bool packed_split(const PackedSeqs& s, const PackedHeads& d, int hd) {
+  return packed_tiles(s.T, s.n) * d.H < (hd == 64 ? 576 : 384);
+}
+
 hipError_t launch_packed_fwd(const void* q, const void* k, const void* v, void* o, void* rest, float* lse,
                              const PackedSeqs& s, const PackedHeads& d, int hd, float scale, hipStream_t st) {
   auto run = [&](auto kernel, int rows) {
@@ -737,10 +760,7 @@ hipError_t launch_packed_fwd(const void* q, const void* k, const void* v, void* 
                                     lse, s, d, scale * kLog2e));
     return hipGetLastError();
   };
-  // under one and a half tiles a CU: 4000 queries of 8 heads of 128 (272 tiles)
-  // 95 -> 73 us, 2000 52 -> 39, 500 18 -> 15; from two a CU on level or slower
-  // (4000 queries of 16 heads 106 -> 112, of 32 171 -> 199)
-  const bool split = packed_tiles(s.T, s.n) * d.H < 384;
+  const bool split = packed_split(s, d, hd);
   if (hd == 64) return split ? run(packed_fwd_kernel<64, 2>, 64) : run(packed_fwd_kernel<64, 1>, 128);
   return split ? run(packed_fwd_kernel<128, 2>, 64) : run(packed_fwd_kernel<128, 1>, 128);
 }
@@ -792,8 +812,7 @@ hipError_t launch_packed_bwd(const void* q, const void* k, const void* v, const 
     return hipGetLastError();
   };
   if (s.T > 0) {
-    // as in the forward: 4000 queries of 8 heads of 128 100 -> 77 us, of 16 (level)
-    const bool split = packed_tiles(s.T, s.n) * d.H < 384;
+    const bool split = packed_split(s, d, hd);
     const hipError_t e = hd == 64 ? (split ? run_dq(packed_bwd_dq_kernel<64, 2>, 64)
                                            : run_dq(packed_bwd_dq_kernel<64, 1>, 128))
                                   : (split ? run_dq(packed_bwd_dq_kernel<128, 2>, 64)

@@ -1,8 +1,8 @@
 // Which tile of which packed sequence a workgroup takes (packed attention).
 //
 // Sequences are given by their offsets alone, which are on the device, so the
-// grid has the most tiles that T rows in n sequences can have, and each wave
-// finds its workgroup's tile from the offsets: no plan to build, nothing to
+// grid has the most tiles that T rows in n sequences can have, and a workgroup's
+// first wave finds its tile from the offsets: no plan to build, nothing to
 // copy, no extra launch.  Tiles are ranked by their work, in levels of 128
 // rows of the other operand, longest first: F(x) = number of tiles with more
 // than x rows is a sum over the sequences (one wave reduction), so a binary

@@ -11,10 +11,10 @@
 //
 // Work is dealt in steps of 32 tokens: each slice's (key head's) steps of all
 // sequences form one list, cut into equal ranges for its workgroups and those
-// into quarters for their waves, so a long sequence among short ones keeps no
+// into four for their waves, so a long sequence among short ones keeps no
 // wave waiting.  The waves of a workgroup join what they hold of one sequence
-// in LDS; what several workgroups hold of it goes to a second kernel as (max,
-// sum, o) partials.  Lengths stay on the device: each wave finds its range's
+// in LDS, all of it read at once; what several workgroups hold of it goes to a
+// second kernel as (max, sum, o) partials.  Lengths stay on the device: each wave finds its range's
 // first sequence by a scan over them.
 //
 // Per step a wave forms S^T = K Q^T (v_mfma_f32_16x16x32_bf16: 16 tokens x up
@@ -26,8 +26,9 @@
 // needed.  Loads bypass the caches: 64 sequences of up to 4096 tokens, 8 key
 // heads of 128, 588 MB: 113 -> 103 us (5.7 TB/s; the kernel 97 us, the join and
 // its launch 6).  Three contexts of 65537 .. 131072 tokens, e4m3, 747 MB: 151 ->
-// 124 us (6.0 TB/s); in steps of 64 tokens 134 us (256 registers).  One sequence of
-// 500 tokens, 16 heads of 64: 7.9 us, of which 5 are launch and dependent loads.
+// 122 us (6.1 TB/s); in steps of 64 tokens 134 us (256 registers).  One sequence of
+// 500 tokens, 16 heads of 64: 7.0 us, a chain of dependent loads (length, page,
+// rows) that fill nothing.
 #include "common.h"
 #include "launch.h"
 #include "packed_tiles.h"
@@ -41,7 +42,7 @@ namespace naylis {
 namespace {
 
 constexpr int kRowsMfma = 16;       // query heads of a product
-constexpr int kPagedStep = 32;         // tokens of a step
+constexpr int kPagedStep = 32;      // tokens of a step
 constexpr int kPagedMaxWgs = 512;   // workgroups that share a slice's steps
 
 __device__ __forceinline__ f32x4 mfma16(const bf16x8& a, const bf16x8& b, const f32x4& c) {
