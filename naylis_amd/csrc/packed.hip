@@ -16,14 +16,14 @@
 // fp32, with no atomics.  Probabilities and dS enter their products as bf16
 // (at most half a step, 2^-9 of a value's binade); all sums are fp32.
 //
-// Bound by power and by the softmax's vector work beside the matrix units.  Over
+// Bound by power, then by the softmax's vector work beside the matrix units.  Over
 // 16k tokens, with the products that each gradient kernel forms again counted, the
 // forward runs at 1.07 PFLOP/s with 16 heads of 128 (a large matrix product at 1.14
-// for as long) and 0.94 of 64, dQ at 1.24 and 1.0, dK/dV at 1.05 and 1.0; on tensors
-// of zeros, which take less power, all at 1.2 to 1.6.  Nine sequences of 48 .. 3885
-// tokens, 16 heads of 64: 107 us forward, 423 with the gradients; four of 499 .. 4093,
-// 32 / 8 heads of 128: 213 and 960.  The first loads of a tile and the last tiles'
-// tail are a quarter of such batches.
+// for as long) and 0.93 of 64, dQ at 1.20 and 0.98, dK/dV at 1.13 and 0.97; on tensors
+// of zeros, which take less power, at 1.4 and 1.2, 1.7 and 1.5, 1.5 and 1.45.  Nine
+// sequences of 48 .. 3885 tokens, 16 heads of 64: 107 us forward, 428 with the
+// gradients; four of 499 .. 4093, 32 / 8 heads of 128: 209 and 920.  The first loads of
+// a tile and the last tiles' tail are a quarter of such batches.
 #include "common.h"
 #include "launch.h"
 #include "packed_tiles.h"
@@ -234,6 +234,38 @@ __device__ __forceinline__ void load_rows(bf16x8 (&f)[HD / 16], __amdgpu_buffer_
     f[ks] = __builtin_bit_cast(bf16x8, __builtin_amdgcn_raw_buffer_load_b128(rs, off + 32 * ks, 0, 0));
 }
 
+// The fragments are here from now on.  Without this the compiler, which does not
+// see wait_loads' waits, waits for them at every use, and so in every round for
+// the stages under way (forward, 16k tokens, 16 heads of 128: 1055 -> 1032 us).
+template <int N>
+__device__ __forceinline__ void arrived(bf16x8 (&f)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+v"(f[i]));
+}
+
+// Order of a block of products whose operands come from LDS: N1 products of R1
+// reads each, then N2 of R2; the reads of two products ahead of the products, and
+// FIRST other reads before them.  Left alone the compiler reads each operand right
+// before its product, into the registers of the last one, and waits there: dK/dV of
+// four sequences of 499 .. 4093, 32 / 8 heads of 128, 488 -> 421 us, dQ 324 -> 317.
+// Three products ahead: level.
+template <int N1, int R1, int N2 = 0, int R2 = 0, int FIRST = 0>
+__device__ __forceinline__ void read_ahead() {
+  constexpr int MFMA = 0x8, DS_READ = 0x100;
+  __builtin_amdgcn_sched_group_barrier(DS_READ, FIRST + 2 * R1, 0);
+#pragma unroll
+  for (int i = 0; i < N1 - 2; ++i) {
+    __builtin_amdgcn_sched_group_barrier(MFMA, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(DS_READ, R1, 0);
+  }
+#pragma unroll
+  for (int i = 0; i < N2; ++i) {
+    __builtin_amdgcn_sched_group_barrier(MFMA, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(DS_READ, R2, 0);
+  }
+  __builtin_amdgcn_sched_group_barrier(MFMA, 2, 0);
+}
+
 // Transposed accumulators (lane = row, registers = features 32 t + 16 g + v)
 // times x to a row of HD bf16.
 template <int HD>
@@ -411,6 +443,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void packed_fwd_kernel(
         for (int i = 0; i < 16 / NK; ++i) weigh(ks * (16 / NK) + i);
       }
       add_pv();
+      read_ahead<NK, 1, 2 * NT, 2>();
       settle(y, t + SPLIT);
       x = y;
     } else {
@@ -423,6 +456,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void packed_fwd_kernel(
   lk.load(ring0, 0);
   lv.load(ring0 + 2 * STAGE, 0);
   lk.load(ring0 + STAGE, 1);
+  arrived(qf);
   wait_loads<StageLoad<HD>::N>();
   if (share < nt) {
     x = f32x16{};
@@ -551,6 +585,8 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void packed_bwd_dq_kernel(
   const int nst = (max(keys, 0) + kStageRows - 1) / kStageRows;
   lk.load(ring0, 0);
   lv.load(ring0 + 2 * STAGE, 0);
+  arrived(qf);
+  arrived(df);
   for (int st = 0; st < nst; ++st) {
     wait_loads<0>();  // stage st is in LDS, st - 1 read by every wave
     lk.load(ring0 + ((st + 1) & 1) * STAGE, st + 1);
@@ -567,6 +603,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void packed_bwd_dq_kernel(
         x = mfma32(rf.get(ring, 32 * sub, ks), qf[ks], x);
         dp = mfma32(rf.get(ring + 2 * STAGE, 32 * sub, ks), df[ks], dp);
       }
+      read_ahead<HD / 8, 1>();
       if (kv0 + 31 > q0 + shift) {
         asm volatile("");  // a branch, not 16 selects for every tile
 #pragma unroll
@@ -580,6 +617,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void packed_bwd_dq_kernel(
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int t = 0; t < NT; ++t) acc[t] = mfma32(tf.get(ring, 32 * sub + 16 * h, t), sf[h], acc[t]);
+      read_ahead<2 * NT, 2>();
     }
     rf.move(STAGE);
     tf.move(STAGE);
@@ -596,8 +634,8 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void packed_bwd_dq_kernel(
 // head of the group, the queries from the diagonal to the end pass through LDS with
 // their -lse / c and -delta, which start the accumulators of S and dP.  Queries past
 // the sequence are zeros throughout: their P is 1, their dO and dS 0.  Eight waves
-// on stages of 128 queries take longer than two workgroups of four (472 -> 510 us
-// for four sequences of 499 .. 4093, 32 / 8 heads of 128).
+// on stages of 128 queries take longer than two workgroups of four (470 -> 510 us,
+// before read_ahead, for four sequences of 499 .. 4093, 32 / 8 heads of 128).
 // parts > 1, for grids that leave CUs idle: a workgroup walks a part of the
 // group's heads and leaves fp32 sums (parts, Tk, Hkv, HD) for packed_sum_kernel.
 template <int HD, int KB>
@@ -651,6 +689,8 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void packed_bwd_dkdv_kernel(
   };
   int head = 0, st = st0;
   load(steps > 0 ? 0 : group, st, 0);
+  arrived(kf);
+  arrived(vf);
   for (int step = 0; step < steps; ++step) {
     const int buf = step & 1, cur = st;
     if (++st == st0 + nst) {  // the next stage, or the next head's first
@@ -680,6 +720,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void packed_bwd_dkdv_kernel(
         x = mfma32(fr.get(ring, 32 * sub, ks), kf[ks], x);
         dp = mfma32(fr.get(ring + 2 * STAGE, 32 * sub, ks), vf[ks], dp);
       }
+      read_ahead<HD / 8, 1, 0, 0, 8>();
 #pragma unroll
       for (int i = 0; i < 16; ++i) x[i] = __builtin_amdgcn_exp2f(x[i] * c);
       if (kv0 + 31 > q0 + shift) {
@@ -699,6 +740,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void packed_bwd_dkdv_kernel(
           av[t] = mfma32(fr.get_t(ring + 2 * STAGE, 32 * sub + 16 * h, t), pf[h], av[t]);
           ak[t] = mfma32(fr.get_t(ring, 32 * sub + 16 * h, t), sf[h], ak[t]);
         }
+      read_ahead<4 * NT, 2>();
     }
     fr.move(STAGE);
   }
