@@ -22,7 +22,7 @@
 // Many rows are bound by HBM: 4096 x 50001 bf16 69 us (5.9 TB/s; fp32 127 us, 6.5
 // TB/s), with the top 20, read twice, 122; a thread that keeps values as fp32
 // between maximum and sum, 8 chunks at a time, takes 200 registers and 105 us.
-// The gradient 180 us (4.6 TB/s read and written; a copy reaches 4.95).  Few rows
+// The gradient 154 us (5.3 TB/s read and written; a large copy 4.95).  Few rows
 // are bound by the steps within a workgroup: 64 x 32768 with the top 20 8.9 us
 // (1024 threads; 19.6 with 512 and a second read), of which 3 are launch and
 // first load.  One row of 151999 in 8 parts 13.7 us, in one 21.9; 64 of them 17.4
@@ -449,16 +449,24 @@ __global__ __launch_bounds__(256) void logprobs_join_kernel(const T* __restrict_
   }
 }
 
-// d logits of one row; g_logp and g_entropy may be null (no gradient).
+// d logits of a slab of `slab` chunks of a row (the first one takes the elements
+// beside the chunks too); slabs of a row are neighbours in the grid, so that what
+// is under way at a time lies together in memory.  4096 x 50001 bf16: 154 us (5.3
+// TB/s; a workgroup a row 183, of 1024 threads 157), fp32 287 (362); 300 x 151999 30
+// (53).  Slabs of 512 chunks: 160, 267, 35.  g_logp and g_entropy may be null (no
+// gradient).
+constexpr int kBwdChunks = 4;  // of a thread, loaded at once
 template <typename T>
 __global__ __launch_bounds__(256) void logprobs_bwd_kernel(const T* __restrict__ logits, long ld,
                                                            const int64_t* __restrict__ tokens,
                                                            const float* __restrict__ stat,
                                                            const float* __restrict__ g_logp, long gl_stride,
                                                            const float* __restrict__ g_entropy, long ge_stride,
-                                                           T* __restrict__ dlogits, int V, long ignore_index) {
+                                                           T* __restrict__ dlogits, int V, long ignore_index, int slabs,
+                                                           int slab) {
   constexpr int E = Row<T>::E;
-  const long r = blockIdx.x;
+  const long r = blockIdx.x / (unsigned)slabs;
+  const int begin = blockIdx.x % (unsigned)slabs * slab;
   // chunks at the gradient's alignment (its rows are dense); the logits' may differ
   const Row<T> out(dlogits + r * (long)V, V);
   const T* x = logits + r * ld;
@@ -478,18 +486,19 @@ __global__ __launch_bounds__(256) void logprobs_bwd_kernel(const T* __restrict__
     return (j == tok ? gl : 0.f) - p * fmaf(ge, fmaf(z < -1e30f ? -1e30f : z, kLn2, ent), gl);
   };
   T* dx = dlogits + r * (long)V;
-  constexpr int U = 4;
-  for (int c0 = threadIdx.x; c0 < out.chunks; c0 += 256 * U) {
+  constexpr int U = kBwdChunks;
+  const int end = min(out.chunks, begin + slab);
+  for (int c0 = begin + threadIdx.x; c0 < end; c0 += 256 * U) {
     uint4 u[U];
     if (same) {
 #pragma unroll
       for (int i = 0; i < U; ++i)
-        u[i] = *reinterpret_cast<const uint4*>(x + out.first(min(c0 + 256 * i, out.chunks - 1)));
+        u[i] = *reinterpret_cast<const uint4*>(x + out.first(min(c0 + 256 * i, end - 1)));
     }
 #pragma unroll
     for (int i = 0; i < U; ++i) {
       const int j0 = out.first(c0 + 256 * i);
-      if (c0 + 256 * i >= out.chunks) break;
+      if (c0 + 256 * i >= end) break;
       float d[E];
       if (same) {
 #pragma unroll
@@ -511,7 +520,7 @@ __global__ __launch_bounds__(256) void logprobs_bwd_kernel(const T* __restrict__
       __builtin_nontemporal_store(o, reinterpret_cast<f32x4*>(dx + j0));
     }
   }
-  const int je = out.extra(threadIdx.x);
+  const int je = begin == 0 ? out.extra(threadIdx.x) : -1;
   if (je >= 0) {
     const float d = grad(value(x[je]), je);
     if constexpr (E == 8)
@@ -572,9 +581,13 @@ hipError_t launch_logprobs_bwd(const void* logits, bool bf16, long ld, const int
                                void* dlogits, long N, int V, long ignore_index, hipStream_t st) {
   auto run = [&](auto kernel, auto* x) {
     typedef std::remove_const_t<std::remove_pointer_t<decltype(x)>> T;
+    const int chunks = std::max(V / Row<T>::E, 1);
+    int slab = 256 * kBwdChunks;
+    while (N * ((chunks + slab - 1) / slab) >= 1L << 24) slab *= 2;  // (a launch has under 2^32 threads)
+    const int slabs = (chunks + slab - 1) / slab;
     NAYLIS_TIMED("logprobs_bwd", st,
-                 hipLaunchKernelGGL(kernel, dim3((unsigned)N), dim3(256), 0, st, x, ld, tokens, stat, g_logp,
-                                    gl_stride, g_entropy, ge_stride, (T*)dlogits, V, ignore_index));
+                 hipLaunchKernelGGL(kernel, dim3((unsigned)(N * slabs)), dim3(256), 0, st, x, ld, tokens, stat, g_logp,
+                                    gl_stride, g_entropy, ge_stride, (T*)dlogits, V, ignore_index, slabs, slab));
   };
   if (bf16)
     run(logprobs_bwd_kernel<bf16_t>, (const bf16_t*)logits);
