@@ -3,12 +3,19 @@
 // Sequences are given by their offsets alone, which are on the device, so the
 // grid has the most tiles that T rows in n sequences can have, and a workgroup's
 // first wave finds its tile from the offsets: no plan to build, nothing to
-// copy, no extra launch.  Tiles are ranked by their work, in levels of 128
-// rows of the other operand, longest first: F(x) = number of tiles with more
-// than x rows is a sum over the sequences (one wave reduction), so a binary
-// search over x finds a rank's level and one scan over the sequences its
-// tile.  About 0.5 us of a workgroup's time for up to 62 sequences (their
-// offsets stay in registers); more of them are read again at every step.
+// copy, no extra launch.
+//
+// Up to 22 sequences (a range a lane): tiles are ranked by their work, in levels
+// of 128 rows of the other operand, longest first.  F(x) = number of tiles with
+// more than x rows is a sum over the sequences (one wave reduction), so a binary
+// search over x finds a rank's level and one scan over the sequences its tile,
+// about 0.5 us of a workgroup's time.
+//
+// More sequences: in their order, sequence i from slot start / TILE + i on, which
+// leaves room for its tiles; a slot's sequence is found by a search of 64 at a
+// time, two loads for up to 4094.  15 sequences of up to 2000 tokens, 8 heads of
+// 128, take 72 us ranked and 82 in order (forward), 30 level, 60 332 and 317; 128 of
+// up to 64 tokens, 16 heads of 64, 25 and 18, 4096 6200 and 600.
 //
 // The rows before the first offset and behind the last one are sequences 0
 // and n + 1, without anything to attend to: their results are zeros.  Offsets
@@ -22,8 +29,12 @@ namespace naylis {
 
 constexpr int kTileRows = 128;
 
-// most tiles of `tile` rows that `rows` rows in n sequences have, the two outer ranges included
-inline long packed_tiles(long rows, long n, int tile = kTileRows) { return (rows + (tile - 1) * (n + 2)) / tile; }
+constexpr int kRankedRanges = 24;  // most ranges (sequences and the two outer ones) whose tiles are ranked
+
+// most tiles (ranked), or slots, of `tile` rows that `rows` rows in n sequences have, the two outer ranges included
+inline long packed_tiles(long rows, long n, int tile = kTileRows) {
+  return n + 2 <= kRankedRanges ? (rows + (tile - 1) * (n + 2)) / tile : rows / tile + n + 2;
+}
 
 struct PackedTile {
   int q0, lq, k0, lk;  // the sequence: first rows and lengths
@@ -73,25 +84,28 @@ __device__ __forceinline__ int tiles_over(const PackedSpan& p, bool outer, int x
   return y < 0 ? all : y >= p.lq ? 0 : all - y / TILE;
 }
 
+// Tile `nth` of a range's tiles (query tiles from the last one on: longest first).
 template <bool KEYS, int TILE>
-__device__ __forceinline__ PackedTile search_tile(const PackedSeqs& s, int rank) {
-  const int lane = threadIdx.x & 63, count = s.n + 2;
+__device__ __forceinline__ PackedTile tile_of(const PackedSpan& p, bool outer, int nth) {
+  PackedTile tile{p.q0, p.lq, p.k0, p.lk, 0, false};
+  if (outer) (KEYS ? tile.lq : tile.lk) = 0;
+  const int all = ((KEYS ? tile.lk : tile.lq) + TILE - 1) / TILE;
+  tile.block = KEYS ? nth : all - 1 - nth;
+  tile.live = nth >= 0 && nth < all;
+  return tile;
+}
+
+template <bool KEYS, int TILE>
+__device__ __forceinline__ PackedTile search_ranked(const PackedSeqs& s, int rank) {
+  const int lane = threadIdx.x & 63;
   const PackedSpan mine = packed_span(s, lane);
-  const auto outer = [&](int i) { return i == 0 || i == s.n + 1; };
+  const bool outer = lane == 0 || lane == s.n + 1;
   const auto total = [&](int x) {
-    int t = tiles_over<KEYS, TILE>(mine, outer(lane), x);
-    for (int base = 64; base < count; base += 64)
-      t += tiles_over<KEYS, TILE>(packed_span(s, base + lane), outer(base + lane), x);
-    return __builtin_amdgcn_readfirstlane(wave_allsum_i32(t));
+    return __builtin_amdgcn_readfirstlane(wave_allsum_i32(tiles_over<KEYS, TILE>(mine, outer, x)));
   };
-  PackedTile tile{0, 0, 0, 0, 0, false};
-  if (rank >= total(-1)) return tile;
+  if (rank >= total(-1)) return PackedTile{0, 0, 0, 0, 0, false};
   // the first level whose work no tile before `rank` lies under: F(128 lo) <= rank
-  int most = KEYS ? mine.lq : mine.lk;
-  for (int base = 64; base < count; base += 64) {
-    const PackedSpan p = packed_span(s, base + lane);
-    most = max(most, KEYS ? p.lq : p.lk);
-  }
+  const int most = KEYS ? mine.lq : mine.lk;
   int lo = 0, hi = (-wave_allmin_i32(-most) + kTileRows - 1) / kTileRows;
   hi = __builtin_amdgcn_readfirstlane(hi);
   while (lo < hi) {
@@ -102,34 +116,36 @@ __device__ __forceinline__ PackedTile search_tile(const PackedSeqs& s, int rank)
       lo = mid + 1;
   }
   const int x = lo * kTileRows, above = lo == 0 ? -1 : x - kTileRows;
-  int left = rank - total(x);
-  for (int base = 0; base < count; base += 64) {
-    const PackedSpan p = base == 0 ? mine : packed_span(s, base + lane);
-    const int over = tiles_over<KEYS, TILE>(p, outer(base + lane), x);
-    const int here = tiles_over<KEYS, TILE>(p, outer(base + lane), above) - over;
-    int sum = here;  // inclusive scan
+  const int left = rank - total(x);
+  const int over = tiles_over<KEYS, TILE>(mine, outer, x), here = tiles_over<KEYS, TILE>(mine, outer, above) - over;
+  int sum = here;  // inclusive scan
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int t = __shfl_up(sum, o, 64);
-      if (lane >= o) sum += t;
-    }
-    const unsigned long long past = __ballot(sum > left);
-    if (past) {
-      const int src = __ffsll(past) - 1;
-      const int nth = left - __builtin_amdgcn_readlane(sum - here, src), o = __builtin_amdgcn_readlane(over, src);
-      tile.q0 = __builtin_amdgcn_readlane(p.q0, src);
-      tile.lq = __builtin_amdgcn_readlane(p.lq, src);
-      tile.k0 = __builtin_amdgcn_readlane(p.k0, src);
-      tile.lk = __builtin_amdgcn_readlane(p.lk, src);
-      if (base + src == 0 || base + src == s.n + 1) (KEYS ? tile.lq : tile.lk) = 0;
-      const int all = ((KEYS ? tile.lk : tile.lq) + TILE - 1) / TILE;
-      tile.block = KEYS ? o + nth : all - 1 - o - nth;
-      tile.live = tile.block >= 0 && tile.block < all;
-      return tile;
-    }
-    left -= __builtin_amdgcn_readlane(sum, 63);
+  for (int o = 1; o < 64; o <<= 1) {
+    const int t = __shfl_up(sum, o, 64);
+    if (lane >= o) sum += t;
   }
-  return tile;
+  const unsigned long long past = __ballot(sum > left);
+  if (!past) return PackedTile{0, 0, 0, 0, 0, false};
+  const int src = __ffsll(past) - 1;
+  const auto of = [&](int v) { return __builtin_amdgcn_readlane(v, src); };
+  return tile_of<KEYS, TILE>(PackedSpan{of(mine.q0), of(mine.lq), of(mine.k0), of(mine.lk)},
+                             src == 0 || src == s.n + 1, of(over) + left - of(sum - here));
+}
+
+template <bool KEYS, int TILE>
+__device__ __forceinline__ PackedTile search_slots(const PackedSeqs& s, int at) {
+  const int lane = threadIdx.x & 63, rows = KEYS ? s.Tk : s.T;
+  const int32_t* cu = KEYS ? s.cu_k : s.cu_q;
+  const auto slot = [&](int i) { return (i == 0 ? 0 : min(max(cu[i - 1], 0), rows)) / TILE + i; };
+  int lo = 0, ranges = s.n + 2;  // the last of these whose slot is no later (range 0 has slot 0)
+  while (ranges > 1) {
+    const int stride = (ranges + 63) / 64, i = lane * stride;
+    const unsigned long long early = __ballot(i < ranges && slot(lo + min(i, ranges - 1)) <= at) | 1;
+    const int skip = (63 - __clzll(early)) * stride;
+    lo += skip;
+    ranges = min(stride, ranges - skip);
+  }
+  return tile_of<KEYS, TILE>(packed_span(s, lo), lo == 0 || lo == s.n + 1, at - slot(lo));
 }
 
 // The workgroup's tile: searched by its first wave alone (the others' vector
@@ -138,7 +154,8 @@ template <bool KEYS, int TILE = kTileRows>
 __device__ __forceinline__ PackedTile find_tile(const PackedSeqs& s, int rank) {
   __shared__ PackedTile found;
   if (threadIdx.x < 64) {
-    const PackedTile t = search_tile<KEYS, TILE>(s, rank);
+    const PackedTile t =
+        s.n + 2 <= kRankedRanges ? search_ranked<KEYS, TILE>(s, rank) : search_slots<KEYS, TILE>(s, rank);
     if (threadIdx.x == 0) found = t;
   }
   __syncthreads();

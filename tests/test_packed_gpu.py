@@ -161,6 +161,17 @@ def test_packed_rising_scores(top, hd, dev):
     _check(_run(*x, 0.7), _reference(*x, 0.7))
 
 
+@pytest.mark.parametrize("n,longest", [(22, 200), (23, 200), (63, 90), (4200, 3)])
+def test_packed_many_sequences(n, longest, dev):
+    """Either side of the count from which sequences are taken in their order,
+    and more than a search of two rounds covers; empty ones among them."""
+    r = random.Random(n)
+    lq = [r.choice([0, 1, r.randint(0, longest)]) for _ in range(n)]
+    lk = [a + r.choice([0, r.randint(0, longest)]) for a in lq]
+    x = _inputs(lq, lk, 2, 1, 64, 3, 140, dev)
+    _check(_run(*x, 0.125), _reference(*x, 0.125))
+
+
 def test_packed_is_causal(dev):
     x = _inputs([333], [400], 4, 4, 64, 0, 0, dev)
     y = [t.clone() for t in x]
