@@ -130,45 +130,68 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedCacheDims c, con
 
 namespace {
 
-// Steps of the sequences before b, of all of them, and the steps of a wave's range.
+// The list of all sequences' steps.  A lane looks after an equal chunk of the
+// sequences, so that a place is found with one scan over the lanes and one over
+// a chunk, whatever their number.
 struct StepList {
   const int32_t* lens;
   int B, cap;  // sequences, tokens that a table row holds
 
-  __device__ __forceinline__ int len(int b) const { return b < B ? min(max(lens[b], 0), cap) : 0; }
+  // (any b: loads of several at once are not held up by a comparison)
+  __device__ __forceinline__ int len(int b) const {
+    const int n = lens[min(b, B - 1)];
+    return b < B ? min(max(n, 0), cap) : 0;
+  }
   __device__ __forceinline__ int steps(int b) const { return (len(b) + kPagedStep - 1) / kPagedStep; }
 
-  // sum of steps over sequences [0, b)
-  __device__ __forceinline__ int before(int b) const {
+  static __device__ __forceinline__ int inclusive(int x) {
     const int lane = threadIdx.x & 63;
-    int t = 0;
-    for (int i = lane; i < b; i += 64) t += steps(i);
-    return __builtin_amdgcn_readfirstlane(wave_allsum_i32(t));
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int t = __shfl_up(x, o, 64);
+      if (lane >= o) x += t;
+    }
+    return x;
   }
 
-  // the sequence that holds step `at` (at < before(B)) and its first step
-  __device__ __forceinline__ void find(int at, int& b, int& first) const {
-    const int lane = threadIdx.x & 63;
-    int done = 0;
-    for (int base = 0; base < B; base += 64) {
-      const int here = steps(base + lane);
-      int sum = here;
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const int t = __shfl_up(sum, o, 64);
-        if (lane >= o) sum += t;
-      }
-      const unsigned long long past = __ballot(done + sum > at);
+  __device__ __forceinline__ int chunk() const { return (B + 63) / 64; }
+  // steps of the lane's chunk, and of all up to it
+  __device__ __forceinline__ int2 chunks() const {
+    const int n = chunk(), b = (threadIdx.x & 63) * n;
+    int own = 0;
+#pragma unroll 8
+    for (int i = 0; i < n; ++i) own += steps(b + i);
+    return make_int2(own, inclusive(own));
+  }
+
+  // the sequence that holds step `at` (one of the list's) and its first step
+  __device__ __forceinline__ void find(int at, const int2& sums, int& b, int& first) const {
+    const int lane = threadIdx.x & 63, n = chunk();
+    const int src = max(__ffsll((unsigned long long)__ballot(sums.y > at)) - 1, 0);
+    b = src * n;
+    first = __builtin_amdgcn_readlane(sums.y - sums.x, src);
+    if (n == 1) return;
+    for (int i = 0; i < n; i += 64) {
+      const int own = i + lane < n ? steps(b + lane) : 0, sum = inclusive(own);
+      const unsigned long long past = __ballot(first + sum > at);
       if (past) {
-        const int src = __ffsll(past) - 1;
-        b = base + src;
-        first = done + __builtin_amdgcn_readlane(sum - here, src);
+        const int in = __ffsll(past) - 1;
+        b += in;
+        first += __builtin_amdgcn_readlane(sum - own, in);
         return;
       }
-      done += __builtin_amdgcn_readlane(sum, 63);
+      b += 64;
+      first += __builtin_amdgcn_readlane(sum, 63);
     }
-    b = B;
-    first = done;
+  }
+
+  // the first sequence from b on that has tokens, or B
+  __device__ __forceinline__ int next(int b) const {
+    for (; b < B; b += 64) {
+      const unsigned long long live = __ballot(len(b + (int)(threadIdx.x & 63)) > 0);
+      if (live) return b + __ffsll(live) - 1;
+    }
+    return B;
   }
 };
 
@@ -214,7 +237,8 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedCacheDims c, co
                                                             long hsq, const int32_t* __restrict__ table,
                                                             const int32_t* __restrict__ lens,
                                                             bf16_t* __restrict__ out, float* __restrict__ part,
-                                                            float2* __restrict__ stat, PagedSplit p, float sc) {
+                                                            float2* __restrict__ stat, int* __restrict__ starts,
+                                                            PagedSplit p, float sc) {
   constexpr int TOK = kPagedStep;        // tokens of a step
   constexpr int NS = TOK / 16;           // its 16-token products
   constexpr int KS = HD / 32;            // products along the features
@@ -236,11 +260,14 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedCacheDims c, co
   const StepList list{lens, c.B, c.W * c.page};
 
   int wg0, wg1, at, end, b = wg, first = 0;
+  int2 sums = make_int2(0, 0);
   if (p.whole) {
     wg0 = 0;
     wg1 = list.steps(wg);
   } else {
-    const int total = list.before(c.B), range = max((total + p.wgs - 1) / p.wgs, 1);
+    sums = list.chunks();
+    const int total = __builtin_amdgcn_readlane(sums.y, 63), range = max((total + p.wgs - 1) / p.wgs, 1);
+    if (tid == 0 && wg == 0 && slice == 0) starts[c.B] = total;
     wg0 = min(wg * range, total);
     wg1 = min(wg0 + range, total);
   }
@@ -249,7 +276,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedCacheDims c, co
     at = min(wg0 + wave * share, wg1);
     end = min(at + share, wg1);
   }
-  if (!p.whole && at < end) list.find(at, b, first);
+  if (!p.whole && at < end) list.find(at, sums, b, first);
   if (lane < 2) seqs[2 * wave + lane].b = -1;
 
   const int shift = 31 - __clz(c.page);
@@ -262,6 +289,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedCacheDims c, co
     const int n = list.len(b), nsteps = (n + TOK - 1) / TOK;
     const int s0 = at - first, s1 = min(end - first, nsteps);  // this wave's steps of sequence b
     bool bad = lens[b] > list.cap;                             // longer than its table
+    if (!p.whole && s0 == 0 && slice == 0 && lane == 0) starts[b] = first;
 
     bf16x8 qf[KS];
     {
@@ -448,7 +476,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedCacheDims c, co
     at = first + s1;
     first += nsteps;
     ++b;
-    while (b < c.B && list.steps(b) == 0) ++b;  // sequences without tokens hold no step
+    if (at < end) b = list.next(b);  // sequences without tokens hold no step
   }
   __syncthreads();
 
@@ -503,12 +531,15 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedCacheDims c, co
       a = f32x4{};
     }
   }
-  // zeros for the sequences without tokens
-  if (p.whole ? wg1 == 0 : wg == 0) {
-    for (int z = p.whole ? wg : 0; z < (p.whole ? wg + 1 : c.B); ++z)
-      if (list.len(z) == 0)
-        for (int i = tid; i < nh * (HD / 4); i += 256)
-          *reinterpret_cast<bf16x4*>(out + ((long)z * H + hbase) * HD + 4 * i) = bf16x4{};
+  // zeros for the sequences without tokens: 64 sequences a wave, or the workgroup's own
+  for (int z0 = p.whole ? wg : (wg * 4 + wave) * 64; z0 < c.B; z0 += p.whole ? c.B : p.wgs * 256) {
+    if (p.whole && wave > 0) break;
+    unsigned long long none = __ballot(z0 + lane < c.B && (!p.whole || lane == 0) && list.len(z0 + lane) == 0);
+    for (; none; none &= none - 1) {
+      const long z = z0 + __ffsll(none) - 1;
+      for (int i = lane; i < nh * (HD / 4); i += 64)
+        *reinterpret_cast<bf16x4*>(out + (z * H + hbase) * HD + 4 * i) = bf16x4{};
+    }
   }
 }
 
@@ -517,18 +548,18 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedCacheDims c, co
 template <int HD>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedCacheDims c, const int32_t* __restrict__ lens,
                                                          bf16_t* __restrict__ out, const float* __restrict__ part,
-                                                         const float2* __restrict__ stat, PagedSplit p) {
+                                                         const float2* __restrict__ stat, const int* __restrict__ starts,
+                                                         PagedSplit p) {
   constexpr int TR = HD / 4, NG = 256 / TR;  // threads of a partial; partials read at once
   __shared__ float weight[kPagedMaxWgs];
   __shared__ float red[4];
   __shared__ f32x4 sums[NG][TR];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int h = blockIdx.x, b = blockIdx.y;
-  const StepList list{lens, c.B, c.W * c.page};
-  const int n = list.steps(b);
+  const int n = StepList{lens, c.B, c.W * c.page}.steps(b);
   if (n == 0) return;
-  const int total = list.before(c.B), range = max((total + p.wgs - 1) / p.wgs, 1);
-  const int first = list.before(b), w0 = first / range, w1 = (first + n - 1) / range;
+  const int total = starts[c.B], range = max((total + p.wgs - 1) / p.wgs, 1);
+  const int first = starts[b], w0 = first / range, w1 = (first + n - 1) / range;
   if (w0 == w1) return;
   const int kvh = h / c.G, hr = h % c.G, slice = kvh * p.head_tiles + hr / kRowsMfma;
   const int count = w1 - w0 + 1;
@@ -603,9 +634,10 @@ size_t paged_part_floats(const PagedCacheDims& c, const PagedSplit& p, int hd) {
   return p.whole ? 0 : (size_t)c.Hkv * p.head_tiles * p.wgs * 2 * p.rows * hd;
 }
 
+// partials, their (maximum, sum), and each sequence's first step with the number of all behind the last
 size_t paged_ws_bytes(const PagedCacheDims& c, int hd) {
   const size_t n = paged_part_floats(c, paged_split(c), hd);
-  return n * 4 + n / hd * 8;
+  return n == 0 ? 0 : n * 4 + n / hd * 8 + ((size_t)c.B + 1) * 4;
 }
 
 hipError_t launch_paged_append(const PagedCacheDims& c, int hd, bool fp8, const void* k, const void* v,
@@ -629,11 +661,13 @@ hipError_t launch_paged_attn(const PagedCacheDims& c, int hd, bool fp8, const vo
                              hipStream_t st) {
   const PagedSplit p = paged_split(c);
   float* part = (float*)ws;
-  float2* stat = (float2*)(part + paged_part_floats(c, p, hd));
+  const size_t n = paged_part_floats(c, p, hd);
+  float2* stat = (float2*)(part + n);
+  int* starts = (int*)(stat + n / hd);
   auto run = [&](auto kernel) {
     NAYLIS_TIMED("paged_attn", st,
                  hipLaunchKernelGGL(kernel, dim3(p.wgs, c.Hkv * p.head_tiles), dim3(256), 0, st, c,
-                                    (const bf16_t*)q, ldq, hsq, table, lens, (bf16_t*)out, part, stat, p,
+                                    (const bf16_t*)q, ldq, hsq, table, lens, (bf16_t*)out, part, stat, starts, p,
                                     scale * kLog2e));
   };
   auto pick = [&](auto rows) {
@@ -649,7 +683,7 @@ hipError_t launch_paged_attn(const PagedCacheDims& c, int hd, bool fp8, const vo
   auto join = [&](auto kernel) {
     NAYLIS_TIMED("paged_join", st,
                  hipLaunchKernelGGL(kernel, dim3(c.Hkv * c.G, c.B), dim3(256), 0, st, c, lens, (bf16_t*)out,
-                                    (const float*)part, (const float2*)stat, p));
+                                    (const float*)part, (const float2*)stat, (const int*)starts, p));
   };
   hd == 64 ? join(paged_join_kernel<64>) : join(paged_join_kernel<128>);
   return hipGetLastError();

@@ -22,6 +22,9 @@ CASES = [
     ([(37 * i) % 400 for i in range(130)], 6, 2, 64, 32, False),
     ([70001], 4, 2, 128, 64, True),
     ([(53 * i) % 900 for i in range(65)], 32, 8, 128, 16, True),
+    ([0] * 70 + [600] + [0] * 200 + [(29 * i) % 90 for i in range(100)] + [0], 2, 1, 64, 16, False),
+    ([0] * 90 + [5] + [0] * 40, 2, 2, 128, 16, True),
+    ([0 if i % 3 else (i * i) % 23 for i in range(4200)] + [530], 2, 1, 64, 16, False),  # chunks of 66 sequences
 ]
 
 
