@@ -14,8 +14,10 @@
 // into four for their waves, so a long sequence among short ones keeps no
 // wave waiting.  The waves of a workgroup join what they hold of one sequence
 // in LDS, all of it read at once; what several workgroups hold of it goes to a
-// second kernel as (max, sum, o) partials.  Lengths stay on the device: each wave finds its range's
-// first sequence by a scan over them.
+// second kernel as (max, sum, o) partials.  Lengths stay on the device: each wave
+// finds its range's first sequence by two scans over them, and leaves each
+// sequence's first step for the second kernel (4096 sequences of up to 1024 tokens,
+// one key head of 64: 104 us and 25; with scans of 64 sequences a round 393 and 234).
 //
 // Per step a wave forms S^T = K Q^T (v_mfma_f32_16x16x32_bf16: 16 tokens x up
 // to 16 query heads of the key head, zeros for missing ones) with K straight
@@ -23,12 +25,11 @@
 // which transposes it; P leaves the accumulators as the B operand, rounded to
 // bf16 (with e4m3 pages, times V's scale).  The next step's K is loaded as soon
 // as the products have read this one's, V as soon as LDS has, and no barrier is
-// needed.  Loads bypass the caches: 64 sequences of up to 4096 tokens, 8 key
-// heads of 128, 588 MB: 113 -> 103 us (5.7 TB/s; the kernel 97 us, the join and
-// its launch 6).  Three contexts of 65537 .. 131072 tokens, e4m3, 747 MB: 151 ->
-// 122 us (6.1 TB/s); in steps of 64 tokens 134 us (256 registers).  One sequence of
-// 500 tokens, 16 heads of 64: 7.0 us, a chain of dependent loads (length, page,
-// rows) that fill nothing.
+// needed.  Loads bypass the caches (a tenth of the time): 64 sequences of up to 4096
+// tokens, 8 key heads of 128, 588 MB: 98 us (6.0 TB/s; 5 of them the join and its
+// launch).  Three contexts of 65537 .. 131072 tokens, e4m3, 747 MB: 123 us (6.1 TB/s);
+// in steps of 64 tokens 134 (256 registers).  One sequence of 500 tokens, 16 heads of
+// 64: 7.0 us, a chain of dependent loads (length, page, rows) that fill nothing.
 #include "common.h"
 #include "launch.h"
 #include "packed_tiles.h"
@@ -531,15 +532,18 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedCacheDims c, co
       a = f32x4{};
     }
   }
-  // zeros for the sequences without tokens: 64 sequences a wave, or the workgroup's own
-  for (int z0 = p.whole ? wg : (wg * 4 + wave) * 64; z0 < c.B; z0 += p.whole ? c.B : p.wgs * 256) {
-    if (p.whole && wave > 0) break;
-    unsigned long long none = __ballot(z0 + lane < c.B && (!p.whole || lane == 0) && list.len(z0 + lane) == 0);
-    for (; none; none &= none - 1) {
-      const long z = z0 + __ffsll(none) - 1;
-      for (int i = lane; i < nh * (HD / 4); i += 64)
-        *reinterpret_cast<bf16x4*>(out + (z * H + hbase) * HD + 4 * i) = bf16x4{};
-    }
+  // zeros for the sequences without tokens: the workgroup's own, or 64 sequences a wave
+  const auto empty = [&](long z) {
+    for (int i = lane; i < nh * (HD / 4); i += 64)
+      *reinterpret_cast<bf16x4*>(out + (z * H + hbase) * HD + 4 * i) = bf16x4{};
+  };
+  if (p.whole) {
+    if (wg1 == 0 && wave == 0 && wg < c.B) empty(wg);
+    return;
+  }
+  for (int z = (wg * 4 + wave) * 64; z < c.B; z += p.wgs * 256) {
+    unsigned long long none = __ballot(z + lane < c.B && list.len(z + lane) == 0);
+    for (; none; none &= none - 1) empty(z + __ffsll(none) - 1);
   }
 }
 
