@@ -250,6 +250,23 @@ def test_packed_far_rows(dev):
     assert all(torch.equal(got[n], want[n]) for n in got)
 
 
+def test_packed_large_tensors(dev):
+    """Queries, results and gradients of more than 2^31 elements."""
+    n, L, H = 16400, 64, 32
+    q, k, v, d, _, _ = _inputs([L] * 3, None, H, 1, 64, 0, 0, dev)
+    cu = torch.arange(0, n * L + 1, L, dtype=torch.int32, device=dev)
+    want = _reference(q, k, v, d, cu[:4], cu[:4], 0.125)
+    x = [torch.zeros(n * L, *t.shape[1:], dtype=t.dtype, device=dev) for t in (q, k, v, d)]
+    assert x[0].numel() > 2 ** 31
+    for big, small in zip(x, (q, k, v, d)):
+        big[-3 * L:] = small
+        big[:3 * L] = small
+    got = _run(*x, cu, cu, 0.125)
+    _check({name: t[:3 * L] for name, t in got.items()}, want)
+    for name, t in got.items():
+        assert torch.equal(t[:3 * L], t[-3 * L:]) and not bool(t[3 * L:-3 * L].any()), name
+
+
 def test_packed_empty_tensors(dev):
     from naylis_amd.mom_kernels import packed_attention
     z = lambda n, h: torch.zeros(n, h, 64, dtype=torch.bfloat16, device=dev, requires_grad=True)  # noqa: E731
