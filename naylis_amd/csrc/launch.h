@@ -124,7 +124,8 @@ hipError_t launch_attn_bwd(const void* q, const void* k, const void* v, const vo
 // Causal attention over packed sequences (packed.hip): q, o (T, H, hd) and k, v
 // (Tk, Hkv, hd) bf16, hd 64 or 128; sequence i holds query rows cu_q[i] ..
 // cu_q[i + 1] - 1 and key rows cu_k[i] .. (device arrays of n + 1 offsets).
-// lse (H, T; log2 domain) fp32; rest: o less its rounding (bf16, o's shape).  lse and rest are null in a forward without a backward.
+// lse (H, T; log2 domain) fp32; rest: o less its rounding (bf16, o's shape).  lse
+// and rest are null in a forward without a backward.
 struct PackedSeqs {
   const int32_t* cu_q;
   const int32_t* cu_k;
