@@ -807,10 +807,12 @@ hipError_t launch_packed_fwd(const void* q, const void* k, const void* v, void* 
   return split ? run(packed_fwd_kernel<128, 2>, 64) : run(packed_fwd_kernel<128, 1>, 128);
 }
 
-// Tiles of 64 keys for heads of 128, and for heads of 64 where those of 128 keys
-// are under three a CU.
-static int packed_key_tile(const PackedSeqs& s, const PackedHeads& d, int hd) {
-  return hd == 128 || packed_tiles(s.Tk, s.n) * d.Hkv < 768 ? 64 : 128;
+// Tiles of 64 keys, whose waves share 32 of them, where those of 128 are under three
+// a CU: 4000 tokens, 16 heads of 64, 88 -> 73 us; beyond it the join and the barriers
+// cost more (nine sequences of 16376, 16 heads of 64, 189 -> 229; 8 x 2048, 16 heads of
+// 128, 263 -> 322; 4000, 32 of 128, 233 -> 261).
+static int packed_key_tile(const PackedSeqs& s, const PackedHeads& d) {
+  return packed_tiles(s.Tk, s.n) * d.Hkv < 768 ? 64 : 128;
 }
 
 // Parts of a group where its key tiles are few, up to 1536 workgroups: 2000 tokens,
@@ -819,7 +821,7 @@ static int packed_key_tile(const PackedSeqs& s, const PackedHeads& d, int hd) {
 // tokens take 309 us (and 25) for 293.  Not for short sequences, whose tiles have
 // little to do (8 of 30 .. 128 tokens 12 -> 19 us).
 static int packed_parts(const PackedSeqs& s, const PackedHeads& d, int hd) {
-  const long wgs = std::max(packed_tiles(s.Tk, s.n, packed_key_tile(s, d, hd)) * d.Hkv, 1L);
+  const long wgs = std::max(packed_tiles(s.Tk, s.n, packed_key_tile(s, d)) * d.Hkv, 1L);
   if (s.T < 192L * s.n) return 1;
   return (int)std::max(1L, std::min((long)d.H / d.Hkv, 1536 / wgs));
 }
@@ -862,9 +864,11 @@ hipError_t launch_packed_bwd(const void* q, const void* k, const void* v, const 
     if (e != hipSuccess) return e;
   }
   if (s.Tk == 0) return hipSuccess;
-  const hipError_t e = hd == 128 ? run_dkdv(packed_bwd_dkdv_kernel<128, 64>, 64)
-                       : packed_key_tile(s, d, hd) == 64 ? run_dkdv(packed_bwd_dkdv_kernel<64, 64>, 64)
-                                                         : run_dkdv(packed_bwd_dkdv_kernel<64, 128>, 128);
+  const bool wide = packed_key_tile(s, d) == 128;
+  const hipError_t e = hd == 64 ? (wide ? run_dkdv(packed_bwd_dkdv_kernel<64, 128>, 128)
+                                        : run_dkdv(packed_bwd_dkdv_kernel<64, 64>, 64))
+                                : (wide ? run_dkdv(packed_bwd_dkdv_kernel<128, 128>, 128)
+                                        : run_dkdv(packed_bwd_dkdv_kernel<128, 64>, 64));
   if (e != hipSuccess || parts == 1) return e;
   NAYLIS_TIMED("packed_sum", st,
                hipLaunchKernelGGL(packed_sum_kernel, dim3((unsigned)((n / 4 + 255) / 256), 2), dim3(256), 0, st,

@@ -27,6 +27,7 @@ CASES = [
     ([1537, 130], None, 16, 2, 128, 0, 130),
     ([900, 1500], None, 32, 8, 128, 0, 0),              # grids that fill the chip: whole tiles a workgroup
     ([1500], None, 64, 64, 64, 0, 3),
+    ([1500], [1600], 64, 64, 128, 0, 3),
     ([(7 * i) % 150 for i in range(70)], None, 4, 2, 64, 10, 10),
     ([(11 * i) % 40 for i in range(130)], [(11 * i) % 40 + (i % 3) * 50 for i in range(130)], 2, 1, 128, 0, 0),
 ]
