@@ -19,10 +19,10 @@
 // Bound by power, then by the softmax's vector work beside the matrix units.  Over
 // 16k tokens, with the products that each gradient kernel forms again counted, the
 // forward runs at 1.07 PFLOP/s with 16 heads of 128 (a large matrix product at 1.14
-// for as long) and 0.93 of 64, dQ at 1.20 and 0.98, dK/dV at 1.13 and 0.97; on tensors
-// of zeros, which take less power, at 1.4 and 1.2, 1.7 and 1.5, 1.5 and 1.45.  Nine
-// sequences of 48 .. 3885 tokens, 16 heads of 64: 107 us forward, 428 with the
-// gradients; four of 499 .. 4093, 32 / 8 heads of 128: 209 and 920.  The first loads of
+// for as long) and 0.93 of 64, dQ at 1.25 and 1.0, dK/dV at 1.27 and 1.0; on tensors
+// of zeros, which take less power, at 1.4 and 1.2, 1.7 and 1.5, 1.6 and 1.45.  Nine
+// sequences of 48 .. 3885 tokens, 16 heads of 64: 107 us forward, 415 with the
+// gradients; four of 499 .. 4093, 32 / 8 heads of 128: 209 and 885.  The first loads of
 // a tile and the last tiles' tail are a quarter of such batches.
 #include "common.h"
 #include "launch.h"
@@ -391,7 +391,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void packed_fwd_kernel(
   // key tiles that the wave's queries see (a wave behind the sequence has none)
   const int nt = q0 < tile.lq ? min(max(q0 + 32 + shift + 31, 0) / 32, 2 * nst) : 0;
 
-  f32x16 acc[NT], x;  // x: scores, then weights, of the tile at hand
+  f32x16 acc[NT], x;  // x: scores of the tile at hand
   clear(acc);
   float m = kNegBig, l = 0.f;
   // mask of tile t, its maximum, and the sums rescaled where that is far above the reference
@@ -416,9 +416,9 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void packed_fwd_kernel(
         for (int i = 0; i < 16; ++i) acc[u][i] *= al;
     }
   };
-  auto weigh = [&](int i) {
-    x[i] = __builtin_amdgcn_exp2f(fmaf(x[i], c, -m));
-    l += x[i];
+  auto weigh = [&](f32x16& p, int i) {
+    p[i] = __builtin_amdgcn_exp2f(SPLIT == 1 ? p[i] : fmaf(p[i], c, -m));
+    l += p[i];
   };
   // Tile t (the first or second of its stage) with its scores in x; leaves those of
   // the wave's next one, t + SPLIT, there.  The lanes' LDS offsets move to the other
@@ -427,28 +427,32 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void packed_fwd_kernel(
     constexpr int HALF = 32 * 2 * HD, SECOND = decltype(second)::value;
     const uint8_t* vb = ring + SECOND * HALF;
     const uint8_t* kb = ring + (SECOND != (SPLIT == 1) ? HALF : 0);
+    f32x16 p = x;  // weights; their exponents before the branch, so that the next scores can take x's registers
+    if constexpr (SPLIT == 1) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) p[i] = fmaf(x[i], c, -m);
+    }
     auto add_pv = [&]() {
-      const bf16x8 pf[2] = {pack8(x, 0), pack8(x, 8)};
+      const bf16x8 pf[2] = {pack8(p, 0), pack8(p, 8)};
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int u = 0; u < NT; ++u) acc[u] = mfma32(tf.get(vb, 16 * h, u), pf[h], acc[u]);
     };
     if (t + SPLIT < nt) {
-      f32x16 y = f32x16{};
+      x = f32x16{};
 #pragma unroll
       for (int ks = 0; ks < NK; ++ks) {
-        y = mfma32(rf.get(kb, 0, ks), qf[ks], y);
+        x = mfma32(rf.get(kb, 0, ks), qf[ks], x);
 #pragma unroll
-        for (int i = 0; i < 16 / NK; ++i) weigh(ks * (16 / NK) + i);
+        for (int i = 0; i < 16 / NK; ++i) weigh(p, ks * (16 / NK) + i);
       }
       add_pv();
       read_ahead<NK, 1, 2 * NT, 2>();
-      settle(y, t + SPLIT);
-      x = y;
+      settle(x, t + SPLIT);
     } else {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) weigh(i);
+      for (int i = 0; i < 16; ++i) weigh(p, i);
       add_pv();
     }
   };
