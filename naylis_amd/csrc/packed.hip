@@ -18,11 +18,11 @@
 //
 // Bound by power, then by the softmax's vector work beside the matrix units.  Over
 // 16k tokens, with the products that each gradient kernel forms again counted, the
-// forward runs at 1.07 PFLOP/s with 16 heads of 128 (a large matrix product at 1.14
-// for as long) and 0.93 of 64, dQ at 1.25 and 1.0, dK/dV at 1.27 and 1.0; on tensors
-// of zeros, which take less power, at 1.4 and 1.2, 1.7 and 1.5, 1.6 and 1.45.  Nine
-// sequences of 48 .. 3885 tokens, 16 heads of 64: 107 us forward, 415 with the
-// gradients; four of 499 .. 4093, 32 / 8 heads of 128: 209 and 885.  The first loads of
+// forward runs at 1.1 PFLOP/s with 16 heads of 128 (a large matrix product at 1.14
+// for as long) and 0.95 of 64, dQ at 1.25 and 1.0, dK/dV at 1.26 and 1.0; on tensors
+// of zeros, which take less power, at 1.4 and 1.2, 1.65 and 1.5, 1.6 and 1.45.  Nine
+// sequences of 48 .. 3885 tokens, 16 heads of 64: 103 us forward, 405 with the
+// gradients; four of 499 .. 4093, 32 / 8 heads of 128: 210 and 888.  The first loads of
 // a tile and the last tiles' tail are a quarter of such batches.
 #include "common.h"
 #include "launch.h"
@@ -393,7 +393,9 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void packed_fwd_kernel(
 
   f32x16 acc[NT], x;  // x: scores of the tile at hand
   clear(acc);
-  float m = kNegBig, l = 0.f;
+  float m = kNegBig, l = 0.f, inf;
+  // (a known infinity would turn the median below into a maximum of three instructions)
+  asm("s_mov_b32 %0, 0x7f800000" : "=s"(inf));
   // mask of tile t, its maximum, and the sums rescaled where that is far above the reference
   auto settle = [&](f32x16& z, int t) {
     if (32 * t + 31 > q0 + shift) {
@@ -402,7 +404,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void packed_fwd_kernel(
       for (int i = 0; i < 16; ++i)
         if (32 * t + acc_row(g, i) > row + shift) z[i] = -INFINITY;
     }
-    const float over = fmaf(max_of(fmaxf(z[0], z[1]), z), c, -kSlack);
+    const float over = fmaf(max_of(__builtin_amdgcn_fmed3f(z[0], z[1], inf), z), c, -kSlack);
     if (__builtin_expect(__any(over > m), 0)) {
       // per query, so that a row's result does not depend on its neighbours'
       const float most = xor32_f32(over, [](float a, float b) { return fmaxf(a, b); });
