@@ -23,9 +23,10 @@ def packed_attention(q, k, v, cu_seqlens, cu_seqlens_k=None, scale=None):
     outside the sequences.  Offsets must not descend and are not copied to the
     host; they are clamped to the tensors.  scale defaults to hd ** -0.5.
     Returns (T, H, hd).  Sequences do not see each other's rows, whatever these
-    hold; within one, a weight of 0 multiplies v as it is, so a NaN or an infinity
-    in a row of v reaches queries up to 31 rows before it too.  A forward with
-    gradients keeps, beside its inputs and the output, what the output's rounding
-    left (as much again) and (H, T) fp32.  The derivative of the backward raises."""
+    hold; within one, a weight of 0 multiplies v (dout in the backward) as it is,
+    so a NaN or an infinity in a row of it reaches up to 62 rows that do not see
+    it.  A forward with gradients keeps, beside its inputs and the output, what
+    the output's rounding left (as much again) and (H, T) fp32.  The derivative of
+    the backward raises."""
     return _torch_ext.load().packed_attention(q, k, v, cu_seqlens,
                                               cu_seqlens if cu_seqlens_k is None else cu_seqlens_k, scale, 0)

@@ -181,6 +181,29 @@ def test_packed_is_causal(dev):
     assert torch.equal(_run(*x, 0.125)["o"][:200], _run(*y, 0.125)["o"][:200])
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("shift", [0, 5, 31])
+def test_packed_garbage_stays_near(shift, hd, dev):
+    """A NaN in a row of v or k reaches, beside the queries that see it, at most
+    62 queries before them (k: none); one in dO at most 62 keys behind it."""
+    from naylis_amd.mom_kernels import packed_attention
+    q, k, v, d, cq, ck = _inputs([300], [300 + shift], 4, 2, hd, 0, 0, dev)
+    want = _run(q, k, v, d, cq, ck, 0.1)
+    for row in (64, 161, 200):
+        bad = [t.clone() for t in (q, k, v, d)]
+        bad[2][row] = math.nan
+        o = packed_attention(*bad[:3], cq, ck, scale=0.1)
+        first = row - shift  # the first query that sees it
+        assert torch.equal(o[:max(first - 62, 0)], want["o"][:max(first - 62, 0)]) and bool(o[first:].isnan().all())
+        bad[2], bad[1][row] = v, math.nan
+        o = packed_attention(*bad[:3], cq, ck, scale=0.1)
+        assert torch.equal(o[:first], want["o"][:first]) and bool(o[first:].isnan().all())
+        bad[1], bad[3][row] = k, math.nan
+        dv = _run(*bad, cq, ck, 0.1)["dv"]
+        last = row + shift  # the last key that it sees
+        assert torch.equal(dv[last + 63:], want["dv"][last + 63:]) and bool(dv[:last + 1].isnan().all())
+
+
 def test_packed_equals_the_batch_kernel(dev):
     """Equal lengths and heads of 64: the framework's batch attention within
     both kernels' bounds."""
