@@ -1194,8 +1194,10 @@ static int check_paged(int64_t pages, int64_t Hkv, int64_t page_size, int64_t B,
     return fail(NAYLIS_ERR_ARG, "%s: head_dim %lld must be 64 or 128", who, (long long)head_dim);
   if (page_size < 16 || page_size > 256 || (page_size & (page_size - 1)) != 0)
     return fail(NAYLIS_ERR_ARG, "%s: page_size %lld must be a power of two in [16, 256]", who, (long long)page_size);
+  // tokens of a table row: the kernels look up to 64 groups of 16 past a sequence's end in 32 bits
   if (pages < 1 || pages >= ((int64_t)1 << 31) || Hkv < 1 || Hkv > 4096 || G < 1 || G > 4096 || B < 0 || W < 1 ||
-      B > 65535 || W * page_size >= ((int64_t)1 << 31) || B * ((W * page_size + 31) / 32) >= ((int64_t)1 << 30))
+      B > 65535 || W > (((int64_t)1 << 31) - 2048) / page_size ||
+      B * ((W * page_size + 31) / 32) >= ((int64_t)1 << 30))
     return fail(NAYLIS_ERR_ARG, "%s: bad shape pages=%lld Hkv=%lld group=%lld B=%lld table width %lld", who,
                 (long long)pages, (long long)Hkv, (long long)G, (long long)B, (long long)W);
   return NAYLIS_OK;

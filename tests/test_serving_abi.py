@@ -107,6 +107,18 @@ def test_paged_attention_workspace(lib):
     assert _attn(lib, B=0) == _lib.NAYLIS_OK
 
 
+@pytest.mark.parametrize("page", [16, 256])
+def test_paged_tables_of_2_to_the_31_tokens(lib, page):
+    """A table row may hold 2^31 - 2048 tokens and no more: behind a longer sequence's
+    end the kernels' 32-bit token numbers would wrap, and their table reads with them."""
+    last = (2 ** 31 - 2048) // page
+    for W in (last + 1, last + 2, 2 ** 31 // page - 1, 2 ** 31 // page, 2 ** 60):
+        assert lib.naylis_mom_paged_attn_workspace_bytes(1, 1, 4, 2, page, 64, W) == 0
+        _refused(lib, _attn(lib, B=1, page=page, W=W), "bad shape")
+        _refused(lib, _append(lib, T=1, B=1, page=page, W=W), "bad shape")
+    assert lib.naylis_mom_paged_attn_workspace_bytes(1, 1, 4, 2, page, 64, last) > 0
+
+
 def _logprobs(lib, dtype=1, ld=100, N=3, V=100, top=0, x=P, tok=P, ids=P, ws=P, ws_bytes=1 << 40):
     return lib.naylis_mom_logprobs_fwd(x, dtype, ld, tok, P, P, P, ids, ids, ws, ws_bytes, N, V, top, -100, None)
 
