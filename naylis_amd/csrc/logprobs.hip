@@ -42,10 +42,12 @@ constexpr int kCand = 1024;     // candidates ranked at once
 constexpr int kMaxParts = 8;    // parts of a row
 constexpr float kLn2 = 0.6931471805599453f;
 
-// order of torch's descending sort as an unsigned key: NaN first, -0 equal to 0
+// order of torch's descending sort as an unsigned key: NaN first, -0 equal to 0.
+// No key is all ones: with column 0 that would make the rank key that stands
+// for "before every logit".
 __device__ __forceinline__ uint32_t sort_key(float x) {
   const uint32_t u = __float_as_uint(x + 0.f);
-  return x != x ? 0xffffffffu : (u >> 31) ? ~u : u | 0x80000000u;
+  return x != x ? 0xfffffffeu : (u >> 31) ? ~u : u | 0x80000000u;
 }
 
 template <typename T>
@@ -386,7 +388,7 @@ __global__ __launch_bounds__(NT) void logprobs_fwd_kernel(const T* __restrict__ 
       return;
     }
     // one pass for each: the best logit behind the last one taken
-    unsigned long long last = ~0ull;
+    unsigned long long last = ~0ull;  // no logit's key
     for (int i = 0; i < top; ++i) {
       unsigned long long best = 0;
       const auto see = [&](float f, int j) {

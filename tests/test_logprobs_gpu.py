@@ -137,6 +137,25 @@ def test_logprobs_ties_masks_and_nan(V, dev):
             assert abs(float(r.entropy[0]) - math.log(V)) < 1e-4  # V / 512 additions and more, each 2^-24
 
 
+@pytest.mark.parametrize("V", [70, 5003, 70001])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+def test_logprobs_nan_in_the_first_column(dtype, V, dev):
+    """A NaN in column 0 comes first like any other: rows of NaN, of -inf with a
+    NaN, of equal logits with a NaN (more of them than the ranking holds at once)."""
+    from naylis_amd.mom_kernels import token_logprobs
+    x = torch.full((5, V), math.nan, dtype=dtype, device=dev)
+    x[1] = -math.inf
+    x[2] = 1.0
+    x[1:3, 0] = math.nan
+    x[3] = -math.inf
+    x[3, [0, 60, V - 1]] = math.nan
+    x[4, V // 2:] = 0.0
+    for top in (1, 17, 64):
+        got = token_logprobs(x, torch.zeros(5, dtype=torch.long, device=dev), top=top)
+        assert torch.equal(got.top_ids, torch.sort(x, dim=-1, descending=True, stable=True)[1][:, :top]), top
+        assert bool(got.logp.isnan().all() and got.entropy.isnan().all() and got.top_logp.isnan().all())
+
+
 @pytest.mark.parametrize("V", [1003, 70001])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
 def test_logprobs_of_lowest_values(dtype, V, dev):
