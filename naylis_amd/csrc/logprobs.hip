@@ -336,8 +336,11 @@ __global__ __launch_bounds__(NT) void logprobs_fwd_kernel(const T* __restrict__ 
       const int w = __popcll(__ballot(lane < 16 && counts[round & 1][lane & 15] >= top)) - 1;
       bound |= (uint32_t)max(w, 0) << shift;
     }
-    // (bound 0: fewer threads than `top` have a logit)
-    const float least = bound == 0 ? -INFINITY : logit((unsigned long long)bound << (64 - KEYBITS));
+    // that value: bf16's keys lack the low half, zeros in a positive number's and ones in a
+    // negative one's.  -inf where fewer than `top` threads hold a larger logit: all are
+    // collected then
+    const float least = logit((unsigned long long)bound << (64 - KEYBITS) |
+                              (KEYBITS == 16 && bound >> 15 == 0 ? 0xffffull << 32 : 0));
     const bool plain = a.s == a.s;  // no NaN, which a maximum leaves out
     auto collect = [&](float f, int j) {
       if (f < least) return;
