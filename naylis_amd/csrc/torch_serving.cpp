@@ -20,8 +20,15 @@ at::TensorOptions f32_like(const at::Tensor& t) { return t.options().dtype(at::k
 bool wants_grad(std::initializer_list<at::Tensor> ts) {
   if (!at::GradMode::is_enabled()) return false;
   for (const at::Tensor& t : ts)
-    if (t.requires_grad()) return true;
+    if (t.defined() && t.requires_grad()) return true;
   return false;
+}
+
+// Dual tensors need no requires_grad: a call that looked at that alone would
+// return a constant for them.
+void no_tangents(std::initializer_list<at::Tensor> ts, const char* who) {
+  for (const at::Tensor& t : ts)
+    TORCH_CHECK(!t.defined() || !t._fw_grad(0).defined(), who, ": the forward-mode derivative is not implemented");
 }
 
 void on_gpu(const at::Tensor& t, const char* who, const char* name) {
@@ -159,6 +166,7 @@ at::Tensor packed_attention(const at::Tensor& q, const at::Tensor& k, const at::
   const at::Tensor ck = cu_k.is_same(cu_q) ? cq : indices(cu_k, q, who, "cu_seqlens_k");
   TORCH_CHECK(cq.dim() == 1 && cq.size(0) >= 2 && ck.sizes() == cq.sizes(), who,
               ": cu_seqlens and cu_seqlens_k must hold n + 1 offsets of the same n >= 1 sequences");
+  no_tangents({q, k, v}, who);
   const double scale = scale_of(scale_in, q.size(2));
   void* st = stream_of(stream, q);
   if (wants_grad({q, k, v})) return PackedAttention::apply(q, k, v, cq, ck, scale, reinterpret_cast<int64_t>(st));
@@ -213,7 +221,8 @@ void paged_append(const at::Tensor& kp, const at::Tensor& vp, const c10::optiona
   const char* who = "paged_append";
   const Cache c = cache_of(kp, vp, ks, vs, who);
   at::DeviceGuard guard(kp.device());
-  TORCH_CHECK(!wants_grad({k_in, v_in, kp, vp}), who, " has no backward: call it without gradients");
+  no_tangents({k_in, v_in, kp, vp, c.ks, c.vs}, who);
+  TORCH_CHECK(!wants_grad({k_in, v_in, kp, vp, c.ks, c.vs}), who, " has no backward: call it without gradients");
   at::NoGradGuard no_grad;
   TORCH_CHECK(k_in.dim() == 3 && v_in.sizes() == k_in.sizes() && k_in.size(1) == c.Hkv && k_in.size(2) == c.hd &&
                   k_in.scalar_type() == at::kBFloat16 && v_in.scalar_type() == at::kBFloat16,
@@ -243,7 +252,8 @@ at::Tensor paged_attention(const at::Tensor& q_in, const at::Tensor& kp, const a
   const char* who = "paged_attention";
   const Cache c = cache_of(kp, vp, ks, vs, who);
   at::DeviceGuard guard(kp.device());
-  TORCH_CHECK(!wants_grad({q_in, kp, vp}), who, " has no backward: call it without gradients");
+  no_tangents({q_in, kp, vp, c.ks, c.vs}, who);
+  TORCH_CHECK(!wants_grad({q_in, kp, vp, c.ks, c.vs}), who, " has no backward: call it without gradients");
   at::NoGradGuard no_grad;
   TORCH_CHECK(q_in.dim() == 3 && q_in.scalar_type() == at::kBFloat16 && q_in.size(2) == c.hd && c.Hkv > 0 &&
                   q_in.size(1) > 0 && q_in.size(1) % c.Hkv == 0,
@@ -361,6 +371,7 @@ variable_list token_logprobs(const at::Tensor& logits, const at::Tensor& tokens_
   same_device(tokens_in, logits, who, "tokens");
   TORCH_CHECK(tokens_in.scalar_type() == at::kLong || tokens_in.scalar_type() == at::kInt, who,
               ": tokens must be int64 or int32");
+  no_tangents({logits}, who);
   const at::Tensor tokens = tokens_in.reshape({-1}).to(at::kLong).contiguous();
   const at::Tensor x = logit_rows(logits);  // part of the graph where it copies
   void* st = stream_of(stream, logits);

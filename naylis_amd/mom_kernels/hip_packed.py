@@ -27,6 +27,6 @@ def packed_attention(q, k, v, cu_seqlens, cu_seqlens_k=None, scale=None):
     so a NaN or an infinity in a row of it reaches up to 62 rows that do not see
     it.  A forward with gradients keeps, beside its inputs and the output, what
     the output's rounding left (as much again) and (H, T) fp32.  The derivative of
-    the backward raises."""
+    the backward and forward-mode derivatives raise."""
     return _torch_ext.load().packed_attention(q, k, v, cu_seqlens,
                                               cu_seqlens if cu_seqlens_k is None else cu_seqlens_k, scale, 0)

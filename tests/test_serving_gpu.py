@@ -146,3 +146,40 @@ def test_operators_under_trace(dev):
         assert all(torch.equal(a, b) for a, b in pairs)
     with pytest.raises(RuntimeError, match="in place"):
         torch.jit.trace(lambda k: mk.paged_append(cache, k, k, table, lens), (rand(2, 2, 64),))
+
+
+def test_forward_mode_is_refused(dev):
+    """A dual tensor (which needs no requires_grad), with and without reverse mode,
+    raises in every operator that it reaches: no result without its tangent."""
+    from torch.autograd import forward_ad
+
+    from naylis_amd import mom_kernels as mk
+    g = torch.Generator(device=dev).manual_seed(7)
+    rand = lambda *s: torch.randn(*s, generator=g, device=dev).bfloat16()  # noqa: E731
+    cu, tok = torch.tensor([0, 5, 20], dtype=torch.int32, device=dev), torch.arange(4, device=dev)
+    bf, e4 = (mk.new_paged_cache(4, 2, 16, 64, dev, fp8=fp8) for fp8 in (False, True))
+    table = torch.arange(4, dtype=torch.int32, device=dev).view(2, 2)
+    lens = torch.tensor([1, 2], dtype=torch.int32, device=dev)
+    kv = lambda: (rand(2, 2, 64), rand(2, 2, 64))  # noqa: E731
+    calls = [(lambda q, k, v: mk.packed_attention(q, k, v, cu), (rand(20, 4, 64), rand(20, 2, 64), rand(20, 2, 64))),
+             (lambda x: mk.token_logprobs(x, tok), (rand(4, 100),)),
+             (lambda x: mk.token_logprobs(x, tok, top=3), (rand(4, 100).float(),)),
+             (lambda k, v: mk.paged_append(bf, k, v, table, lens), kv()),
+             (lambda q, k, v: mk.paged_attention(q, mk.PagedCache(k, v), table, lens), (rand(2, 4, 64), bf.k, bf.v)),
+             (lambda s, t: mk.paged_attention(rand(2, 4, 64), mk.PagedCache(e4.k, e4.v, s, t), table, lens),
+              (e4.k_scale, e4.v_scale)),
+             (lambda s, t: mk.paged_append(mk.PagedCache(e4.k, e4.v, s, t), *kv(), table, lens), (e4.k_scale, e4.v_scale))]
+    for call, args in calls:
+        call(*args)
+        for i, a in enumerate(args):
+            for grads in (False, True):
+                with torch.set_grad_enabled(grads), forward_ad.dual_level():
+                    dual = forward_ad.make_dual(a, torch.ones_like(a))
+                    with pytest.raises(RuntimeError, match="forward-mode"):
+                        call(*args[:i], dual, *args[i + 1:])
+            with pytest.raises(RuntimeError):
+                torch.func.jvp(lambda t: call(*args[:i], t, *args[i + 1:]), (a,), (torch.ones_like(a),))
+    for i in range(2):  # nor a cache's scales that want a gradient
+        for call, args in calls[-2:]:
+            with pytest.raises(RuntimeError, match="no backward"):
+                call(*(a.clone().requires_grad_(j == i) for j, a in enumerate(args)))
