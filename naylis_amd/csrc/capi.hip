@@ -1206,9 +1206,9 @@ static int check_paged(int64_t pages, int64_t Hkv, int64_t page_size, int64_t B,
 static int check_cache(const PagedCacheDims& c, int dtype, const char* who) {
   int rc = check_pointers({c.k, c.v}, who);
   if (rc) return rc;
-  if (dtype == NAYLIS_DTYPE_E4M3 && (!c.k_scale || !c.v_scale))
-    return fail(NAYLIS_ERR_ARG, "%s: an e4m3 cache needs its scales", who);
-  return NAYLIS_OK;
+  if (dtype != NAYLIS_DTYPE_E4M3) return NAYLIS_OK;
+  if (!c.k_scale || !c.v_scale) return fail(NAYLIS_ERR_ARG, "%s: an e4m3 cache needs its scales", who);
+  return check_pointers({c.k_scale, c.v_scale}, who);  // (read four at a time)
 }
 
 int naylis_mom_paged_append(void* k_pages, void* v_pages, float* k_scale, float* v_scale, int cache_dtype,

@@ -194,7 +194,7 @@ Cache cache_of(const at::Tensor& k, const at::Tensor& v, const c10::optional<at:
                   v.device() == k.device() && k.is_contiguous() && v.is_contiguous() &&
                   (uintptr_t)k.data_ptr() % 16 == 0 && (uintptr_t)v.data_ptr() % 16 == 0,
               who, ": the cache's k and v must be dense (pages, Hkv, page_size, head_dim) tensors of one type and ",
-              "device; got ", k.sizes(), " ", k.scalar_type(), ", ", v.sizes(), " ", v.scalar_type());
+              "device, 16-byte aligned; got ", k.sizes(), " ", k.scalar_type(), ", ", v.sizes(), " ", v.scalar_type());
   const bool codes = k.scalar_type() == at::kByte;
   TORCH_CHECK(codes || k.scalar_type() == at::kBFloat16, who,
               ": the cache must be bf16, or e4m3 codes in uint8 with scales; got ", k.scalar_type());
@@ -205,8 +205,8 @@ Cache cache_of(const at::Tensor& k, const at::Tensor& v, const c10::optional<at:
   if (codes)
     for (const at::Tensor& s : {c.ks, c.vs})
       TORCH_CHECK(s.scalar_type() == at::kFloat && s.is_contiguous() && s.device() == k.device() &&
-                      s.sizes() == k.sizes().slice(0, 3),
-                  who, ": k_scale and v_scale must be dense fp32 (pages, Hkv, page_size) tensors");
+                      s.sizes() == k.sizes().slice(0, 3) && (uintptr_t)s.data_ptr() % 16 == 0,
+                  who, ": k_scale and v_scale must be dense fp32 (pages, Hkv, page_size) tensors, 16-byte aligned");
   return c;
 }
 

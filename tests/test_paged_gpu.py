@@ -315,3 +315,19 @@ def test_paged_refusals(dev):
             paged_append(*args)
     assert paged_attention(q[:0], cache, table[:0], lens[:0]).shape == (0, 4, 64)
     paged_append(cache, k[:0], v[:0], table, pos[:0])
+
+
+def test_paged_scales_out_of_line_are_refused(dev):
+    """Dense scales that begin off a 16-byte boundary of a larger buffer."""
+    from naylis_amd.mom_kernels import PagedCache, paged_append, paged_attention
+    c = _case([20, 3], 4, 2, 64, 16, True, dev)
+    k, v, ks, vs = c["cache"]
+    for off in (1, 2, 3):
+        buf = torch.ones(ks.numel() + off, device=dev)
+        odd = buf[off:].view(ks.shape)
+        assert odd.is_contiguous()
+        for cache in (PagedCache(k, v, odd, vs), PagedCache(k, v, ks, odd)):
+            with pytest.raises(RuntimeError, match="paged_attention.*aligned"):
+                paged_attention(c["q"], cache, c["table"], c["lens"])
+            with pytest.raises(RuntimeError, match="paged_append.*aligned"):
+                paged_append(cache, c["k"][:2], c["v"][:2], c["table"], c["pos"][:2])

@@ -107,6 +107,18 @@ def test_paged_attention_workspace(lib):
     assert _attn(lib, B=0) == _lib.NAYLIS_OK
 
 
+@pytest.mark.parametrize("which", [0, 1])
+def test_scales_out_of_line_are_refused(lib, which):
+    """The kernels read an e4m3 cache's scales four at a time."""
+    for off in (4, 8, 12):
+        s = [P, P]
+        s[which] = ctypes.c_void_p(P.value + off)
+        _refused(lib, lib.naylis_mom_paged_attn(P, P, P, *s, 2, P, P, P, P, 1 << 40, _i64(256, 64), 0.1, 2, 4, 8, 2, 16, 64, 3,
+                                                None), "aligned")
+        _refused(lib, lib.naylis_mom_paged_append(P, P, *s, 2, P, P, _i64(128, 64, 128, 64), P, P, None, 4, 8, 2, 16, 64, 4, 3,
+                                                  None), "aligned")
+
+
 @pytest.mark.parametrize("page", [16, 256])
 def test_paged_tables_of_2_to_the_31_tokens(lib, page):
     """A table row may hold 2^31 - 2048 tokens and no more: behind a longer sequence's
