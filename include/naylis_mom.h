@@ -567,7 +567,8 @@ int naylis_mom_paged_attn(const void* q, const void* k_pages, const void* v_page
  * NULL; strides in elements, 0 for one value for all rows),
  *   dlogits_j = g_logp (1[j = token] - p_j) - g_entropy p_j (lp_j + entropy)
  * dense (N, V), in the logits' type; g_logp counts as 0 where the token is
- * ignore_index.
+ * ignore_index, and the row is 0 where g_entropy is 0 there too, whatever its
+ * logits.
  * logits (N, V) in dtype (bf16 or fp32), row stride row_stride elements, any V
  * and any address that its elements allow; N < 2^24, top <= min(64, V).  Workspace of the
  * forward: naylis_mom_logprobs_workspace_bytes, 8-byte aligned (0 bytes for

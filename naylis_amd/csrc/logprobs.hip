@@ -493,6 +493,13 @@ __global__ __launch_bounds__(256) void logprobs_bwd_kernel(const T* __restrict__
   T* dx = dlogits + r * (long)V;
   constexpr int U = kBwdChunks;
   const int end = min(out.chunks, begin + slab);
+  const int je = begin == 0 ? out.extra(threadIdx.x) : -1;
+  if (tok == ignore_index && ge == 0.f) {  // zeros, also where the row has no probabilities (-inf or NaN)
+    for (int c = begin + threadIdx.x; c < end; c += 256)
+      *reinterpret_cast<uint4*>(dx + out.first(c)) = make_uint4(0, 0, 0, 0);
+    if (je >= 0) dx[je] = T(0);
+    return;
+  }
   for (int c0 = begin + threadIdx.x; c0 < end; c0 += 256 * U) {
     uint4 u[U];
     if (same) {
@@ -525,7 +532,6 @@ __global__ __launch_bounds__(256) void logprobs_bwd_kernel(const T* __restrict__
       __builtin_nontemporal_store(o, reinterpret_cast<f32x4*>(dx + j0));
     }
   }
-  const int je = begin == 0 ? out.extra(threadIdx.x) : -1;
   if (je >= 0) {
     const float d = grad(value(x[je]), je);
     if constexpr (E == 8)

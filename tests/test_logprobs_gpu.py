@@ -199,6 +199,31 @@ def test_logprobs_ignored_and_bad_tokens(dev):
     assert bool((d[[0, 4]] == 0).all() and d[1:4].isnan().all())
 
 
+@pytest.mark.parametrize("V", [7, 300, 70001])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+def test_logprobs_ignored_rows_without_probabilities(dtype, V, dev):
+    """Padding rows of -inf or NaN, or with an infinity, whose token is ignored:
+    log probability 0, and a gradient of exactly 0 from it."""
+    from naylis_amd.mom_kernels import token_logprobs
+    x, tok = _rows(6, V, dtype, dev)
+    x[1] = -math.inf
+    x[2, V // 2] = math.nan
+    x[3] = math.nan
+    x[4, 3] = math.inf
+    tok[1:5] = -100
+    wide = torch.zeros(6, V + 3, dtype=dtype, device=dev)
+    wide[:, 1:V + 1] = x
+    for y in (x, wide[:, 1:V + 1].detach()):  # rows at the gradient's alignment, and at others
+        y.requires_grad_()
+        r = token_logprobs(y, tok)
+        assert bool((r.logp[1:5] == 0).all() and r.entropy[1:5].isnan().all())
+        d, = torch.autograd.grad(r.logp, y, torch.ones(6, device=dev), retain_graph=True)
+        assert bool((d[1:5] == 0).all() and d.isfinite().all() and d[[0, 5]].any(-1).all())
+        some = torch.tensor([1.0, 0.0, 0.0, 0.0, 0.0, 0.5], device=dev)  # the ignored rows' entropies are left out
+        d, = torch.autograd.grad((r.logp, r.entropy), y, (torch.ones(6, device=dev), some))
+        assert bool((d[1:5] == 0).all() and d.isfinite().all() and d[[0, 5]].any(-1).all())
+
+
 def test_logprobs_views_and_shapes(dev):
     """Rows of a padded buffer (any stride and address), leading dimensions,
     int32 tokens, sums' expanded gradients, streams."""
