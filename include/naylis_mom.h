@@ -559,10 +559,10 @@ int naylis_mom_paged_attn(const void* q, const void* k_pages, const void* v_page
  *   entropy (N) fp32 = -sum_j p_j lp_j
  *   top_ids (N, top) int64, top_logp (N, top) fp32: the `top` largest logits,
  *   descending, equal ones by the lowest index, NaN before all numbers
- *   stat (N, 3) fp32 for the backward (reference and log2 of the sum in powers
- *   of two, entropy); may be NULL
+ *   stat (N, 3) fp32 for the backward (largest logit, log2 of the sum in powers
+ *   of two against it, entropy); may be NULL
  * Columns of -inf have p = 0 and add nothing; a row without a finite logit is
- * NaN.  Logits over 2^24 either way count as 2^24.
+ * NaN.
  * The backward writes, for the gradients of logp and entropy (either may be
  * NULL; strides in elements, 0 for one value for all rows),
  *   dlogits_j = g_logp (1[j = token] - p_j) - g_entropy p_j (lp_j + entropy)

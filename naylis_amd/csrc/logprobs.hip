@@ -8,11 +8,10 @@
 // One workgroup per row (a few wide rows: one per part of a row, and a second
 // launch that joins them), any V, any row stride and address: 16-byte chunks
 // from the row's first 16-byte boundary, the few elements beside them one a
-// thread.  Forward: one pass with a running reference c (log2 of the largest
-// e^x so far), s = sum 2^z and t = sum 2^z z, z = x log2 e - c, per thread;
-// H = (log2 s - t / s) ln 2.  All statistics are fp32, saved as (c, log2 s, H):
-// lp = (x log2 e - c - log2 s) ln 2 keeps the last bits that a single
-// log-sum-exp would lose.
+// thread.  Forward: one pass with a running reference m (the largest logit so
+// far), s = sum 2^z and t = sum 2^z z, z the log2 of e^x over e^m, per thread; H =
+// (log2 s - t / s) ln 2.  All statistics are fp32, saved as (m, log2 s, H): lp =
+// (z - log2 s) ln 2 keeps the last bits that a single log-sum-exp would lose.
 //
 // The top k come from a second look at the row (registers, or the caches): the
 // k-th largest of the threads' maxima is a value that at least k logits reach,
@@ -112,26 +111,45 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return r;
 }
 
-// Logits over 2^24 either way count as 2^24, infinities stay: a row masked by the
-// type's lowest value is even, not NaN.  x log2 e - c below keeps what rounding c
-// left of the product, at most 1 for the largest x up to here and 2^102 at 2e38.
-constexpr float kMost = 16777216.f;
-__device__ __forceinline__ float tame(float x) {
-  return fabsf(x) > kMost && fabsf(x) != INFINITY ? copysignf(kMost, x) : x;
+// The reference of a sum of powers of two is its largest logit m, as c = m log2 e
+// rounded once: all its terms x log2 e - c use the same c, so its rounding drops
+// out.  Past 2^24 that rounding is more than an exponent may be off (and c can
+// overflow): there the reference is m itself, and the terms are (x - m) log2 e.
+constexpr float kFar = 16777216.f;
+__device__ __forceinline__ bool is_far(float m) { return fabsf(m) > kFar; }
+
+// log2 of e^m over e^w for the references m and w, no less than -1e20 (finite
+// times any sum)
+__device__ __forceinline__ float ref_step(float m, float w) {
+#pragma clang fp contract(off)
+  const float c = m * kLog2e, cw = w * kLog2e;
+  float d = c - cw;
+  if (is_far(m) || is_far(w)) {
+    d = is_far(m) ? is_far(w) ? (m - w) * kLog2e : fmaf(m, kLog2e, -cw) : -fmaf(w, kLog2e, -c);
+    d = d < -1e20f ? -1e20f : d;
+  }
+  return d;
 }
 
-// Sums of a part of a row in powers of two, against a reference c (the log2 of
-// its largest e^x, rounded once: all terms of a sum use the same number, so its
-// rounding drops out): s = sum 2^z, t = sum 2^z z with z = x log2 e - c.
-// m is the largest x itself.
+// log2 of e^x over e^m for the reference m (near: one within 2^24)
+__device__ __forceinline__ float log2_near(float x, float m) {
+  const float c = m * kLog2e;
+  return fmaf(x, kLog2e, -c);
+}
+__device__ __forceinline__ float log2_ratio(float x, float m) {
+  return is_far(m) ? (x - m) * kLog2e : log2_near(x, m);
+}
+
+// Sums of a part of a row against its largest x, m: s = sum 2^z, t = sum 2^z z
+// with z the log2 of e^x over e^m.
 struct Sums {
-  float m, c, s, t;
+  float m, s, t;
   // against the reference of a whole; an empty part (m = -inf) weighs nothing
-  __device__ __forceinline__ void rescale(float cw) {
-    const float d = c - cw, a = __builtin_amdgcn_exp2f(d);
+  __device__ __forceinline__ void rescale(float w) {
+    const float d = ref_step(m, w), a = __builtin_amdgcn_exp2f(d);
     t = m == -INFINITY ? 0.f : a * fmaf(d, s, t);
     s = m == -INFINITY ? 0.f : a * s;
-    c = cw;
+    m = w;
   }
 };
 
@@ -151,28 +169,27 @@ __device__ __forceinline__ void add_chunks(Sums& a, const uint4 (&u)[U], bool& n
       for (int e = 0; e < E; ++e) nan |= element<E>(u[i], e) != element<E>(u[i], e);
     return;
   }
-  const float c = tame(m) * kLog2e;
   if (a.m == -INFINITY)
-    a.c = c;
+    a.m = m;
   else if (m > a.m)
-    a.rescale(c);
-  a.m = m;
+    a.rescale(m);
   float s[2] = {a.s, 0.f}, t[2] = {a.t, 0.f};  // two chains
-  auto add = [&](auto cut) {
+  auto add = [&](auto log2_of) {
 #pragma unroll
     for (int i = 0; i < U; ++i)
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        const float z = fmaf(cut(element<E>(u[i], e)), kLog2e, -a.c), p = __builtin_amdgcn_exp2f(z);
+        const float z = log2_of(element<E>(u[i], e)), p = __builtin_amdgcn_exp2f(z);
         s[e & 1] += p;
         t[e & 1] = fmaf(p, fmaxf(z, -1e30f), t[e & 1]);  // 0 log 0 = 0
       }
   };
-  // beside a largest value within 2^24 a lower one weighs nothing, cut or not
-  if (__ballot(fabsf(m) > kMost) == 0)
-    add([](float x) { return x; });
-  else
-    add(tame);
+  if (__ballot(is_far(m)) == 0) {
+    add([&](float x) { return log2_near(x, a.m); });
+  } else {  // log2_ratio of both kinds of lanes in one form
+    const float from = is_far(m) ? a.m : 0.f, c = is_far(m) ? 0.f : a.m * kLog2e;
+    add([&](float x) { return fmaf(x - from, kLog2e, -c); });
+  }
   a.s = s[0] + s[1];
   a.t = t[0] + t[1];
 }
@@ -181,15 +198,11 @@ __device__ __forceinline__ void add_chunks(Sums& a, const uint4 (&u)[U], bool& n
 __device__ __forceinline__ void add_one(Sums& a, float x, bool& nan) {
   nan |= x != x;
   if (!(x > -INFINITY)) return;
-  const float y = tame(x);
-  if (a.m == -INFINITY) {
+  if (a.m == -INFINITY)
     a.m = x;
-    a.c = y * kLog2e;
-  } else if (x > a.m) {
-    a.m = x;
-    a.rescale(y * kLog2e);
-  }
-  const float z = fmaf(y, kLog2e, -a.c), p = __builtin_amdgcn_exp2f(z);
+  else if (x > a.m)
+    a.rescale(x);
+  const float z = log2_ratio(x, a.m), p = __builtin_amdgcn_exp2f(z);
   a.s += p;
   a.t = fmaf(p, fmaxf(z, -1e30f), a.t);
 }
@@ -204,16 +217,17 @@ __device__ __forceinline__ float logit(unsigned long long k) {
   return __uint_as_float((u >> 31) ? u & 0x7fffffffu : ~u);
 }
 
-// log p of a logit from its row's reference and log2 of its sum
-__device__ __forceinline__ float log_prob(float x, float c, float ls) {
-  return (fmaf(tame(x), kLog2e, -c) - ls) * kLn2;
+// log p of a logit from its row's reference and log2 of its sum; a far logit's in
+// its own units, where its product with log2 e may overflow
+__device__ __forceinline__ float log_prob(float x, float m, float ls) {
+  return is_far(x) || is_far(m) ? (x - m) - ls * kLn2 : (log2_near(x, m) - ls) * kLn2;
 }
 
 // Joins the sums of `count` <= 64 parts that stand in LDS; every lane gets them.
-__device__ __forceinline__ Sums join_parts(const float* c, const float* s, const float* t, int count) {
+__device__ __forceinline__ Sums join_parts(const float* m, const float* s, const float* t, int count) {
   const int lane = threadIdx.x & 63, i = min(lane, count - 1);
-  Sums a{c[i], c[i], s[i], t[i]};
-  a.rescale(wave_allmax(a.c));
+  Sums a{m[i], s[i], t[i]};
+  a.rescale(wave_allmax(a.m));
   a.s = wave_allsum(lane < count ? a.s : 0.f);
   a.t = wave_allsum(lane < count ? a.t : 0.f);
   return a;
@@ -228,14 +242,14 @@ struct LogprobsOut {
 };
 
 // A row's numbers from its sums (one thread); returns log2 s.  A row without a
-// finite logit: c = -inf, NaN throughout.
+// finite logit: m = -inf, NaN throughout.
 __device__ __forceinline__ void write_row(const LogprobsOut& o, long r, const Sums& a, float ls, float xt, bool ignored,
                                           bool in_range) {
   const float ent = (ls - a.t / a.s) * kLn2;
-  o.logp[r] = ignored ? 0.f : in_range ? log_prob(xt, a.c, ls) : __builtin_nanf("");
+  o.logp[r] = ignored ? 0.f : in_range ? log_prob(xt, a.m, ls) : __builtin_nanf("");
   o.entropy[r] = ent;
   if (o.stat) {
-    o.stat[3 * r] = a.c;
+    o.stat[3 * r] = a.m;
     o.stat[3 * r + 1] = ls;
     o.stat[3 * r + 2] = ent;
   }
@@ -271,7 +285,7 @@ __global__ __launch_bounds__(NT) void logprobs_fwd_kernel(const T* __restrict__ 
   const int je = row.extra(tid);
   const float xe = je >= 0 ? value(row.x[je]) : -INFINITY;
 
-  Sums a{-INFINITY, -INFINITY, 0.f, 0.f};
+  Sums a{-INFINITY, 0.f, 0.f};
   bool nan = false;
   uint4 u[U];
   if constexpr (HELD) {
@@ -285,12 +299,12 @@ __global__ __launch_bounds__(NT) void logprobs_fwd_kernel(const T* __restrict__ 
   }
   add_one(a, xe, nan);
   const float mine = a.m;  // one of the logits, or -inf
-  if (nan) a = Sums{0.f, 0.f, __builtin_nanf(""), 0.f};
-  a.rescale(wave_allmax(a.c));
+  if (nan) a = Sums{0.f, __builtin_nanf(""), 0.f};
+  a.rescale(wave_allmax(a.m));
   a.s = wave_allsum(a.s);
   a.t = wave_allsum(a.t);
   if (lane == 0) {
-    red[0][wave] = a.c;
+    red[0][wave] = a.m;
     red[1][wave] = a.s;
     red[2][wave] = a.t;
   }
@@ -302,7 +316,7 @@ __global__ __launch_bounds__(NT) void logprobs_fwd_kernel(const T* __restrict__ 
     if (parts == 1) {
       write_row(o, r, a, ls, xt, tok == ignore_index, in_range);
     } else {
-      part_sums[3 * part] = a.c;
+      part_sums[3 * part] = a.m;
       part_sums[3 * part + 1] = a.s;
       part_sums[3 * part + 2] = a.t;
     }
@@ -374,7 +388,7 @@ __global__ __launch_bounds__(NT) void logprobs_fwd_kernel(const T* __restrict__ 
     auto write = [&](int rank, unsigned long long k) {
       if (parts == 1) {
         o.top_ids[r * top + rank] = column(k);
-        o.top_logp[r * top + rank] = log_prob(logit(k), a.c, ls);
+        o.top_logp[r * top + rank] = log_prob(logit(k), a.m, ls);
       } else {
         part_keys[part * top + rank] = k;
       }
@@ -449,7 +463,7 @@ __global__ __launch_bounds__(256) void logprobs_join_kernel(const T* __restrict_
     for (int j = 0; j < n; ++j) rank += cand[j] > k;
     if (rank < top) {
       o.top_ids[r * top + rank] = column(k);
-      o.top_logp[r * top + rank] = log_prob(logit(k), a.c, ls);
+      o.top_logp[r * top + rank] = log_prob(logit(k), a.m, ls);
     }
   }
 }
@@ -482,13 +496,10 @@ __global__ __launch_bounds__(256) void logprobs_bwd_kernel(const T* __restrict__
                    : tok >= 0 && tok < V          ? g_logp[r * gl_stride]
                                                   : __builtin_nanf("");
   const float ge = g_entropy ? g_entropy[r * ge_stride] : 0.f;
-  // beside a largest value within 2^24 a lower one weighs nothing, cut or not
-  const bool far = fabsf(ref) >= kMost * kLog2e;
   // z ln 2 = log p; 0 log 0 = 0 (the comparison keeps NaN)
   const auto grad = [&](float f, int j) {
-    if (far) f = tame(f);
-    const float z = fmaf(f, kLog2e, -ref) - ls, p = __builtin_amdgcn_exp2f(z);
-    return (j == tok ? gl : 0.f) - p * fmaf(ge, fmaf(z < -1e30f ? -1e30f : z, kLn2, ent), gl);
+    const float z = log2_ratio(f, ref) - ls, p = __builtin_amdgcn_exp2f(z);
+    return (j == tok ? gl : 0.f) - p * fmaf(ge, fmaf(z < -1e3f ? -1e3f : z, kLn2, ent), gl);
   };
   T* dx = dlogits + r * (long)V;
   constexpr int U = kBwdChunks;

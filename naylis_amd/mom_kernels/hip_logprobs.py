@@ -28,8 +28,8 @@ def token_logprobs(logits, tokens, top=0, ignore_index=-100) -> TokenLogprobs:
 
     logp is 0 (with no gradient) where the token is ignore_index, NaN where it
     is neither that nor in [0, V).  Columns of -inf have no probability and add
-    nothing, logits over 2^24 either way count as 2^24.  top (up to 64) gives
-    each row's largest logits, equal ones by the lowest index.  The derivative of
+    nothing; finite logits may be of any size.  top (up to 64) gives each row's
+    largest logits, equal ones by the lowest index.  The derivative of
     the backward and forward-mode derivatives raise."""
     logp, entropy, ids, lps = _torch_ext.load().token_logprobs(logits, tokens, int(top), int(ignore_index), 0)
     return TokenLogprobs(logp, entropy, ids if top else None, lps if top else None)

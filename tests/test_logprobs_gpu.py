@@ -182,6 +182,56 @@ def test_logprobs_of_lowest_values(dtype, V, dev):
     assert abs(float(d[0, 7]) - (1 - 1 / V)) < 2.0 ** -8
 
 
+@pytest.mark.parametrize("V", [9, 1003, 70001])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+def test_logprobs_of_logits_of_any_size(dtype, V, dev):
+    """Logits past 2^24, where x log2 e is off by more than 1: rows of a few far
+    values apart, close together, on both sides of 2^24, up to the type's ends, and
+    tokens masked by a large negative number; against fp64 of the same values.
+
+    Bounds: of e^(x - m), x - m is exact where it matters (fp32, under 2^7, and its
+    operands within a factor of two), so the sums' errors are those of _reference; a
+    log probability of -d with d large is one rounding of x - m, one of it less log
+    s and two of a product with log2 e and back (2^-22 d in all); of the near rows,
+    whose reference is rounded, d itself is off by 2^-24 of the logits' size."""
+    from naylis_amd.mom_kernels import token_logprobs
+    low, big = torch.finfo(dtype).min, torch.finfo(dtype).max
+    step = 2.0 ** 24 * torch.finfo(dtype).eps  # neighbouring values at 2^24
+    rows = [[2e7, 3e7], [-3e7, -2e7], [2.0 ** 24, 2.0 ** 24 + 2 * step], [2.0 ** 24, 2.0 ** 24 - step],
+            [-2.0 ** 24 - 2 * step, -2.0 ** 24 + step], [1e30, 1.5e30], [low, 0.0], [low, 5.0], [-1e9, 3.0],
+            [low, big], [big, big], [low, low], [-1e30, 2e7], [-2e7, 1e7], [0.0, 1e38]]
+    g = torch.Generator(device=dev).manual_seed(9)
+    pick = torch.randint(0, 2, (len(rows), V), generator=g, device=dev)
+    pick[:, 0], pick[:, 1], pick[:, V - 1] = 0, 1, 0
+    x = torch.tensor(rows, dtype=torch.float64, device=dev).to(dtype).gather(1, pick)
+    x[:, 3] = -math.inf
+    x.requires_grad_()
+    z = x.detach().double()
+    for col in (0, 1, V - 1):
+        tok = torch.full((len(rows),), col, device=dev)
+        r = token_logprobs(x, tok, top=5)
+        lp = torch.log_softmax(z, -1)
+        p = lp.exp()
+        want, entropy = lp[:, col], -torch.where(p > 0, p * lp, 0.0).sum(-1)
+        m = z.amax(-1)
+        near = torch.where(m.abs() <= 2.0 ** 24, m.abs(), 0.0) * 2.0 ** -22
+        d = torch.where(p > 0, p * (z - m[:, None]), 0.0).abs().sum(-1)
+        s_err = (V / 512 + 80 + 2 * d) * 2.0 ** -23
+        err = s_err + want.abs() * 2.0 ** -22 + math.log(V) * 2.0 ** -22 + torch.where(want < -1, near, 0.0)
+        fits = want.float().isfinite()  # (low less big rounds to no fp32 number; low less a logarithm rounds to low)
+        assert bool((r.logp.double() - want).abs()[fits].le(err[fits]).all()), (r.logp, want)
+        assert bool((r.logp[~fits] == -math.inf).all())
+        assert bool(((r.entropy.double() - entropy).abs() <= 2 * s_err * (1 + d) + (d + 12) * 2.0 ** -22).all())
+        assert torch.equal(r.top_ids, torch.sort(x.detach(), dim=-1, descending=True, stable=True)[1][:, :5])
+        dx, = torch.autograd.grad(r.logp.sum() + r.entropy.sum(), x)
+        hot = torch.zeros_like(lp)
+        hot[:, col] = 1
+        grad = hot - p - torch.where(p > 0, p * (lp + entropy[:, None]), 0.0)
+        size = hot + p + torch.where(p > 0, p * (lp.abs() + entropy[:, None]), 0.0)
+        tol = torch.finfo(dtype).eps / 2 * grad.abs() + (s_err * (3 + d) + (d + 12) * 2.0 ** -21)[:, None] * size + 1e-30
+        assert bool(((dx.double() - grad).abs() <= tol).all()), float(((dx.double() - grad).abs() / tol).max())
+
+
 def test_logprobs_ignored_and_bad_tokens(dev):
     from naylis_amd.mom_kernels import token_logprobs
     x, _ = _rows(5, 300, torch.bfloat16, dev)
