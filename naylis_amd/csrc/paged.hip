@@ -306,7 +306,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedCacheDims c, co
     f32x4 acc[NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) acc[t] = f32x4{};
-    float m = kNegBig, l = 0.f;
+    float m = kLowest, l = 0.f;
 
     // pages of the next 64 products' tokens, one a lane
     int ids = 0, ids_at = -64;
@@ -504,7 +504,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedCacheDims c, co
       px[e] = *reinterpret_cast<const f32x4*>(
           reinterpret_cast<const float*>(lds + (e >> 1) * kWaveLds<HD, ROWS> + part_offset<HD>(e & 1)) + r * HD + f);
     }
-    float m = kNegBig, l = 0.f;
+    float m = kLowest, l = 0.f;
     f32x4 a = f32x4{};
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -527,7 +527,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedCacheDims c, co
         *reinterpret_cast<f32x4*>(part + row * HD + f) = a;
         if (f == 0) stat[row] = make_float2(m, l);
       }
-      m = kNegBig;
+      m = kLowest;
       l = 0.f;
       a = f32x4{};
     }
@@ -586,11 +586,11 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedCacheDims c, const
   const auto piece = [&](int i) { return *reinterpret_cast<const f32x4*>(part + row(i) * HD + 4 * f); };
   const f32x4 mine = piece(min(gi, count - 1));
   float2 st[kPagedMaxWgs / 256];
-  float m = kNegBig, l = 0.f;
+  float m = kLowest, l = 0.f;
 #pragma unroll
   for (int u = 0; u < kPagedMaxWgs / 256; ++u) {
     const int i = tid + 256 * u;
-    st[u] = i < count ? stat[row(i)] : float2{kNegBig, 0.f};
+    st[u] = i < count ? stat[row(i)] : float2{kLowest, 0.f};
     m = fmaxf(m, st[u].x);
   }
   m = block(m, [](float a, float b) { return fmaxf(a, b); });

@@ -331,3 +331,33 @@ def test_paged_scales_out_of_line_are_refused(dev):
                 paged_attention(c["q"], cache, c["table"], c["lens"])
             with pytest.raises(RuntimeError, match="paged_append.*aligned"):
                 paged_append(cache, c["k"][:2], c["v"][:2], c["table"], c["pos"][:2])
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("lens", [[1, 40, 33, 300], [3000, 1, 70]])  # tables of one launch, and of two
+@pytest.mark.parametrize("size", [2.0 ** 17, 2.0 ** 50, 2.0 ** 60])
+def test_paged_scores_of_any_size(size, lens, hd, fp8, dev):
+    """Scores of +-2^30, 2^96 and 2^116: each sequence has a few tokens with the
+    highest one, so its result is their mean; once with all scores negative, once
+    positive.  Weights are 0 or 1, their sum exact, e4m3 values times their scale
+    rounded once to bf16, and the result once: 2^-8 each of the values."""
+    from naylis_amd.mom_kernels import PagedCache, paged_append, paged_attention
+    c = _case(lens, 4, 2, hd, 16, fp8, dev)
+    k, q = torch.zeros_like(c["k"]), torch.zeros_like(c["q"])
+    q[..., 3] = size
+    best = (c["pos"] * 7 + c["rows"]) % 11 == 0
+    first = torch.nn.functional.pad(c["lens"].cumsum(0), (1, 0))[:-1].long()
+    best[first] = True
+    for sign in (-1, 1):
+        k[..., 3] = sign * size * torch.where(best, 1.0 if sign > 0 else 0.5, 0.5 if sign > 0 else 1.0)[:, None]
+        paged_append(c["cache"], k, c["v"], c["table"], c["pos"], c["rows"])
+        got = paged_attention(q, c["cache"], c["table"], c["lens"], scale=0.125).double()
+        _, v = PagedCache(*c["cache"]).dequantize()
+        page, off = c["table"][c["rows"].long(), c["pos"].long() // 16].long(), c["pos"].long() % 16
+        v = v.double()[page, :, off]
+        for b in range(len(lens)):
+            mine = v[(c["rows"] == b) & best]
+            want = mine.mean(0).repeat_interleave(2, 0)
+            bound = mine.abs().mean(0).repeat_interleave(2, 0) * (2.0 ** -7 + 2.0 ** -20)
+            assert bool(((got[b] - want).abs() <= bound).all()), (b, sign)
