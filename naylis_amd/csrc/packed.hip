@@ -41,6 +41,9 @@ constexpr int kStageRows = 64;
 // weights reach 2^8, which costs fp32 sums and bf16 weights nothing, and few
 // tiles rescale the sums (of 32 queries one has a new maximum in most tiles).
 constexpr float kSlack = 8.f;
+// Past this (log2 domain) the reference's own rounding is more than 2^16 in a
+// weight, as a fused score - reference leaves it; there scores are rounded first.
+constexpr float kFarScore = 268435456.f;
 
 // LDS rows of HD bf16 without padding; 16-byte chunk c of row r sits in slot
 // c ^ swz(r).  16 consecutive rows' chunk c then cover 256 bytes (row
@@ -393,21 +396,38 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void packed_fwd_kernel(
 
   f32x16 acc[NT], x;  // x: scores of the tile at hand
   clear(acc);
-  float m = kNegBig, l = 0.f, inf;
+  float m = kLowest, l = 0.f, inf;
+  float ce = c;      // what scores are multiplied by: 1 in lanes whose scores are far and were multiplied before
+  bool far = false;  // whether the wave has such lanes
   // (a known infinity would turn the median below into a maximum of three instructions)
   asm("s_mov_b32 %0, 0x7f800000" : "=s"(inf));
   // mask of tile t, its maximum, and the sums rescaled where that is far above the reference
   auto settle = [&](f32x16& z, int t) {
-    if (32 * t + 31 > q0 + shift) {
+    auto times_c = [&](bool mine) {
+      const float f = mine ? c : 1.f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) z[i] *= f;
+    };
+    if (32 * t + 31 > q0 + shift || far) {
       asm volatile("");  // a branch, not 16 selects for every tile
 #pragma unroll
       for (int i = 0; i < 16; ++i)
         if (32 * t + acc_row(g, i) > row + shift) z[i] = -INFINITY;
+      if (far) times_c(ce != c);
     }
-    const float over = fmaf(max_of(__builtin_amdgcn_fmed3f(z[0], z[1], inf), z), c, -kSlack);
+    auto over_of = [&]() { return fmaf(max_of(__builtin_amdgcn_fmed3f(z[0], z[1], inf), z), ce, -kSlack); };
+    const float over = over_of();
     if (__builtin_expect(__any(over > m), 0)) {
       // per query, so that a row's result does not depend on its neighbours'
-      const float most = xor32_f32(over, [](float a, float b) { return fmaxf(a, b); });
+      const auto fmx = [](float a, float b) { return fmaxf(a, b); };
+      float most = xor32_f32(over, fmx);
+      const bool turns = fabsf(most) > kFarScore && most != -INFINITY && ce == c;
+      if (__any(turns)) {
+        far = true;
+        times_c(turns);
+        if (turns) ce = 1.f;
+        most = xor32_f32(over_of(), fmx);
+      }
       const float mn = most > m ? most + kSlack : m;
       const float al = __builtin_amdgcn_exp2f(m - mn);
       m = mn;
@@ -419,7 +439,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void packed_fwd_kernel(
     }
   };
   auto weigh = [&](f32x16& p, int i) {
-    p[i] = __builtin_amdgcn_exp2f(SPLIT == 1 ? p[i] : fmaf(p[i], c, -m));
+    p[i] = __builtin_amdgcn_exp2f(SPLIT == 1 ? p[i] : fmaf(p[i], ce, -m));
     l += p[i];
   };
   // Tile t (the first or second of its stage) with its scores in x; leaves those of
@@ -432,7 +452,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void packed_fwd_kernel(
     f32x16 p = x;  // weights; their exponents before the branch, so that the next scores can take x's registers
     if constexpr (SPLIT == 1) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) p[i] = fmaf(x[i], c, -m);
+      for (int i = 0; i < 16; ++i) p[i] = fmaf(x[i], ce, -m);
     }
     auto add_pv = [&]() {
       const bf16x8 pf[2] = {pack8(p, 0), pack8(p, 8)};
@@ -497,7 +517,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void packed_fwd_kernel(
     }
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the late loads (zeros) land before LDS goes to another workgroup
-  if constexpr (SPLIT == 2) {  // the odd tiles' sums to the even ones' (m is -1e30 and all else 0 where there were none)
+  if constexpr (SPLIT == 2) {  // the odd tiles' sums to the even ones' (m is kLowest and all else 0 where there were none)
     float* sums = reinterpret_cast<float*>(ring) + wave / 2 * (HD / 2 + 2) * 64 + lane;
     lds_barrier();
     if (share == 1) {

@@ -204,6 +204,69 @@ def test_packed_garbage_stays_near(shift, hd, dev):
         assert torch.equal(dv[last + 63:], want["dv"][last + 63:]) and bool(dv[:last + 1].isnan().all())
 
 
+def _far_inputs(size, sign, lens, H, Hkv, hd, dev):
+    """Scores of up to size^2 / 8 either way, each of few values (equal ones equal
+    bit for bit, others far apart), and queries so small that theirs are ordinary."""
+    q, k, v, d, cq, ck = _inputs(*lens, H, Hkv, hd, 0, 0, dev)
+    i, j = (torch.arange(t.shape[0], device=dev)[:, None] for t in (q, k))
+    q, k = torch.zeros_like(q), torch.zeros_like(k)
+    q[..., 3] = torch.where(i % 3 == 0, 2.0 ** -6 / size, size * 2.0 ** -(i % 2))
+    grade = torch.where((j * 5) % 13 == 0, 4.0, 2.0) * torch.where(j < 70, 0.25, 1.0)  # rises within a walk
+    k[..., 3] = sign * size / 4 * (grade if sign > 0 else 5 - grade)
+    return q, k, v, d, cq, ck
+
+
+FAR = [2.0 ** 10, 2.0 ** 17, 2.0 ** 30, 2.0 ** 60]
+FAR_LENS = [([300, 1, 33], None), ([90, 200], [400, 260]), ([40], [20])]
+
+
+@pytest.mark.parametrize("hd,H", [(64, 4), (128, 4), (64, 600), (128, 400)])  # two waves for 32 queries, and one
+@pytest.mark.parametrize("lens", FAR_LENS, ids=["same", "earlier", "none"])
+@pytest.mark.parametrize("sign", [-1, 1])
+@pytest.mark.parametrize("size", FAR)
+def test_packed_scores_of_any_size(size, sign, lens, hd, H, dev):
+    """Weights of far scores are 0 or equal ones; the bounds are the ordinary ones."""
+    from naylis_amd.mom_kernels import packed_attention
+    q, k, v, d, cq, ck = _far_inputs(size, sign, lens, 4, 2, hd, dev)
+    want = _reference(q, k, v, d, cq, ck, 0.125)["o"]
+    wide = lambda t: t.repeat(1, H // 4, 1)  # noqa: E731
+    heads = torch.arange(H, device=dev) % 2 if H > 4 else torch.arange(2, device=dev)
+    o = packed_attention(wide(q), k[:, heads], v[:, heads], cq, ck, scale=0.125)
+    for h in range(0, H, max(H // 8, 1)):
+        kv = int(heads[h]) if H > 4 else h // 2
+        err = (o[:, h].double() - want[0][:, 2 * kv]).abs()
+        assert bool((err <= want[1][:, 2 * kv] + 1e-30).all()), (h, float(err.max()))
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("size", [2.0 ** 8, 2.0 ** 16, 2.0 ** 30])
+def test_packed_far_random_scores(size, hd, dev):
+    """Random far scores: where a query's highest lies clear of the next one by
+    more than fp32 sums of hd products may be off, its result is that key's v (within
+    the roundings of P and of the result); an
+    ordinary query's does not depend on its far neighbours, bit for bit."""
+    from naylis_amd.mom_kernels import packed_attention
+    q, k, v, d, cq, ck = _inputs([200, 130], [350, 130], 4, 2, hd, 0, 0, dev)
+    usual = packed_attention(q, k, v, cq, ck)
+    far = torch.arange(330, device=dev) % 5 != 0
+    q = torch.where(far[:, None, None], q * size * size, q)
+    o = packed_attention(q, k, v, cq, ck)
+    assert bool(o.isfinite().all()) and torch.equal(o[~far], usual[~far])
+    clear = 0
+    for a, b, e, f in ((0, 200, 0, 350), (200, 330, 350, 480)):
+        see = torch.ones(b - a, f - e, dtype=torch.bool, device=dev).tril(f - e - b + a)
+        for h in range(4):
+            x, y = q[a:b, h].double(), k[e:f, h // 2].double()
+            s = (x @ y.T * hd ** -0.5).masked_fill(~see, -math.inf)
+            noise = (x.abs() @ y.abs().T * hd ** -0.5).amax(-1) * hd * 2.0 ** -23
+            top, at = s.topk(2, -1)
+            sure = far[a:b] & (top[:, 0] - top[:, 1] > 2 * noise + 40)
+            clear += int(sure.sum())
+            best = v[e:f, h // 2][at[sure, 0]].double()  # (times P / l, whose P is rounded to bf16, and rounded once)
+            assert bool(((o[a:b, h][sure].double() - best).abs() <= best.abs() * (2.0 ** -7 + 2.0 ** -10)).all())
+    assert clear > 300
+
+
 def test_packed_equals_the_batch_kernel(dev):
     """Equal lengths and heads of 64: the framework's batch attention within
     both kernels' bounds."""
