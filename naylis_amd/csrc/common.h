@@ -219,6 +219,7 @@ __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNegBig = -1.0e30f;  // finite "minus infinity" for running maxima
-constexpr float kLowest = -3.4028234664e38f;  // the lowest fp32 number: a running maximum that any finite score takes part in
+// the lowest fp32 number: a running maximum that any finite score takes part in
+constexpr float kLowest = -3.4028234664e38f;
 
 }  // namespace naylis

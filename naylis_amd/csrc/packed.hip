@@ -44,6 +44,17 @@ constexpr float kSlack = 8.f;
 // Past this (log2 domain) the reference's own rounding is more than 2^16 in a
 // weight, as a fused score - reference leaves it; there scores are rounded first.
 constexpr float kFarScore = 268435456.f;
+// Past this the log-sum-exp's rounding shows in the weights of the gradients
+// (2^-12 at most up to here): such rows' weights are formed against it and divided by
+// their sum.
+constexpr float kFarLse = 4096.f;
+
+// log2 of a weight against the log-sum-exp `lse` of far scores
+__device__ __forceinline__ float far_exponent(float x, float c, float lse) {
+#pragma clang fp contract(off)
+  const float rounded = x * c;
+  return fabsf(lse) > kFarScore ? rounded - lse : fmaf(x, c, -lse);
+}
 
 // LDS rows of HD bf16 without padding; 16-byte chunk c of row r sits in slot
 // c ^ swz(r).  16 consecutive rows' chunk c then cover 256 bytes (row
@@ -320,9 +331,10 @@ __device__ __forceinline__ void clear(f32x16 (&a)[N]) {
 
 // N accumulators of the odd wave of a pair added to the even one's through LDS
 // (`sums`: the pair's 64 N x 64 bytes), which the workgroup no longer needs
-// otherwise.  The odd wave's work ends here.
+// otherwise, and so `one` where it is given (256 bytes more).  The odd wave's
+// work ends here.
 template <int N>
-__device__ __forceinline__ void join_pair(f32x16 (&a)[N], uint8_t* sums, int share, int lane) {
+__device__ __forceinline__ void join_pair(f32x16 (&a)[N], uint8_t* sums, int share, int lane, float* one = nullptr) {
   f32x4* p = reinterpret_cast<f32x4*>(sums) + lane;
   lds_barrier();
   if (share == 1) {
@@ -331,9 +343,11 @@ __device__ __forceinline__ void join_pair(f32x16 (&a)[N], uint8_t* sums, int sha
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         p[(4 * t + i) * 64] = f32x4{a[t][4 * i], a[t][4 * i + 1], a[t][4 * i + 2], a[t][4 * i + 3]};
+    if (one) reinterpret_cast<float*>(sums + N * 4096)[lane] = *one;
   }
   lds_barrier();
   if (share == 1) return;
+  if (one) *one += reinterpret_cast<const float*>(sums + N * 4096)[lane];
 #pragma unroll
   for (int t = 0; t < N; ++t)
 #pragma unroll
@@ -557,7 +571,8 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void packed_fwd_kernel(
 // dK/dV kernel: -lse / c and -delta, delta = rowsum(dO o) of the forward's o
 // before its rounding (o + rest): with the rounded o alone the error of dQ and dK
 // (2-norm, against fp64) is 2.6e-3, with both 2.4e-3, of which each rounding that
-// remains, of dS and of the result, makes 1.7e-3.
+// remains, of dS and of the result, makes 1.7e-3.  Rows of far scores leave -inf
+// and log2 of the sum of their weights against the log-sum-exp.
 // SPLIT as in the forward.
 template <int HD, int SPLIT>
 __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void packed_bwd_dq_kernel(
@@ -587,6 +602,11 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void packed_bwd_dq_kernel(
   const long stat = (long)hd.h * s.T + tile.q0 + min(row, tile.lq - 1);
   const float ml = -lse[stat];
   float md = 0.f;  // -delta of the lane's query
+  // per query, so that a row's gradient does not depend on its neighbours'
+  const bool renew = ml != -INFINITY && !(fabsf(ml) <= fminf(kFarLse, 1e30f * c));
+  const bool far = __any(renew);
+  const float ce = renew && fabsf(ml) > kFarScore ? 1.f : c;  // (1: scores are multiplied and rounded first)
+  float sum = 0.f;                                            // of a renewed row's weights
   {
     bf16x8 of[HD / 16], lf[HD / 16];
     load_rows<HD>(of, rows_rsrc(o + ob, (long)d.H * HD, q0, tile.lq, 32, HD), d.H * HD, lane);
@@ -597,8 +617,8 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void packed_bwd_dq_kernel(
       for (int e = 0; e < 8; ++e) md = fmaf(-(float)df[ks][e], (float)of[ks][e] + (float)lf[ks][e], md);
     md = xor32_f32(md, [](float a, float b) { return a + b; });
     if (g == 0 && share == 0 && row < tile.lq) {
-      stats[stat] = ml / c;
-      stats[(long)d.H * s.T + stat] = md;
+      stats[stat] = renew ? -INFINITY : ml == -INFINITY ? 0.f : ml / c;  // (a row without keys is masked throughout)
+      if (!renew) stats[(long)d.H * s.T + stat] = md;
     }
   }
   const StageLoad<HD> lk(kb, d.ldk, tile.lk, wave, lane), lv(vb, d.ldv, tile.lk, wave, lane);
@@ -630,14 +650,22 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void packed_bwd_dq_kernel(
         dp = mfma32(rf.get(ring + 2 * STAGE, 32 * sub, ks), df[ks], dp);
       }
       read_ahead<HD / 8, 1>();
-      if (kv0 + 31 > q0 + shift) {
+      if (kv0 + 31 > q0 + shift || far) {
         asm volatile("");  // a branch, not 16 selects for every tile
 #pragma unroll
         for (int i = 0; i < 16; ++i)
           if (kv0 + acc_row(g, i) > row + shift) x[i] = -INFINITY;
+        if (far) {
+          const float f = ce != c ? c : 1.f;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            x[i] *= f;
+            sum += __builtin_amdgcn_exp2f(fmaf(x[i], ce, ml));
+          }
+        }
       }
 #pragma unroll
-      for (int i = 0; i < 16; ++i) x[i] = __builtin_amdgcn_exp2f(fmaf(x[i], c, ml)) * dp[i];
+      for (int i = 0; i < 16; ++i) x[i] = __builtin_amdgcn_exp2f(fmaf(x[i], ce, ml)) * dp[i];
       const bf16x8 sf[2] = {pack8(x, 0), pack8(x, 8)};
 #pragma unroll
       for (int h = 0; h < 2; ++h)
@@ -650,10 +678,94 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void packed_bwd_dq_kernel(
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the late loads (zeros) land before LDS goes to another workgroup
   if constexpr (SPLIT == 2) {
-    join_pair(acc, ring + wave / 2 * 2 * STAGE, share, lane);
+    join_pair(acc, ring + wave / 2 * 2 * STAGE, share, lane, &sum);
     if (share == 1) return;
   }
-  if (row < tile.lq) store_row<HD>(dq + (((long)tile.q0 + row) * d.H + hd.h) * HD, acc, scale, g);
+  float by = scale;
+  if (far) {
+    sum = xor32_f32(sum, [](float a, float b) { return a + b; });
+    if (renew) by /= sum;
+    if (renew && g == 0 && row < tile.lq) stats[(long)d.H * s.T + stat] = log2f(sum);
+  }
+  if (row < tile.lq) store_row<HD>(dq + (((long)tile.q0 + row) * d.H + hd.h) * HD, acc, by, g);
+}
+
+// What only add_far_rows reads, of the workgroup's sequence and first heads: in LDS,
+// because the scalar registers are the main loop's.
+struct FarOperands {
+  const bf16_t *k, *v, *o, *rest;
+  const float* lse;
+  int ldk, ldv;
+};
+__device__ __forceinline__ int lane_again() { return __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0)); }
+template <typename T>
+__device__ __forceinline__ T* uniform(T* p) {
+  const uint64_t a = (uint64_t)p;
+  return (T*)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)a) |
+              (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(a >> 32)) << 32);
+}
+
+// The far rows (-inf in stats) of 32 queries of head `head`, added to 32 keys' dK and
+// dV one by one, without LDS; scores from the same products as in dQ, so that they
+// are the same bits there and here.
+template <int HD>
+__device__ __forceinline__ void add_far_rows(f32x16 (&ak)[HD / 32], f32x16 (&av)[HD / 32], const FarOperands& in,
+                                             const bf16_t* q, const bf16_t* dout, const float* stats, int head, int T,
+                                             const PackedTile& tile, const PackedHeads& d, int q0, int kv0, float c,
+                                             int lane) {
+  const int col = lane & 31, g = lane >> 5, r0 = min(q0 + col, tile.lq - 1), shift = tile.lk - tile.lq;
+  const bool far = q0 + col < tile.lq && stats[r0] == -INFINITY;
+  unsigned todo = (unsigned)__ballot(far);
+  if (!todo) return;
+  const float ls = stats[(long)d.H * T + r0], big = uniform(in.lse)[(long)head * T + r0];
+  const int ldk = __builtin_amdgcn_readfirstlane(in.ldk), ldv = __builtin_amdgcn_readfirstlane(in.ldv), ldo = d.H * HD;
+  const auto qr = rows_rsrc(q, d.ldq, q0, tile.lq, 32, HD), dr = rows_rsrc(dout, d.ldd, q0, tile.lq, 32, HD),
+             kr = rows_rsrc(uniform(in.k), ldk, kv0, tile.lk, 32, HD),
+             vr = rows_rsrc(uniform(in.v), ldv, kv0, tile.lk, 32, HD),
+             outr = rows_rsrc(uniform(in.o) + head * HD, ldo, q0, tile.lq, 32, HD),
+             restr = rows_rsrc(uniform(in.rest) + head * HD, ldo, q0, tile.lq, 32, HD);
+  const auto piece = [&](__amdgpu_buffer_rsrc_t rs, int ld, int ks) {
+    return __builtin_bit_cast(bf16x8, __builtin_amdgcn_raw_buffer_load_b128(rs, (col * ld + 8 * g) * 2 + 32 * ks, 0, 0));
+  };
+  f32x16 x = f32x16{}, dp = f32x16{};
+  float md = 0.f;  // -delta
+#pragma unroll 1
+  for (int ks = 0; ks < HD / 16; ++ks) {
+    const bf16x8 df = piece(dr, (int)d.ldd, ks), of = piece(outr, ldo, ks), lf = piece(restr, ldo, ks);
+    x = mfma32(piece(qr, (int)d.ldq, ks), piece(kr, ldk, ks), x);
+    dp = mfma32(df, piece(vr, ldv, ks), dp);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) md = fmaf(-(float)df[e], (float)of[e] + (float)lf[e], md);
+  }
+  md = xor32_f32(md, [](float a, float b) { return a + b; });
+  for (; todo; todo &= todo - 1) {
+    const int r = __ffs(todo) - 1, at = 4 * (r >> 3) + (r & 3);
+    float p = 0.f, ds = 0.f;  // of the query r and the lane's key
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      p = i == at ? x[i] : p;
+      ds = i == at ? dp[i] : ds;
+    }
+    p = __shfl(p, col + 32 * ((r >> 2) & 1), 64);
+    ds = __shfl(ds, col + 32 * ((r >> 2) & 1), 64);
+    p = __builtin_amdgcn_exp2f(far_exponent(p, c, __shfl(big, r, 64)) - __shfl(ls, r, 64));
+    ds = p * (ds + __shfl(md, r, 64));
+    if (kv0 + col > q0 + r + shift) p = ds = 0.f;
+    const bf16_t* qp = q + (long)(q0 + r) * d.ldq + 16 * g;
+    const bf16_t* dop = dout + (long)(q0 + r) * d.ldd + 16 * g;
+#pragma unroll
+    for (int t = 0; t < HD / 32; ++t)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const bf16x8 qv = *reinterpret_cast<const bf16x8*>(qp + 32 * t + 8 * h);
+        const bf16x8 dv = *reinterpret_cast<const bf16x8*>(dop + 32 * t + 8 * h);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          ak[t][8 * h + e] = fmaf(ds, (float)qv[e], ak[t][8 * h + e]);
+          av[t][8 * h + e] = fmaf(p, (float)dv[e], av[t][8 * h + e]);
+        }
+      }
+  }
 }
 
 // dK, dV: waves of 32 keys, whose K and V rows stay in registers; for each query
@@ -662,17 +774,21 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void packed_bwd_dq_kernel(
 // the sequence are zeros throughout: their P is 1, their dO and dS 0.  Eight waves
 // on stages of 128 queries take longer than two workgroups of four (470 -> 510 us,
 // before read_ahead, for four sequences of 499 .. 4093, 32 / 8 heads of 128).
+// Rows of far scores, whose -lse / c is -inf, have no weight there and are added at the
+// end, in fp32.
 // parts > 1, for grids that leave CUs idle: a workgroup walks a part of the
 // group's heads and leaves fp32 sums (parts, Tk, Hkv, HD) for packed_sum_kernel.
 template <int HD, int KB>
 __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void packed_bwd_dkdv_kernel(
     const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, const bf16_t* __restrict__ v,
-    const bf16_t* __restrict__ dout, const float* __restrict__ stats,
-    bf16_t* __restrict__ dk, bf16_t* __restrict__ dv, float* __restrict__ part_k, float* __restrict__ part_v,
-    int parts, PackedSeqs s, PackedHeads d, float scale) {
+    const bf16_t* __restrict__ o, const bf16_t* __restrict__ rest, const float* __restrict__ lse,
+    const bf16_t* __restrict__ dout, const float* __restrict__ stats, bf16_t* __restrict__ dk,
+    bf16_t* __restrict__ dv, float* __restrict__ part_k, float* __restrict__ part_v, int parts, PackedSeqs s,
+    PackedHeads d, float scale) {
   constexpr int NT = HD / 32, STAGE = kStageRows * 2 * HD;
   __shared__ __align__(1024) uint8_t ring[4 * STAGE];      // Q even, Q odd, dO even, dO odd
   __shared__ __align__(1024) float rows[2][2][kStageRows];  // [buffer][-lse / c, -delta][query]
+  __shared__ FarOperands far_operands;
   constexpr int SPLIT = 128 / KB;  // waves that share 32 keys, each with a part of every stage's queries
   const PackedTile tile = find_tile<true, KB>(s, blockIdx.x / (d.Hkv * parts));
   if (!tile.live) return;
@@ -686,6 +802,10 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void packed_bwd_dkdv_kernel(
   const bf16_t* qb = q + (long)tile.q0 * d.ldq + (long)h0 * d.hsq;
   const bf16_t* db = dout + (long)tile.q0 * d.ldd + (long)h0 * d.hsd;
   const long sb = (long)h0 * s.T + tile.q0;
+  if (tid == 0) {
+    const long ob = ((long)tile.q0 * d.H + h0) * HD;
+    far_operands = FarOperands{kb, vb, o + ob, rest + ob, lse + sb, (int)d.ldk, (int)d.ldv};
+  }
   const int shift = tile.lk - tile.lq;
   const int kv0 = tile.block * KB + wave / SPLIT * 32, row = kv0 + col, share = wave % SPLIT;
   const float c = scale * kLog2e;
@@ -703,6 +823,9 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void packed_bwd_dkdv_kernel(
   const int st0 = first / kStageRows;
   const int nst = max((tile.lq + kStageRows - 1) / kStageRows - st0, 0), steps = nst * group;
   StageLoad<HD> lq(qb, d.ldq, tile.lq, wave, lane), ld(db, d.ldd, tile.lq, wave, lane);
+  // whether there were rows of far scores, whose weights are 0 in the products below (the look at each tile's
+  // rows takes 1 % with heads of 64, 2 with 128; one wave's for all 3, a walk over them at the end 6)
+  unsigned long long far = 0;
   // stage st of head `head` into buffer buf; past the last head nothing
   auto load = [&](int head, int st, int buf) {
     lq.base = qb + (long)head * d.hsq;
@@ -731,6 +854,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void packed_bwd_dkdv_kernel(
       if (kv0 > q0 + 31 + shift || q0 >= tile.lq || kv0 >= tile.lk) continue;  // above the diagonal, or outside
       fr.renew();
       f32x16 x, dp;
+      far |= __ballot(rows[buf][0][32 * sub + (lane_again() & 31)] == -INFINITY);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const f32x4 a = *reinterpret_cast<const f32x4*>(&rows[buf][0][32 * sub + 8 * i + 4 * g]);
@@ -746,7 +870,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void packed_bwd_dkdv_kernel(
         x = mfma32(fr.get(ring, 32 * sub, ks), kf[ks], x);
         dp = mfma32(fr.get(ring + 2 * STAGE, 32 * sub, ks), vf[ks], dp);
       }
-      read_ahead<HD / 8, 1, 0, 0, 8>();
+      read_ahead<HD / 8, 1, 0, 0, 9>();
 #pragma unroll
       for (int i = 0; i < 16; ++i) x[i] = __builtin_amdgcn_exp2f(x[i] * c);
       if (kv0 + 31 > q0 + shift) {
@@ -771,6 +895,13 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void packed_bwd_dkdv_kernel(
     fr.move(STAGE);
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the late loads (zeros) land before LDS goes to another workgroup
+  if (__builtin_expect(far != 0, 0)) {
+    for (int i = 0; i < group; ++i)
+      for (int q0 = st0 * kStageRows + (SPLIT == 1 ? 0 : 32 * share); q0 < tile.lq; q0 += 32 * SPLIT)
+        if (kv0 <= q0 + 31 + shift && kv0 < tile.lk)
+          add_far_rows<HD>(ak, av, far_operands, qb + (long)i * d.hsq, db + (long)i * d.hsd,
+                           stats + sb + (long)i * s.T, i, s.T, tile, d, q0, kv0, c, lane_again());
+  }
   if constexpr (SPLIT == 2) {  // in two steps of half the ring
     join_pair(ak, ring + wave / 2 * STAGE, share, lane);
     join_pair(av, ring + (2 + wave / 2) * STAGE, share, lane);
@@ -877,8 +1008,9 @@ hipError_t launch_packed_bwd(const void* q, const void* k, const void* v, const 
     NAYLIS_TIMED("packed_bwd_dkdv", st,
                  hipLaunchKernelGGL(kernel, dim3((unsigned)(packed_tiles(s.Tk, s.n, rows) * d.Hkv * parts)),
                                     dim3(256), 0, st, (const bf16_t*)q, (const bf16_t*)k, (const bf16_t*)v,
-                                    (const bf16_t*)dout, (const float*)stats, (bf16_t*)dk, (bf16_t*)dv, part_k,
-                                    part_v, parts, s, d, scale));
+                                    (const bf16_t*)o, (const bf16_t*)rest, lse, (const bf16_t*)dout,
+                                    (const float*)stats, (bf16_t*)dk, (bf16_t*)dv, part_k, part_v, parts, s, d,
+                                    scale));
     return hipGetLastError();
   };
   if (s.T > 0) {

@@ -267,6 +267,65 @@ def test_packed_far_random_scores(size, hd, dev):
     assert clear > 300
 
 
+@pytest.mark.parametrize("hd,copies", [(64, 1), (128, 1), (64, 150), (128, 100)])  # pairs of waves, and tiles a wave
+@pytest.mark.parametrize("lens", FAR_LENS, ids=["same", "earlier", "none"])
+@pytest.mark.parametrize("sign", [-1, 1])
+@pytest.mark.parametrize("size", [2.0 ** 6, 2.0 ** 8] + FAR)
+def test_packed_gradients_of_scores_of_any_size(size, sign, lens, hd, copies, dev):
+    """The ordinary bounds, for ordinary queries and far ones among each other; a
+    far query's weights are 0 or equal ones.  Copies of the heads give the same bits."""
+    H, Hkv = (4, 2) if copies == 1 else (2, 2)
+    x = _far_inputs(size, sign, lens, H, Hkv, hd, dev)
+    want = _reference(*x, 0.125)
+    got = _run(*(t.repeat(1, copies, 1) for t in x[:4]), *x[4:], 0.125)
+    if copies > 1:
+        for n, t in got.items():
+            parts = t.view(t.shape[0], copies, -1, hd)
+            assert torch.equal(parts, parts[:, :1].expand_as(parts)), n
+            got[n] = parts[:, 0]
+    _check(got, want)
+
+
+@pytest.mark.parametrize("hd,H,Hkv", [(64, 4, 2), (128, 4, 2), (64, 300, 300), (128, 200, 200)])
+@pytest.mark.parametrize("size", [2.0 ** 6, 2.0 ** 16, 2.0 ** 30])
+def test_packed_gradients_of_far_random_scores(size, hd, H, Hkv, dev):
+    """Random far scores: queries whose highest lies clear of the next by more than
+    fp32 sums may be off are one key's each (the others get no gradient); ordinary
+    queries' dq, and with far queries' dO zero all of dk and dv, do not depend on
+    the far ones, bit for bit."""
+    q, k, v, d, cq, ck = _inputs([200, 130], [350, 130], 4, 2, hd, 0, 0, dev)
+    q, d = (t.repeat(1, H // 4, 1) for t in (q, d))
+    k, v = (t.repeat(1, Hkv // 2, 1) for t in (k, v))
+    far = (torch.arange(330, device=dev) % 5 != 0)[:, None, None]
+    scale = hd ** -0.5
+    usual = _run(q, k, v, d.masked_fill(far, 0.0), cq, ck, scale)
+    q = torch.where(far, q * size * size, q)
+    none = _run(q, k, v, d.masked_fill(far, 0.0), cq, ck, scale)
+    assert torch.equal(none["dk"], usual["dk"]) and torch.equal(none["dv"], usual["dv"])
+    if H > 4:  # (the reference goes head by head)
+        q, d = (t[:, :4].contiguous() for t in (q, d))
+        k, v = (t[:, :4].contiguous() for t in (k, v))
+    G, clear = q.shape[1] // k.shape[1], 0
+    for a, b, e, f in ((0, 200, 0, 350), (200, 330, 350, 480)):
+        see = torch.ones(b - a, f - e, dtype=torch.bool, device=dev).tril(f - e - b + a)
+        for h in range(4):
+            x, y = q[a:b, h].double(), k[e:f, h // G].double()
+            top = (x @ y.T * scale).masked_fill(~see, -math.inf).topk(2, -1)[0]
+            noise = (x.abs() @ y.abs().T * scale).amax(-1) * hd * 2.0 ** -23
+            sure = (top[:, 0] - top[:, 1] > 2 * noise + 40) | ~far[a:b, 0, 0]
+            clear += int(sure.sum())
+            d[a:b, h] = torch.where(sure[:, None], d[a:b, h], 0.0)
+    assert clear > 600
+    want = _reference(q, k, v, d, cq, ck, scale)
+    if H > 4:
+        q, k, v, d = (t.repeat(1, H // 4, 1) for t in (q, k, v, d))
+    got = _run(q, k, v, d, cq, ck, scale)
+    plain = ~far[:, 0, 0]
+    assert torch.equal(got["dq"][plain], usual["dq"][plain])
+    # o of the queries that are not clear is not the reference's
+    _check({n: t[:, :want[n][0].shape[1]] for n, t in got.items() if n != "o"}, {n: w for n, w in want.items() if n != "o"})
+
+
 def test_packed_equals_the_batch_kernel(dev):
     """Equal lengths and heads of 64: the framework's batch attention within
     both kernels' bounds."""
