@@ -557,6 +557,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void packed_fwd_kernel(
   if (row < tile.lq) {
     // a query without keys: zeros, and a log-sum-exp under which every backward weight is 0
     const bool none = row + shift < 0;
+    if (none) clear(acc);  // (0 times a NaN of rows that its neighbours see)
     const long at = (long)tile.q0 + row;
     const long off = (at * d.H + hd.h) * HD;
     if (lse)
@@ -687,6 +688,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void packed_bwd_dq_kernel(
     if (renew) by /= sum;
     if (renew && g == 0 && row < tile.lq) stats[(long)d.H * s.T + stat] = log2f(sum);
   }
+  if (row + shift < 0) clear(acc);  // as in the forward
   if (row < tile.lq) store_row<HD>(dq + (((long)tile.q0 + row) * d.H + hd.h) * HD, acc, by, g);
 }
 

@@ -326,6 +326,21 @@ def test_packed_gradients_of_far_random_scores(size, hd, H, Hkv, dev):
     _check({n: t[:, :want[n][0].shape[1]] for n, t in got.items() if n != "o"}, {n: w for n, w in want.items() if n != "o"})
 
 
+@pytest.mark.parametrize("hd,H", [(64, 4), (128, 4), (64, 600), (128, 400)])
+@pytest.mark.parametrize("bad", ["k", "v"])
+def test_packed_queries_without_keys_are_zero(bad, hd, H, dev):
+    """Whatever the sequence's keys and values hold, a query that sees none of them
+    gives 0 and has a gradient of 0."""
+    x = _inputs([90, 40], [30, 33], H, H // 2, hd, 0, 0, dev)
+    for value in (math.nan, math.inf):
+        t = x[1 if bad == "k" else 2]
+        t[3] = t[35] = value
+        got = _run(*x, 0.125)
+        for n in ("o", "dq"):
+            assert bool((got[n][:60] == 0).all() and (got[n][90:97] == 0).all()), n
+            assert not bool(got[n][60:90].isfinite().all())
+
+
 def test_packed_equals_the_batch_kernel(dev):
     """Equal lengths and heads of 64: the framework's batch attention within
     both kernels' bounds."""
