@@ -22,10 +22,12 @@ def packed_attention(q, k, v, cu_seqlens, cu_seqlens_k=None, scale=None):
     earlier one a key less; a query that sees none gives 0, and so do rows
     outside the sequences.  Offsets must not descend and are not copied to the
     host; they are clamped to the tensors.  scale defaults to hd ** -0.5.
-    Returns (T, H, hd).  Sequences do not see each other's rows, whatever these
-    hold; within one, a weight of 0 multiplies v (dout in the backward) as it is,
-    so a NaN or an infinity in a row of it reaches up to 62 rows that do not see
-    it.  A forward with gradients keeps, beside its inputs and the output, what
+    Returns (T, H, hd).  Scores may be of any size that fp32 holds.  Sequences do
+    not see each other's rows, whatever these hold; within one, a weight of 0
+    multiplies what it stands for as it is, so a NaN or an infinity reaches up to 62
+    rows that have nothing to do with it: from a row of v the results, and of k or v
+    the dq, of queries that see keys but not this one; from a row of dout the dv,
+    and of q or dout the dk, of keys that its query does not see.  A forward with gradients keeps, beside its inputs and the output, what
     the output's rounding left (as much again) and (H, T) fp32.  The derivative of
     the backward and forward-mode derivatives raise."""
     return _torch_ext.load().packed_attention(q, k, v, cu_seqlens,

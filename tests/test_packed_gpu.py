@@ -326,6 +326,33 @@ def test_packed_gradients_of_far_random_scores(size, hd, H, Hkv, dev):
     _check({n: t[:, :want[n][0].shape[1]] for n, t in got.items() if n != "o"}, {n: w for n, w in want.items() if n != "o"})
 
 
+@pytest.mark.parametrize("hd,copies", [(64, 1), (128, 1), (64, 150), (128, 100)])
+@pytest.mark.parametrize("shift", [0, 5, 31])
+def test_packed_garbage_stays_near_in_the_gradients(shift, hd, copies, dev):
+    """A NaN in a row of k or v reaches, beside dq of the queries that see it, that of
+    at most 62 before them; one in q or dO, beside dk of the keys that its query
+    sees, that of at most 62 behind them, and one in q no further key's dv."""
+    H = 4 * copies
+    q, k, v, d, cq, ck = _inputs([300], [300 + shift], H, H // 2, hd, 0, 0, dev)
+    want = _run(q, k, v, d, cq, ck, 0.1)
+    for row in (64, 161, 200):
+        first, last = row - shift, row + shift  # the first query that sees the key, the last key that the query sees
+        for i in (1, 2):
+            bad = [t.clone() if j == i else t for j, t in enumerate((q, k, v, d))]
+            bad[i][row] = math.nan
+            dq = _run(*bad, cq, ck, 0.1)["dq"]
+            near = max(first - 62, 0)
+            assert torch.equal(dq[:near], want["dq"][:near]) and bool(dq[first:].isnan().all())
+        for i in (0, 3):
+            bad = [t.clone() if j == i else t for j, t in enumerate((q, k, v, d))]
+            bad[i][row] = math.nan
+            got = _run(*bad, cq, ck, 0.1)
+            assert torch.equal(got["dk"][last + 63:], want["dk"][last + 63:]) and bool(got["dk"][:last + 1].isnan().all())
+            assert torch.equal(got["dq"][:row], want["dq"][:row]) and torch.equal(got["dq"][row + 1:], want["dq"][row + 1:])
+            if i == 0:
+                assert torch.equal(got["dv"][last + 1:], want["dv"][last + 1:]) and bool(got["dv"][:last + 1].isnan().all())
+
+
 @pytest.mark.parametrize("hd,H", [(64, 4), (128, 4), (64, 600), (128, 400)])
 @pytest.mark.parametrize("bad", ["k", "v"])
 def test_packed_queries_without_keys_are_zero(bad, hd, H, dev):
