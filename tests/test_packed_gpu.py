@@ -286,6 +286,26 @@ def test_packed_gradients_of_scores_of_any_size(size, sign, lens, hd, copies, de
     _check(got, want)
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("size", [2.0 ** 10, 2.0 ** 30])
+def test_packed_far_scores_in_parts_and_views(size, hd, dev):
+    """A group's heads in parts (few key tiles, many heads), rows outside the
+    sequences, operands of any stride, an expanded gradient: the bits of dense ones."""
+    q, k, v, d, cq, ck = _far_inputs(size, 1, ([700, 260], [900, 260]), 8, 2, hd, dev)
+    edge = lambda t: torch.cat([t[:7], t, t[:50]])  # noqa: E731
+    x = [edge(t) for t in (q, k, v, d)] + [cq + 7, ck + 7]
+    got = _run(*x, 0.125)
+    _check(got, _reference(*x, 0.125))
+    assert all(torch.equal(a, b) for a, b in zip(got.values(), _run(*x, 0.125).values()))
+    wide = torch.cat([x[0].flatten(1), x[3].flatten(1)], 1)
+    views = [wide[:, :8 * hd].view(-1, 8, hd), x[1].transpose(0, 1).contiguous().transpose(0, 1),
+             torch.cat([x[2], x[2]], 2)[..., hd:], wide[:, -8 * hd:].view(-1, 8, hd)]
+    assert all(torch.equal(a, b) for a, b in zip(got.values(), _run(*views, *x[4:], 0.125).values()))
+    ones = torch.ones(1, 1, 1, dtype=q.dtype, device=dev).expand_as(x[0])
+    same = _run(*x[:3], torch.ones_like(x[3]), *x[4:], 0.125)
+    assert all(torch.equal(a, b) for a, b in zip(same.values(), _run(*x[:3], ones, *x[4:], 0.125).values()))
+
+
 @pytest.mark.parametrize("hd,H,Hkv", [(64, 4, 2), (128, 4, 2), (64, 300, 300), (128, 200, 200)])
 @pytest.mark.parametrize("size", [2.0 ** 6, 2.0 ** 16, 2.0 ** 30])
 def test_packed_gradients_of_far_random_scores(size, hd, H, Hkv, dev):
