@@ -497,6 +497,7 @@ int naylis_mom_decode_step(const double* state_in, double* state_out, const int3
  *   workspace: naylis_mom_packed_attn_bwd_workspace_bytes
  * The backward writes dense dq, dk, dv; the gradients of a key head are summed
  * over its query heads in one fixed order in fp32.
+ * Scores may be of any size that fp32 holds.
  * Constraints: head_dim 64 or 128, H a multiple of Hkv, scale > 0, pointers
  * 16-byte aligned, strides multiples of 8, token strides and H head_dim under
  * 2^23, 2^24 tiles of 64 rows and heads. */

@@ -21,7 +21,7 @@
 // Many rows are bound by HBM: 4096 x 50001 bf16 69 us (5.9 TB/s; fp32 127 us, 6.5
 // TB/s), with the top 20, read twice, 122; a thread that keeps values as fp32
 // between maximum and sum, 8 chunks at a time, takes 200 registers and 105 us.
-// The gradient 154 us (5.3 TB/s read and written; a large copy 4.95).  Few rows
+// The gradient 143 to 154 us (5.3 to 5.7 TB/s read and written; a large copy 4.95).  Few rows
 // are bound by the steps within a workgroup: 64 x 32768 with the top 20 8.9 us
 // (1024 threads; 19.6 with 512 and a second read), of which 3 are launch and
 // first load.  One row of 151999 in 8 parts 13.7 us, in one 21.9; 64 of them 17.4
@@ -470,9 +470,9 @@ __global__ __launch_bounds__(256) void logprobs_join_kernel(const T* __restrict_
 
 // d logits of a slab of `slab` chunks of a row (the first one takes the elements
 // beside the chunks too); slabs of a row are neighbours in the grid, so that what
-// is under way at a time lies together in memory.  4096 x 50001 bf16: 154 us (5.3
-// TB/s; a workgroup a row 183, of 1024 threads 157), fp32 287 (362); 300 x 151999 30
-// (53).  Slabs of 512 chunks: 160, 267, 35.  g_logp and g_entropy may be null (no
+// is under way at a time lies together in memory.  4096 x 50001 bf16: 143 to 154 us by
+// card (beside 154, a workgroup a row 183, of 1024 threads 157), fp32 287 (362); 300 x
+// 151999 30 (53).  Slabs of 512 chunks: 160, 267, 35.  g_logp and g_entropy may be null (no
 // gradient).
 constexpr int kBwdChunks = 4;  // of a thread, loaded at once
 template <typename T>

@@ -16,14 +16,16 @@
 // fp32, with no atomics.  Probabilities and dS enter their products as bf16
 // (at most half a step, 2^-9 of a value's binade); all sums are fp32.
 //
-// Bound by power, then by the softmax's vector work beside the matrix units.  Over
-// 16k tokens, with the products that each gradient kernel forms again counted, the
-// forward runs at 1.1 PFLOP/s with 16 heads of 128 (a large matrix product at 1.14
-// for as long) and 0.95 of 64, dQ at 1.25 and 1.0, dK/dV at 1.26 and 1.0; on tensors
-// of zeros, which take less power, at 1.4 and 1.2, 1.65 and 1.5, 1.6 and 1.45.  Nine
-// sequences of 48 .. 3885 tokens, 16 heads of 64: 103 us forward, 405 with the
-// gradients; four of 499 .. 4093, 32 / 8 heads of 128: 210 and 888.  The first loads of
-// a tile and the last tiles' tail are a quarter of such batches.
+// Bound by power, and by the softmax's vector work, which in the gradient kernels
+// follows a wave's products instead of running beside them.  Over 16k tokens, with the
+// products that each gradient kernel forms again counted, the forward runs at 1.0 to
+// 1.1 PFLOP/s with 16 heads of 128 (a large matrix product at 1.14 for as long) and 0.88
+// to 0.95 of 64, dQ at 1.15 to 1.25 and 1.0, dK/dV at 1.17 to 1.26 and 1.0, by card and
+// clock; on tensors of zeros, which take less power, at 1.4 and 1.2, 1.65 and 1.5, 1.6
+// and 1.45.  Nine sequences of 48 .. 3885 tokens, 16 heads of 64: 103 to 123 us forward,
+// 405 to 433 with the gradients; four of 499 .. 4093, 32 / 8 heads of 128: 208 to 239 and
+// 890 to 941.  The first loads of a tile and the last tiles' tail are a quarter of such
+// batches.
 #include "common.h"
 #include "launch.h"
 #include "packed_tiles.h"
@@ -531,7 +533,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void packed_fwd_kernel(
     }
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the late loads (zeros) land before LDS goes to another workgroup
-  if constexpr (SPLIT == 2) {  // the odd tiles' sums to the even ones' (m is kLowest and all else 0 where there were none)
+  if constexpr (SPLIT == 2) {  // the odd tiles' sums to the even ones' (kLowest and zeros where there were none)
     float* sums = reinterpret_cast<float*>(ring) + wave / 2 * (HD / 2 + 2) * 64 + lane;
     lds_barrier();
     if (share == 1) {
@@ -699,7 +701,10 @@ struct FarOperands {
   const float* lse;
   int ldk, ldv;
 };
-__device__ __forceinline__ int lane_again() { return __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0)); }
+// The lane, in no register until then.
+__device__ __forceinline__ int lane_again() {
+  return __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0));
+}
 template <typename T>
 __device__ __forceinline__ T* uniform(T* p) {
   const uint64_t a = (uint64_t)p;
@@ -727,7 +732,8 @@ __device__ __forceinline__ void add_far_rows(f32x16 (&ak)[HD / 32], f32x16 (&av)
              outr = rows_rsrc(uniform(in.o) + head * HD, ldo, q0, tile.lq, 32, HD),
              restr = rows_rsrc(uniform(in.rest) + head * HD, ldo, q0, tile.lq, 32, HD);
   const auto piece = [&](__amdgpu_buffer_rsrc_t rs, int ld, int ks) {
-    return __builtin_bit_cast(bf16x8, __builtin_amdgcn_raw_buffer_load_b128(rs, (col * ld + 8 * g) * 2 + 32 * ks, 0, 0));
+    const int off = (col * ld + 8 * g) * 2 + 32 * ks;
+    return __builtin_bit_cast(bf16x8, __builtin_amdgcn_raw_buffer_load_b128(rs, off, 0, 0));
   };
   f32x16 x = f32x16{}, dp = f32x16{};
   float md = 0.f;  // -delta
