@@ -712,68 +712,61 @@ __device__ __forceinline__ T* uniform(T* p) {
               (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(a >> 32)) << 32);
 }
 
-// The far rows (-inf in stats) of 32 queries of head `head`, added to 32 keys' dK and
-// dV one by one, without LDS; scores from the same products as in dQ, so that they
-// are the same bits there and here.
-template <int HD>
+// The far rows (-inf in `starts`, and the log2 of their weights' sum a stage behind) of
+// 32 queries of head `head`, whose Q and dO are in LDS at row 32 sub, added to 32 keys'
+// dK and dV.  Scores from the same products as in dQ, so that they are the same bits
+// there and here; K, V and what -delta needs are read from memory again, because the
+// registers are the main loop's.
+template <int HD, typename Frag>
 __device__ __forceinline__ void add_far_rows(f32x16 (&ak)[HD / 32], f32x16 (&av)[HD / 32], const FarOperands& in,
-                                             const bf16_t* q, const bf16_t* dout, const float* stats, int head, int T,
-                                             const PackedTile& tile, const PackedHeads& d, int q0, int kv0, float c,
-                                             int lane) {
-  const int col = lane & 31, g = lane >> 5, r0 = min(q0 + col, tile.lq - 1), shift = tile.lk - tile.lq;
-  const bool far = q0 + col < tile.lq && stats[r0] == -INFINITY;
-  unsigned todo = (unsigned)__ballot(far);
-  if (!todo) return;
-  const float ls = stats[(long)d.H * T + r0], big = uniform(in.lse)[(long)head * T + r0];
+                                             const Frag& fr, const uint8_t* ring, const float* starts,
+                                             const bf16_t* dout, int head, int T, const PackedTile& tile,
+                                             const PackedHeads& d, int q0, int sub, int kv0, float c, int lane) {
+  constexpr int NT = HD / 32, STAGE = kStageRows * 2 * HD;
+  const int col = lane & 31, g = lane >> 5, shift = tile.lk - tile.lq;
+  if (!__any(starts[32 * sub + col] == -INFINITY)) return;
+  const float big = uniform(in.lse)[(long)head * T + min(q0 + col, tile.lq - 1)];
   const int ldk = __builtin_amdgcn_readfirstlane(in.ldk), ldv = __builtin_amdgcn_readfirstlane(in.ldv), ldo = d.H * HD;
-  const auto qr = rows_rsrc(q, d.ldq, q0, tile.lq, 32, HD), dr = rows_rsrc(dout, d.ldd, q0, tile.lq, 32, HD),
-             kr = rows_rsrc(uniform(in.k), ldk, kv0, tile.lk, 32, HD),
+  const auto kr = rows_rsrc(uniform(in.k), ldk, kv0, tile.lk, 32, HD),
              vr = rows_rsrc(uniform(in.v), ldv, kv0, tile.lk, 32, HD),
+             dr = rows_rsrc(dout, d.ldd, q0, tile.lq, 32, HD),
              outr = rows_rsrc(uniform(in.o) + head * HD, ldo, q0, tile.lq, 32, HD),
              restr = rows_rsrc(uniform(in.rest) + head * HD, ldo, q0, tile.lq, 32, HD);
   const auto piece = [&](__amdgpu_buffer_rsrc_t rs, int ld, int ks) {
     const int off = (col * ld + 8 * g) * 2 + 32 * ks;
     return __builtin_bit_cast(bf16x8, __builtin_amdgcn_raw_buffer_load_b128(rs, off, 0, 0));
   };
-  f32x16 x = f32x16{}, dp = f32x16{};
-  float md = 0.f;  // -delta
-#pragma unroll 1
+  float md = 0.f;  // -delta of query col
+#pragma unroll 2
   for (int ks = 0; ks < HD / 16; ++ks) {
     const bf16x8 df = piece(dr, (int)d.ldd, ks), of = piece(outr, ldo, ks), lf = piece(restr, ldo, ks);
-    x = mfma32(piece(qr, (int)d.ldq, ks), piece(kr, ldk, ks), x);
-    dp = mfma32(df, piece(vr, ldv, ks), dp);
 #pragma unroll
     for (int e = 0; e < 8; ++e) md = fmaf(-(float)df[e], (float)of[e] + (float)lf[e], md);
   }
   md = xor32_f32(md, [](float a, float b) { return a + b; });
-  for (; todo; todo &= todo - 1) {
-    const int r = __ffs(todo) - 1, at = 4 * (r >> 3) + (r & 3);
-    float p = 0.f, ds = 0.f;  // of the query r and the lane's key
+  f32x16 x = f32x16{}, dp = f32x16{};
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      p = i == at ? x[i] : p;
-      ds = i == at ? dp[i] : ds;
-    }
-    p = __shfl(p, col + 32 * ((r >> 2) & 1), 64);
-    ds = __shfl(ds, col + 32 * ((r >> 2) & 1), 64);
-    p = __builtin_amdgcn_exp2f(far_exponent(p, c, __shfl(big, r, 64)) - __shfl(ls, r, 64));
-    ds = p * (ds + __shfl(md, r, 64));
-    if (kv0 + col > q0 + r + shift) p = ds = 0.f;
-    const bf16_t* qp = q + (long)(q0 + r) * d.ldq + 16 * g;
-    const bf16_t* dop = dout + (long)(q0 + r) * d.ldd + 16 * g;
-#pragma unroll
-    for (int t = 0; t < HD / 32; ++t)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const bf16x8 qv = *reinterpret_cast<const bf16x8*>(qp + 32 * t + 8 * h);
-        const bf16x8 dv = *reinterpret_cast<const bf16x8*>(dop + 32 * t + 8 * h);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          ak[t][8 * h + e] = fmaf(ds, (float)qv[e], ak[t][8 * h + e]);
-          av[t][8 * h + e] = fmaf(p, (float)dv[e], av[t][8 * h + e]);
-        }
-      }
+  for (int ks = 0; ks < HD / 16; ++ks) {
+    x = mfma32(fr.get(ring, 32 * sub, ks), piece(kr, ldk, ks), x);
+    dp = mfma32(fr.get(ring + 2 * STAGE, 32 * sub, ks), piece(vr, ldv, ks), dp);
   }
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int r = acc_row(g, i);
+    const float z = far_exponent(x[i], c, __shfl(big, r, 64)) - starts[kStageRows + 32 * sub + r];
+    const float delta = __shfl(md, r, 64);
+    const bool none = starts[32 * sub + r] != -INFINITY || kv0 + col > q0 + r + shift;
+    x[i] = none ? 0.f : __builtin_amdgcn_exp2f(z);
+    dp[i] = none ? 0.f : x[i] * (dp[i] + delta);
+  }
+  const bf16x8 pf[2] = {pack8(x, 0), pack8(x, 8)}, sf[2] = {pack8(dp, 0), pack8(dp, 8)};
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      av[t] = mfma32(fr.get_t(ring + 2 * STAGE, 32 * sub + 16 * h, t), pf[h], av[t]);
+      ak[t] = mfma32(fr.get_t(ring, 32 * sub + 16 * h, t), sf[h], ak[t]);
+    }
 }
 
 // dK, dV: waves of 32 keys, whose K and V rows stay in registers; for each query
@@ -782,8 +775,8 @@ __device__ __forceinline__ void add_far_rows(f32x16 (&ak)[HD / 32], f32x16 (&av)
 // the sequence are zeros throughout: their P is 1, their dO and dS 0.  Eight waves
 // on stages of 128 queries take longer than two workgroups of four (470 -> 510 us,
 // before read_ahead, for four sequences of 499 .. 4093, 32 / 8 heads of 128).
-// Rows of far scores, whose -lse / c is -inf, have no weight there and are added at the
-// end, in fp32.
+// Rows of far scores, whose -lse / c is -inf, have no weight there; where a workgroup
+// met some, it walks again for them (all rows far: 6 to 7 times as long).
 // parts > 1, for grids that leave CUs idle: a workgroup walks a part of the
 // group's heads and leaves fp32 sums (parts, Tk, Hkv, HD) for packed_sum_kernel.
 template <int HD, int KB>
@@ -797,6 +790,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void packed_bwd_dkdv_kernel(
   __shared__ __align__(1024) uint8_t ring[4 * STAGE];      // Q even, Q odd, dO even, dO odd
   __shared__ __align__(1024) float rows[2][2][kStageRows];  // [buffer][-lse / c, -delta][query]
   __shared__ FarOperands far_operands;
+  __shared__ bool any_far;
   constexpr int SPLIT = 128 / KB;  // waves that share 32 keys, each with a part of every stage's queries
   const PackedTile tile = find_tile<true, KB>(s, blockIdx.x / (d.Hkv * parts));
   if (!tile.live) return;
@@ -813,6 +807,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void packed_bwd_dkdv_kernel(
   if (tid == 0) {
     const long ob = ((long)tile.q0 * d.H + h0) * HD;
     far_operands = FarOperands{kb, vb, o + ob, rest + ob, lse + sb, (int)d.ldk, (int)d.ldv};
+    any_far = false;
   }
   const int shift = tile.lk - tile.lq;
   const int kv0 = tile.block * KB + wave / SPLIT * 32, row = kv0 + col, share = wave % SPLIT;
@@ -903,12 +898,29 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void packed_bwd_dkdv_kernel(
     fr.move(STAGE);
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the late loads (zeros) land before LDS goes to another workgroup
-  if (__builtin_expect(far != 0, 0)) {
-    for (int i = 0; i < group; ++i)
-      for (int q0 = st0 * kStageRows + (SPLIT == 1 ? 0 : 32 * share); q0 < tile.lq; q0 += 32 * SPLIT)
-        if (kv0 <= q0 + 31 + shift && kv0 < tile.lk)
-          add_far_rows<HD>(ak, av, far_operands, qb + (long)i * d.hsq, db + (long)i * d.hsd,
-                           stats + sb + (long)i * s.T, i, s.T, tile, d, q0, kv0, c, lane_again());
+  if (far) any_far = true;
+  lds_barrier();
+  if (__builtin_expect(any_far, 0)) {  // the walk again, for those rows alone
+    head = 0;
+    st = st0;
+    load(0, st, steps & 1);
+    for (int step = steps; step < 2 * steps; ++step) {
+      const int buf = step & 1, cur = st, cur_head = head;
+      if (++st == st0 + nst) {
+        st = st0;
+        ++head;
+      }
+      wait_loads<0>();
+      load(head, st, buf ^ 1);
+      for (int sub = SPLIT == 1 ? 0 : share; sub < 2; sub += SPLIT) {
+        const int q0 = cur * kStageRows + 32 * sub;
+        if (kv0 > q0 + 31 + shift || q0 >= tile.lq || kv0 >= tile.lk) continue;
+        add_far_rows<HD>(ak, av, far_operands, fr, ring, &rows[buf][0][0], db + (long)cur_head * d.hsd, cur_head, s.T,
+                         tile, d, q0, sub, kv0, c, lane_again());
+      }
+      fr.move(STAGE);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   }
   if constexpr (SPLIT == 2) {  // in two steps of half the ring
     join_pair(ak, ring + wave / 2 * STAGE, share, lane);
