@@ -24,7 +24,7 @@
 extern "C" {
 #endif
 
-#define NAYLIS_MOM_ABI_VERSION 22
+#define NAYLIS_MOM_ABI_VERSION 23
 
 #define NAYLIS_OK 0
 #define NAYLIS_ERR_ARG 1       /* invalid shape / argument (the reference raises RuntimeError) */
@@ -34,6 +34,7 @@ extern "C" {
 #define NAYLIS_DTYPE_F32 0
 #define NAYLIS_DTYPE_BF16 1
 #define NAYLIS_DTYPE_E4M3 2 /* OCP fp8 codes with one fp32 scale per row (caches) */
+#define NAYLIS_DTYPE_E2M1 3 /* OCP fp4 codes, two in a byte, with a power of two per 32 (caches) */
 
 /* noise_kind of naylis_mom_router_fwd */
 #define NAYLIS_NOISE_ADDITIVE 0        /* noise holds the perturbation itself */
@@ -513,13 +514,18 @@ int naylis_mom_packed_attn_bwd(const void* q, const void* k, const void* v, cons
                                int64_t head_dim, void* stream);
 
 /* --------------------------------------------------------- paged cache ---
- * Keys and values of earlier tokens in pages, and the attention of one new
- * token per sequence over them (the reference keeps no cache: use_cache=False,
+ * Keys and values of earlier tokens in pages, and the attention of a few new
+ * tokens per sequence over them (the reference keeps no cache: use_cache=False,
  * pretrain.py:198).
- *   k_pages, v_pages (pages, Hkv, page_size, head_dim), cache_dtype bf16, or
+ *   k_pages, v_pages (pages, Hkv, page_size, head_dim), cache_dtype bf16; or
  *   e4m3 codes with k_scale, v_scale (pages, Hkv, page_size) fp32: scale =
  *   max|row| / 448 (1 for a row of zeros), code = e4m3(x / scale) rounded to
- *   nearest even; scales NULL for bf16
+ *   nearest even; or e2m1 codes, (pages, Hkv, page_size, head_dim / 2) bytes with
+ *   the even feature in the low four bits, and k_scale, v_scale (pages, Hkv,
+ *   page_size, head_dim / 32) bytes e: 32 features times 2^(e - 127), e - 127 =
+ *   floor(log2(max|x|)) - 2, at least -126, codes rounded to nearest even and to 6
+ *   at most; e = 255 (a block with an infinity or a NaN) reads as NaN; scales NULL
+ *   for bf16
  *   table (B, W) int32: the pages of each sequence's tokens 0 .., in order
  *
  * naylis_mom_paged_append: k, v (T, Hkv, head_dim) bf16 with the token and
@@ -529,27 +535,93 @@ int naylis_mom_packed_attn_bwd(const void* q, const void* k, const void* v, cons
  * (padding: position -1) is left out, and nothing else is written.  No two
  * tokens of a call may have the same place.
  *
+ * naylis_mom_paged_append_rope: the same with k rotated to its position, and
+ * q_out (T, H, head_dim) bf16 dense = q (T, H, head_dim) rotated to it (those of
+ * tokens that are left out too; H = 0: none).  Of a row's first 2 half features
+ * the pair (i, i + half) turns by the angle positions[t] * inv_freq[i] (fp32;
+ * formed in fp64; cos and sin rounded to fp32, times `scaling`), the others
+ * stay; products and sum in fp32, rounded once to the cache's type or bf16.
+ * strides: q's, k's, v's.  half a multiple of 8 up to head_dim / 2, T < 2^24.
+ *
+ * naylis_mom_paged_gather: k_out, v_out (T, Hkv, head_dim) bf16 dense = the
+ * first cu_seqlens[b + 1] - cu_seqlens[b] tokens of each sequence b, in rows
+ * cu_seqlens[b] .. (int32, B + 1, not descending; rows outside all sequences are
+ * 0), NaN where the page lies outside the cache or the token past the table's
+ * row.  T < 2^28.
+ *
  * naylis_mom_paged_attn: out (B, H, head_dim) bf16 dense = softmax_n(scale
  * q . k_n) v_n over the tokens n < lens[b] (int32); 0 where lens[b] <= 0; NaN
  * for a sequence longer than its table row, or with a page outside the cache.
  * Table entries and page rows past the sequence's end are not used, whatever
  * they hold.  q (B, H, head_dim) bf16, q_strides: host array, its batch and
  * head strides.
+ *
+ * naylis_mom_paged_attn_tokens: N new tokens of each sequence, q and out (B, N,
+ * H, head_dim), q_strides its batch, token and head strides.  The last of them
+ * sees all lens[b] tokens, each earlier one a token less.  q_lens (B) int32:
+ * new tokens of each sequence, clamped to [0, N], the first ones of its N rows
+ * (NULL: N); rows behind them, and rows that see no token, are 0.
  * Constraints: head_dim 64 or 128, page_size a power of two in [16, 256], H a
- * multiple of Hkv, Hkv ceil(H / Hkv / 16) and B <= 65535, W page_size <= 2^31 -
- * 2048, B ceil(W page_size / 32) < 2^30, scale > 0, pointers (tables and lengths
- * apart) 16-byte aligned, strides multiples of 8, the first of a pair under 2^23. */
-int naylis_mom_paged_append(void* k_pages, void* v_pages, float* k_scale, float* v_scale, int cache_dtype,
+ * multiple of Hkv, N H / Hkv <= 4096, Hkv ceil(N H / Hkv / 16) and B <= 65535, W
+ * page_size <= 2^31 - 2048, B ceil(W page_size / 32) < 2^30, scale > 0, pointers
+ * (tables and lengths apart) 16-byte aligned, strides multiples of 8, all but the
+ * last under 2^23. */
+int naylis_mom_paged_append(void* k_pages, void* v_pages, void* k_scale, void* v_scale, int cache_dtype,
                             const void* k, const void* v, const int64_t* strides, const int32_t* table,
                             const int32_t* positions, const int32_t* rows, int64_t T, int64_t pages, int64_t Hkv,
                             int64_t page_size, int64_t head_dim, int64_t B, int64_t W, void* stream);
+int naylis_mom_paged_append_rope(void* k_pages, void* v_pages, void* k_scale, void* v_scale, int cache_dtype,
+                                 const void* q, const void* k, const void* v, const int64_t* strides,
+                                 const float* inv_freq, float scaling, const int32_t* table, const int32_t* positions,
+                                 const int32_t* rows, void* q_out, int64_t T, int64_t H, int64_t half, int64_t pages,
+                                 int64_t Hkv, int64_t page_size, int64_t head_dim, int64_t B, int64_t W, void* stream);
+int naylis_mom_paged_gather(const void* k_pages, const void* v_pages, const void* k_scale, const void* v_scale,
+                            int cache_dtype, const int32_t* table, const int32_t* cu_seqlens, void* k_out, void* v_out,
+                            int64_t T, int64_t pages, int64_t Hkv, int64_t page_size, int64_t head_dim, int64_t B,
+                            int64_t W, void* stream);
 size_t naylis_mom_paged_attn_workspace_bytes(int cache_dtype, int64_t B, int64_t H, int64_t Hkv, int64_t page_size,
                                              int64_t head_dim, int64_t W);
-int naylis_mom_paged_attn(const void* q, const void* k_pages, const void* v_pages, const float* k_scale,
-                          const float* v_scale, int cache_dtype, const int32_t* table, const int32_t* lens, void* out,
+int naylis_mom_paged_attn(const void* q, const void* k_pages, const void* v_pages, const void* k_scale,
+                          const void* v_scale, int cache_dtype, const int32_t* table, const int32_t* lens, void* out,
                           void* workspace, size_t workspace_bytes, const int64_t* q_strides, float scale, int64_t B,
                           int64_t H, int64_t pages, int64_t Hkv, int64_t page_size, int64_t head_dim, int64_t W,
                           void* stream);
+size_t naylis_mom_paged_attn_tokens_workspace_bytes(int cache_dtype, int64_t B, int64_t N, int64_t H, int64_t Hkv,
+                                                    int64_t page_size, int64_t head_dim, int64_t W);
+int naylis_mom_paged_attn_tokens(const void* q, const void* k_pages, const void* v_pages, const void* k_scale,
+                                 const void* v_scale, int cache_dtype, const int32_t* table, const int32_t* lens,
+                                 const int32_t* q_lens, void* out, void* workspace, size_t workspace_bytes,
+                                 const int64_t* q_strides, float scale, int64_t B, int64_t N, int64_t H, int64_t pages,
+                                 int64_t Hkv, int64_t page_size, int64_t head_dim, int64_t W, void* stream);
+
+/* ----------------------------------------------- drafts' verification ---
+ * Drafted tokens held against a model's logits, from given random numbers (the
+ * reference generates nothing).  For each sequence b with drafts d_0 .. d_{n-1}
+ * drawn from q_i, p_i = softmax(logits[b, i] / T) and u = uniforms[b]:
+ *   draft i is kept while u[i] q_i(d_i) < p_i(d_i); accepted[b] = a, how many
+ *   the token behind them is drawn from max(0, p_a - q_a) where draft a was
+ *   turned away (from p_a where that is 0 everywhere), from p_n where none was:
+ *   the first j whose cumulative weight exceeds u[N] of the whole
+ *   tokens[b] (N + 1) int64: the kept drafts, that token, -1 behind it
+ * so the tokens are distributed as p's own.  Weights and sums are fp64.
+ *   logits (B, N + 1, V) in dtype (bf16 or fp32), draft_probs (B, N, V) bf16 or
+ *   fp32, both with host arrays of their batch and token strides, last
+ *   dimension dense, any address that their elements allow; draft_probs NULL:
+ *   drafts found by a rule, q_i(d_i) = 1
+ *   drafts (B, N) int64 (an id outside [0, V) is never kept), uniforms (B, N + 1)
+ *   fp32 in [0, 1), the last one for the token behind; draft_lens (B) int32, the
+ *   drafts of each sequence, clamped to [0, N] (NULL: N)
+ *   temperatures (B) fp32, or NULL for one temperature; 0 (or less, or NaN):
+ *   all of p on the largest logit, the first of equal ones
+ * A row that has no distribution (a NaN, +inf, or nothing but -inf) keeps no
+ * draft and gives token -1.  Rows behind a sequence's drafts are not read.
+ * B <= 65535, N <= 1023, V <= 2^28; workspace 16-byte aligned. */
+size_t naylis_mom_verify_drafts_workspace_bytes(int64_t B, int64_t N, int64_t V, int draft_probs);
+int naylis_mom_verify_drafts(const void* logits, int dtype, const int64_t* logits_strides, const int64_t* drafts,
+                             const float* uniforms, const void* draft_probs, int probs_dtype,
+                             const int64_t* probs_strides, const int32_t* draft_lens, const float* temperatures,
+                             float temperature, int64_t* tokens, int32_t* accepted, void* workspace,
+                             size_t workspace_bytes, int64_t B, int64_t N, int64_t V, void* stream);
 
 /* --------------------------------------------------- log probabilities ---
  * Of given tokens under rows of logits (the reference keeps the summed loss of

@@ -14,7 +14,7 @@ import threading
 
 LIB_DIR = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib")
 LIB_PATH = os.path.join(LIB_DIR, "libnaylis_mom.so")
-ABI_VERSION = 22
+ABI_VERSION = 23
 
 NAYLIS_OK = 0
 NAYLIS_ERR_ARG = 1
@@ -91,6 +91,15 @@ SIGNATURES = {
     "naylis_mom_paged_attn_workspace_bytes": (_size_t, [_int] + [_i64] * 6),
     "naylis_mom_paged_attn": (_int, [_c_void_p] * 5 + [_int] + [_c_void_p] * 4 + [_size_t, _c_void_p, _float]
                               + [_i64] * 7 + [_c_void_p]),
+    "naylis_mom_paged_attn_tokens_workspace_bytes": (_size_t, [_int] + [_i64] * 7),
+    "naylis_mom_paged_attn_tokens": (_int, [_c_void_p] * 5 + [_int] + [_c_void_p] * 5 + [_size_t, _c_void_p, _float]
+                                     + [_i64] * 8 + [_c_void_p]),
+    "naylis_mom_paged_append_rope": (_int, [_c_void_p] * 4 + [_int] + [_c_void_p] * 5 + [_float] + [_c_void_p] * 4
+                                     + [_i64] * 9 + [_c_void_p]),
+    "naylis_mom_paged_gather": (_int, [_c_void_p] * 4 + [_int] + [_c_void_p] * 4 + [_i64] * 7 + [_c_void_p]),
+    "naylis_mom_verify_drafts_workspace_bytes": (_size_t, [_i64] * 3 + [_int]),
+    "naylis_mom_verify_drafts": (_int, [_c_void_p, _int] + [_c_void_p] * 4 + [_int] + [_c_void_p] * 3 + [_float]
+                                 + [_c_void_p] * 3 + [_size_t] + [_i64] * 3 + [_c_void_p]),
     "naylis_mom_logprobs_workspace_bytes": (_size_t, [_i64] * 3),
     "naylis_mom_logprobs_fwd": (_int, [_c_void_p, _int, _i64] + [_c_void_p] * 7 + [_size_t] + [_i64] * 4
                                 + [_c_void_p]),

@@ -1188,8 +1188,8 @@ int naylis_mom_packed_attn_bwd(const void* q, const void* k, const void* v, cons
 
 static int check_paged(int64_t pages, int64_t Hkv, int64_t page_size, int64_t B, int64_t W, int64_t G,
                        int64_t head_dim, int dtype, const char* who) {
-  if (dtype != NAYLIS_DTYPE_BF16 && dtype != NAYLIS_DTYPE_E4M3)
-    return fail(NAYLIS_ERR_ARG, "%s: cache dtype %d must be bf16 or e4m3", who, dtype);
+  if (dtype != NAYLIS_DTYPE_BF16 && dtype != NAYLIS_DTYPE_E4M3 && dtype != NAYLIS_DTYPE_E2M1)
+    return fail(NAYLIS_ERR_ARG, "%s: cache dtype %d must be bf16, e4m3 or e2m1", who, dtype);
   if (head_dim != 64 && head_dim != 128)
     return fail(NAYLIS_ERR_ARG, "%s: head_dim %lld must be 64 or 128", who, (long long)head_dim);
   if (page_size < 16 || page_size > 256 || (page_size & (page_size - 1)) != 0)
@@ -1206,12 +1206,17 @@ static int check_paged(int64_t pages, int64_t Hkv, int64_t page_size, int64_t B,
 static int check_cache(const PagedCacheDims& c, int dtype, const char* who) {
   int rc = check_pointers({c.k, c.v}, who);
   if (rc) return rc;
-  if (dtype != NAYLIS_DTYPE_E4M3) return NAYLIS_OK;
-  if (!c.k_scale || !c.v_scale) return fail(NAYLIS_ERR_ARG, "%s: an e4m3 cache needs its scales", who);
+  if (dtype == NAYLIS_DTYPE_BF16) return NAYLIS_OK;
+  if (!c.k_scale || !c.v_scale)
+    return fail(NAYLIS_ERR_ARG, "%s: an %s cache needs its scales", who, dtype == NAYLIS_DTYPE_E4M3 ? "e4m3" : "e2m1");
   return check_pointers({c.k_scale, c.v_scale}, who);  // (read four at a time)
 }
 
-int naylis_mom_paged_append(void* k_pages, void* v_pages, float* k_scale, float* v_scale, int cache_dtype,
+static PagedFormat paged_format(int dtype) {
+  return dtype == NAYLIS_DTYPE_BF16 ? kPagedBf16 : dtype == NAYLIS_DTYPE_E4M3 ? kPagedE4m3 : kPagedE2m1;
+}
+
+int naylis_mom_paged_append(void* k_pages, void* v_pages, void* k_scale, void* v_scale, int cache_dtype,
                             const void* k, const void* v, const int64_t* strides, const int32_t* table,
                             const int32_t* positions, const int32_t* rows, int64_t T, int64_t pages, int64_t Hkv,
                             int64_t page_size, int64_t head_dim, int64_t B, int64_t W, void* stream) {
@@ -1230,21 +1235,77 @@ int naylis_mom_paged_append(void* k_pages, void* v_pages, float* k_scale, float*
       (rc = check_strides(strides + 2, "v", who)))
     return rc;
   const PagedNew src{(long)T, strides[0], strides[1], strides[2], strides[3]};
-  return hip_status(launch_paged_append(c, (int)head_dim, cache_dtype == NAYLIS_DTYPE_E4M3, k, v, table, positions,
-                                        rows, src, (hipStream_t)stream),
+  return hip_status(launch_paged_append(c, (int)head_dim, paged_format(cache_dtype), k, v, table, positions, rows, src,
+                                        (hipStream_t)stream),
                     who);
 }
 
-static PagedCacheDims paged_dims(int64_t H, int64_t pages, int64_t Hkv, int64_t page_size, int64_t B, int64_t W) {
-  return PagedCacheDims{nullptr, nullptr, nullptr, nullptr, (int)pages, (int)Hkv, (int)page_size,
-                        (int)B,  (int)W,  (int)(H / Hkv)};
+int naylis_mom_paged_append_rope(void* k_pages, void* v_pages, void* k_scale, void* v_scale, int cache_dtype,
+                                 const void* q, const void* k, const void* v, const int64_t* strides,
+                                 const float* inv_freq, float scaling, const int32_t* table, const int32_t* positions,
+                                 const int32_t* rows, void* q_out, int64_t T, int64_t H, int64_t half, int64_t pages,
+                                 int64_t Hkv, int64_t page_size, int64_t head_dim, int64_t B, int64_t W, void* stream) {
+  const char* who = "mom_paged_append_rope";
+  const PagedCacheDims c{k_pages, v_pages, k_scale, v_scale, (int)pages, (int)Hkv, (int)page_size, (int)B, (int)W, 1};
+  int rc = check_paged(pages, Hkv, page_size, B, W, 1, head_dim, cache_dtype, who);
+  if (rc || (rc = check_cache(c, cache_dtype, who))) return rc;
+  if (T < 0 || T >= (1 << 24))  // a workgroup of 256 threads a token
+    return fail(NAYLIS_ERR_ARG, "%s: bad token count %lld", who, (long long)T);
+  if (H < 0 || H > (1 << 23) / head_dim) return fail(NAYLIS_ERR_ARG, "%s: bad shape H=%lld", who, (long long)H);
+  if (half < 8 || half % 8 != 0 || 2 * half > head_dim)
+    return fail(NAYLIS_ERR_ARG, "%s: %lld frequencies must be a multiple of 8 up to head_dim / 2", who, (long long)half);
+  if (!std::isfinite(scaling)) return fail(NAYLIS_ERR_ARG, "%s: the scaling must be finite", who);
+  if (!rows && T > B)
+    return fail(NAYLIS_ERR_ARG, "%s: %lld tokens without rows for a table of %lld sequences", who, (long long)T,
+                (long long)B);
+  if (T == 0) return NAYLIS_OK;
+  if (!strides || !inv_freq || (!table && B > 0) || !positions)
+    return fail(NAYLIS_ERR_ARG, "%s: null pointer argument", who);
+  if ((rc = check_pointers({k, v}, who)) || (rc = check_strides(strides + 2, "k", who)) ||
+      (rc = check_strides(strides + 4, "v", who)))
+    return rc;
+  if (H > 0 && ((rc = check_pointers({q, q_out}, who)) || (rc = check_strides(strides, "q", who)))) return rc;
+  const PagedRope r{q,          k,          v,          q_out,      inv_freq,   (long)T, strides[0], strides[1],
+                    strides[2], strides[3], strides[4], strides[5], (int)H, (int)half, scaling};
+  return hip_status(launch_paged_append_rope(c, (int)head_dim, paged_format(cache_dtype), r, table, positions, rows,
+                                             (hipStream_t)stream),
+                    who);
 }
 
-static int check_paged_attn(int cache_dtype, int64_t B, int64_t H, int64_t pages, int64_t Hkv, int64_t page_size,
-                            int64_t head_dim, int64_t W, const char* who) {
+int naylis_mom_paged_gather(const void* k_pages, const void* v_pages, const void* k_scale, const void* v_scale,
+                            int cache_dtype, const int32_t* table, const int32_t* cu_seqlens, void* k_out, void* v_out,
+                            int64_t T, int64_t pages, int64_t Hkv, int64_t page_size, int64_t head_dim, int64_t B,
+                            int64_t W, void* stream) {
+  const char* who = "mom_paged_gather";
+  const PagedCacheDims c{const_cast<void*>(k_pages), const_cast<void*>(v_pages), const_cast<void*>(k_scale),
+                         const_cast<void*>(v_scale), (int)pages, (int)Hkv, (int)page_size, (int)B, (int)W, 1};
+  int rc = check_paged(pages, Hkv, page_size, B, W, 1, head_dim, cache_dtype, who);
+  if (rc || (rc = check_cache(c, cache_dtype, who))) return rc;
+  if (B < 1) return fail(NAYLIS_ERR_ARG, "%s: bad shape B=%lld", who, (long long)B);
+  if (T < 0 || T >= (1 << 28))  // a workgroup of 256 threads for 16 tokens
+    return fail(NAYLIS_ERR_ARG, "%s: bad token count %lld", who, (long long)T);
+  if (T == 0) return NAYLIS_OK;
+  if (!table || !cu_seqlens) return fail(NAYLIS_ERR_ARG, "%s: null pointer argument", who);
+  if ((rc = check_pointers({k_out, v_out}, who))) return rc;
+  return hip_status(launch_paged_gather(c, (int)head_dim, paged_format(cache_dtype), table, cu_seqlens, k_out, v_out,
+                                        (long)T, (hipStream_t)stream),
+                    who);
+}
+
+static PagedCacheDims paged_dims(int64_t N, int64_t H, int64_t pages, int64_t Hkv, int64_t page_size, int64_t B,
+                                 int64_t W) {
+  return PagedCacheDims{nullptr, nullptr, nullptr, nullptr, (int)pages, (int)Hkv, (int)page_size,
+                        (int)B,  (int)W,  (int)(H / Hkv), (int)N};
+}
+
+static int check_paged_attn(int cache_dtype, int64_t B, int64_t N, int64_t H, int64_t pages, int64_t Hkv,
+                            int64_t page_size, int64_t head_dim, int64_t W, const char* who) {
   if (Hkv < 1 || H < 1 || H % Hkv != 0)
     return fail(NAYLIS_ERR_ARG, "%s: %lld query heads for %lld key heads", who, (long long)H, (long long)Hkv);
-  if (Hkv * ((H / Hkv + 15) / 16) > 65535)  // one grid row for 16 query heads of a key head
+  if (N < 1 || N > 4096 || N * (H / Hkv) > 4096)
+    return fail(NAYLIS_ERR_ARG, "%s: %lld new tokens of %lld query heads a key head are too many", who, (long long)N,
+                (long long)(H / Hkv));
+  if (Hkv * ((N * (H / Hkv) + 15) / 16) > 65535)  // one grid row for 16 query rows of a key head
     return fail(NAYLIS_ERR_ARG, "%s: %lld query heads for %lld key heads are too many", who, (long long)H,
                 (long long)Hkv);
   return check_paged(pages, Hkv, page_size, B, W, H / Hkv, head_dim, cache_dtype, who);
@@ -1252,34 +1313,116 @@ static int check_paged_attn(int cache_dtype, int64_t B, int64_t H, int64_t pages
 
 size_t naylis_mom_paged_attn_workspace_bytes(int cache_dtype, int64_t B, int64_t H, int64_t Hkv, int64_t page_size,
                                              int64_t head_dim, int64_t W) {
-  if (check_paged_attn(cache_dtype, B, H, 1, Hkv, page_size, head_dim, W, "mom_paged_attn")) return 0;
-  const PagedCacheDims c = paged_dims(H, 1, Hkv, page_size, B, W);
-  return paged_ws_bytes(c, (int)head_dim);
+  return naylis_mom_paged_attn_tokens_workspace_bytes(cache_dtype, B, 1, H, Hkv, page_size, head_dim, W);
 }
 
-int naylis_mom_paged_attn(const void* q, const void* k_pages, const void* v_pages, const float* k_scale,
-                          const float* v_scale, int cache_dtype, const int32_t* table, const int32_t* lens, void* out,
+size_t naylis_mom_paged_attn_tokens_workspace_bytes(int cache_dtype, int64_t B, int64_t N, int64_t H, int64_t Hkv,
+                                                    int64_t page_size, int64_t head_dim, int64_t W) {
+  if (check_paged_attn(cache_dtype, B, N, H, 1, Hkv, page_size, head_dim, W, "mom_paged_attn")) return 0;
+  const PagedCacheDims c = paged_dims(N, H, 1, Hkv, page_size, B, W);
+  return paged_ws_bytes(c, (int)head_dim, paged_format(cache_dtype));
+}
+
+int naylis_mom_paged_attn(const void* q, const void* k_pages, const void* v_pages, const void* k_scale,
+                          const void* v_scale, int cache_dtype, const int32_t* table, const int32_t* lens, void* out,
                           void* workspace, size_t workspace_bytes, const int64_t* q_strides, float scale, int64_t B,
                           int64_t H, int64_t pages, int64_t Hkv, int64_t page_size, int64_t head_dim, int64_t W,
                           void* stream) {
+  const int64_t strides[3] = {q_strides ? q_strides[0] : 0, 0, q_strides ? q_strides[1] : 0};
+  return naylis_mom_paged_attn_tokens(q, k_pages, v_pages, k_scale, v_scale, cache_dtype, table, lens, nullptr, out,
+                                      workspace, workspace_bytes, q_strides ? strides : nullptr, scale, B, 1, H, pages,
+                                      Hkv, page_size, head_dim, W, stream);
+}
+
+int naylis_mom_paged_attn_tokens(const void* q, const void* k_pages, const void* v_pages, const void* k_scale,
+                                 const void* v_scale, int cache_dtype, const int32_t* table, const int32_t* lens,
+                                 const int32_t* q_lens, void* out, void* workspace, size_t workspace_bytes,
+                                 const int64_t* q_strides, float scale, int64_t B, int64_t N, int64_t H, int64_t pages,
+                                 int64_t Hkv, int64_t page_size, int64_t head_dim, int64_t W, void* stream) {
   const char* who = "mom_paged_attn";
-  int rc = check_paged_attn(cache_dtype, B, H, pages, Hkv, page_size, head_dim, W, who);
+  int rc = check_paged_attn(cache_dtype, B, N, H, pages, Hkv, page_size, head_dim, W, who);
   if (rc || (rc = check_scale(scale, who)) || B == 0) return rc;
-  PagedCacheDims c = paged_dims(H, pages, Hkv, page_size, B, W);
+  PagedCacheDims c = paged_dims(N, H, pages, Hkv, page_size, B, W);
   c.k = const_cast<void*>(k_pages);
   c.v = const_cast<void*>(v_pages);
-  c.k_scale = const_cast<float*>(k_scale);
-  c.v_scale = const_cast<float*>(v_scale);
+  c.k_scale = const_cast<void*>(k_scale);
+  c.v_scale = const_cast<void*>(v_scale);
   if ((rc = check_cache(c, cache_dtype, who))) return rc;
   if (!table || !lens || !q_strides) return fail(NAYLIS_ERR_ARG, "%s: null pointer argument", who);
-  if ((rc = check_pointers({q, out}, who)) || (rc = check_strides(q_strides, "q", who))) return rc;
-  const size_t need = paged_ws_bytes(c, (int)head_dim);
+  const int64_t outer[2] = {q_strides[0], q_strides[2]}, inner[2] = {q_strides[1], q_strides[2]};
+  if ((rc = check_pointers({q, out}, who)) || (rc = check_strides(outer, "q", who)) ||
+      (rc = check_strides(inner, "q", who)))
+    return rc;
+  const size_t need = paged_ws_bytes(c, (int)head_dim, paged_format(cache_dtype));
   if (need && (rc = check_pointers({workspace}, who))) return rc;
   if (workspace_bytes < need)
     return fail(NAYLIS_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", who, workspace_bytes, need);
-  return hip_status(launch_paged_attn(c, (int)head_dim, cache_dtype == NAYLIS_DTYPE_E4M3, q, q_strides[0],
-                                      q_strides[1], table, lens, out, workspace, scale, (hipStream_t)stream),
+  const PagedQueries queries{q, (long)q_strides[0], (long)q_strides[1], (long)q_strides[2], q_lens};
+  return hip_status(launch_paged_attn(c, (int)head_dim, paged_format(cache_dtype), queries, table, lens, out,
+                                      workspace, scale, (hipStream_t)stream),
                     who);
+}
+
+// B, N, V of a verification, and whether the drafts have probabilities: its shape as the kernels take it
+static int check_verify(VerifyArgs* a, int64_t B, int64_t N, int64_t V, bool probs, const char* who) {
+  if (B < 0 || B > 65535 || N < 0 || N > 1023 || V < 1 || V > (1 << 28))
+    return fail(NAYLIS_ERR_ARG, "%s: bad shape B=%lld N=%lld V=%lld", who, (long long)B, (long long)N, (long long)V);
+  *a = VerifyArgs{};
+  a->B = (int)B;
+  a->N = (int)N;
+  a->V = (int)V;
+  a->probs = probs ? "" : nullptr;
+  return NAYLIS_OK;
+}
+
+size_t naylis_mom_verify_drafts_workspace_bytes(int64_t B, int64_t N, int64_t V, int draft_probs) {
+  VerifyArgs a;
+  if (check_verify(&a, B, N, V, draft_probs != 0, "mom_verify_drafts")) return 0;
+  return std::max<size_t>(verify_ws_bytes(a), 16);
+}
+
+int naylis_mom_verify_drafts(const void* logits, int dtype, const int64_t* logits_strides, const int64_t* drafts,
+                             const float* uniforms, const void* draft_probs, int probs_dtype,
+                             const int64_t* probs_strides, const int32_t* draft_lens, const float* temperatures,
+                             float temperature, int64_t* tokens, int32_t* accepted, void* workspace,
+                             size_t workspace_bytes, int64_t B, int64_t N, int64_t V, void* stream) {
+  const char* who = "mom_verify_drafts";
+  VerifyArgs a;
+  int rc = check_dtype(dtype, who);
+  if (rc || (rc = check_verify(&a, B, N, V, draft_probs != nullptr, who))) return rc;
+  if (draft_probs && (rc = check_dtype(probs_dtype, who))) return rc;
+  if (!temperatures && !(temperature >= 0.f && std::isfinite(temperature)))
+    return fail(NAYLIS_ERR_ARG, "%s: the temperature must not be negative", who);
+  if (B == 0) return NAYLIS_OK;
+  if (!logits || !logits_strides || (N > 0 && !drafts) || !uniforms || !tokens || !accepted ||
+      (draft_probs && !probs_strides))
+    return fail(NAYLIS_ERR_ARG, "%s: null pointer argument", who);
+  const auto strides_ok = [](const int64_t* s) {
+    return s[0] >= 0 && s[1] >= 0 && s[0] < ((int64_t)1 << 40) && s[1] < ((int64_t)1 << 40);
+  };
+  if (!strides_ok(logits_strides) || (draft_probs && !strides_ok(probs_strides)))
+    return fail(NAYLIS_ERR_ARG, "%s: strides must not be negative", who);
+  if ((uintptr_t)logits % (dtype == NAYLIS_DTYPE_BF16 ? 2 : 4) != 0 ||
+      (uintptr_t)draft_probs % (probs_dtype == NAYLIS_DTYPE_BF16 ? 2 : 4) != 0)
+    return fail(NAYLIS_ERR_ARG, "%s: logits and draft_probs must be aligned to their elements", who);
+  if (workspace_bytes < verify_ws_bytes(a))
+    return fail(NAYLIS_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", who, workspace_bytes,
+                verify_ws_bytes(a));
+  if ((rc = check_pointers({workspace}, who))) return rc;
+  a.drafts = drafts;
+  a.uniforms = uniforms;
+  a.probs = draft_probs;
+  a.probs_bf16 = probs_dtype == NAYLIS_DTYPE_BF16;
+  a.lens = draft_lens;
+  a.temps = temperatures;
+  a.temp = temperature;
+  a.tokens = tokens;
+  a.accepted = accepted;
+  a.ldb = logits_strides[0];
+  a.ldt = logits_strides[1];
+  a.lqb = draft_probs ? probs_strides[0] : 0;
+  a.lqt = draft_probs ? probs_strides[1] : 0;
+  return hip_status(launch_verify(a, logits, dtype == NAYLIS_DTYPE_BF16, workspace, (hipStream_t)stream), who);
 }
 
 static int check_logprobs(const void* logits, int dtype, int64_t ld, const int64_t* tokens, int64_t N, int64_t V,

@@ -143,28 +143,36 @@ hipError_t launch_packed_bwd(const void* q, const void* k, const void* v, const 
                              const float* lse, const void* dout, void* dq, void* dk, void* dv, void* ws,
                              const PackedSeqs& s, const PackedHeads& d, int hd, float scale, hipStream_t st);
 
-// Paged key / value cache (paged.hip): pages (P, Hkv, page, hd) bf16 or e4m3
-// codes with scales (P, Hkv, page); table (B, W) page ids; G query heads for a
-// key head.
+// Paged key / value cache (paged.hip): pages (P, Hkv, page, hd) bf16, e4m3
+// codes with fp32 scales (P, Hkv, page), or pairs of e2m1 codes (.., hd / 2) with
+// the exponents of their scales (P, Hkv, page, hd / 32) in bytes; table (B, W)
+// page ids; G query heads for a key head, N new tokens of a sequence.
+enum PagedFormat { kPagedBf16 = 0, kPagedE4m3 = 1, kPagedE2m1 = 2 };
 struct PagedCacheDims {
   void* k;
   void* v;
-  float* k_scale;
-  float* v_scale;
+  void* k_scale;
+  void* v_scale;
   int P, Hkv, page, B, W, G;
+  int N = 1;
 };
 struct PagedNew {
   long T, ldk, hsk, ldv, hsv;  // new tokens, token and head strides of their k and v
 };
 struct PagedSplit {
-  int wgs, rows, head_tiles;  // workgroups of a slice, its most query heads, slices of a key head
+  int wgs, rows, head_tiles;  // workgroups of a slice, its most query rows, slices of a key head
   bool whole;                 // a workgroup takes a sequence
 };
-size_t paged_ws_bytes(const PagedCacheDims& c, int hd);
-hipError_t launch_paged_append(const PagedCacheDims& c, int hd, bool fp8, const void* k, const void* v,
+struct PagedQueries {
+  const void* q;
+  long ldb, ldt, hs;      // sequence, token and head strides
+  const int32_t* live;    // (B) new tokens of each sequence, NULL for N
+};
+size_t paged_ws_bytes(const PagedCacheDims& c, int hd, PagedFormat fmt);
+hipError_t launch_paged_append(const PagedCacheDims& c, int hd, PagedFormat fmt, const void* k, const void* v,
                                const int32_t* table, const int32_t* positions, const int32_t* rows,
                                const PagedNew& src, hipStream_t st);
-hipError_t launch_paged_attn(const PagedCacheDims& c, int hd, bool fp8, const void* q, long ldq, long hsq,
+hipError_t launch_paged_attn(const PagedCacheDims& c, int hd, PagedFormat fmt, const PagedQueries& q,
                              const int32_t* table, const int32_t* lens, void* out, void* ws, float scale,
                              hipStream_t st);
 
@@ -178,6 +186,42 @@ hipError_t launch_logprobs_fwd(const void* logits, bool bf16, long ld, const int
 hipError_t launch_logprobs_bwd(const void* logits, bool bf16, long ld, const int64_t* tokens, const float* stat,
                                const float* g_logp, long gl_stride, const float* g_entropy, long ge_stride,
                                void* dlogits, long N, int V, long ignore_index, hipStream_t st);
+
+// A chunk of new tokens rotated and into the cache, and sequences of the cache
+// back dense (paged_chunk.hip).
+struct PagedRope {
+  const void* q;  // (T, H, hd), or NULL with H = 0
+  const void* k;
+  const void* v;
+  void* q_out;            // dense
+  const float* inv_freq;  // (half)
+  long T, ldq, hsq, ldk, hsk, ldv, hsv;
+  int H, half;
+  float scaling;
+};
+hipError_t launch_paged_append_rope(const PagedCacheDims& c, int hd, PagedFormat fmt, const PagedRope& r,
+                                    const int32_t* table, const int32_t* positions, const int32_t* rows,
+                                    hipStream_t st);
+hipError_t launch_paged_gather(const PagedCacheDims& c, int hd, PagedFormat fmt, const int32_t* table,
+                               const int32_t* cu, void* k_out, void* v_out, long T, hipStream_t st);
+
+// Drafted tokens against logits (verify.hip): logits (B, N + 1, V) with strides
+// ldb, ldt, probs (B, N, V) of the drafts with lqb, lqt, or NULL.
+struct VerifyArgs {
+  const int64_t* drafts;  // (B, N)
+  const float* uniforms;  // (B, N + 1)
+  const void* probs;
+  const int32_t* lens;  // (B), NULL for N
+  const float* temps;   // (B), NULL for temp
+  int64_t* tokens;      // (B, N + 1)
+  int32_t* accepted;    // (B)
+  long ldb, ldt, lqb, lqt;
+  float temp;
+  int B, N, V, parts;
+  bool probs_bf16;
+};
+size_t verify_ws_bytes(const VerifyArgs& a);
+hipError_t launch_verify(VerifyArgs a, const void* logits, bool bf16, void* ws, hipStream_t st);
 
 // SwiGLU of the decoder MLP (swiglu.hip): h = silu(g) * u forward; backward
 // writes dg and du from dh; n elements, a multiple of 8.

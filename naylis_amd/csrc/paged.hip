@@ -33,6 +33,7 @@
 #include "common.h"
 #include "launch.h"
 #include "packed_tiles.h"
+#include "paged_common.h"
 #include "timing.h"
 
 #include <algorithm>
@@ -43,27 +44,12 @@ namespace naylis {
 namespace {
 
 constexpr int kRowsMfma = 16;       // query heads of a product
-constexpr int kPagedStep = 32;      // tokens of a step
+// tokens of a step (4 bits: as many bytes under way take more tokens)
+constexpr int paged_step(PagedFormat f) { return f == kPagedE2m1 ? 64 : 32; }
 constexpr int kPagedMaxWgs = 512;   // workgroups that share a slice's steps
 
 __device__ __forceinline__ f32x4 mfma16(const bf16x8& a, const bf16x8& b, const f32x4& c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
-}
-
-// eight e4m3 codes as bf16 (exact)
-__device__ __forceinline__ bf16x8 widen8(uint32_t lo, uint32_t hi) {
-  bf16x8 r;
-  const uint32_t w[2] = {lo, hi};
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const auto a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[i], false);
-    const auto b = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[i], true);
-    r[4 * i] = (__bf16)a[0];
-    r[4 * i + 1] = (__bf16)a[1];
-    r[4 * i + 2] = (__bf16)b[0];
-    r[4 * i + 3] = (__bf16)b[1];
-  }
-  return r;
 }
 
 // The wave's own LDS writes before its reads, and the other way round: LDS
@@ -73,15 +59,12 @@ __device__ __forceinline__ void lds_order() {
   __builtin_amdgcn_wave_barrier();
 }
 
-// Whether a table entry is a page.
-__device__ __forceinline__ bool page_ok(int id, int pages) { return id >= 0 && id < pages; }
-
 }  // namespace
 
 // New rows into the cache, HD / 8 lanes a row.  Token t goes to sequence
 // rows[t] (t itself without rows) at positions[t]; a position or a page outside
 // the table or the cache (padding) writes nothing.
-template <int HD, bool FP8>
+template <int HD, PagedFormat FMT>
 __global__ __launch_bounds__(256) void paged_append_kernel(PagedCacheDims c, const bf16_t* __restrict__ k,
                                                            const bf16_t* __restrict__ v,
                                                            const int32_t* __restrict__ table,
@@ -101,31 +84,18 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedCacheDims c, con
   const bf16_t* x = is_v ? v + t * src.ldv + h * src.hsv : k + t * src.ldk + h * src.hsk;
   const uint4 u = *reinterpret_cast<const uint4*>(x + 8 * piece);
   const long row = ((long)pg * c.Hkv + h) * c.page + pos % c.page;
-  if constexpr (!FP8) {
+  if constexpr (FMT == kPagedBf16) {
     reinterpret_cast<uint4*>(is_v ? c.v : c.k)[row * LANES + piece] = u;
   } else {
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-    float f[8], top = 0.f;
+    float f[8];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       f[2 * i] = __uint_as_float(w[i] << 16);
       f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-      top = fmaxf(top, fmaxf(fabsf(f[2 * i]), fabsf(f[2 * i + 1])));
     }
     // the row's lanes are all here: they share t and so every return above
-    const auto mx = [](float a, float b) { return fmaxf(a, b); };
-    top = mx(top, dpp_f32<0xb1>(top));
-    top = mx(top, dpp_f32<0x4e>(top));
-    top = mx(top, dpp_f32<0x141>(top));
-    if constexpr (LANES == 16) top = mx(top, dpp_f32<0x140>(top));
-    const float s = top > 0.f ? top / 448.f : 1.f;
-    int lo = 0, hi = 0;
-    lo = __builtin_amdgcn_cvt_pk_fp8_f32(f[0] / s, f[1] / s, lo, false);
-    lo = __builtin_amdgcn_cvt_pk_fp8_f32(f[2] / s, f[3] / s, lo, true);
-    hi = __builtin_amdgcn_cvt_pk_fp8_f32(f[4] / s, f[5] / s, hi, false);
-    hi = __builtin_amdgcn_cvt_pk_fp8_f32(f[6] / s, f[7] / s, hi, true);
-    reinterpret_cast<uint2*>(is_v ? c.v : c.k)[row * LANES + piece] = make_uint2((uint32_t)lo, (uint32_t)hi);
-    if (piece == 0) (is_v ? c.v_scale : c.k_scale)[row] = s;
+    store_codes<HD, FMT>(c, is_v, row, piece, f);
   }
 }
 
@@ -134,6 +104,7 @@ namespace {
 // The list of all sequences' steps.  A lane looks after an equal chunk of the
 // sequences, so that a place is found with one scan over the lanes and one over
 // a chunk, whatever their number.
+template <int STEP>
 struct StepList {
   const int32_t* lens;
   int B, cap;  // sequences, tokens that a table row holds
@@ -143,7 +114,7 @@ struct StepList {
     const int n = lens[min(b, B - 1)];
     return b < B ? min(max(n, 0), cap) : 0;
   }
-  __device__ __forceinline__ int steps(int b) const { return (len(b) + kPagedStep - 1) / kPagedStep; }
+  __device__ __forceinline__ int steps(int b) const { return (len(b) + STEP - 1) / STEP; }
 
   static __device__ __forceinline__ int inclusive(int x) {
     const int lane = threadIdx.x & 63;
@@ -221,6 +192,33 @@ __device__ __forceinline__ int v_slot(int row, int chunk) {  // byte of a 16-byt
 __device__ __forceinline__ uint4 load_once16(const uint8_t* p) {
   return __builtin_bit_cast(uint4, __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(p)));
 }
+template <int N>
+struct Words {
+  uint32_t w[N];
+};
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+template <int N>
+__device__ __forceinline__ Words<N> load_once(const uint8_t* p) {
+  using V = std::conditional_t<N == 4, u32x4, u32x2>;
+  static_assert(N == 2 || N == 4, "8 or 16 bytes");
+  return __builtin_bit_cast(Words<N>, __builtin_nontemporal_load(reinterpret_cast<const V*>(p)));
+}
+
+// A query row of a key head is (new token, query head): token-major, so that one
+// product's 16 rows see nearly the same keys.
+struct Rows {
+  int G, N, H;
+  __device__ __forceinline__ int token(int row) const { return row / G; }
+  // row `row` of key head kvh in out (B, N, H, hd), in heads
+  __device__ __forceinline__ long at(int b, int kvh, int row) const {
+    return ((long)b * N + row / G) * H + kvh * G + row % G;
+  }
+};
+
+// Tokens that new token i of a sequence of n sees, where the last of `live` sees
+// all; 0 for one that is none or sees nothing.
+__device__ __forceinline__ int seen(int n, int live, int i) { return i < live ? max(n - (live - 1 - i), 0) : 0; }
 
 }  // namespace
 
@@ -229,25 +227,28 @@ __device__ __forceinline__ long part_row(const PagedSplit& p, int slice, int wg,
   return (((long)slice * p.wgs + wg) * 2 + slot) * p.rows;
 }
 
-// grid (workgroups of a slice, slices): slice = (key head, 16 of its query heads).
+// grid (workgroups of a slice, slices): slice = (key head, 16 of its query rows).
 // A workgroup takes a range of the step list, or (p.whole) the sequence of its
 // number, its waves an equal share each.
-// ROWS: partials' rows, at least the query heads of a slice.
-template <int HD, bool FP8, int ROWS>
-__global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedCacheDims c, const bf16_t* __restrict__ q, long ldq,
-                                                            long hsq, const int32_t* __restrict__ table,
+// ROWS: partials' rows, at least the query rows of a slice.  MANY: more than one
+// new token, or a number of them that each sequence has of its own.
+template <int HD, PagedFormat FMT, int ROWS, bool MANY>
+__global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedCacheDims c, PagedQueries q,
+                                                            const int32_t* __restrict__ table,
                                                             const int32_t* __restrict__ lens,
                                                             bf16_t* __restrict__ out, float* __restrict__ part,
                                                             float2* __restrict__ stat, int* __restrict__ starts,
                                                             PagedSplit p, float sc) {
-  constexpr int TOK = kPagedStep;        // tokens of a step
+  constexpr bool FP8 = FMT == kPagedE4m3, FP4 = FMT == kPagedE2m1;
+  constexpr int TOK = paged_step(FMT);   // tokens of a step
   constexpr int NS = TOK / 16;           // its 16-token products
   constexpr int KS = HD / 32;            // products along the features
   constexpr int NT = HD / 16;            // 16-feature tiles of the output
-  constexpr int RB = FP8 ? HD : 2 * HD;  // bytes of a cache row
-  constexpr int KL = RB / 64;            // 16-byte loads of a lane for 16 tokens of K
-  constexpr int VR = 1024 / RB;          // rows of V that a load of 64 lanes covers
+  constexpr int RB = FP4 ? HD / 2 : FP8 ? HD : 2 * HD;  // bytes of a cache row
+  constexpr int KL = FP4 ? 1 : RB / 64;  // 16-byte loads of a lane for 16 tokens of K
+  constexpr int VR = FP4 ? 16 : 1024 / RB;  // rows of V that a load of 64 lanes covers
   constexpr int VL = TOK / VR;           // such loads
+  constexpr int NW = HD / 32;            // 4 bits: words of such a load, HD / 4 features
   __shared__ __align__(16) uint8_t lds[4 * kWaveLds<HD, ROWS>];
   __shared__ PartSeq seqs[8];
   __shared__ float2 stats[8][ROWS];
@@ -256,9 +257,17 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedCacheDims c, co
   uint8_t* vt = lds + wave * kWaveLds<HD, ROWS>;
   const int wg = blockIdx.x, slice = blockIdx.y;
   const int kvh = slice / p.head_tiles, h0 = kRowsMfma * (slice % p.head_tiles);
-  const int nh = min(kRowsMfma, c.G - h0);  // live query heads of the slice
+  const int nh = min(kRowsMfma, (MANY ? c.G * c.N : c.G) - h0);  // live query rows of the slice
   const int H = c.Hkv * c.G, hbase = kvh * c.G + h0;
-  const StepList list{lens, c.B, c.W * c.page};
+  const Rows rows{c.G, c.N, H};
+  // the slice's row r of sequence b in out
+  const auto out_row = [&](long b, int r) {
+    return out + (MANY ? rows.at((int)b, kvh, h0 + r) : b * H + hbase + r) * HD;
+  };
+  const auto live_of = [&](int b) { return q.live ? min(max(q.live[b], 0), c.N) : c.N; };
+  // whether the slice's row r sees no token of sequence b
+  const auto blind = [&](int b, int r) { return MANY && seen(lens[b], live_of(b), rows.token(h0 + r)) == 0; };
+  const StepList<TOK> list{lens, c.B, c.W * c.page};
 
   int wg0, wg1, at, end, b = wg, first = 0;
   int2 sums = make_int2(0, 0);
@@ -281,24 +290,32 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedCacheDims c, co
   if (lane < 2) seqs[2 * wave + lane].b = -1;
 
   const int shift = 31 - __clz(c.page);
-  const int voff = lane * 16;          // V: row lane / (RB / 16), piece lane % (RB / 16)
-  const int koff = r16 * RB + g * 16;  // K: row r16, pieces g, g + 4, ..
-  const int vrow = lane / (RB / 16), vpc = lane % (RB / 16);
+  // bytes of a lane's loads.  V: row vrow, piece vpc; K: row r16, pieces g, g + 4, ..
+  const int voff = lane * (FP4 ? 4 * NW : 16), koff = r16 * RB + g * (FP4 ? 4 * NW : 16);
+  const int vrow = FP4 ? lane / 4 : lane / (RB / 16), vpc = FP4 ? lane % 4 : lane % (RB / 16);
   const int begin = at;
 
   while (at < end && b < c.B) {
     const int n = list.len(b), nsteps = (n + TOK - 1) / TOK;
     const int s0 = at - first, s1 = min(end - first, nsteps);  // this wave's steps of sequence b
     bool bad = lens[b] > list.cap;                             // longer than its table
+    // tokens that the lane's row sees, and the fewest that one does
+    const int live = MANY ? live_of(b) : 1, all = n - (live - 1);
+    const int mine = MANY ? n - max(live - 1 - rows.token(h0 + r16), 0) : n;
     if (!p.whole && s0 == 0 && slice == 0 && lane == 0) starts[b] = first;
 
     bf16x8 qf[KS];
     {
-      const bf16_t* qp = q + (long)b * ldq + (long)(hbase + min(r16, nh - 1)) * hsq;
+      const int row = h0 + min(r16, nh - 1);
+      const bf16_t* qp = (const bf16_t*)q.q + (long)b * q.ldb +
+                         (MANY ? rows.token(row) * q.ldt + (long)(kvh * c.G + row % c.G) * q.hs
+                               : (long)(kvh * c.G + row) * q.hs);
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
         // feature order of the products: as the lane's 16-byte pieces of K hold them
-        const int f = FP8 ? 64 * (ks >> 1) + 16 * g + 8 * (ks & 1) : 32 * ks + 8 * g;
+        const int f = FP4   ? 8 * NW * g + 8 * ks
+                      : FP8 ? 64 * (ks >> 1) + 16 * g + 8 * (ks & 1)
+                            : 32 * ks + 8 * g;
         qf[ks] = *reinterpret_cast<const bf16x8*>(qp + f);
         if (r16 >= nh) qf[ks] = bf16x8{};
       }
@@ -311,7 +328,9 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedCacheDims c, co
     // pages of the next 64 products' tokens, one a lane
     int ids = 0, ids_at = -64;
     uint4 kx[NS][KL], vx[VL];
-    f32x4 ksc[NS], vsc[NS];  // scales of tokens 16 i + 4 g ..
+    Words<NW> kw[NS], vw[NS];  // 4 bits
+    uint32_t ke[NS], ve[NS];   // their scales' exponents
+    f32x4 ksc[NS], vsc[NS];    // scales of tokens 16 i + 4 g ..
     long row16[NS];          // cache row of each 16-token group of the step being loaded
     auto find_pages = [&](int step) {
 #pragma unroll
@@ -333,24 +352,36 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedCacheDims c, co
     auto load_k = [&]() {
 #pragma unroll
       for (int i = 0; i < NS; ++i) {
+        if constexpr (FP4) {
+          kw[i] = load_once<NW>((const uint8_t*)c.k + row16[i] * RB + koff);
+          ke[i] = ((const uint8_t*)c.k_scale)[row16[i] * NW + r16 * NW + g * NW / 4];
+        } else {
 #pragma unroll
-        for (int j = 0; j < KL; ++j) kx[i][j] = load_once16((const uint8_t*)c.k + row16[i] * RB + koff + 64 * j);
+          for (int j = 0; j < KL; ++j) kx[i][j] = load_once16((const uint8_t*)c.k + row16[i] * RB + koff + 64 * j);
+        }
         if constexpr (FP8) {
-          ksc[i] = *reinterpret_cast<const f32x4*>(c.k_scale + row16[i] + 4 * g);
-          vsc[i] = *reinterpret_cast<const f32x4*>(c.v_scale + row16[i] + 4 * g);
+          ksc[i] = *reinterpret_cast<const f32x4*>((const float*)c.k_scale + row16[i] + 4 * g);
+          vsc[i] = *reinterpret_cast<const f32x4*>((const float*)c.v_scale + row16[i] + 4 * g);
         }
       }
     };
-    auto load_v = [&]() {
+    // 16-token groups i0 ..
+    auto load_v = [&](int i0, int n) {
 #pragma unroll
-      for (int i = 0; i < NS; ++i)
+      for (int i = i0; i < i0 + n; ++i) {
+        if constexpr (FP4) {
+          vw[i] = load_once<NW>((const uint8_t*)c.v + row16[i] * RB + voff);
+          ve[i] = ((const uint8_t*)c.v_scale)[row16[i] * NW + lane * NW / 4];
+        } else {
 #pragma unroll
-        for (int j = 0; j < VL / NS; ++j)
-          vx[i * (VL / NS) + j] = load_once16((const uint8_t*)c.v + row16[i] * RB + voff + 1024 * j);
+          for (int j = 0; j < VL / NS; ++j)
+            vx[i * (VL / NS) + j] = load_once16((const uint8_t*)c.v + row16[i] * RB + voff + 1024 * j);
+        }
+      }
     };
     find_pages(s0);
     load_k();
-    load_v();
+    load_v(0, NS);
     for (int s = s0; s < s1; ++s) {
       const int tok0 = s * TOK;
       // S^T: lane = query head r16, registers = tokens 16 i + 4 g + v
@@ -361,7 +392,9 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedCacheDims c, co
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
           bf16x8 kf;
-          if constexpr (FP8) {
+          if constexpr (FP4) {
+            kf = widen8_e2m1(kw[i].w[ks], ke[i]);
+          } else if constexpr (FP8) {
             const uint4 u = kx[i][ks >> 1];
             kf = (ks & 1) ? widen8(u.z, u.w) : widen8(u.x, u.y);
           } else {
@@ -370,9 +403,26 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedCacheDims c, co
           x[i] = mfma16(kf, qf[ks], x[i]);
         }
       }
-      const bool tail = tok0 + TOK > n;
-      // V rows to LDS as bf16; rows past the sequence as zeros, whatever the page holds there
-      auto store_v = [&]() {
+      const bool tail = tok0 + TOK > (MANY ? all : n);
+      // V rows to LDS as bf16, 32 tokens from `half` on; rows past the sequence as zeros, whatever the page holds there
+      auto store_v = [&](int half) {
+        if constexpr (FP4) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int row = 16 * i + vrow;
+            Words<NW> u = vw[2 * half + i];
+            uint32_t e = ve[2 * half + i];
+            if (tail && tok0 + 32 * half + row >= n) {
+              u = Words<NW>{};
+              e = 127;
+            }
+#pragma unroll
+            for (int w = 0; w < NW; ++w)
+              *reinterpret_cast<bf16x8*>(vt + v_slot<HD>(row, NW * vpc + w)) = widen8_e2m1(u.w[w], e);
+          }
+          lds_order();
+          return;
+        }
 #pragma unroll
         for (int j = 0; j < VL; ++j) {
           const int row = j * VR + vrow;
@@ -401,15 +451,15 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedCacheDims c, co
         find_pages(s + 1);
         load_k();
       }
-      store_v();
-      if (more) load_v();
+      store_v(0);
+      if (more) load_v(0, FP4 ? 2 : NS);
       float mx = -INFINITY;
 #pragma unroll
       for (int i = 0; i < NS; ++i)
 #pragma unroll
         for (int v = 0; v < 4; ++v) {
           x[i][v] *= FP8 ? kss[i][v] : sc;
-          if (tail && tok0 + 16 * i + 4 * g + v >= n) {
+          if (tail && tok0 + 16 * i + 4 * g + v >= mine) {
             x[i][v] = -INFINITY;
             if constexpr (FP8) vss[i][v] = 0.f;
           }
@@ -430,24 +480,31 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedCacheDims c, co
           l += x[i][v];
           if constexpr (FP8) x[i][v] *= vss[i][v];
         }
-      // O^T += V^T P^T: registers of the two products are the B operand
-      bf16x8 pf;
+      // O^T += V^T P^T: registers of two products are the B operand
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        pf[e] = (__bf16)x[0][e];
-        pf[4 + e] = (__bf16)x[1][e];
-      }
-      const int rlo = 4 * g + (r16 >> 2), rhi = rlo + 16;
+      for (int half = 0; half < TOK / 32; ++half) {
+        if (half) {
+          store_v(half);
+          if (more) load_v(2 * half, 2);
+        }
+        bf16x8 pf;
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        const int ch = 2 * t + ((r16 & 3) >> 1), b8 = 8 * (r16 & 1);
-        const v4i16 lo = lds_read_tr16(reinterpret_cast<const bf16_t*>(vt + v_slot<HD>(rlo, ch) + b8));
-        const v4i16 hi = lds_read_tr16(reinterpret_cast<const bf16_t*>(vt + v_slot<HD>(rhi, ch) + b8));
-        typedef short v8i16 __attribute__((ext_vector_type(8)));
-        const v8i16 vf = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-        acc[t] = mfma16(__builtin_bit_cast(bf16x8, vf), pf, acc[t]);
+        for (int e = 0; e < 4; ++e) {
+          pf[e] = (__bf16)x[2 * half][e];
+          pf[4 + e] = (__bf16)x[2 * half + 1][e];
+        }
+        const int rlo = 4 * g + (r16 >> 2), rhi = rlo + 16;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          const int ch = 2 * t + ((r16 & 3) >> 1), b8 = 8 * (r16 & 1);
+          const v4i16 lo = lds_read_tr16(reinterpret_cast<const bf16_t*>(vt + v_slot<HD>(rlo, ch) + b8));
+          const v4i16 hi = lds_read_tr16(reinterpret_cast<const bf16_t*>(vt + v_slot<HD>(rhi, ch) + b8));
+          typedef short v8i16 __attribute__((ext_vector_type(8)));
+          const v8i16 vf = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+          acc[t] = mfma16(__builtin_bit_cast(bf16x8, vf), pf, acc[t]);
+        }
+        lds_order();
       }
-      lds_order();
     }
     const auto add = [](float a, float b2) { return a + b2; };
     l = xor32_f32(xor16_f32(l, add), add);
@@ -455,12 +512,14 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedCacheDims c, co
     if (s0 == 0 && s1 == nsteps) {
       if (r16 < nh) {
         const float inv = 1.f / l;
+        const bool none = blind(b, r16);
+        bf16_t* to = out_row(b, r16);
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
           bf16x4 o;
 #pragma unroll
-          for (int v = 0; v < 4; ++v) o[v] = (__bf16)(acc[t][v] * inv);
-          *reinterpret_cast<bf16x4*>(out + ((long)b * H + hbase + r16) * HD + 16 * t + 4 * g) = o;
+          for (int v = 0; v < 4; ++v) o[v] = (__bf16)(none ? 0.f : acc[t][v] * inv);
+          *reinterpret_cast<bf16x4*>(to + 16 * t + 4 * g) = o;
         }
       }
     } else {
@@ -518,10 +577,11 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedCacheDims c, co
       if (next[e] == cur.b) continue;
       if (cur.first >= wg0 && cur.first + cur.steps <= wg1) {
         const float inv = 1.f / l;
+        const bool none = blind(cur.b, r);
         bf16x4 o;
 #pragma unroll
-        for (int v = 0; v < 4; ++v) o[v] = (__bf16)(a[v] * inv);
-        *reinterpret_cast<bf16x4*>(out + ((long)cur.b * H + hbase + r) * HD + f) = o;
+        for (int v = 0; v < 4; ++v) o[v] = (__bf16)(none ? 0.f : a[v] * inv);
+        *reinterpret_cast<bf16x4*>(out_row(cur.b, r) + f) = o;
       } else {
         const long row = part_row(p, slice, wg, cur.first <= wg0 ? 0 : 1) + r;
         *reinterpret_cast<f32x4*>(part + row * HD + f) = a;
@@ -535,7 +595,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedCacheDims c, co
   // zeros for the sequences without tokens: the workgroup's own, or 64 sequences a wave
   const auto empty = [&](long z) {
     for (int i = lane; i < nh * (HD / 4); i += 64)
-      *reinterpret_cast<bf16x4*>(out + (z * H + hbase) * HD + 4 * i) = bf16x4{};
+      *reinterpret_cast<bf16x4*>(out_row(z, i / (HD / 4)) + 4 * (i % (HD / 4))) = bf16x4{};
   };
   if (p.whole) {
     if (wg1 == 0 && wave == 0 && wg < c.B) empty(wg);
@@ -548,24 +608,25 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedCacheDims c, co
 }
 
 // Joins the workgroups' partials of a sequence; nothing where one of them held
-// it whole.  Grid (H, B).
-template <int HD>
-__global__ __launch_bounds__(256) void paged_join_kernel(PagedCacheDims c, const int32_t* __restrict__ lens,
-                                                         bf16_t* __restrict__ out, const float* __restrict__ part,
-                                                         const float2* __restrict__ stat, const int* __restrict__ starts,
-                                                         PagedSplit p) {
+// it whole.  Grid (N H, B).
+template <int HD, int STEP>
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedCacheDims c, const int32_t* __restrict__ live,
+                                                         const int32_t* __restrict__ lens, bf16_t* __restrict__ out,
+                                                         const float* __restrict__ part, const float2* __restrict__ stat,
+                                                         const int* __restrict__ starts, PagedSplit p) {
   constexpr int TR = HD / 4, NG = 256 / TR;  // threads of a partial; partials read at once
   __shared__ float weight[kPagedMaxWgs];
   __shared__ float red[4];
   __shared__ f32x4 sums[NG][TR];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int h = blockIdx.x, b = blockIdx.y;
-  const int n = StepList{lens, c.B, c.W * c.page}.steps(b);
+  const int H = c.Hkv * c.G, token = blockIdx.x / H, h = blockIdx.x % H, b = blockIdx.y;
+  const StepList<STEP> list{lens, c.B, c.W * c.page};
+  const int n = list.steps(b);
   if (n == 0) return;
   const int total = starts[c.B], range = max((total + p.wgs - 1) / p.wgs, 1);
   const int first = starts[b], w0 = first / range, w1 = (first + n - 1) / range;
   if (w0 == w1) return;
-  const int kvh = h / c.G, hr = h % c.G, slice = kvh * p.head_tiles + hr / kRowsMfma;
+  const int kvh = h / c.G, hr = token * c.G + h % c.G, slice = kvh * p.head_tiles + hr / kRowsMfma;
   const int count = w1 - w0 + 1;
   // a workgroup's first sequence, unless its range begins before this one
   const auto row = [&](int i) {
@@ -609,11 +670,12 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedCacheDims c, const
   if (gi) return;
 #pragma unroll
   for (int i = 1; i < NG; ++i) a += sums[i][f];
+  const bool none = seen(lens[b], live ? min(max(live[b], 0), c.N) : c.N, token) == 0;
   const float inv = 1.f / l;
   bf16x4 o;
 #pragma unroll
-  for (int v = 0; v < 4; ++v) o[v] = (__bf16)(a[v] * inv);
-  *reinterpret_cast<bf16x4*>(out + ((long)b * c.Hkv * c.G + h) * HD + 4 * f) = o;
+  for (int v = 0; v < 4; ++v) o[v] = (__bf16)(none ? 0.f : a[v] * inv);
+  *reinterpret_cast<bf16x4*>(out + (((long)b * c.N + token) * H + h) * HD + 4 * f) = o;
 }
 
 // A workgroup for each sequence where tables hold at most 16 steps, four for each
@@ -622,12 +684,13 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedCacheDims c, const
 // slices, and no finer than a step a wave.
 // Three or four a CU take longer (three contexts of 65537 .. 131072 tokens, e4m3:
 // 124 us with 512 workgroups, 147 with 768, 130 with 1024).
-PagedSplit paged_split(const PagedCacheDims& c) {
+PagedSplit paged_split(const PagedCacheDims& c, PagedFormat fmt) {
   PagedSplit p;
-  p.head_tiles = (c.G + kRowsMfma - 1) / kRowsMfma;
-  p.rows = c.G <= 4 ? 4 : kRowsMfma;
+  const int step = paged_step(fmt), rows = c.G * c.N;
+  p.head_tiles = (rows + kRowsMfma - 1) / kRowsMfma;
+  p.rows = rows <= 4 ? 4 : kRowsMfma;
   const long slices = (long)c.Hkv * p.head_tiles;
-  const long cap = ((long)c.W * c.page + kPagedStep - 1) / kPagedStep;
+  const long cap = ((long)c.W * c.page + step - 1) / step;
   p.whole = cap <= 16;
   p.wgs = (int)(p.whole ? std::max(c.B, 1)
                         : std::max(1L, std::min({512 / slices, (c.B * cap + 3) / 4, (long)kPagedMaxWgs})));
@@ -639,57 +702,75 @@ size_t paged_part_floats(const PagedCacheDims& c, const PagedSplit& p, int hd) {
 }
 
 // partials, their (maximum, sum), and each sequence's first step with the number of all behind the last
-size_t paged_ws_bytes(const PagedCacheDims& c, int hd) {
-  const size_t n = paged_part_floats(c, paged_split(c), hd);
+size_t paged_ws_bytes(const PagedCacheDims& c, int hd, PagedFormat fmt) {
+  const size_t n = paged_part_floats(c, paged_split(c, fmt), hd);
   return n == 0 ? 0 : n * 4 + n / hd * 8 + ((size_t)c.B + 1) * 4;
 }
 
-hipError_t launch_paged_append(const PagedCacheDims& c, int hd, bool fp8, const void* k, const void* v,
+namespace {
+
+template <PagedFormat F>
+using Format = std::integral_constant<PagedFormat, F>;
+
+// f(head dim, format) as compile-time constants
+template <typename F>
+void with_format(int hd, PagedFormat fmt, F f) {
+  auto go = [&](auto d) {
+    if (fmt == kPagedBf16)
+      f(d, Format<kPagedBf16>{});
+    else if (fmt == kPagedE4m3)
+      f(d, Format<kPagedE4m3>{});
+    else
+      f(d, Format<kPagedE2m1>{});
+  };
+  hd == 64 ? go(std::integral_constant<int, 64>{}) : go(std::integral_constant<int, 128>{});
+}
+
+}  // namespace
+
+hipError_t launch_paged_append(const PagedCacheDims& c, int hd, PagedFormat fmt, const void* k, const void* v,
                                const int32_t* table, const int32_t* positions, const int32_t* rows,
                                const PagedNew& src, hipStream_t st) {
   const long threads = src.T * c.Hkv * 2 * (hd / 8);
-  auto run = [&](auto kernel) {
+  with_format(hd, fmt, [&](auto d, auto f) {
     NAYLIS_TIMED("paged_append", st,
-                 hipLaunchKernelGGL(kernel, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, st, c,
-                                    (const bf16_t*)k, (const bf16_t*)v, table, positions, rows, src));
-  };
-  if (hd == 64)
-    fp8 ? run(paged_append_kernel<64, true>) : run(paged_append_kernel<64, false>);
-  else
-    fp8 ? run(paged_append_kernel<128, true>) : run(paged_append_kernel<128, false>);
+                 hipLaunchKernelGGL((paged_append_kernel<decltype(d)::value, decltype(f)::value>),
+                                    dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, st, c, (const bf16_t*)k,
+                                    (const bf16_t*)v, table, positions, rows, src));
+  });
   return hipGetLastError();
 }
 
-hipError_t launch_paged_attn(const PagedCacheDims& c, int hd, bool fp8, const void* q, long ldq, long hsq,
+hipError_t launch_paged_attn(const PagedCacheDims& c, int hd, PagedFormat fmt, const PagedQueries& q,
                              const int32_t* table, const int32_t* lens, void* out, void* ws, float scale,
                              hipStream_t st) {
-  const PagedSplit p = paged_split(c);
+  const PagedSplit p = paged_split(c, fmt);
   float* part = (float*)ws;
   const size_t n = paged_part_floats(c, p, hd);
   float2* stat = (float2*)(part + n);
   int* starts = (int*)(stat + n / hd);
   auto run = [&](auto kernel) {
     NAYLIS_TIMED("paged_attn", st,
-                 hipLaunchKernelGGL(kernel, dim3(p.wgs, c.Hkv * p.head_tiles), dim3(256), 0, st, c,
-                                    (const bf16_t*)q, ldq, hsq, table, lens, (bf16_t*)out, part, stat, starts, p,
-                                    scale * kLog2e));
+                 hipLaunchKernelGGL(kernel, dim3(p.wgs, c.Hkv * p.head_tiles), dim3(256), 0, st, c, q, table, lens,
+                                    (bf16_t*)out, part, stat, starts, p, scale * kLog2e));
   };
-  auto pick = [&](auto rows) {
-    constexpr int R = decltype(rows)::value;
-    if (hd == 64)
-      fp8 ? run(paged_attn_kernel<64, true, R>) : run(paged_attn_kernel<64, false, R>);
+  with_format(hd, fmt, [&](auto d, auto f) {
+    constexpr int HD = decltype(d)::value;
+    constexpr PagedFormat F = decltype(f)::value;
+    if (c.N > 1 || q.live)
+      p.rows == 4 ? run(paged_attn_kernel<HD, F, 4, true>) : run(paged_attn_kernel<HD, F, 16, true>);
     else
-      fp8 ? run(paged_attn_kernel<128, true, R>) : run(paged_attn_kernel<128, false, R>);
-  };
-  p.rows == 4 ? pick(std::integral_constant<int, 4>{}) : pick(std::integral_constant<int, 16>{});
+      p.rows == 4 ? run(paged_attn_kernel<HD, F, 4, false>) : run(paged_attn_kernel<HD, F, 16, false>);
+  });
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || p.whole || p.wgs == 1) return e;
-  auto join = [&](auto kernel) {
+  with_format(hd, fmt, [&](auto d, auto f) {
+    constexpr int HD = decltype(d)::value, STEP = paged_step(decltype(f)::value);
     NAYLIS_TIMED("paged_join", st,
-                 hipLaunchKernelGGL(kernel, dim3(c.Hkv * c.G, c.B), dim3(256), 0, st, c, lens, (bf16_t*)out,
-                                    (const float*)part, (const float2*)stat, (const int*)starts, p));
-  };
-  hd == 64 ? join(paged_join_kernel<64>) : join(paged_join_kernel<128>);
+                 hipLaunchKernelGGL((paged_join_kernel<HD, STEP>), dim3(c.Hkv * c.G * c.N, c.B), dim3(256), 0, st, c,
+                                    q.live, lens, (bf16_t*)out, (const float*)part, (const float2*)stat,
+                                    (const int*)starts, p));
+  });
   return hipGetLastError();
 }
 

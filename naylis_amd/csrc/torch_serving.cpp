@@ -1,6 +1,6 @@
-// Packed attention, the paged cache and token log probabilities: argument
-// checks, the C-ABI calls and the autograd nodes behind
-// mom_kernels/hip_packed.py, hip_paged.py and hip_logprobs.py.  Calls without
+// Packed attention, the paged cache, token log probabilities and the drafts'
+// verification: argument checks, the C-ABI calls and the autograd nodes behind
+// mom_kernels/hip_packed.py, hip_paged.py, hip_logprobs.py and hip_verify.py.  Calls without
 // a gradient make no node; the checks are here, not in Python, because a call
 // for one token costs little more than its host time.
 #include "torch_common.h"
@@ -176,14 +176,14 @@ at::Tensor packed_attention(const at::Tensor& q, const at::Tensor& k, const at::
 
 // ---- paged cache ----------------------------------------------------------------
 
-constexpr int kE4M3 = 2;
+constexpr int kE4M3 = 2, kE2M1 = 3;
 
 struct Cache {
   at::Tensor k, v, ks, vs;
   int dtype;
   int64_t pages, Hkv, page, hd;
-  float* k_scale() const { return ks.defined() ? ks.data_ptr<float>() : nullptr; }
-  float* v_scale() const { return vs.defined() ? vs.data_ptr<float>() : nullptr; }
+  void* k_scale() const { return ptr(ks); }
+  void* v_scale() const { return ptr(vs); }
 };
 
 // The pages are written in place and read where they are, so they have to be dense.
@@ -197,22 +197,54 @@ Cache cache_of(const at::Tensor& k, const at::Tensor& v, const c10::optional<at:
               "device, 16-byte aligned; got ", k.sizes(), " ", k.scalar_type(), ", ", v.sizes(), " ", v.scalar_type());
   const bool codes = k.scalar_type() == at::kByte;
   TORCH_CHECK(codes || k.scalar_type() == at::kBFloat16, who,
-              ": the cache must be bf16, or e4m3 codes in uint8 with scales; got ", k.scalar_type());
+              ": the cache must be bf16, or e4m3 or e2m1 codes in uint8 with scales; got ", k.scalar_type());
   TORCH_CHECK(codes == ks.has_value() && codes == vs.has_value(), who,
-              ": e4m3 pages need k_scale and v_scale, bf16 pages have none");
-  Cache c{k, v, ks.value_or(at::Tensor()), vs.value_or(at::Tensor()), codes ? kE4M3 : kBF16,
-          k.size(0), k.size(1), k.size(2), k.size(3)};
-  if (codes)
+              ": e4m3 and e2m1 pages need k_scale and v_scale, bf16 pages have none");
+  // the scales tell e2m1, two codes in a byte and an exponent's byte for 32, from e4m3
+  const bool fp4 = codes && ks->scalar_type() == at::kByte;
+  Cache c{k, v, ks.value_or(at::Tensor()), vs.value_or(at::Tensor()), fp4 ? kE2M1 : codes ? kE4M3 : kBF16,
+          k.size(0), k.size(1), k.size(2), fp4 ? 2 * k.size(3) : k.size(3)};
+  if (codes) {
+    std::vector<int64_t> shape = k.sizes().slice(0, 3).vec();
+    if (fp4) shape.push_back(c.hd / 32);
     for (const at::Tensor& s : {c.ks, c.vs})
-      TORCH_CHECK(s.scalar_type() == at::kFloat && s.is_contiguous() && s.device() == k.device() &&
-                      s.sizes() == k.sizes().slice(0, 3) && (uintptr_t)s.data_ptr() % 16 == 0,
-                  who, ": k_scale and v_scale must be dense fp32 (pages, Hkv, page_size) tensors, 16-byte aligned");
+      TORCH_CHECK(s.scalar_type() == c.ks.scalar_type() && (fp4 || s.scalar_type() == at::kFloat) &&
+                      s.is_contiguous() && s.device() == k.device() && s.sizes() == shape &&
+                      (uintptr_t)s.data_ptr() % 16 == 0,
+                  who, ": k_scale and v_scale must be dense fp32 (pages, Hkv, page_size) tensors, or uint8 (pages, ",
+                  "Hkv, page_size, head_dim / 32) ones for e2m1 pages, 16-byte aligned");
+  }
   return c;
 }
 
 void written(const at::Tensor& t) {
   if (t.defined() && !t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
+
+// What an append is given beside the cache, checked and as the kernels read it.
+struct NewTokens {
+  at::Tensor k, v, table, pos, row;
+  int64_t T;
+  NewTokens(const Cache& c, const at::Tensor& k_in, const at::Tensor& v_in, const at::Tensor& table_in,
+            const at::Tensor& positions, const c10::optional<at::Tensor>& rows, const char* who) {
+    TORCH_CHECK(k_in.dim() == 3 && v_in.sizes() == k_in.sizes() && k_in.size(1) == c.Hkv && k_in.size(2) == c.hd &&
+                    k_in.scalar_type() == at::kBFloat16 && v_in.scalar_type() == at::kBFloat16,
+                who, ": k and v must be bf16 (T, Hkv, head_dim) of the cache's heads; got ", k_in.sizes(), " ",
+                k_in.scalar_type(), ", ", v_in.sizes(), " ", v_in.scalar_type());
+    same_device(k_in, c.k, who, "k");
+    same_device(v_in, c.k, who, "v");
+    table = indices(table_in, c.k, who, "block_table");
+    pos = indices(positions, c.k, who, "positions");
+    if (rows.has_value()) row = indices(*rows, c.k, who, "rows");
+    T = k_in.size(0);
+    TORCH_CHECK(table.dim() == 2 && table.size(1) > 0, who, ": block_table must be (B, pages of a sequence)");
+    TORCH_CHECK(pos.dim() == 1 && pos.size(0) == T && (!row.defined() || row.sizes() == pos.sizes()), who,
+                ": positions and rows must hold one entry for each of the ", T, " tokens");
+    k = rows_of(k_in);
+    v = rows_of(v_in);
+  }
+  const int32_t* row_ptr() const { return row.defined() ? row.data_ptr<int32_t>() : nullptr; }
+};
 
 void paged_append(const at::Tensor& kp, const at::Tensor& vp, const c10::optional<at::Tensor>& ks,
                   const c10::optional<at::Tensor>& vs, const at::Tensor& k_in, const at::Tensor& v_in,
@@ -224,55 +256,139 @@ void paged_append(const at::Tensor& kp, const at::Tensor& vp, const c10::optiona
   no_tangents({k_in, v_in, kp, vp, c.ks, c.vs}, who);
   TORCH_CHECK(!wants_grad({k_in, v_in, kp, vp, c.ks, c.vs}), who, " has no backward: call it without gradients");
   at::NoGradGuard no_grad;
-  TORCH_CHECK(k_in.dim() == 3 && v_in.sizes() == k_in.sizes() && k_in.size(1) == c.Hkv && k_in.size(2) == c.hd &&
-                  k_in.scalar_type() == at::kBFloat16 && v_in.scalar_type() == at::kBFloat16,
-              who, ": k and v must be bf16 (T, Hkv, head_dim) of the cache's heads; got ", k_in.sizes(), " ",
-              k_in.scalar_type(), ", ", v_in.sizes(), " ", v_in.scalar_type());
-  same_device(k_in, kp, who, "k");
-  same_device(v_in, kp, who, "v");
-  const at::Tensor table = indices(table_in, kp, who, "block_table"), pos = indices(positions, kp, who, "positions");
-  const at::Tensor row = rows.has_value() ? indices(*rows, kp, who, "rows") : at::Tensor();
-  const int64_t T = k_in.size(0);
-  TORCH_CHECK(table.dim() == 2 && table.size(1) > 0, who, ": block_table must be (B, pages of a sequence)");
-  TORCH_CHECK(pos.dim() == 1 && pos.size(0) == T && (!row.defined() || row.sizes() == pos.sizes()), who,
-              ": positions and rows must hold one entry for each of the ", T, " tokens");
-  const at::Tensor k = rows_of(k_in), v = rows_of(v_in);
-  const int64_t strides[4] = {row_stride(k), head_stride(k), row_stride(v), head_stride(v)};
-  check(naylis_mom_paged_append(kp.data_ptr(), vp.data_ptr(), c.k_scale(), c.v_scale(), c.dtype, k.data_ptr(),
-                                v.data_ptr(), strides, table.data_ptr<int32_t>(), pos.data_ptr<int32_t>(),
-                                row.defined() ? row.data_ptr<int32_t>() : nullptr, T, c.pages, c.Hkv, c.page, c.hd,
-                                table.size(0), table.size(1), stream_of(st, kp)));
+  const NewTokens n(c, k_in, v_in, table_in, positions, rows, who);
+  const int64_t strides[4] = {row_stride(n.k), head_stride(n.k), row_stride(n.v), head_stride(n.v)};
+  check(naylis_mom_paged_append(kp.data_ptr(), vp.data_ptr(), c.k_scale(), c.v_scale(), c.dtype, n.k.data_ptr(),
+                                n.v.data_ptr(), strides, n.table.data_ptr<int32_t>(), n.pos.data_ptr<int32_t>(),
+                                n.row_ptr(), n.T, c.pages, c.Hkv, c.page, c.hd, n.table.size(0), n.table.size(1),
+                                stream_of(st, kp)));
   for (const at::Tensor& t : {c.k, c.v, c.ks, c.vs}) written(t);
+}
+
+// Returns the rotated queries (undefined without q).
+at::Tensor paged_append_rope(const at::Tensor& kp, const at::Tensor& vp, const c10::optional<at::Tensor>& ks,
+                             const c10::optional<at::Tensor>& vs, const c10::optional<at::Tensor>& q_in,
+                             const at::Tensor& k_in, const at::Tensor& v_in, const at::Tensor& inv_freq,
+                             const at::Tensor& table_in, const at::Tensor& positions,
+                             const c10::optional<at::Tensor>& rows, double scaling, int64_t st) {
+  const char* who = "paged_append_rope";
+  const Cache c = cache_of(kp, vp, ks, vs, who);
+  at::DeviceGuard guard(kp.device());
+  const at::Tensor q_given = q_in.value_or(at::Tensor());
+  no_tangents({q_given, k_in, v_in, inv_freq, kp, vp, c.ks, c.vs}, who);
+  TORCH_CHECK(!wants_grad({q_given, k_in, v_in, inv_freq, kp, vp, c.ks, c.vs}), who,
+              " has no backward: call it without gradients");
+  at::NoGradGuard no_grad;
+  const NewTokens n(c, k_in, v_in, table_in, positions, rows, who);
+  same_device(inv_freq, kp, who, "inv_freq");
+  TORCH_CHECK(inv_freq.dim() == 1 && inv_freq.scalar_type() == at::kFloat, who, ": inv_freq must be fp32 (half,), got ",
+              inv_freq.sizes(), " ", inv_freq.scalar_type());
+  const at::Tensor freq = inv_freq.contiguous();
+  at::Tensor q, q_out;
+  int64_t H = 0, strides[6] = {0, 0, row_stride(n.k), head_stride(n.k), row_stride(n.v), head_stride(n.v)};
+  if (q_given.defined()) {
+    same_device(q_given, kp, who, "q");
+    TORCH_CHECK(q_given.dim() == 3 && q_given.scalar_type() == at::kBFloat16 && q_given.size(0) == n.T &&
+                    q_given.size(1) > 0 && q_given.size(2) == c.hd,
+                who, ": q must be bf16 (T, H, head_dim) of the same tokens; got ", q_given.sizes(), " ",
+                q_given.scalar_type());
+    q = rows_of(q_given);
+    H = q.size(1);
+    q_out = at::empty({n.T, H, c.hd}, q.options());
+    strides[0] = row_stride(q);
+    strides[1] = head_stride(q);
+  }
+  check(naylis_mom_paged_append_rope(kp.data_ptr(), vp.data_ptr(), c.k_scale(), c.v_scale(), c.dtype, ptr(q),
+                                     n.k.data_ptr(), n.v.data_ptr(), strides, freq.data_ptr<float>(), (float)scaling,
+                                     n.table.data_ptr<int32_t>(), n.pos.data_ptr<int32_t>(), n.row_ptr(), ptr(q_out),
+                                     n.T, H, freq.size(0), c.pages, c.Hkv, c.page, c.hd, n.table.size(0),
+                                     n.table.size(1), stream_of(st, kp)));
+  for (const at::Tensor& t : {c.k, c.v, c.ks, c.vs}) written(t);
+  return q_out;
+}
+
+variable_list paged_gather(const at::Tensor& kp, const at::Tensor& vp, const c10::optional<at::Tensor>& ks,
+                           const c10::optional<at::Tensor>& vs, const at::Tensor& table_in, const at::Tensor& cu_in,
+                           int64_t tokens, int64_t st) {
+  const char* who = "paged_gather";
+  const Cache c = cache_of(kp, vp, ks, vs, who);
+  at::DeviceGuard guard(kp.device());
+  no_tangents({kp, vp, c.ks, c.vs}, who);
+  TORCH_CHECK(!wants_grad({kp, vp, c.ks, c.vs}), who, " has no backward: call it without gradients");
+  at::NoGradGuard no_grad;
+  const at::Tensor table = indices(table_in, kp, who, "block_table"), cu = indices(cu_in, kp, who, "cu_seqlens");
+  TORCH_CHECK(table.dim() == 2 && table.size(0) > 0 && table.size(1) > 0 && cu.dim() == 1 &&
+                  cu.size(0) == table.size(0) + 1,
+              who, ": block_table must be (B, pages of a sequence) and cu_seqlens (B + 1,); got ", table.sizes(),
+              " and ", cu.sizes());
+  TORCH_CHECK(tokens >= 0, who, ": tokens must not be negative, got ", tokens);
+  const at::TensorOptions o = kp.options().dtype(at::kBFloat16);
+  at::Tensor k = at::empty({tokens, c.Hkv, c.hd}, o), v = at::empty({tokens, c.Hkv, c.hd}, o);
+  check(naylis_mom_paged_gather(kp.data_ptr(), vp.data_ptr(), c.k_scale(), c.v_scale(), c.dtype,
+                                table.data_ptr<int32_t>(), cu.data_ptr<int32_t>(), k.data_ptr(), v.data_ptr(), tokens,
+                                c.pages, c.Hkv, c.page, c.hd, table.size(0), table.size(1), stream_of(st, kp)));
+  return {k, v};
+}
+
+// A (B, N, H, hd) operand as the kernels read it; dimensions of one keep no stride.
+at::Tensor tokens_of(const at::Tensor& t, int64_t (&strides)[3]) {
+  const auto stride = [&](const at::Tensor& x, int d) {
+    if (x.size(d) > 1) return x.stride(d);
+    int64_t dense = 1;
+    for (int64_t i = d + 1; i < x.dim(); ++i) dense *= x.size(i);
+    return dense;
+  };
+  const auto fits = [&](const at::Tensor& x) {
+    bool ok = x.stride(3) == 1 && (uintptr_t)x.data_ptr() % 16 == 0;
+    for (int d = 0; d < 3; ++d) {
+      strides[d] = stride(x, d);
+      ok = ok && strides[d] % 8 == 0 && (d == 2 || strides[d] < (1 << 23));
+    }
+    return ok;
+  };
+  if (fits(t)) return t;
+  at::Tensor c = t.contiguous();
+  if ((uintptr_t)c.data_ptr() % 16 != 0) c = c.clone();
+  fits(c);
+  return c;
 }
 
 at::Tensor paged_attention(const at::Tensor& q_in, const at::Tensor& kp, const at::Tensor& vp,
                            const c10::optional<at::Tensor>& ks, const c10::optional<at::Tensor>& vs,
                            const at::Tensor& table_in, const at::Tensor& lens_in, c10::optional<double> scale,
-                           int64_t st) {
+                           const c10::optional<at::Tensor>& q_lens, int64_t st) {
   const char* who = "paged_attention";
   const Cache c = cache_of(kp, vp, ks, vs, who);
   at::DeviceGuard guard(kp.device());
   no_tangents({q_in, kp, vp, c.ks, c.vs}, who);
   TORCH_CHECK(!wants_grad({q_in, kp, vp, c.ks, c.vs}), who, " has no backward: call it without gradients");
   at::NoGradGuard no_grad;
-  TORCH_CHECK(q_in.dim() == 3 && q_in.scalar_type() == at::kBFloat16 && q_in.size(2) == c.hd && c.Hkv > 0 &&
-                  q_in.size(1) > 0 && q_in.size(1) % c.Hkv == 0,
-              who, ": q must be bf16 (B, H, head_dim) with H a multiple of the cache's heads; got ", q_in.sizes(), " ",
-              q_in.scalar_type(), " for a cache of ", c.k.sizes());
+  const bool many = q_in.dim() == 4;
+  const int64_t heads = many ? 2 : 1;
+  TORCH_CHECK((many || q_in.dim() == 3) && q_in.scalar_type() == at::kBFloat16 && q_in.size(heads + 1) == c.hd &&
+                  c.Hkv > 0 && q_in.size(heads) > 0 && q_in.size(heads) % c.Hkv == 0 && q_in.size(heads - 1) >= (many ? 1 : 0),
+              who, ": q must be bf16 (B, H, head_dim) or (B, N, H, head_dim) with N >= 1 and H a multiple of the ",
+              "cache's heads; got ", q_in.sizes(), " ", q_in.scalar_type(), " for a cache of ", c.k.sizes());
   same_device(q_in, kp, who, "q");
   const at::Tensor table = indices(table_in, kp, who, "block_table"), lens = indices(lens_in, kp, who, "seq_lens");
-  const int64_t B = q_in.size(0), H = q_in.size(1);
+  const int64_t B = q_in.size(0), N = many ? q_in.size(1) : 1, H = q_in.size(heads);
   TORCH_CHECK(table.dim() == 2 && table.size(0) == B && table.size(1) > 0 && lens.dim() == 1 && lens.size(0) == B,
               who, ": block_table must be (B, pages of a sequence) and seq_lens (B,) for the ", B, " rows of q");
-  const at::Tensor q = rows_of(q_in);
-  at::Tensor out = at::empty({B, H, c.hd}, q.options());
-  const size_t bytes = naylis_mom_paged_attn_workspace_bytes(c.dtype, B, H, c.Hkv, c.page, c.hd, table.size(1));
+  at::Tensor live;
+  if (q_lens.has_value()) {
+    live = indices(*q_lens, kp, who, "q_lens");
+    TORCH_CHECK(live.dim() == 1 && live.size(0) == B, who, ": q_lens must be (B,) for the ", B, " rows of q");
+  }
+  int64_t strides[3];
+  const at::Tensor q = tokens_of(many ? q_in : q_in.unsqueeze(1), strides);
+  at::Tensor out = at::empty(q_in.sizes(), q_in.options().memory_format(at::MemoryFormat::Contiguous));
+  const size_t bytes = naylis_mom_paged_attn_tokens_workspace_bytes(c.dtype, B, N, H, c.Hkv, c.page, c.hd, table.size(1));
   const at::Tensor ws = bytes ? workspace(bytes, q) : at::Tensor();
-  const int64_t strides[2] = {row_stride(q), head_stride(q)};
-  check(naylis_mom_paged_attn(q.data_ptr(), kp.data_ptr(), vp.data_ptr(), c.k_scale(), c.v_scale(), c.dtype,
-                              table.data_ptr<int32_t>(), lens.data_ptr<int32_t>(), out.data_ptr(), ptr(ws), bytes,
-                              strides, (float)scale_of(scale, c.hd), B, H, c.pages, c.Hkv, c.page, c.hd,
-                              table.size(1), stream_of(st, kp)));
+  check(naylis_mom_paged_attn_tokens(q.data_ptr(), kp.data_ptr(), vp.data_ptr(), c.k_scale(), c.v_scale(), c.dtype,
+                                     table.data_ptr<int32_t>(), lens.data_ptr<int32_t>(),
+                                     live.defined() ? live.data_ptr<int32_t>() : nullptr, out.data_ptr(), ptr(ws),
+                                     bytes, strides, (float)scale_of(scale, c.hd), B, N, H, c.pages, c.Hkv, c.page,
+                                     c.hd, table.size(1), stream_of(st, kp)));
   return out;
 }
 
@@ -388,13 +504,85 @@ variable_list token_logprobs(const at::Tensor& logits, const at::Tensor& tokens_
   return {out[0].view(lead), out[1].view(lead), out[2].view(tops), out[3].view(tops)};
 }
 
+// ---- drafts' verification ---------------------------------------------------------
+
+// (B, n, V) of dense rows
+at::Tensor dense_rows(const at::Tensor& t, int64_t (&strides)[2]) {
+  const at::Tensor x = t.size(2) == 1 || t.stride(2) == 1 ? t : t.contiguous();
+  strides[0] = x.size(0) == 1 ? 0 : x.stride(0);
+  strides[1] = x.size(1) == 1 ? 0 : x.stride(1);
+  return x;
+}
+
+variable_list verify_drafts(const at::Tensor& logits_in, const at::Tensor& drafts_in, const at::Tensor& uniforms_in,
+                            const c10::optional<at::Tensor>& probs_in, const c10::optional<at::Tensor>& lens_in,
+                            const c10::optional<at::Tensor>& temps_in, double temperature, int64_t st) {
+  const char* who = "verify_drafts";
+  on_gpu(logits_in, who, "logits");
+  at::DeviceGuard guard(logits_in.device());
+  const auto real = [](const at::Tensor& t) { return t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kFloat; };
+  TORCH_CHECK(logits_in.dim() == 3 && real(logits_in) && logits_in.size(1) > 0 && logits_in.size(2) > 0, who,
+              ": logits must be bf16 or fp32 (B, N + 1, V), got ", logits_in.sizes(), " ", logits_in.scalar_type());
+  const int64_t B = logits_in.size(0), N = logits_in.size(1) - 1, V = logits_in.size(2);
+  same_device(drafts_in, logits_in, who, "drafts");
+  same_device(uniforms_in, logits_in, who, "uniforms");
+  TORCH_CHECK(drafts_in.dim() == 2 && drafts_in.size(0) == B && drafts_in.size(1) == N &&
+                  (drafts_in.scalar_type() == at::kLong || drafts_in.scalar_type() == at::kInt),
+              who, ": drafts must be int64 or int32 (B, N) for logits (B, N + 1, V); got ", drafts_in.sizes(), " ",
+              drafts_in.scalar_type(), " for ", logits_in.sizes());
+  TORCH_CHECK(uniforms_in.dim() == 2 && uniforms_in.size(0) == B && uniforms_in.size(1) == N + 1 &&
+                  uniforms_in.scalar_type() == at::kFloat,
+              who, ": uniforms must be fp32 (B, N + 1); got ", uniforms_in.sizes(), " ", uniforms_in.scalar_type());
+  const at::Tensor probs_given = probs_in.value_or(at::Tensor()), temps_given = temps_in.value_or(at::Tensor());
+  no_tangents({logits_in, uniforms_in, probs_given, temps_given}, who);
+  TORCH_CHECK(!wants_grad({logits_in, uniforms_in, probs_given, temps_given}), who,
+              " has no backward: call it without gradients");
+  at::NoGradGuard no_grad;
+  int64_t strides[2], probs_strides[2] = {0, 0};
+  const at::Tensor logits = dense_rows(logits_in, strides), drafts = drafts_in.to(at::kLong).contiguous();
+  const at::Tensor uniforms = uniforms_in.contiguous();
+  at::Tensor probs, lens, temps;
+  if (probs_given.defined()) {
+    same_device(probs_given, logits, who, "draft_probs");
+    TORCH_CHECK(probs_given.dim() == 3 && real(probs_given) && probs_given.size(0) == B && probs_given.size(1) == N &&
+                    probs_given.size(2) == V,
+                who, ": draft_probs must be bf16 or fp32 (B, N, V); got ", probs_given.sizes(), " ",
+                probs_given.scalar_type());
+    if (N > 0) probs = dense_rows(probs_given, probs_strides);
+  }
+  if (lens_in.has_value()) {
+    lens = indices(*lens_in, logits, who, "draft_lens");
+    TORCH_CHECK(lens.dim() == 1 && lens.size(0) == B, who, ": draft_lens must be (B,)");
+  }
+  if (temps_given.defined()) {
+    same_device(temps_given, logits, who, "temperature");
+    TORCH_CHECK(temps_given.dim() == 1 && temps_given.size(0) == B && temps_given.scalar_type() == at::kFloat, who,
+                ": temperature must be a number or fp32 (B,)");
+    temps = temps_given.contiguous();
+  }
+  at::Tensor tokens = at::empty({B, N + 1}, logits.options().dtype(at::kLong));
+  at::Tensor accepted = at::empty({B}, logits.options().dtype(at::kInt));
+  const size_t bytes = need(naylis_mom_verify_drafts_workspace_bytes(B, N, V, probs.defined()));
+  const at::Tensor ws = workspace(bytes, logits);
+  check(naylis_mom_verify_drafts(logits.data_ptr(), dtype_code(logits), strides, drafts.data_ptr<int64_t>(),
+                                 uniforms.data_ptr<float>(), ptr(probs), probs.defined() ? dtype_code(probs) : kF32,
+                                 probs_strides, lens.defined() ? lens.data_ptr<int32_t>() : nullptr,
+                                 temps.defined() ? temps.data_ptr<float>() : nullptr, (float)temperature,
+                                 tokens.data_ptr<int64_t>(), accepted.data_ptr<int32_t>(), ws.data_ptr(), bytes, B, N,
+                                 V, stream_of(st, logits)));
+  return {tokens, accepted};
+}
+
 }  // namespace
 
 void bind_serving(pybind11::module_& m) {
   m.def("packed_attention", &packed_attention);
   m.def("paged_append", &paged_append);
   m.def("paged_attention", &paged_attention);
+  m.def("paged_append_rope", &paged_append_rope);
+  m.def("paged_gather", &paged_gather);
   m.def("token_logprobs", &token_logprobs);
+  m.def("verify_drafts", &verify_drafts);
 }
 
 }  // namespace naylis_ext

@@ -14,8 +14,10 @@ projection), used by ``naylis_amd.layer.MoMLayer``; ``quantize_bank_fp8`` and
 ``decode_step``, the one-token inference step over an fp8 bank (the reference
 has no decode path).  Around it, for the trunk's attention and the answers:
 ``packed_attention`` (prompts and packed batches, grouped heads),
-``paged_append`` / ``paged_attention`` (a key / value cache in pages and one new
-token over it) and ``token_logprobs`` (scores, entropies, top alternatives).
+``paged_append`` / ``paged_append_rope`` / ``paged_attention`` / ``paged_gather``
+(a key / value cache in pages, rotated on the way in, a few new tokens over it,
+and dense again), ``verify_drafts`` (drafted tokens against the logits) and
+``token_logprobs`` (scores, entropies, top alternatives).
 """
 from __future__ import annotations
 
@@ -27,15 +29,18 @@ from .hip_decode import decode_step, quantize_bank_fp8
 from .hip_linear import mom_linear
 from .hip_logprobs import TokenLogprobs, token_logprobs
 from .hip_packed import packed_attention
-from .hip_paged import PagedCache, new_paged_cache, paged_append, paged_attention
+from .hip_paged import (PagedCache, new_paged_cache, paged_append, paged_append_rope, paged_attention,
+                        paged_gather)
 from .hip_read import mom_read as _hip_mom_read
 from .hip_rezero import mom_gated_linear, mom_rezero
 from .hip_router import mom_route, mom_router_stats
+from .hip_verify import VerifiedDrafts, verify_drafts
 
 __all__ = ["HAS_HIP", "preflight", "resolve_mode", "mom_read", "announce", "mom_route",
            "mom_bank_kv", "mom_bank_kv_grouped", "mom_linear", "mom_rezero", "mom_gated_linear", "has_hip", "quantize_bank_fp8", "decode_step",
-           "mom_router_stats", "packed_attention", "PagedCache", "new_paged_cache", "paged_append", "paged_attention",
-           "token_logprobs", "TokenLogprobs"]
+           "mom_router_stats", "packed_attention", "PagedCache", "new_paged_cache", "paged_append",
+           "paged_append_rope", "paged_attention", "paged_gather", "token_logprobs", "TokenLogprobs", "verify_drafts",
+           "VerifiedDrafts"]
 
 _ANNOUNCED = {"backend": None}
 
