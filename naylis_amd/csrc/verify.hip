@@ -9,17 +9,22 @@
 // (drafts found by a rule) q_i(d_i) = 1, and the rest of p is p without d_a.
 // T = 0: p is all on the largest logit, the first of equal ones.
 //
-// Weights and their sums are fp64: a token is a place among up to 152000
-// cumulative sums, and an error of fp32's 2^-24 would move the border between two
-// tokens of the tail past u once in a hundred draws.  fp64 runs at fp32's rate
-// here, and 2^x costs ten products (a polynomial of degree 10 fitted at the
-// Chebyshev nodes of [-1/2, 1/2], off by 3e-16).
+// The weights of the row that a token is drawn from, and their sums, are fp64: the
+// token is a place among up to 152000 cumulative sums, and an error of fp32's 2^-24
+// would move the border between two tokens of the tail past u once in a hundred
+// draws.  fp64 runs at fp32's rate here, and 2^x costs ten products (a polynomial of
+// degree 10 fitted at the Chebyshev nodes of [-1/2, 1/2], off by 3e-16).  The sums
+// that only decide which drafts are kept are fp32 where there are many rows: u falls
+// between p and p (1 + 2^-20) once in a million draws.
 //
-// Three launches: a workgroup for each part of each row leaves (largest logit,
-// its place, sum of 2^z against it) -- all that the rows' bytes are read for; a
-// workgroup for each part of a row with a draft turned away sums its remaining
-// weights (only with q); one for each sequence finds the part and the token in it.
-// Each of the last two finds a by itself from the parts' sums, which lie in L2.
+// Launches: (1) a wave for each 2048 logits of each row leaves (largest logit, its
+// place, sum of 2^z against it) -- all that the rows' bytes are read for; (2) for
+// each sequence the drafts kept, and over the row behind them the parts' fp64 sums
+//   S = sum e,  and with q  R = sum max(0, e - S' q),  Q = sum of q where that is not 0,
+// e = e^((x - top) / T) and S' the fp32 sum: what is left of p weighs R + (S' - S) Q,
+// for S is so near to S' that only tokens that weigh nothing change sides;
+// (3) a workgroup for each sequence finds the part and the token in it.  Few logits
+// and no q: (1) in fp64, and no (2).
 #include "common.h"
 #include "launch.h"
 #include "timing.h"
@@ -31,7 +36,11 @@ namespace naylis {
 
 namespace {
 
-constexpr int kStatThreads = 256;
+constexpr int kThreads = 256, kWaves = kThreads / 64;
+constexpr int kPart = 2048;          // logits of a part
+constexpr int kPieces = kPart / 512; // of eight logits a lane
+constexpr int kRows = 16;            // rows whose joined sums a workgroup keeps
+constexpr double kNothing = 0x1p-900;  // weights up to this are none: those of -inf count as 2^-1000
 
 // what the first launch leaves of a part of a row
 struct VerifyStat {
@@ -40,11 +49,16 @@ struct VerifyStat {
   double sum;  // of e^((x - top) / T), the draft's own token left out
 };
 static_assert(sizeof(VerifyStat) == 16, "the workspace is counted in these");
+// what the second leaves of a part of the row behind the kept drafts, against its largest logit
+struct VerifyLeft {
+  double sum, over;  // S (a turned away draft of a rule left out), R
+  float q;           // Q
+};
 
-// 2^t for t <= 0: exact powers from the exponent's bits, 0 below 2^-1000, NaN for NaN
+// 2^t for t <= 0, 2^-1000 and less as 2^-1000 (NaN too: callers look for those)
 __device__ __forceinline__ double pow2(double t) {
   constexpr double kRound = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to a whole number
-  const double c = t < -1000.0 ? -1000.0 : t;
+  const double c = __builtin_fmax(t, -1000.0);
   const double shifted = c + kRound, f = c - (shifted - kRound);
   double p = 0x1.e6064532b85cep-28;
   p = __builtin_fma(p, f, 0x1.b675bd731322bp-24);
@@ -57,13 +71,10 @@ __device__ __forceinline__ double pow2(double t) {
   p = __builtin_fma(p, f, 0x1.ebfbdff82c598p-3);
   p = __builtin_fma(p, f, 0x1.62e42fefa3a19p-1);
   p = __builtin_fma(p, f, 1.0);
-  const uint64_t b = __builtin_bit_cast(uint64_t, p);
-  const uint32_t n = (uint32_t)__builtin_bit_cast(uint64_t, shifted);
-  const double r = __builtin_bit_cast(double, b + ((uint64_t)n << 52));
-  return t < -1000.0 ? 0.0 : r;
+  return __builtin_amdgcn_ldexp(p, (int)(uint32_t)__builtin_bit_cast(uint64_t, shifted));
 }
 
-// e^((x - top) / T), scale = log2(e) / T; 0 for x = -inf
+// e^((x - top) / T), scale = log2(e) / T; next to nothing, 2^-1000, for x = -inf
 __device__ __forceinline__ double weight(float x, float top, double scale) {
   return pow2(((double)x - (double)top) * scale);
 }
@@ -71,31 +82,76 @@ __device__ __forceinline__ double weight(float x, float top, double scale) {
 __device__ __forceinline__ float load1(const bf16_t* p) { return bf16_to_f32(*p); }
 __device__ __forceinline__ float load1(const float* p) { return *p; }
 
-// Eight logits of a row, j0 .. j0 + 7, where j0 - shift is a multiple of 8: the
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+// Eight numbers of a row as they lie in memory.
+template <typename T>
+struct Raw8;
+template <>
+struct Raw8<bf16_t> {
+  u32x4 u;
+  __device__ __forceinline__ float operator[](int e) const {
+    return __uint_as_float(e & 1 ? u[e >> 1] & 0xffff0000u : u[e >> 1] << 16);
+  }
+  __device__ __forceinline__ void set(int e, float x) {  // (x is a bf16)
+    const uint32_t b = __float_as_uint(x);
+    u[e >> 1] = e & 1 ? (u[e >> 1] & 0xffffu) | (b & 0xffff0000u) : (u[e >> 1] & 0xffff0000u) | (b >> 16);
+  }
+};
+template <>
+struct Raw8<float> {
+  f32x4 f[2];
+  __device__ __forceinline__ float operator[](int e) const { return f[e >> 2][e & 3]; }
+  __device__ __forceinline__ void set(int e, float x) { f[e >> 2][e & 3] = x; }
+};
+
+// Logits j0 .. j0 + 7 of a row, where j0 + shift_of(row) is a multiple of 8: the
 // row's 16-byte pieces of memory; -inf outside [0, V).
 template <typename T>
-__device__ __forceinline__ void load8(const T* row, long j0, int V, float (&x)[8]) {
-  if (j0 >= 0 && j0 + 8 <= V) {
-    if constexpr (sizeof(T) == 2) {
-      const uint4 u = *reinterpret_cast<const uint4*>(row + j0);
-      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+__device__ __forceinline__ Raw8<T> load8(const T* row, int j0, int V) {
+  if (j0 >= 0 && j0 + 8 <= V) return *reinterpret_cast<const Raw8<T>*>(row + j0);
+  Raw8<T> x = {};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        x[2 * i] = __uint_as_float(w[i] << 16);
-        x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-      }
-    } else {
-      const f32x4 a = *reinterpret_cast<const f32x4*>(row + j0), b = *reinterpret_cast<const f32x4*>(row + j0 + 4);
+  for (int e = 0; e < 8; ++e) x.set(e, j0 + e >= 0 && j0 + e < V ? load1(row + j0 + e) : -INFINITY);
+  return x;
+}
+
+// A wave's share of a part: eight a lane from `first` on, for each of its pieces.
+// Only a row's first and last part look at their ends.
+template <typename T>
+__device__ __forceinline__ void load_part(const T* row, int first, int V, Raw8<T> (&x)[kPieces]) {
+  const int j0 = first + 8 * (int)(threadIdx.x & 63);
+  if (first >= 0 && first + kPart <= V) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        x[i] = a[i];
-        x[4 + i] = b[i];
-      }
-    }
-    return;
+    for (int c = 0; c < kPieces; ++c) x[c] = *reinterpret_cast<const Raw8<T>*>(row + j0 + 512 * c);
+  } else {
+#pragma unroll
+    for (int c = 0; c < kPieces; ++c) x[c] = load8(row, j0 + 512 * c, V);
   }
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {  // (without making NaNs quiet first)
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+
+// Eight numbers of a row at any address, 0 outside [0, V).
+template <typename T>
+struct __attribute__((packed, aligned(sizeof(T)))) Any8 {
+  Raw8<T> x;
+};
+template <typename T>
+__device__ __forceinline__ Raw8<T> any8(const T* p) {
+  return reinterpret_cast<const Any8<T>*>(p)->x;
+}
+template <typename T>
+__device__ __forceinline__ Raw8<T> load_any8(const T* row, int j0, int V) {
+  if (j0 >= 0 && j0 + 8 <= V) return any8(row + j0);
+  Raw8<T> x = {};
 #pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = j0 + i >= 0 && j0 + i < V ? load1(row + j0 + i) : -INFINITY;
+  for (int e = 0; e < 8; ++e) x.set(e, j0 + e >= 0 && j0 + e < V ? load1(row + j0 + e) : 0.f);
+  return x;
 }
 
 // elements between the last 16-byte boundary and the row's first
@@ -104,11 +160,31 @@ __device__ __forceinline__ int shift_of(const T* row) {
   return (int)(((uintptr_t)row & 15) / sizeof(T));
 }
 
-__device__ __forceinline__ double wave_sum(double x) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) x += __shfl_xor(x, o, 64);
+// a double from the lane that a DPP control names, 0 where there is none
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ double dpp_f64(double x) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)u, CTRL, ROWS, 0xf, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(u >> 32), CTRL, ROWS, 0xf, false);
+  return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
+}
+__device__ __forceinline__ double lane_of(double x, int lane) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = __builtin_amdgcn_readlane((int)u, lane), hi = __builtin_amdgcn_readlane((int)(u >> 32), lane);
+  return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
+}
+// inclusive sum over the lanes: within rows of 16 (row_shr 1, 2, 4, 8), then row 0
+// into 1 and 2 into 3 (row_bcast 15), rows 0 and 1 into 2 and 3 (row_bcast 31)
+__device__ __forceinline__ double wave_scan(double x) {
+  x += dpp_f64<0x111>(x);
+  x += dpp_f64<0x112>(x);
+  x += dpp_f64<0x114>(x);
+  x += dpp_f64<0x118>(x);
+  x += dpp_f64<0x142, 0xa>(x);
+  x += dpp_f64<0x143, 0xc>(x);
   return x;
 }
+__device__ __forceinline__ double wave_sum(double x) { return lane_of(wave_scan(x), 63); }
 
 __device__ __forceinline__ double scale_of(float t) { return 1.4426950408889634074 / (t > 0.f ? (double)t : 1.0); }
 
@@ -119,324 +195,316 @@ __device__ __forceinline__ int verify_drafts_of(const VerifyArgs& a, int b) {
 }
 __device__ __forceinline__ float verify_temperature(const VerifyArgs& a, int b) { return a.temps ? a.temps[b] : a.temp; }
 
-// grid (parts, N + 1, B).  PART logits, eight for a thread at a time.
-template <typename T, int PART>
-__global__ __launch_bounds__(kStatThreads) void verify_stat_kernel(VerifyArgs a, const T* __restrict__ logits,
-                                                                   VerifyStat* __restrict__ stat) {
-  constexpr int C = PART / (8 * kStatThreads), WAVES = kStatThreads / 64;
-  __shared__ float tops[WAVES];
-  __shared__ int ats[WAVES];
-  __shared__ double sums[WAVES];
-  const int part = blockIdx.x, i = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+// grid (parts / 4, N + 1, B), a part for each wave.  EXACT: sums in fp64.
+template <typename T, bool EXACT>
+__global__ __launch_bounds__(kThreads, EXACT || sizeof(T) == 4 ? 1 : 8) void verify_stat_kernel(VerifyArgs a, const T* __restrict__ logits,
+                                                               VerifyStat* __restrict__ stat) {
+  const int i = blockIdx.y, b = blockIdx.z, lane = threadIdx.x & 63;
+  const int part = blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = verify_drafts_of(a, b);
-  if (i > n) return;
+  if (i > n || part >= a.parts) return;
   const T* row = logits + b * a.ldb + i * a.ldt;
-  const double scale = scale_of(verify_temperature(a, b));
+  const int first = part * kPart - shift_of(row), j0 = first + 8 * lane;
+  Raw8<T> x[kPieces];
+  load_part(row, first, a.V, x);
+  const float t = verify_temperature(a, b);
+  const double scale = scale_of(t);
   const long draft = i < n ? a.drafts[(long)b * a.N + i] : -1;
-  const long j0 = (long)part * PART - shift_of(row) + 8 * tid;
-  float x[C][8];
-#pragma unroll
-  for (int c = 0; c < C; ++c) load8(row, j0 + 8 * kStatThreads * c, a.V, x[c]);
   float top = -INFINITY;
   bool nan = false;
 #pragma unroll
-  for (int c = 0; c < C; ++c)
+  for (int c = 0; c < kPieces; ++c)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      top = fmaxf(top, x[c][e]);
-      nan |= x[c][e] != x[c][e];
+    for (int e = 0; e < 8; e += 2) {
+      top = max3(top, x[c][e], x[c][e + 1]);
+      if constexpr (EXACT) nan |= __builtin_isunordered(x[c][e], x[c][e + 1]);
     }
   const float own = top;
   top = wave_allmax(top);
-  if (lane == 0) tops[wave] = top;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < WAVES; ++w) top = fmaxf(top, tops[w]);
   int at = 0x7fffffff;
-  if (own == top)
+  if (!(t > 0.f) && own == top)
 #pragma unroll
-    for (int c = C - 1; c >= 0; --c)
+    for (int c = kPieces - 1; c >= 0; --c)
 #pragma unroll
       for (int e = 7; e >= 0; --e)
-        if (x[c][e] == top) at = (int)(j0 + 8 * kStatThreads * c + e);
-  // a part of -inf alone adds nothing; a row with a NaN or +inf has no weights
-  const float ref = top == -INFINITY ? 0.f : top;
+        if (x[c][e] == top) at = j0 + 512 * c + e;
+  // the draft's own weight stays out: what is left without it is exact however small
+  if (draft >= first && draft < first + kPart) {
+#pragma unroll
+    for (int c = 0; c < kPieces; ++c)
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (j0 + 512 * c + e == (int)draft) {
+          nan |= x[c][e] != x[c][e];
+          x[c].set(e, -INFINITY);
+        }
+  }
+  // a part of -inf alone adds nothing; a row with a NaN (which an fp32 sum keeps) or
+  // +inf has no weights
   double s = 0.0;
+  if (!(top == -INFINITY)) {
+    if constexpr (EXACT) {
 #pragma unroll
-  for (int c = 0; c < C; ++c)
+      for (int c = 0; c < kPieces; ++c)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const double w = weight(x[c][e], ref, scale);
-      s += j0 + 8 * kStatThreads * c + e == draft ? 0.0 : w;
+        for (int e = 0; e < 8; ++e) s += weight(x[c][e], top, scale);
+    } else {
+      const float fs = (float)scale;
+      float sums[kPieces] = {};
+#pragma unroll
+      for (int c = 0; c < kPieces; ++c)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sums[c] += __builtin_amdgcn_exp2f((x[c][e] - top) * fs);
+#pragma unroll
+      for (int c = 0; c < kPieces; ++c) s += sums[c];
     }
-  if (nan || top == INFINITY) s = __builtin_nan("");
-  at = wave_allmin_i32(at);
+  }
+  if (__any(nan) || top == INFINITY) s = __builtin_nan("");
+  if (!(t > 0.f)) at = wave_allmin_i32(at);
   s = wave_sum(s);
-  if (lane == 0) {
-    ats[wave] = at;
-    sums[wave] = s;
-  }
-  __syncthreads();
-  if (tid) return;
-#pragma unroll
-  for (int w = 1; w < WAVES; ++w) {
-    at = min(at, ats[w]);
-    s += sums[w];
-  }
-  stat[((long)b * (a.N + 1) + i) * a.parts + part] = VerifyStat{top, at, s};
+  if (lane == 0) stat[((long)b * (a.N + 1) + i) * a.parts + part] = VerifyStat{top, at, s};
 }
 
 namespace {
 
-// a row's parts joined, by a wave: every lane gets it
+// a row's parts joined: every lane of the wave gets it
 struct RowStat {
   float top;
   int at;
-  double sum;  // with the draft's token
-};
-
-// the draft's weight against the row's largest logit, 0 for an id that is none
-struct DraftWeight {
-  float x = 0.f;
-  bool some = false;
-  __device__ __forceinline__ double operator()(float top, double scale) const {
-    return some ? weight(x, top, scale) : 0.0;
-  }
+  double sum, draft;  // with the draft's weight, and that
 };
 
 template <typename T>
 __device__ __forceinline__ RowStat join_row(const VerifyArgs& a, const VerifyStat* s, const T* row, long draft,
-                                            double scale, double& dw) {
+                                            double scale) {
   const int lane = threadIdx.x & 63;
-  DraftWeight d;
-  if (draft >= 0 && draft < a.V) {
-    d.x = load1(row + draft);
-    d.some = true;
-  }
+  const bool some = draft >= 0 && draft < a.V;
+  const float x = some ? load1(row + draft) : 0.f;
   float top = -INFINITY;
   for (int p = lane; p < a.parts; p += 64) top = fmaxf(top, s[p].top);
   top = wave_allmax(top);
-  const float ref = top == -INFINITY ? 0.f : top;
   int at = 0x7fffffff;
   double sum = 0.0;
   for (int p = lane; p < a.parts; p += 64) {
     const VerifyStat v = s[p];
     if (v.top == top) at = min(at, v.at);
-    sum += v.top == -INFINITY ? v.sum : v.sum * weight(v.top, ref, scale);
+    sum += v.sum * weight(v.top, top, scale);  // (0 for a part of -inf)
   }
-  dw = d(ref, scale);
-  return RowStat{top, wave_allmin_i32(at), wave_sum(sum) + dw};
+  const double d = some && x > -INFINITY ? weight(x, top, scale) : 0.0;
+  return RowStat{top, wave_allmin_i32(at), wave_sum(sum) + d, d};
 }
 
-// What a sequence's decision is: drafts kept, and the row behind them.
+// What a sequence's decision is: drafts kept of n, and the row behind them.
 struct Decision {
   int kept, n;
+  float t;
+  long gone;  // the draft turned away, or -1
   RowStat row;
-  double draft_weight;  // of the draft turned away
 };
 
-// By a whole workgroup; `red` and `out` in LDS.
+// By a whole workgroup: rows 0 .. n, a wave each.
 template <typename T>
-__device__ __forceinline__ Decision decide(const VerifyArgs& a, const T* logits, const VerifyStat* stat, int b,
-                                           int* red, Decision* out) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = blockDim.x >> 6;
+__device__ __forceinline__ Decision decide(const VerifyArgs& a, const T* logits, const VerifyStat* stat, int b) {
+  __shared__ int first;
+  __shared__ RowStat rows[kRows];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = verify_drafts_of(a, b);
   const float t = verify_temperature(a, b);
   const double scale = scale_of(t);
-  if (tid == 0) *red = n;
+  if (tid == 0) first = n;
   __syncthreads();
-  const auto row_of = [&](int i) { return logits + b * a.ldb + i * a.ldt; };
-  const auto stat_of = [&](int i) { return stat + ((long)b * (a.N + 1) + i) * a.parts; };
-  for (int i = wave; i < n; i += waves) {
-    const long d = a.drafts[(long)b * a.N + i];
-    double dw;
-    const RowStat r = join_row(a, stat_of(i), row_of(i), d, scale, dw);
-    bool keep = false;
-    if (d >= 0 && d < a.V) {
-      const double u = a.uniforms[(long)b * (a.N + 1) + i];
-      double q = 1.0;
-      if (a.probs) {
-        const long at = b * a.lqb + i * a.lqt + d;
-        q = a.probs_bf16 ? bf16_to_f32(((const bf16_t*)a.probs)[at]) : ((const float*)a.probs)[at];
-      }
-      const double p = t > 0.f ? dw / r.sum : r.sum > 0.0 && r.at == d ? 1.0 : 0.0;
-      keep = u * q < p;
+  const auto join = [&](int i) {
+    const long d = i < n ? a.drafts[(long)b * a.N + i] : -1;
+    return join_row(a, stat + ((long)b * (a.N + 1) + i) * a.parts, logits + b * a.ldb + i * a.ldt, d, scale);
+  };
+  for (int i = wave; i <= n; i += kWaves) {
+    const long d = i < n ? a.drafts[(long)b * a.N + i] : -1;
+    const bool some = d >= 0 && d < a.V;
+    double q = 1.0;
+    if (some && a.probs) {
+      const long at = b * a.lqb + i * a.lqt + d;
+      q = a.probs_bf16 ? bf16_to_f32(((const bf16_t*)a.probs)[at]) : ((const float*)a.probs)[at];
     }
-    if (!keep && lane == 0) atomicMin(red, i);
+    const double u = a.uniforms[(long)b * (a.N + 1) + i];
+    const RowStat r = join(i);
+    const double p = t > 0.f ? r.draft / r.sum : r.sum > 0.0 && r.at == d ? 1.0 : 0.0;
+    if (lane == 0) {
+      if (i < n && !(some && u * q < p)) atomicMin(&first, i);
+      if (i < kRows) rows[i] = r;
+    }
   }
   __syncthreads();
-  const int kept = *red;
-  if (wave == 0) {
-    const long d = kept < n ? a.drafts[(long)b * a.N + kept] : -1;
-    double dw;
-    const RowStat r = join_row(a, stat_of(kept), row_of(kept), d, scale, dw);
-    if (lane == 0) *out = Decision{kept, n, r, dw};
-  }
-  __syncthreads();
-  return *out;
+  const int kept = first;
+  return Decision{kept, n, t, kept < n ? a.drafts[(long)b * a.N + kept] : -1, kept < kRows ? rows[kept] : join(kept)};
 }
 
-// The weights of eight tokens of the row behind the kept drafts: what is left of p.
+// The row behind the kept drafts, and what is taken from its weights.
 template <typename T>
-struct Left {
+struct Behind {
   const VerifyArgs& a;
   const T* row;
   const void* probs;  // q of the draft turned away, or NULL
-  long without;       // a draft found by a rule that was turned away, or -1
+  long gone;          // that draft, or -1
   float top;
-  int at;  // place of the largest logit
-  double scale, inv;
-  bool greedy;
+  double scale;
 
-  __device__ __forceinline__ void operator()(long j0, double (&w)[8]) const {
-    float x[8];
-    load8(row, j0, a.V, x);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const long j = j0 + e;
-      w[e] = greedy ? (j == at ? 1.0 : 0.0) : weight(x[e], top, scale) * inv;
-      if (probs) {
-        double q = 0.0;
-        if (j >= 0 && j < a.V) q = a.probs_bf16 ? bf16_to_f32(((const bf16_t*)probs)[j]) : ((const float*)probs)[j];
-        const double r = w[e] - q;
-        w[e] = r > 0.0 ? r : 0.0;
-      } else if (j == without) {
-        w[e] = 0.0;
-      }
-    }
-  }
-};
-
-template <typename T>
-__device__ __forceinline__ Left<T> left_of(const VerifyArgs& a, const T* logits, int b, const Decision& d, bool less) {
-  const float t = verify_temperature(a, b);
-  const T* row = logits + b * a.ldb + d.kept * a.ldt;
-  const bool turned = less && d.kept < d.n;
-  const void* probs = nullptr;
-  if (turned && a.probs) {
+  __device__ __forceinline__ Behind(const VerifyArgs& a, const T* logits, int b, const Decision& d)
+      : a(a), row(logits + b * a.ldb + d.kept * a.ldt), probs(nullptr), gone(d.gone), top(d.row.top), scale(scale_of(d.t)) {
+    if (d.kept == d.n || !a.probs) return;
     const long at = b * a.lqb + d.kept * a.lqt;
     probs = a.probs_bf16 ? (const void*)((const bf16_t*)a.probs + at) : (const void*)((const float*)a.probs + at);
   }
-  const long without = turned && !a.probs ? a.drafts[(long)b * a.N + d.kept] : -1;
-  return Left<T>{a, row, probs, without, d.row.top, d.row.at, scale_of(t), 1.0 / d.row.sum, !(t > 0.f)};
-}
+  __device__ __forceinline__ Raw8<T> logits(int j0) const { return load8(row, j0, a.V); }
+  // e of a token; next to nothing for columns of -inf and none
+  __device__ __forceinline__ double operator()(float x) const { return weight(x, top, scale); }
+};
 
 }  // namespace
 
-// grid (parts, B), with q only: the sums of max(0, p - q) over the parts of a row
-// whose draft was turned away.
-template <typename T, int PART>
-__global__ __launch_bounds__(kStatThreads) void verify_left_kernel(VerifyArgs a, const T* __restrict__ logits,
-                                                                   const VerifyStat* __restrict__ stat,
-                                                                   double* __restrict__ left) {
-  __shared__ int red;
-  __shared__ Decision dec;
-  __shared__ double sums[kStatThreads / 64];
-  const int part = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
-  const Decision d = decide(a, logits, stat, b, &red, &dec);
-  if (d.kept == d.n) return;
-  const Left<T> l = left_of(a, logits, b, d, true);
-  const long j0 = (long)part * PART - shift_of(l.row) + 8 * tid;
-  double s = 0.0;
-#pragma unroll 2
-  for (int c = 0; c < PART / (8 * kStatThreads); ++c) {
-    double w[8];
-    l(j0 + 8 * kStatThreads * c, w);
+// grid (parts / 4, B): the drafts kept, and the fp64 sums over the row behind them.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void verify_left_kernel(VerifyArgs a, const T* __restrict__ logits,
+                                                               const VerifyStat* __restrict__ stat,
+                                                               VerifyLeft* __restrict__ left,
+                                                               Decision* __restrict__ decisions) {
+  const int b = blockIdx.y, lane = threadIdx.x & 63;
+  const int part = blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const Decision d = decide(a, logits, stat, b);
+  if (part == 0 && lane == 0) decisions[b] = d;
+  if (!(d.t > 0.f) || !(d.row.sum > 0.0) || part >= a.parts) return;
+  const Behind<T> r(a, logits, b, d);
+  const int first = part * kPart - shift_of(r.row), j0 = first + 8 * lane;
+  double sum = 0.0, over = 0.0;
+  float qs = 0.f;
+  Raw8<T> x[kPieces];
+  load_part(r.row, first, a.V, x);
+  const auto with = [&](const auto* probs) {
+    Raw8<std::remove_const_t<std::remove_reference_t<decltype(*probs)>>> q[kPieces];
+    if (first >= 0 && first + kPart <= a.V) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) s += w[e];
+      for (int c = 0; c < kPieces; ++c) q[c] = any8(probs + j0 + 512 * c);
+    } else {
+#pragma unroll
+      for (int c = 0; c < kPieces; ++c) q[c] = load_any8(probs, j0 + 512 * c, a.V);
+    }
+#pragma unroll
+    for (int c = 0; c < kPieces; ++c)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const double w = r(x[c][e]), m = __builtin_fma(-d.row.sum, (double)q[c][e], w);
+        sum += w;
+        over += fmax(m, 0.0);
+        qs += m > 0.0 ? q[c][e] : 0.f;
+      }
+  };
+  if (!r.probs) {
+#pragma unroll
+    for (int c = 0; c < kPieces; ++c)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum += j0 + 512 * c + e == r.gone ? 0.0 : r(x[c][e]);
+  } else if (a.probs_bf16) {
+    with((const bf16_t*)r.probs);
+  } else {
+    with((const float*)r.probs);
   }
-  s = wave_sum(s);
-  if ((tid & 63) == 0) sums[tid >> 6] = s;
-  __syncthreads();
-  if (tid) return;
-#pragma unroll
-  for (int w = 1; w < kStatThreads / 64; ++w) s += sums[w];
-  left[(long)b * a.parts + part] = s;
+  sum = wave_sum(sum);
+  if (r.probs) {
+    over = wave_sum(over);
+    qs = wave_allsum(qs);
+  }
+  if (lane == 0) left[(long)b * a.parts + part] = VerifyLeft{sum, over, qs};
 }
 
-// grid (B), PART / 8 threads: the part that the random number falls in, the
-// token in it, and the sequence's results.
-template <typename T, int PART>
-__global__ __launch_bounds__(PART / 8) void verify_pick_kernel(VerifyArgs a, const T* __restrict__ logits,
+// grid (B), eight logits of a part for each thread: the part that the random
+// number falls in, the token in it, and the sequence's results.  DECIDED: from the
+// second launch's sums, else from the first's.
+template <typename T, bool DECIDED>
+__global__ __launch_bounds__(kThreads) void verify_pick_kernel(VerifyArgs a, const T* __restrict__ logits,
                                                                const VerifyStat* __restrict__ stat,
-                                                               const double* __restrict__ left) {
-  constexpr int WAVES = PART / 512;
-  __shared__ int red, found, last;
-  __shared__ Decision dec;
-  __shared__ double sums[WAVES], before;
+                                                               const VerifyLeft* __restrict__ left,
+                                                               const Decision* __restrict__ decisions) {
+  static_assert(kPart == 8 * kThreads, "a piece a thread");
+  __shared__ int found, last;
+  __shared__ double sums[kWaves];
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const Decision d = decide(a, logits, stat, b, &red, &dec);
   const double u = a.uniforms[(long)b * (a.N + 1) + a.N];
-  const bool greedy = !(verify_temperature(a, b) > 0.f), some = d.row.sum > 0.0;  // (not NaN)
-  const VerifyStat* s = stat + ((long)b * (a.N + 1) + d.kept) * a.parts;
+  Decision d;
+  if constexpr (DECIDED)
+    d = decisions[b];
+  else
+    d = decide(a, logits, stat, b);
+  if (tid == 0) {
+    found = 0x7fffffff;
+    last = -1;
+  }
+  const bool some = d.row.sum > 0.0;  // (not NaN)
   long token = -1;
-  if (greedy) {
+  if (!(d.t > 0.f)) {
     // what is left of a weight that is all on one token is on it too
     if (some) token = d.row.at;
   } else if (some) {
-    // weight of a part: of what is left of p, or of p where that is nothing
-    const bool turned = d.kept < d.n;
-    const long gone = turned ? a.drafts[(long)b * a.N + d.kept] : -1;
-    const Left<T> whole = left_of(a, logits, b, d, false);
-    const int shift = shift_of(whole.row);
+    const VerifyStat* s = stat + ((long)b * (a.N + 1) + d.kept) * a.parts;
+    const VerifyLeft* l = left + (long)b * a.parts;
+    const Behind<T> r(a, logits, b, d);
+    const int shift = shift_of(r.row), gone_part = r.gone >= 0 && r.gone < a.V ? (int)((r.gone + shift) / kPart) : -1;
+    double S = 0.0;  // over the whole row, of the e that q is taken from
+    if (r.probs) {
+      for (int p = lane; p < a.parts; p += 64) S += l[p].sum;
+      S = wave_sum(S);
+    }
+    // weight of a part: of what is left of p (less), or of p where that is nothing
     const auto part_weight = [&](int p, bool less) {
-      if (less && a.probs) return left[(long)b * a.parts + p];
-      const VerifyStat v = s[p];
-      double w = v.top == -INFINITY ? 0.0 : v.sum * weight(v.top, d.row.top, whole.scale);
-      if (!less && turned && gone >= 0 && (gone + shift) / PART == p) w += d.draft_weight;
-      return w * whole.inv;
+      if (less && r.probs) return fmax(l[p].over + (d.row.sum - S) * l[p].q, 0.0);
+      double w;
+      if constexpr (DECIDED)
+        w = l[p].sum;
+      else
+        w = s[p].sum * weight(s[p].top, d.row.top, r.scale);
+      return !less && !r.probs && p == gone_part ? w + d.row.draft : w;
     };
-    bool less = turned;
-    double total = 0.0;
-    for (int p = lane; p < a.parts; p += 64) total += part_weight(p, less);
-    total = wave_sum(total);
-    if (less && !(total > 0.0)) {
+    const auto sum_of = [&](bool less) {
+      double w = 0.0;
+      for (int p = lane; p < a.parts; p += 64) w += part_weight(p, less);
+      return wave_sum(w);
+    };
+    bool less = d.kept < d.n;
+    double total = sum_of(less);
+    if (less && !(total > kNothing)) {
       less = false;
-      total = 0.0;
-      for (int p = lane; p < a.parts; p += 64) total += part_weight(p, less);
-      total = wave_sum(total);
+      total = sum_of(less);
     }
     const double target = u * total;
-    // the first part whose cumulative weight passes the target, else the last with any
+    // the first part whose cumulative weight passes the target, else the last with
+    // any; every wave finds it by itself
     int part = -1;
-    double base = 0.0;
+    double base = 0.0, start = 0.0;
     for (int p0 = 0, done = 0; p0 < a.parts && !done; p0 += 64) {
       const int p = p0 + lane;
-      const double own = p < a.parts ? part_weight(p, less) : 0.0;
-      double sum = own;
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const double y = __shfl_up(sum, o, 64);
-        if (lane >= o) sum += y;
-      }
-      const unsigned long long past = __ballot(own > 0.0 && base + sum > target), any = __ballot(own > 0.0);
+      const double own = p < a.parts ? part_weight(p, less) : 0.0, sum = wave_scan(own);
+      const unsigned long long past = __ballot(own > kNothing && base + sum > target), any = __ballot(own > kNothing);
       const unsigned long long from = past ? past & -past : any ? 1ull << (63 - __clzll(any)) : 0;
       if (from) {
-        const int l = __ffsll(from) - 1;
-        part = p0 + l;
-        before = base + __shfl(sum - own, l, 64);  // (the same in every thread)
+        const int at = __ffsll(from) - 1;
+        part = p0 + at;
+        start = base + lane_of(sum - own, at);
       }
       done = past != 0;
-      base += __shfl(sum, 63, 64);
+      base += lane_of(sum, 63);
     }
-    if (tid == 0) {
-      found = 0x7fffffff;
-      last = -1;
-    }
-    __syncthreads();
-    const double start = before;
-    const Left<T> l = left_of(a, logits, b, d, less);
-    const long j0 = (long)part * PART - shift + 8 * tid;
+    const int j0 = part * kPart - shift + 8 * tid;
+    const Raw8<T> x = r.logits(j0);
     double w[8], own = 0.0;
-    l(j0, w);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[e] = less && j0 + e == r.gone && !r.probs ? 0.0 : r(x[e]);
+    const auto minus = [&](const auto* probs) {
+      const auto q = load_any8(probs, j0, a.V);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w[e] = fmax(__builtin_fma(-S, (double)q[e], w[e]), 0.0);
+    };
+    if (less && r.probs) a.probs_bf16 ? minus((const bf16_t*)r.probs) : minus((const float*)r.probs);
 #pragma unroll
     for (int e = 0; e < 8; ++e) own += w[e];
-    double sum = own;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const double y = __shfl_up(sum, o, 64);
-      if (lane >= o) sum += y;
-    }
+    const double sum = wave_scan(own);
     if (lane == 63) sums[wave] = sum;
     __syncthreads();
     double at = start + (sum - own);
@@ -445,9 +513,9 @@ __global__ __launch_bounds__(PART / 8) void verify_pick_kernel(VerifyArgs a, con
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       at += w[e];
-      if (w[e] > 0.0) {
-        mine = (int)(j0 + e);
-        if (at > target && hit == 0x7fffffff) hit = (int)(j0 + e);
+      if (w[e] > kNothing) {
+        mine = j0 + e;
+        if (at > target && hit == 0x7fffffff) hit = j0 + e;
       }
     }
     if (hit != 0x7fffffff) atomicMin(&found, hit);
@@ -455,50 +523,53 @@ __global__ __launch_bounds__(PART / 8) void verify_pick_kernel(VerifyArgs a, con
     __syncthreads();
     token = found != 0x7fffffff ? found : last;
   }
-  for (int i = tid; i <= a.N; i += PART / 8)
+  for (int i = tid; i <= a.N; i += kThreads)
     a.tokens[(long)b * (a.N + 1) + i] = i < d.kept ? a.drafts[(long)b * a.N + i] : i == d.kept ? token : -1;
   if (tid == 0) a.accepted[b] = d.kept;
 }
 
 namespace {
 
-// Parts of 8192 logits where they fill the chip, else of 2048.
-int verify_part(const VerifyArgs& a) {
-  const long cells = (long)a.B * (a.N + 1) * a.V;
-  return cells >= 8192l * 1024 ? 8192 : 2048;
-}
 // (a row that begins between two 16-byte boundaries may need one more)
-int verify_parts(const VerifyArgs& a) { return (int)(((long)a.V + 7 + verify_part(a) - 1) / verify_part(a)); }
+int verify_parts(const VerifyArgs& a) { return (int)(((long)a.V + 7 + kPart - 1) / kPart); }
 
 }  // namespace
 
+// Two launches, the first in fp64, where q is not given and the rows are few.
+bool verify_brief(const VerifyArgs& a) {
+  return !a.probs && (long)a.B * (a.N + 1) * a.V <= (1l << 24);
+}
+
 size_t verify_ws_bytes(const VerifyArgs& a) {
   const size_t parts = verify_parts(a);
-  return parts * a.B * (a.N + 1) * sizeof(VerifyStat) + (a.probs ? parts * a.B * sizeof(double) : 0);
+  const size_t stat = parts * a.B * (a.N + 1) * sizeof(VerifyStat);
+  return verify_brief(a) ? stat : stat + a.B * (parts * sizeof(VerifyLeft) + sizeof(Decision));
 }
 
 hipError_t launch_verify(VerifyArgs a, const void* logits, bool bf16, void* ws, hipStream_t st) {
   a.parts = verify_parts(a);
   VerifyStat* stat = (VerifyStat*)ws;
-  double* left = (double*)(stat + (size_t)a.parts * a.B * (a.N + 1));
-  auto run = [&](auto type, auto part) {
+  VerifyLeft* left = (VerifyLeft*)(stat + (size_t)a.parts * a.B * (a.N + 1));
+  Decision* decisions = (Decision*)(left + (size_t)a.parts * a.B);
+  const unsigned groups = (a.parts + kWaves - 1) / kWaves;
+  auto run = [&](auto type, auto brief) {
     using T = decltype(type);
-    constexpr int PART = decltype(part)::value;
+    constexpr bool BRIEF = decltype(brief)::value;
     const T* x = (const T*)logits;
     NAYLIS_TIMED("verify_stat", st,
-                 hipLaunchKernelGGL((verify_stat_kernel<T, PART>), dim3(a.parts, a.N + 1, a.B), dim3(kStatThreads), 0,
-                                    st, a, x, stat));
-    if (a.probs && a.N > 0) {
+                 hipLaunchKernelGGL((verify_stat_kernel<T, BRIEF>), dim3(groups, a.N + 1, a.B), dim3(kThreads), 0, st,
+                                    a, x, stat));
+    if constexpr (!BRIEF) {
       NAYLIS_TIMED("verify_left", st,
-                   hipLaunchKernelGGL((verify_left_kernel<T, PART>), dim3(a.parts, a.B), dim3(kStatThreads), 0, st, a,
-                                      x, (const VerifyStat*)stat, left));
+                   hipLaunchKernelGGL((verify_left_kernel<T>), dim3(groups, a.B), dim3(kThreads), 0, st, a, x,
+                                      (const VerifyStat*)stat, left, decisions));
     }
     NAYLIS_TIMED("verify_pick", st,
-                 hipLaunchKernelGGL((verify_pick_kernel<T, PART>), dim3(a.B), dim3(PART / 8), 0, st, a, x,
-                                    (const VerifyStat*)stat, (const double*)left));
+                 hipLaunchKernelGGL((verify_pick_kernel<T, !BRIEF>), dim3(a.B), dim3(kThreads), 0, st, a, x,
+                                    (const VerifyStat*)stat, (const VerifyLeft*)left, (const Decision*)decisions));
   };
-  auto pick = [&](auto part) { bf16 ? run(bf16_t{}, part) : run(float{}, part); };
-  verify_part(a) == 8192 ? pick(std::integral_constant<int, 8192>{}) : pick(std::integral_constant<int, 2048>{});
+  auto pick = [&](auto type) { verify_brief(a) ? run(type, std::true_type{}) : run(type, std::false_type{}); };
+  bf16 ? pick(bf16_t{}) : pick(float{});
   return hipGetLastError();
 }
 

@@ -191,6 +191,21 @@ def test_verify_rows_without_a_distribution(t, probs, bad, dev):
         assert torch.equal(got.tokens[b], fine.tokens[b])
 
 
+@pytest.mark.parametrize("B", [2, 600])  # sums in fp64, and in fp32
+def test_verify_signalling_nans(B, dev):
+    """NaNs of every bit pattern, one and a whole part of them."""
+    from naylis_amd.mom_kernels import verify_drafts
+    V = 20000
+    x = torch.zeros(B, 2, V, dtype=torch.bfloat16, device=dev)
+    drafts, u = torch.full((B, 1), 17, device=dev), torch.zeros(B, 2, device=dev)
+    for bits in (0x7f81, 0x7fc0, 0xff81 - 65536, 0xffff - 65536):
+        for where in (slice(17, 18), slice(9000, 9001), slice(2048, 6144), slice(None)):
+            y = x.clone()
+            y.view(torch.int16)[1, 0, where] = bits
+            got = verify_drafts(y, drafts, u)
+            assert got.accepted[:2].tolist() == [1, 0] and got.tokens[:2].tolist() == [[17, 0], [-1, -1]]
+
+
 def test_verify_drafts_that_are_none(dev):
     """Ids outside the vocabulary are turned away and take nothing from p."""
     c = _case(40, 3, 900, torch.float32, None, dev)
