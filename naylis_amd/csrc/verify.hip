@@ -259,6 +259,14 @@ __global__ __launch_bounds__(kThreads, EXACT || sizeof(T) == 4 ? 1 : 8) void ver
       for (int c = 0; c < kPieces; ++c) s += sums[c];
     }
   }
+  if constexpr (!EXACT) {
+    if (top == -INFINITY) {  // of nothing but -inf and NaNs
+#pragma unroll
+      for (int c = 0; c < kPieces; ++c)
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) nan |= __builtin_isunordered(x[c][e], x[c][e + 1]);
+    }
+  }
   if (__any(nan) || top == INFINITY) s = __builtin_nan("");
   if (!(t > 0.f)) at = wave_allmin_i32(at);
   s = wave_sum(s);
