@@ -160,7 +160,7 @@ struct PagedNew {
   long T, ldk, hsk, ldv, hsv;  // new tokens, token and head strides of their k and v
 };
 struct PagedSplit {
-  int wgs, rows, head_tiles;  // workgroups of a slice, its most query rows, slices of a key head
+  int wgs, rows, tile, head_tiles;  // workgroups of a slice, its partials' rows, its query rows, slices of a key head
   bool whole;                 // a workgroup takes a sequence
 };
 struct PagedQueries {

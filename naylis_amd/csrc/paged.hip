@@ -43,9 +43,8 @@ namespace naylis {
 
 namespace {
 
-constexpr int kRowsMfma = 16;       // query heads of a product
-// tokens of a step (4 bits: as many bytes under way take more tokens)
-constexpr int paged_step(PagedFormat f) { return f == kPagedE2m1 ? 64 : 32; }
+constexpr int kRowsMfma = 16;       // query rows of a product
+constexpr int kPagedStep = 32;      // tokens of a step
 constexpr int kPagedMaxWgs = 512;   // workgroups that share a slice's steps
 
 __device__ __forceinline__ f32x4 mfma16(const bf16x8& a, const bf16x8& b, const f32x4& c) {
@@ -104,7 +103,6 @@ namespace {
 // The list of all sequences' steps.  A lane looks after an equal chunk of the
 // sequences, so that a place is found with one scan over the lanes and one over
 // a chunk, whatever their number.
-template <int STEP>
 struct StepList {
   const int32_t* lens;
   int B, cap;  // sequences, tokens that a table row holds
@@ -114,7 +112,7 @@ struct StepList {
     const int n = lens[min(b, B - 1)];
     return b < B ? min(max(n, 0), cap) : 0;
   }
-  __device__ __forceinline__ int steps(int b) const { return (len(b) + STEP - 1) / STEP; }
+  __device__ __forceinline__ int steps(int b) const { return (len(b) + kPagedStep - 1) / kPagedStep; }
 
   static __device__ __forceinline__ int inclusive(int x) {
     const int lane = threadIdx.x & 63;
@@ -173,13 +171,19 @@ struct PartSeq {
   int b, first, steps;  // sequence (-1: none), its first step in the list, its steps
 };
 
-// LDS of a wave: its V tile (32 tokens), where its last partial goes too (16
-// rows of fp32, once the tile is no longer needed), then its first partial.
-template <int HD, int ROWS>
-constexpr int kWaveLds = 32 * 2 * HD + ROWS * HD * 4;
+// Whether the partial of a sequence that ends within a wave's range goes to the
+// workspace, not to LDS: few waves have one, and of 32 rows, or of 16 beside pages
+// of 4 bits, its LDS would leave room for fewer workgroups a CU than the registers do.
+constexpr bool ends_outside(PagedFormat f, int rows) { return rows > kRowsMfma || (f == kPagedE2m1 && rows > 4); }
+
+// LDS of a wave: its V tile (32 tokens), where the partial at the end of its range
+// goes too (fp32 rows, once the tile is no longer needed), then that of a sequence
+// that ends within the range.
+template <int HD, PagedFormat FMT, int ROWS>
+constexpr int kWaveLds = std::max(32 * 2 * HD, ROWS * HD * 4) + (ends_outside(FMT, ROWS) ? 0 : ROWS * HD * 4);
 template <int HD>
 __device__ __forceinline__ int part_offset(int slot) {
-  static_assert(kRowsMfma * 4 == 32 * 2, "a partial fits the V tile");
+  static_assert(kRowsMfma * 4 == 32 * 2, "a partial of 16 rows fits the V tile");
   return slot == 0 ? 32 * 2 * HD : 0;
 }
 
@@ -227,20 +231,22 @@ __device__ __forceinline__ long part_row(const PagedSplit& p, int slice, int wg,
   return (((long)slice * p.wgs + wg) * 2 + slot) * p.rows;
 }
 
-// grid (workgroups of a slice, slices): slice = (key head, 16 of its query rows).
+// grid (workgroups of a slice, slices): slice = (key head, 16 or 32 of its query rows).
 // A workgroup takes a range of the step list, or (p.whole) the sequence of its
 // number, its waves an equal share each.
-// ROWS: partials' rows, at least the query rows of a slice.  MANY: more than one
+// ROWS: partials' rows, at least the query rows of a slice; a product's 16 or, of 32,
+// two products' for each read of the cache.  MANY: more than one
 // new token, or a number of them that each sequence has of its own.
 template <int HD, PagedFormat FMT, int ROWS, bool MANY>
-__global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedCacheDims c, PagedQueries q,
+__global__ __launch_bounds__(256, FMT == kPagedE2m1 && ROWS <= kRowsMfma ? 3 : 2) void paged_attn_kernel(PagedCacheDims c, PagedQueries q,
                                                             const int32_t* __restrict__ table,
                                                             const int32_t* __restrict__ lens,
                                                             bf16_t* __restrict__ out, float* __restrict__ part,
                                                             float2* __restrict__ stat, int* __restrict__ starts,
-                                                            PagedSplit p, float sc) {
+                                                            float* __restrict__ ended, PagedSplit p, float sc) {
+  constexpr int QT = ROWS > kRowsMfma ? 2 : 1;  // 16-row tiles
   constexpr bool FP8 = FMT == kPagedE4m3, FP4 = FMT == kPagedE2m1;
-  constexpr int TOK = paged_step(FMT);   // tokens of a step
+  constexpr int TOK = kPagedStep;        // tokens of a step
   constexpr int NS = TOK / 16;           // its 16-token products
   constexpr int KS = HD / 32;            // products along the features
   constexpr int NT = HD / 16;            // 16-feature tiles of the output
@@ -249,15 +255,17 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedCacheDims c, Pa
   constexpr int VR = FP4 ? 16 : 1024 / RB;  // rows of V that a load of 64 lanes covers
   constexpr int VL = TOK / VR;           // such loads
   constexpr int NW = HD / 32;            // 4 bits: words of such a load, HD / 4 features
-  __shared__ __align__(16) uint8_t lds[4 * kWaveLds<HD, ROWS>];
+  __shared__ __align__(16) uint8_t lds[4 * kWaveLds<HD, FMT, ROWS>];
   __shared__ PartSeq seqs[8];
   __shared__ float2 stats[8][ROWS];
   const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  uint8_t* vt = lds + wave * kWaveLds<HD, ROWS>;
+  uint8_t* vt = lds + wave * kWaveLds<HD, FMT, ROWS>;
   const int wg = blockIdx.x, slice = blockIdx.y;
-  const int kvh = slice / p.head_tiles, h0 = kRowsMfma * (slice % p.head_tiles);
-  const int nh = min(kRowsMfma, (MANY ? c.G * c.N : c.G) - h0);  // live query rows of the slice
+  const int kvh = slice / p.head_tiles, h0 = QT * kRowsMfma * (slice % p.head_tiles);
+  const int nh = min(QT * kRowsMfma, (MANY ? c.G * c.N : c.G) - h0);  // live query rows of the slice
+  constexpr bool OUTSIDE = ends_outside(FMT, ROWS);
+  if constexpr (OUTSIDE) ended += (((long)slice * p.wgs + wg) * 4) * ROWS * HD;  // a wave's partial that ends within its range
   const int H = c.Hkv * c.G, hbase = kvh * c.G + h0;
   const Rows rows{c.G, c.N, H};
   // the slice's row r of sequence b in out
@@ -267,7 +275,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedCacheDims c, Pa
   const auto live_of = [&](int b) { return q.live ? min(max(q.live[b], 0), c.N) : c.N; };
   // whether the slice's row r sees no token of sequence b
   const auto blind = [&](int b, int r) { return MANY && seen(lens[b], live_of(b), rows.token(h0 + r)) == 0; };
-  const StepList<TOK> list{lens, c.B, c.W * c.page};
+  const StepList list{lens, c.B, c.W * c.page};
 
   int wg0, wg1, at, end, b = wg, first = 0;
   int2 sums = make_int2(0, 0);
@@ -291,9 +299,9 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedCacheDims c, Pa
 
   const int shift = 31 - __clz(c.page);
   // bytes of a lane's loads.  V: row vrow, piece vpc; K: row r16, pieces g, g + 4, ..
-  const int voff = lane * (FP4 ? 4 * NW : 16), koff = r16 * RB + g * (FP4 ? 4 * NW : 16);
+  const uint32_t voff = lane * (FP4 ? 4 * NW : 16), koff = r16 * RB + g * (FP4 ? 4 * NW : 16);
+  const uint32_t veoff = lane * NW / 4, keoff = r16 * NW + g * NW / 4;
   const int vrow = FP4 ? lane / 4 : lane / (RB / 16), vpc = FP4 ? lane % 4 : lane % (RB / 16);
-  const int begin = at;
 
   while (at < end && b < c.B) {
     const int n = list.len(b), nsteps = (n + TOK - 1) / TOK;
@@ -301,12 +309,15 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedCacheDims c, Pa
     bool bad = lens[b] > list.cap;                             // longer than its table
     // tokens that the lane's row sees, and the fewest that one does
     const int live = MANY ? live_of(b) : 1, all = n - (live - 1);
-    const int mine = MANY ? n - max(live - 1 - rows.token(h0 + r16), 0) : n;
+    int mine[QT];
+#pragma unroll
+    for (int u = 0; u < QT; ++u) mine[u] = MANY ? n - max(live - 1 - rows.token(h0 + 16 * u + r16), 0) : n;
     if (!p.whole && s0 == 0 && slice == 0 && lane == 0) starts[b] = first;
 
-    bf16x8 qf[KS];
-    {
-      const int row = h0 + min(r16, nh - 1);
+    bf16x8 qf[QT][KS];
+#pragma unroll
+    for (int u = 0; u < QT; ++u) {
+      const int row = h0 + min(16 * u + r16, nh - 1);
       const bf16_t* qp = (const bf16_t*)q.q + (long)b * q.ldb +
                          (MANY ? rows.token(row) * q.ldt + (long)(kvh * c.G + row % c.G) * q.hs
                                : (long)(kvh * c.G + row) * q.hs);
@@ -316,48 +327,60 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedCacheDims c, Pa
         const int f = FP4   ? 8 * NW * g + 8 * ks
                       : FP8 ? 64 * (ks >> 1) + 16 * g + 8 * (ks & 1)
                             : 32 * ks + 8 * g;
-        qf[ks] = *reinterpret_cast<const bf16x8*>(qp + f);
-        if (r16 >= nh) qf[ks] = bf16x8{};
+        qf[u][ks] = *reinterpret_cast<const bf16x8*>(qp + f);
+        if (16 * u + r16 >= nh) qf[u][ks] = bf16x8{};
       }
     }
-    f32x4 acc[NT];
+    f32x4 acc[QT][NT];
+    float m[QT], l[QT];
 #pragma unroll
-    for (int t = 0; t < NT; ++t) acc[t] = f32x4{};
-    float m = kLowest, l = 0.f;
+    for (int u = 0; u < QT; ++u) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t) acc[u][t] = f32x4{};
+      m[u] = kLowest;
+      l[u] = 0.f;
+    }
 
-    // pages of the next 64 products' tokens, one a lane
-    int ids = 0, ids_at = -64;
     uint4 kx[NS][KL], vx[VL];
     Words<NW> kw[NS], vw[NS];  // 4 bits
     uint32_t ke[NS], ve[NS];   // their scales' exponents
     f32x4 ksc[NS], vsc[NS];    // scales of tokens 16 i + 4 g ..
     long row16[NS];          // cache row of each 16-token group of the step being loaded
-    auto find_pages = [&](int step) {
+    // pages a step ahead, by scalar loads: a wait for them leaves the rows' loads in
+    // flight.  Groups past the end take the last token's page, and nothing of it counts.
+    const int32_t* pages = table + (long)b * c.W;
+    int ids[NS];
+    auto fetch_pages = [&](int step) {
+#pragma unroll
+      for (int i = 0; i < NS; ++i) ids[i] = pages[min((step * NS + i) << 4, n - 1) >> shift];
+    };
+    auto take_pages = [&](int step) {
 #pragma unroll
       for (int i = 0; i < NS; ++i) {
-        const int t16 = step * NS + i;  // 16-token group of the sequence
-        if (t16 >= ids_at + 64) {
-          ids_at = t16;
-          const int tok = (t16 + lane) << 4;
-          ids = tok < n ? table[(long)b * c.W + (tok >> shift)] : 0;
-        }
-        int id = __builtin_amdgcn_readlane(ids, t16 - ids_at);
+        int id = ids[i];
         if (!page_ok(id, c.P)) {
           bad = true;
           id = 0;
         }
-        row16[i] = ((long)id * c.Hkv + kvh) * c.page + ((t16 << 4) & (c.page - 1));
+        row16[i] = ((long)id * c.Hkv + kvh) * c.page + (((step * NS + i) << 4) & (c.page - 1));
       }
     };
+    // (a lane's offset is new to the compiler each time, so that the uniform part of
+    // an address stays in scalar registers)
+    const auto lane_offset = [](uint32_t x) {
+      asm("" : "+v"(x));
+      return x;
+    };
     auto load_k = [&]() {
+      const uint32_t off = lane_offset(koff), eoff = lane_offset(keoff);
 #pragma unroll
       for (int i = 0; i < NS; ++i) {
         if constexpr (FP4) {
-          kw[i] = load_once<NW>((const uint8_t*)c.k + row16[i] * RB + koff);
-          ke[i] = ((const uint8_t*)c.k_scale)[row16[i] * NW + r16 * NW + g * NW / 4];
+          kw[i] = load_once<NW>((const uint8_t*)c.k + row16[i] * RB + off);
+          ke[i] = __builtin_nontemporal_load((const uint8_t*)c.k_scale + row16[i] * NW + eoff);
         } else {
 #pragma unroll
-          for (int j = 0; j < KL; ++j) kx[i][j] = load_once16((const uint8_t*)c.k + row16[i] * RB + koff + 64 * j);
+          for (int j = 0; j < KL; ++j) kx[i][j] = load_once16((const uint8_t*)c.k + row16[i] * RB + 64 * j + off);
         }
         if constexpr (FP8) {
           ksc[i] = *reinterpret_cast<const f32x4*>((const float*)c.k_scale + row16[i] + 4 * g);
@@ -365,30 +388,33 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedCacheDims c, Pa
         }
       }
     };
-    // 16-token groups i0 ..
-    auto load_v = [&](int i0, int n) {
+    auto load_v = [&]() {
+      const uint32_t off = lane_offset(voff), eoff = lane_offset(veoff);
 #pragma unroll
-      for (int i = i0; i < i0 + n; ++i) {
+      for (int i = 0; i < NS; ++i) {
         if constexpr (FP4) {
-          vw[i] = load_once<NW>((const uint8_t*)c.v + row16[i] * RB + voff);
-          ve[i] = ((const uint8_t*)c.v_scale)[row16[i] * NW + lane * NW / 4];
+          vw[i] = load_once<NW>((const uint8_t*)c.v + row16[i] * RB + off);
+          ve[i] = __builtin_nontemporal_load((const uint8_t*)c.v_scale + row16[i] * NW + eoff);
         } else {
 #pragma unroll
           for (int j = 0; j < VL / NS; ++j)
-            vx[i * (VL / NS) + j] = load_once16((const uint8_t*)c.v + row16[i] * RB + voff + 1024 * j);
+            vx[i * (VL / NS) + j] = load_once16((const uint8_t*)c.v + row16[i] * RB + 1024 * j + off);
         }
       }
     };
-    find_pages(s0);
+    fetch_pages(s0);
+    take_pages(s0);
+    fetch_pages(s0 + 1);
     load_k();
-    load_v(0, NS);
+    load_v();
     for (int s = s0; s < s1; ++s) {
       const int tok0 = s * TOK;
       // S^T: lane = query head r16, registers = tokens 16 i + 4 g + v
-      f32x4 x[NS];
+      f32x4 x[QT][NS];
 #pragma unroll
       for (int i = 0; i < NS; ++i) {
-        x[i] = f32x4{};
+#pragma unroll
+        for (int u = 0; u < QT; ++u) x[u][i] = f32x4{};
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
           bf16x8 kf;
@@ -400,25 +426,24 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedCacheDims c, Pa
           } else {
             kf = __builtin_bit_cast(bf16x8, kx[i][ks]);
           }
-          x[i] = mfma16(kf, qf[ks], x[i]);
+#pragma unroll
+          for (int u = 0; u < QT; ++u) x[u][i] = mfma16(kf, qf[u][ks], x[u][i]);
         }
       }
       const bool tail = tok0 + TOK > (MANY ? all : n);
-      // V rows to LDS as bf16, 32 tokens from `half` on; rows past the sequence as zeros, whatever the page holds there
-      auto store_v = [&](int half) {
+      // V rows to LDS as bf16; rows past the sequence as zeros, whatever the page holds there
+      auto store_v = [&]() {
         if constexpr (FP4) {
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
+          for (int i = 0; i < NS; ++i) {
             const int row = 16 * i + vrow;
-            Words<NW> u = vw[2 * half + i];
-            uint32_t e = ve[2 * half + i];
-            if (tail && tok0 + 32 * half + row >= n) {
-              u = Words<NW>{};
-              e = 127;
+            if (tail && tok0 + row >= n) {
+              vw[i] = Words<NW>{};
+              ve[i] = 127;
             }
 #pragma unroll
             for (int w = 0; w < NW; ++w)
-              *reinterpret_cast<bf16x8*>(vt + v_slot<HD>(row, NW * vpc + w)) = widen8_e2m1(u.w[w], e);
+              *reinterpret_cast<bf16x8*>(vt + v_slot<HD>(row, NW * vpc + w)) = widen8_e2m1(vw[i].w[w], ve[i]);
           }
           lds_order();
           return;
@@ -426,8 +451,8 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedCacheDims c, Pa
 #pragma unroll
         for (int j = 0; j < VL; ++j) {
           const int row = j * VR + vrow;
-          uint4 u = vx[j];
-          if (tail && tok0 + row >= n) u = make_uint4(0, 0, 0, 0);
+          if (tail && tok0 + row >= n) vx[j] = make_uint4(0, 0, 0, 0);
+          const uint4 u = vx[j];
           if constexpr (FP8) {
             *reinterpret_cast<bf16x8*>(vt + v_slot<HD>(row, 2 * vpc)) = widen8(u.x, u.y);
             *reinterpret_cast<bf16x8*>(vt + v_slot<HD>(row, 2 * vpc + 1)) = widen8(u.z, u.w);
@@ -448,91 +473,106 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedCacheDims c, Pa
       // registers go to the next step's loads as soon as they are read
       const bool more = s + 1 < s1;
       if (more) {
-        find_pages(s + 1);
+        take_pages(s + 1);
+        fetch_pages(s + 2);
         load_k();
       }
-      store_v(0);
-      if (more) load_v(0, FP4 ? 2 : NS);
-      float mx = -INFINITY;
+      store_v();
+      if (more) load_v();
 #pragma unroll
-      for (int i = 0; i < NS; ++i)
+      for (int u = 0; u < QT; ++u) {
+        float mx = -INFINITY;
 #pragma unroll
-        for (int v = 0; v < 4; ++v) {
-          x[i][v] *= FP8 ? kss[i][v] : sc;
-          if (tail && tok0 + 16 * i + 4 * g + v >= mine) {
-            x[i][v] = -INFINITY;
-            if constexpr (FP8) vss[i][v] = 0.f;
+        for (int i = 0; i < NS; ++i)
+#pragma unroll
+          for (int v = 0; v < 4; ++v) x[u][i][v] *= FP8 ? kss[i][v] : sc;
+        if (__builtin_expect(tail, 0))
+#pragma unroll
+          for (int i = 0; i < NS; ++i)
+#pragma unroll
+            for (int v = 0; v < 4; ++v)
+              if (tok0 + 16 * i + 4 * g + v >= mine[u]) x[u][i][v] = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < NS; ++i)
+#pragma unroll
+          for (int v = 0; v < 4; ++v) mx = fmaxf(mx, x[u][i][v]);
+        const auto fmx = [](float a, float b) { return fmaxf(a, b); };
+        mx = xor32_f32(xor16_f32(mx, fmx), fmx);
+        const float mn = fmaxf(m[u], mx), al = __builtin_amdgcn_exp2f(m[u] - mn);
+        // (times 1 where no row has a new maximum)
+        if (__any(mn > m[u])) {
+          l[u] *= al;
+#pragma unroll
+          for (int t = 0; t < NT; ++t) acc[u][t] *= al;
+        }
+        m[u] = mn;
+#pragma unroll
+        for (int i = 0; i < NS; ++i)
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            x[u][i][v] = __builtin_amdgcn_exp2f(x[u][i][v] - mn);
+            l[u] += x[u][i][v];
+            if constexpr (FP8) x[u][i][v] *= vss[i][v];
           }
-          mx = fmaxf(mx, x[i][v]);
-        }
-      const auto fmx = [](float a, float b) { return fmaxf(a, b); };
-      mx = xor32_f32(xor16_f32(mx, fmx), fmx);
-      const float mn = fmaxf(m, mx), al = __builtin_amdgcn_exp2f(m - mn);
-      m = mn;
-      l *= al;
+        // rows past the end: their weight is 0, their scale may be anything
+        if (FP8 && __builtin_expect(tail, 0))
 #pragma unroll
-      for (int t = 0; t < NT; ++t) acc[t] *= al;
+          for (int i = 0; i < NS; ++i)
 #pragma unroll
-      for (int i = 0; i < NS; ++i)
+            for (int v = 0; v < 4; ++v)
+              if (tok0 + 16 * i + 4 * g + v >= mine[u]) x[u][i][v] = 0.f;
+      }
+      // O^T += V^T P^T: registers of the two products are the B operand
+      bf16x8 pf[QT];
 #pragma unroll
-        for (int v = 0; v < 4; ++v) {
-          x[i][v] = __builtin_amdgcn_exp2f(x[i][v] - mn);
-          l += x[i][v];
-          if constexpr (FP8) x[i][v] *= vss[i][v];
-        }
-      // O^T += V^T P^T: registers of two products are the B operand
-#pragma unroll
-      for (int half = 0; half < TOK / 32; ++half) {
-        if (half) {
-          store_v(half);
-          if (more) load_v(2 * half, 2);
-        }
-        bf16x8 pf;
+      for (int u = 0; u < QT; ++u)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          pf[e] = (__bf16)x[2 * half][e];
-          pf[4 + e] = (__bf16)x[2 * half + 1][e];
+          pf[u][e] = (__bf16)x[u][0][e];
+          pf[u][4 + e] = (__bf16)x[u][1][e];
         }
-        const int rlo = 4 * g + (r16 >> 2), rhi = rlo + 16;
+      const int rlo = 4 * g + (r16 >> 2), rhi = rlo + 16;
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          const int ch = 2 * t + ((r16 & 3) >> 1), b8 = 8 * (r16 & 1);
-          const v4i16 lo = lds_read_tr16(reinterpret_cast<const bf16_t*>(vt + v_slot<HD>(rlo, ch) + b8));
-          const v4i16 hi = lds_read_tr16(reinterpret_cast<const bf16_t*>(vt + v_slot<HD>(rhi, ch) + b8));
-          typedef short v8i16 __attribute__((ext_vector_type(8)));
-          const v8i16 vf = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-          acc[t] = mfma16(__builtin_bit_cast(bf16x8, vf), pf, acc[t]);
-        }
-        lds_order();
+      for (int t = 0; t < NT; ++t) {
+        const int ch = 2 * t + ((r16 & 3) >> 1), b8 = 8 * (r16 & 1);
+        const v4i16 lo = lds_read_tr16(reinterpret_cast<const bf16_t*>(vt + v_slot<HD>(rlo, ch) + b8));
+        const v4i16 hi = lds_read_tr16(reinterpret_cast<const bf16_t*>(vt + v_slot<HD>(rhi, ch) + b8));
+        typedef short v8i16 __attribute__((ext_vector_type(8)));
+        const v8i16 vf = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+        for (int u = 0; u < QT; ++u) acc[u][t] = mfma16(__builtin_bit_cast(bf16x8, vf), pf[u], acc[u][t]);
       }
+      lds_order();
     }
     const auto add = [](float a, float b2) { return a + b2; };
-    l = xor32_f32(xor16_f32(l, add), add);
-    if (bad) l = __builtin_nanf("");  // a page that is none: the sequence's result is NaN
-    if (s0 == 0 && s1 == nsteps) {
-      if (r16 < nh) {
-        const float inv = 1.f / l;
-        const bool none = blind(b, r16);
-        bf16_t* to = out_row(b, r16);
+    const bool whole = s0 == 0 && s1 == nsteps;
+    const int slot = first + s1 < end ? 0 : 1;  // ends within the range, or with it
+#pragma unroll
+    for (int u = 0; u < QT; ++u) {
+      const int r = 16 * u + r16;
+      l[u] = xor32_f32(xor16_f32(l[u], add), add);
+      if (bad) l[u] = __builtin_nanf("");  // a page that is none: the sequence's result is NaN
+      if (r >= nh) continue;
+      if (whole) {
+        const float inv = 1.f / l[u];
+        const bool none = blind(b, r);
+        bf16_t* to = out_row(b, r);
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
           bf16x4 o;
 #pragma unroll
-          for (int v = 0; v < 4; ++v) o[v] = (__bf16)(none ? 0.f : acc[t][v] * inv);
+          for (int v = 0; v < 4; ++v) o[v] = (__bf16)(none ? 0.f : acc[u][t][v] * inv);
           *reinterpret_cast<bf16x4*>(to + 16 * t + 4 * g) = o;
         }
-      }
-    } else {
-      const int slot = at == begin ? 0 : 1;
-      if (r16 < nh) {
+      } else {
+        float* to = OUTSIDE && slot == 0 ? ended + (long)wave * ROWS * HD
+                                         : reinterpret_cast<float*>(vt + part_offset<HD>(slot));
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
-          *reinterpret_cast<f32x4*>(reinterpret_cast<float*>(vt + part_offset<HD>(slot)) + r16 * HD + 16 * t + 4 * g) =
-              acc[t];
-        if (g == 0) stats[2 * wave + slot][r16] = make_float2(m, l);
+        for (int t = 0; t < NT; ++t) *reinterpret_cast<f32x4*>(to + r * HD + 16 * t + 4 * g) = acc[u][t];
+        if (g == 0) stats[2 * wave + slot][r] = make_float2(m[u], l[u]);
       }
-      if (lane == 0) seqs[2 * wave + slot] = PartSeq{b, first, nsteps};
     }
+    if (!whole && lane == 0) seqs[2 * wave + slot] = PartSeq{b, first, nsteps};
     at = first + s1;
     first += nsteps;
     ++b;
@@ -560,8 +600,12 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedCacheDims c, Pa
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       st[e] = stats[e][r];
-      px[e] = *reinterpret_cast<const f32x4*>(
-          reinterpret_cast<const float*>(lds + (e >> 1) * kWaveLds<HD, ROWS> + part_offset<HD>(e & 1)) + r * HD + f);
+      if (OUTSIDE && e % 2 == 0) {
+        if (ps[e].b >= 0) px[e] = *reinterpret_cast<const f32x4*>(ended + ((e >> 1) * ROWS + r) * HD + f);
+      } else {
+        px[e] = *reinterpret_cast<const f32x4*>(
+            reinterpret_cast<const float*>(lds + (e >> 1) * kWaveLds<HD, FMT, ROWS> + part_offset<HD>(e & 1)) + r * HD + f);
+      }
     }
     float m = kLowest, l = 0.f;
     f32x4 a = f32x4{};
@@ -609,7 +653,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedCacheDims c, Pa
 
 // Joins the workgroups' partials of a sequence; nothing where one of them held
 // it whole.  Grid (N H, B).
-template <int HD, int STEP>
+template <int HD>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedCacheDims c, const int32_t* __restrict__ live,
                                                          const int32_t* __restrict__ lens, bf16_t* __restrict__ out,
                                                          const float* __restrict__ part, const float2* __restrict__ stat,
@@ -620,18 +664,18 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedCacheDims c, const
   __shared__ f32x4 sums[NG][TR];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int H = c.Hkv * c.G, token = blockIdx.x / H, h = blockIdx.x % H, b = blockIdx.y;
-  const StepList<STEP> list{lens, c.B, c.W * c.page};
+  const StepList list{lens, c.B, c.W * c.page};
   const int n = list.steps(b);
   if (n == 0) return;
   const int total = starts[c.B], range = max((total + p.wgs - 1) / p.wgs, 1);
   const int first = starts[b], w0 = first / range, w1 = (first + n - 1) / range;
   if (w0 == w1) return;
-  const int kvh = h / c.G, hr = token * c.G + h % c.G, slice = kvh * p.head_tiles + hr / kRowsMfma;
+  const int kvh = h / c.G, hr = token * c.G + h % c.G, slice = kvh * p.head_tiles + hr / p.tile;
   const int count = w1 - w0 + 1;
   // a workgroup's first sequence, unless its range begins before this one
   const auto row = [&](int i) {
     const int w = w0 + i;
-    return part_row(p, slice, w, w * range >= first ? 0 : 1) + hr % kRowsMfma;
+    return part_row(p, slice, w, w * range >= first ? 0 : 1) + hr % p.tile;
   };
   const auto block = [&](float x, auto op) {
     x = wave_allreduce_f32(x, op);
@@ -678,33 +722,86 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedCacheDims c, const
   *reinterpret_cast<bf16x4*>(out + (((long)b * c.N + token) * H + h) * HD + 4 * f) = o;
 }
 
+// The same with HD / 4 threads a row, one partial after another: for a few partials
+// of many rows.  Grid (1024 / HD rows of a key head, key heads, B).
+template <int HD>
+__global__ __launch_bounds__(256) void paged_join_few_kernel(PagedCacheDims c, const int32_t* __restrict__ live,
+                                                             const int32_t* __restrict__ lens, bf16_t* __restrict__ out,
+                                                             const float* __restrict__ part,
+                                                             const float2* __restrict__ stat,
+                                                             const int* __restrict__ starts, PagedSplit p) {
+  constexpr int TR = HD / 4, NG = 256 / TR;
+  const int hr = blockIdx.x * NG + threadIdx.x / TR, f = threadIdx.x % TR, kvh = blockIdx.y, b = blockIdx.z;
+  const StepList list{lens, c.B, c.W * c.page};
+  const int n = list.steps(b);
+  if (n == 0 || hr >= c.G * c.N) return;
+  const int total = starts[c.B], range = max((total + p.wgs - 1) / p.wgs, 1);
+  const int first = starts[b], w0 = first / range, w1 = (first + n - 1) / range;
+  if (w0 == w1) return;
+  const int slice = kvh * p.head_tiles + hr / p.tile;
+  const auto row = [&](int w) { return part_row(p, slice, w, w * range >= first ? 0 : 1) + hr % p.tile; };
+  float m = kLowest, l = 0.f;
+  f32x4 a = f32x4{};
+#pragma unroll 4
+  for (int w = w0; w <= w1; ++w) {
+    const float2 s = stat[row(w)];
+    const f32x4 x = *reinterpret_cast<const f32x4*>(part + row(w) * HD + 4 * f);
+    const float mn = fmaxf(m, s.x), wa = __builtin_amdgcn_exp2f(m - mn), wb = __builtin_amdgcn_exp2f(s.x - mn);
+    a = a * wa + x * wb;
+    l = l * wa + s.y * wb;
+    m = mn;
+  }
+  const int token = hr / c.G;
+  const bool none = seen(lens[b], live ? min(max(live[b], 0), c.N) : c.N, token) == 0;
+  const float inv = 1.f / l;
+  bf16x4 o;
+#pragma unroll
+  for (int v = 0; v < 4; ++v) o[v] = (__bf16)(none ? 0.f : a[v] * inv);
+  *reinterpret_cast<bf16x4*>(out + Rows{c.G, c.N, c.Hkv * c.G}.at(b, kvh, hr) * HD + 4 * f) = o;
+}
+
 // A workgroup for each sequence where tables hold at most 16 steps, four for each
 // wave, and no second launch (128 sequences of up to 500 tokens, 8 key heads of
 // 128: 38 us against 50).  Else the list is cut for two workgroups a CU over all
 // slices, and no finer than a step a wave.
 // Three or four a CU take longer (three contexts of 65537 .. 131072 tokens, e4m3:
-// 124 us with 512 workgroups, 147 with 768, 130 with 1024).
+// 124 us with 512 workgroups, 147 with 768, 130 with 1024); pages of 4 bits, with
+// half the loads of a step, leave registers for three and gain by them (three
+// contexts of 99396 .. 131072 tokens, four new ones each: 71 us against 76).
 PagedSplit paged_split(const PagedCacheDims& c, PagedFormat fmt) {
   PagedSplit p;
-  const int step = paged_step(fmt), rows = c.G * c.N;
-  p.head_tiles = (rows + kRowsMfma - 1) / kRowsMfma;
-  p.rows = rows <= 4 ? 4 : kRowsMfma;
+  const int rows = c.G * c.N;
+  // several tokens' rows beyond a product's go two products a read of the cache
+  p.tile = c.N > 1 && rows > kRowsMfma ? 2 * kRowsMfma : kRowsMfma;
+  p.head_tiles = (rows + p.tile - 1) / p.tile;
+  p.rows = rows <= 4 ? 4 : p.tile;
   const long slices = (long)c.Hkv * p.head_tiles;
-  const long cap = ((long)c.W * c.page + step - 1) / step;
+  const long cap = ((long)c.W * c.page + kPagedStep - 1) / kPagedStep;
   p.whole = cap <= 16;
+  const long most = fmt == kPagedE2m1 && p.tile == kRowsMfma ? 768 : 512;
   p.wgs = (int)(p.whole ? std::max(c.B, 1)
-                        : std::max(1L, std::min({512 / slices, (c.B * cap + 3) / 4, (long)kPagedMaxWgs})));
+                        : std::max(1L, std::min({most / slices, (c.B * cap + 3) / 4, (long)kPagedMaxWgs})));
   return p;
 }
+
+// Several tokens of sequences that have eight partials each or so at most: a launch of
+// a thousand workgroups less takes a microsecond less.
+bool paged_join_few(const PagedCacheDims& c, const PagedSplit& p) { return c.N > 1 && p.wgs <= 8 * c.B; }
 
 size_t paged_part_floats(const PagedCacheDims& c, const PagedSplit& p, int hd) {
   return p.whole ? 0 : (size_t)c.Hkv * p.head_tiles * p.wgs * 2 * p.rows * hd;
 }
 
 // partials, their (maximum, sum), and each sequence's first step with the number of all behind the last
+size_t paged_joined_bytes(const PagedCacheDims& c, const PagedSplit& p, int hd) {
+  const size_t n = paged_part_floats(c, p, hd);
+  return n == 0 ? 0 : n * 4 + n / hd * 8 + (((size_t)c.B + 1) * 4 + 15) / 16 * 16;
+}
+
+// and where they are outside LDS, the partials that end within a wave's range
 size_t paged_ws_bytes(const PagedCacheDims& c, int hd, PagedFormat fmt) {
-  const size_t n = paged_part_floats(c, paged_split(c, fmt), hd);
-  return n == 0 ? 0 : n * 4 + n / hd * 8 + ((size_t)c.B + 1) * 4;
+  const PagedSplit p = paged_split(c, fmt);
+  return paged_joined_bytes(c, p, hd) + (ends_outside(fmt, p.rows) ? paged_part_floats(c, p, hd) * 2 * 4 : 0);
 }
 
 namespace {
@@ -749,28 +846,36 @@ hipError_t launch_paged_attn(const PagedCacheDims& c, int hd, PagedFormat fmt, c
   const size_t n = paged_part_floats(c, p, hd);
   float2* stat = (float2*)(part + n);
   int* starts = (int*)(stat + n / hd);
+  float* ended = (float*)((char*)ws + paged_joined_bytes(c, p, hd));
   auto run = [&](auto kernel) {
     NAYLIS_TIMED("paged_attn", st,
                  hipLaunchKernelGGL(kernel, dim3(p.wgs, c.Hkv * p.head_tiles), dim3(256), 0, st, c, q, table, lens,
-                                    (bf16_t*)out, part, stat, starts, p, scale * kLog2e));
+                                    (bf16_t*)out, part, stat, starts, ended, p, scale * kLog2e));
   };
   with_format(hd, fmt, [&](auto d, auto f) {
     constexpr int HD = decltype(d)::value;
     constexpr PagedFormat F = decltype(f)::value;
     if (c.N > 1 || q.live)
-      p.rows == 4 ? run(paged_attn_kernel<HD, F, 4, true>) : run(paged_attn_kernel<HD, F, 16, true>);
+      p.rows == 4    ? run(paged_attn_kernel<HD, F, 4, true>)
+      : p.rows == 16 ? run(paged_attn_kernel<HD, F, 16, true>)
+                     : run(paged_attn_kernel<HD, F, 32, true>);
     else
       p.rows == 4 ? run(paged_attn_kernel<HD, F, 4, false>) : run(paged_attn_kernel<HD, F, 16, false>);
   });
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || p.whole || p.wgs == 1) return e;
-  with_format(hd, fmt, [&](auto d, auto f) {
-    constexpr int HD = decltype(d)::value, STEP = paged_step(decltype(f)::value);
+  auto join = [&](auto kernel, dim3 grid) {
     NAYLIS_TIMED("paged_join", st,
-                 hipLaunchKernelGGL((paged_join_kernel<HD, STEP>), dim3(c.Hkv * c.G * c.N, c.B), dim3(256), 0, st, c,
-                                    q.live, lens, (bf16_t*)out, (const float*)part, (const float2*)stat,
-                                    (const int*)starts, p));
-  });
+                 hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, c, q.live, lens, (bf16_t*)out, (const float*)part,
+                                    (const float2*)stat, (const int*)starts, p));
+  };
+  if (paged_join_few(c, p)) {
+    const dim3 grid((c.G * c.N * hd + 1023) / 1024, c.Hkv, c.B);
+    hd == 64 ? join(paged_join_few_kernel<64>, grid) : join(paged_join_few_kernel<128>, grid);
+  } else {
+    const dim3 grid(c.Hkv * c.G * c.N, c.B);
+    hd == 64 ? join(paged_join_kernel<64>, grid) : join(paged_join_kernel<128>, grid);
+  }
   return hipGetLastError();
 }
 
