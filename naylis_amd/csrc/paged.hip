@@ -485,7 +485,7 @@ __global__ __launch_bounds__(256, FMT == kPagedE2m1 && ROWS <= kRowsMfma ? 3 : 2
 #pragma unroll
         for (int i = 0; i < NS; ++i)
 #pragma unroll
-          for (int v = 0; v < 4; ++v) x[u][i][v] *= FP8 ? kss[i][v] : sc;
+          for (int v = 0; v < 4; ++v) x[u][i][v] = mul_rn(x[u][i][v], FP8 ? kss[i][v] : sc);
         if (__builtin_expect(tail, 0))
 #pragma unroll
           for (int i = 0; i < NS; ++i)
@@ -501,7 +501,6 @@ __global__ __launch_bounds__(256, FMT == kPagedE2m1 && ROWS <= kRowsMfma ? 3 : 2
         const float mn = fmaxf(m[u], mx), al = __builtin_amdgcn_exp2f(m[u] - mn);
         // (times 1 where no row has a new maximum)
         if (__any(mn > m[u])) {
-          l[u] *= al;
 #pragma unroll
           for (int t = 0; t < NT; ++t) acc[u][t] *= al;
         }
@@ -511,7 +510,7 @@ __global__ __launch_bounds__(256, FMT == kPagedE2m1 && ROWS <= kRowsMfma ? 3 : 2
 #pragma unroll
           for (int v = 0; v < 4; ++v) {
             x[u][i][v] = __builtin_amdgcn_exp2f(x[u][i][v] - mn);
-            l[u] += x[u][i][v];
+            l[u] = i + v ? l[u] + x[u][i][v] : __builtin_fmaf(l[u], al, x[u][i][v]);
             if constexpr (FP8) x[u][i][v] *= vss[i][v];
           }
         // rows past the end: their weight is 0, their scale may be anything
