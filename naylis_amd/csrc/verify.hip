@@ -282,23 +282,48 @@ struct RowStat {
   double sum, draft;  // with the draft's weight, and that
 };
 
+// What a row's decision reads, all of it under way at once: 128 parts, the draft and
+// what depends on it.
+struct RowIn {
+  VerifyStat first[2];
+  long draft;
+  float x, q, u;
+  bool some;
+};
 template <typename T>
-__device__ __forceinline__ RowStat join_row(const VerifyArgs& a, const VerifyStat* s, const T* row, long draft,
-                                            double scale) {
+__device__ __forceinline__ RowIn read_row(const VerifyArgs& a, const T* logits, const VerifyStat* stat, int b, int i) {
   const int lane = threadIdx.x & 63;
-  const bool some = draft >= 0 && draft < a.V;
-  const float x = some ? load1(row + draft) : 0.f;
-  float top = -INFINITY;
-  for (int p = lane; p < a.parts; p += 64) top = fmaxf(top, s[p].top);
+  const long at = (long)b * (a.N + 1) + i;
+  RowIn r;
+  r.draft = i < a.N ? a.drafts[(long)b * a.N + i] : -1;
+#pragma unroll
+  for (int v = 0; v < 2; ++v) r.first[v] = stat[at * a.parts + min(lane + 64 * v, a.parts - 1)];
+  r.u = a.uniforms[at];
+  r.some = r.draft >= 0 && r.draft < a.V;
+  r.x = r.some ? load1(logits + b * a.ldb + i * a.ldt + r.draft) : -INFINITY;
+  r.q = 1.f;
+  if (r.some && a.probs) {
+    const long j = b * a.lqb + i * a.lqt + r.draft;
+    r.q = a.probs_bf16 ? bf16_to_f32(((const bf16_t*)a.probs)[j]) : ((const float*)a.probs)[j];
+  }
+  return r;
+}
+__device__ __forceinline__ RowStat join_row(const VerifyArgs& a, const VerifyStat* s, const RowIn& r, double scale,
+                                            bool drafted) {
+  const int lane = threadIdx.x & 63;
+  float top = fmaxf(r.first[0].top, r.first[1].top);  // (a part twice where there are few)
+  for (int p = lane + 128; p < a.parts; p += 64) top = fmaxf(top, s[p].top);
   top = wave_allmax(top);
   int at = 0x7fffffff;
   double sum = 0.0;
-  for (int p = lane; p < a.parts; p += 64) {
-    const VerifyStat v = s[p];
+  const auto add = [&](const VerifyStat& v) {
     if (v.top == top) at = min(at, v.at);
     sum += v.sum * weight(v.top, top, scale);  // (0 for a part of -inf)
-  }
-  const double d = some && x > -INFINITY ? weight(x, top, scale) : 0.0;
+  };
+  if (lane < a.parts) add(r.first[0]);
+  if (lane + 64 < a.parts) add(r.first[1]);
+  for (int p = lane + 128; p < a.parts; p += 64) add(s[p]);
+  const double d = drafted && r.x > -INFINITY ? weight(r.x, top, scale) : 0.0;
   return RowStat{top, wave_allmin_i32(at), wave_sum(sum) + d, d};
 }
 
@@ -310,40 +335,42 @@ struct Decision {
   RowStat row;
 };
 
-// By a whole workgroup: rows 0 .. n, a wave each.
+// By a whole workgroup: rows 0 .. n, two for each wave at a time.
 template <typename T>
 __device__ __forceinline__ Decision decide(const VerifyArgs& a, const T* logits, const VerifyStat* stat, int b) {
   __shared__ int first;
   __shared__ RowStat rows[kRows];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  // (rows behind the drafts are read here too, and do not count)
+  RowIn in[2];
+#pragma unroll
+  for (int v = 0; v < 2; ++v) in[v] = read_row(a, logits, stat, b, min(wave + kWaves * v, a.N));
   const int n = verify_drafts_of(a, b);
   const float t = verify_temperature(a, b);
   const double scale = scale_of(t);
   if (tid == 0) first = n;
   __syncthreads();
-  const auto join = [&](int i) {
-    const long d = i < n ? a.drafts[(long)b * a.N + i] : -1;
-    return join_row(a, stat + ((long)b * (a.N + 1) + i) * a.parts, logits + b * a.ldb + i * a.ldt, d, scale);
-  };
-  for (int i = wave; i <= n; i += kWaves) {
-    const long d = i < n ? a.drafts[(long)b * a.N + i] : -1;
-    const bool some = d >= 0 && d < a.V;
-    double q = 1.0;
-    if (some && a.probs) {
-      const long at = b * a.lqb + i * a.lqt + d;
-      q = a.probs_bf16 ? bf16_to_f32(((const bf16_t*)a.probs)[at]) : ((const float*)a.probs)[at];
-    }
-    const double u = a.uniforms[(long)b * (a.N + 1) + i];
-    const RowStat r = join(i);
-    const double p = t > 0.f ? r.draft / r.sum : r.sum > 0.0 && r.at == d ? 1.0 : 0.0;
+  const auto stat_of = [&](int i) { return stat + ((long)b * (a.N + 1) + i) * a.parts; };
+  const auto judge = [&](int i, const RowIn& r) {
+    if (i > n) return;
+    const RowStat s = join_row(a, stat_of(i), r, scale, i < n);
+    const double p = t > 0.f ? s.draft / s.sum : s.sum > 0.0 && s.at == r.draft ? 1.0 : 0.0;
     if (lane == 0) {
-      if (i < n && !(some && u * q < p)) atomicMin(&first, i);
-      if (i < kRows) rows[i] = r;
+      if (i < n && !(r.some && (double)r.u * (double)r.q < p)) atomicMin(&first, i);
+      if (i < kRows) rows[i] = s;
     }
-  }
+  };
+  judge(wave, in[0]);
+  judge(wave + kWaves, in[1]);
+  for (int i = wave + 2 * kWaves; i <= n; i += kWaves) judge(i, read_row(a, logits, stat, b, i));
   __syncthreads();
   const int kept = first;
-  return Decision{kept, n, t, kept < n ? a.drafts[(long)b * a.N + kept] : -1, kept < kRows ? rows[kept] : join(kept)};
+  RowStat row;
+  if (kept < kRows)
+    row = rows[kept];
+  else
+    row = join_row(a, stat_of(kept), read_row(a, logits, stat, b, kept), scale, kept < n);
+  return Decision{kept, n, t, kept < n ? a.drafts[(long)b * a.N + kept] : -1, row};
 }
 
 // The row behind the kept drafts, and what is taken from its weights.
@@ -432,7 +459,7 @@ __global__ __launch_bounds__(kThreads) void verify_pick_kernel(VerifyArgs a, con
                                                                const VerifyLeft* __restrict__ left,
                                                                const Decision* __restrict__ decisions) {
   static_assert(kPart == 8 * kThreads, "a piece a thread");
-  __shared__ int found, last;
+  __shared__ int found[kWaves], last[kWaves];
   __shared__ double sums[kWaves];
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const double u = a.uniforms[(long)b * (a.N + 1) + a.N];
@@ -441,10 +468,6 @@ __global__ __launch_bounds__(kThreads) void verify_pick_kernel(VerifyArgs a, con
     d = decisions[b];
   else
     d = decide(a, logits, stat, b);
-  if (tid == 0) {
-    found = 0x7fffffff;
-    last = -1;
-  }
   const bool some = d.row.sum > 0.0;  // (not NaN)
   long token = -1;
   if (!(d.t > 0.f)) {
@@ -526,10 +549,21 @@ __global__ __launch_bounds__(kThreads) void verify_pick_kernel(VerifyArgs a, con
         if (at > target && hit == 0x7fffffff) hit = j0 + e;
       }
     }
-    if (hit != 0x7fffffff) atomicMin(&found, hit);
-    if (mine >= 0) atomicMax(&last, mine);
+    const unsigned long long hits = __ballot(hit != 0x7fffffff), some_here = __ballot(mine >= 0);
+    if (lane == 0) {
+      found[wave] = 0x7fffffff;
+      last[wave] = -1;
+    }
+    if (hits && lane == __ffsll(hits) - 1) found[wave] = hit;
+    if (some_here && lane == 63 - __clzll(some_here)) last[wave] = mine;
     __syncthreads();
-    token = found != 0x7fffffff ? found : last;
+    int from = 0x7fffffff, to = -1;
+#pragma unroll
+    for (int v = 0; v < kWaves; ++v) {
+      from = min(from, found[v]);
+      to = max(to, last[v]);
+    }
+    token = from != 0x7fffffff ? from : to;
   }
   for (int i = tid; i <= a.N; i += kThreads)
     a.tokens[(long)b * (a.N + 1) + i] = i < d.kept ? a.drafts[(long)b * a.N + i] : i == d.kept ? token : -1;
