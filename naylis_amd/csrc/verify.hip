@@ -37,9 +37,9 @@ namespace naylis {
 namespace {
 
 constexpr int kThreads = 256, kWaves = kThreads / 64;
-constexpr int kPart = 2048;          // logits of a part
-constexpr int kPieces = kPart / 512; // of eight logits a lane
-constexpr int kRows = 16;            // rows whose joined sums a workgroup keeps
+constexpr int kPiece = 512;          // logits of a wave at a time, eight a lane
+constexpr int kPieces = 4;           // pieces of a part: PIECES 4, or 1 where one workgroup does it all
+constexpr int kSmallParts = 128, kSmallWaves = 16;  // the workgroup that does it all
 constexpr double kNothing = 0x1p-900;  // weights up to this are none: those of -inf count as 2^-1000
 
 // what the first launch leaves of a part of a row
@@ -105,28 +105,37 @@ struct Raw8<float> {
   __device__ __forceinline__ void set(int e, float x) { f[e >> 2][e & 3] = x; }
 };
 
+// Numbers j0 .. j0 + 7 of a row one by one, `none` outside [0, V).
+template <typename T>
+__device__ __forceinline__ Raw8<T> ends8(const T* row, int j0, int V, float none) {
+  Raw8<T> x = {};
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float y = load1(row + min(max(j0 + e, 0), V - 1));
+    x.set(e, j0 + e >= 0 && j0 + e < V ? y : none);
+  }
+  return x;
+}
+
 // Logits j0 .. j0 + 7 of a row, where j0 + shift_of(row) is a multiple of 8: the
 // row's 16-byte pieces of memory; -inf outside [0, V).
 template <typename T>
 __device__ __forceinline__ Raw8<T> load8(const T* row, int j0, int V) {
   if (j0 >= 0 && j0 + 8 <= V) return *reinterpret_cast<const Raw8<T>*>(row + j0);
-  Raw8<T> x = {};
-#pragma unroll
-  for (int e = 0; e < 8; ++e) x.set(e, j0 + e >= 0 && j0 + e < V ? load1(row + j0 + e) : -INFINITY);
-  return x;
+  return ends8(row, j0, V, -INFINITY);
 }
 
 // A wave's share of a part: eight a lane from `first` on, for each of its pieces.
 // Only a row's first and last part look at their ends.
-template <typename T>
-__device__ __forceinline__ void load_part(const T* row, int first, int V, Raw8<T> (&x)[kPieces]) {
+template <int PIECES, typename T>
+__device__ __forceinline__ void load_part(const T* row, int first, int V, Raw8<T> (&x)[PIECES]) {
   const int j0 = first + 8 * (int)(threadIdx.x & 63);
-  if (first >= 0 && first + kPart <= V) {
+  if (first >= 0 && first + PIECES * kPiece <= V) {
 #pragma unroll
-    for (int c = 0; c < kPieces; ++c) x[c] = *reinterpret_cast<const Raw8<T>*>(row + j0 + 512 * c);
+    for (int c = 0; c < PIECES; ++c) x[c] = *reinterpret_cast<const Raw8<T>*>(row + j0 + 512 * c);
   } else {
 #pragma unroll
-    for (int c = 0; c < kPieces; ++c) x[c] = load8(row, j0 + 512 * c, V);
+    for (int c = 0; c < PIECES; ++c) x[c] = load8(row, j0 + 512 * c, V);
   }
 }
 
@@ -145,14 +154,32 @@ template <typename T>
 __device__ __forceinline__ Raw8<T> any8(const T* p) {
   return reinterpret_cast<const Any8<T>*>(p)->x;
 }
-template <typename T>
-__device__ __forceinline__ Raw8<T> load_any8(const T* row, int j0, int V) {
-  if (j0 >= 0 && j0 + 8 <= V) return any8(row + j0);
-  Raw8<T> x = {};
+
+// q, in either type, eight at a time; 0 outside [0, V) and without q.
+struct Q8 {
+  Raw8<float> f;
+  __device__ __forceinline__ Q8(const void* probs, bool bf16, int j0, int V) : f{} {
+    if (!probs) return;
+    const bool inside = j0 >= 0 && j0 + 8 <= V;
+    if (bf16) {
+      const bf16_t* p = (const bf16_t*)probs;
+      const Raw8<bf16_t> h = inside ? any8(p + j0) : ends8(p, j0, V, 0.f);
+      f.f[0] = __builtin_bit_cast(f32x4, h.u);
+      half = true;
+    } else {
+      const float* p = (const float*)probs;
+      f = inside ? any8(p + j0) : ends8(p, j0, V, 0.f);
+    }
+  }
+  // (converted where it is used: the load stays under way until then)
+  __device__ __forceinline__ void widen() {
+    if (!half) return;
+    const Raw8<bf16_t> h{__builtin_bit_cast(u32x4, f.f[0])};
 #pragma unroll
-  for (int e = 0; e < 8; ++e) x.set(e, j0 + e >= 0 && j0 + e < V ? load1(row + j0 + e) : 0.f);
-  return x;
-}
+    for (int e = 0; e < 8; ++e) f.set(e, h[e]);
+  }
+  bool half = false;
+};
 
 // elements between the last 16-byte boundary and the row's first
 template <typename T>
@@ -195,17 +222,15 @@ __device__ __forceinline__ int verify_drafts_of(const VerifyArgs& a, int b) {
 }
 __device__ __forceinline__ float verify_temperature(const VerifyArgs& a, int b) { return a.temps ? a.temps[b] : a.temp; }
 
-// grid (parts / 4, N + 1, B), a part for each wave.  EXACT: sums in fp64.
-template <typename T, bool EXACT>
-__global__ __launch_bounds__(kThreads, EXACT || sizeof(T) == 4 ? 1 : 8) void verify_stat_kernel(VerifyArgs a, const T* __restrict__ logits,
-                                                               VerifyStat* __restrict__ stat) {
-  const int i = blockIdx.y, b = blockIdx.z, lane = threadIdx.x & 63;
-  const int part = blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int n = verify_drafts_of(a, b);
-  if (i > n || part >= a.parts) return;
+namespace {
+
+// A part of row i of sequence b, by a wave.  EXACT: sums in fp64.
+template <int PIECES, bool EXACT, typename T>
+__device__ __forceinline__ VerifyStat stat_part(const VerifyArgs& a, const T* logits, int b, int i, int n, int part) {
+  const int lane = threadIdx.x & 63;
   const T* row = logits + b * a.ldb + i * a.ldt;
-  const int first = part * kPart - shift_of(row), j0 = first + 8 * lane;
-  Raw8<T> x[kPieces];
+  const int first = part * PIECES * kPiece - shift_of(row), j0 = first + 8 * lane;
+  Raw8<T> x[PIECES];
   load_part(row, first, a.V, x);
   const float t = verify_temperature(a, b);
   const double scale = scale_of(t);
@@ -213,7 +238,7 @@ __global__ __launch_bounds__(kThreads, EXACT || sizeof(T) == 4 ? 1 : 8) void ver
   float top = -INFINITY;
   bool nan = false;
 #pragma unroll
-  for (int c = 0; c < kPieces; ++c)
+  for (int c = 0; c < PIECES; ++c)
 #pragma unroll
     for (int e = 0; e < 8; e += 2) {
       top = max3(top, x[c][e], x[c][e + 1]);
@@ -224,14 +249,14 @@ __global__ __launch_bounds__(kThreads, EXACT || sizeof(T) == 4 ? 1 : 8) void ver
   int at = 0x7fffffff;
   if (!(t > 0.f) && own == top)
 #pragma unroll
-    for (int c = kPieces - 1; c >= 0; --c)
+    for (int c = PIECES - 1; c >= 0; --c)
 #pragma unroll
       for (int e = 7; e >= 0; --e)
         if (x[c][e] == top) at = j0 + 512 * c + e;
   // the draft's own weight stays out: what is left without it is exact however small
-  if (draft >= first && draft < first + kPart) {
+  if (draft >= first && draft < first + PIECES * kPiece) {
 #pragma unroll
-    for (int c = 0; c < kPieces; ++c)
+    for (int c = 0; c < PIECES; ++c)
 #pragma unroll
       for (int e = 0; e < 8; ++e)
         if (j0 + 512 * c + e == (int)draft) {
@@ -244,36 +269,38 @@ __global__ __launch_bounds__(kThreads, EXACT || sizeof(T) == 4 ? 1 : 8) void ver
   double s = 0.0;
   if (!(top == -INFINITY)) {
     if constexpr (EXACT) {
+      // (a loop in code too, here and below: what runs once a wave waits for its
+      // instructions longer than for its numbers)
+#pragma unroll 1
+      for (int c = 0; c < PIECES; ++c) {
 #pragma unroll
-      for (int c = 0; c < kPieces; ++c)
+        for (int e = 0; e < 8; ++e) s += weight(x[0][e], top, scale);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) s += weight(x[c][e], top, scale);
+        for (int k = 1; k < PIECES; ++k) x[k - 1] = x[k];
+      }
     } else {
       const float fs = (float)scale;
-      float sums[kPieces] = {};
+      float sums[PIECES] = {};
 #pragma unroll
-      for (int c = 0; c < kPieces; ++c)
+      for (int c = 0; c < PIECES; ++c)
 #pragma unroll
         for (int e = 0; e < 8; ++e) sums[c] += __builtin_amdgcn_exp2f((x[c][e] - top) * fs);
 #pragma unroll
-      for (int c = 0; c < kPieces; ++c) s += sums[c];
+      for (int c = 0; c < PIECES; ++c) s += sums[c];
     }
   }
   if constexpr (!EXACT) {
     if (top == -INFINITY) {  // of nothing but -inf and NaNs
 #pragma unroll
-      for (int c = 0; c < kPieces; ++c)
+      for (int c = 0; c < PIECES; ++c)
 #pragma unroll
         for (int e = 0; e < 8; e += 2) nan |= __builtin_isunordered(x[c][e], x[c][e + 1]);
     }
   }
   if (__any(nan) || top == INFINITY) s = __builtin_nan("");
   if (!(t > 0.f)) at = wave_allmin_i32(at);
-  s = wave_sum(s);
-  if (lane == 0) stat[((long)b * (a.N + 1) + i) * a.parts + part] = VerifyStat{top, at, s};
+  return VerifyStat{top, at, wave_sum(s)};
 }
-
-namespace {
 
 // a row's parts joined: every lane of the wave gets it
 struct RowStat {
@@ -282,23 +309,21 @@ struct RowStat {
   double sum, draft;  // with the draft's weight, and that
 };
 
-// What a row's decision reads, all of it under way at once: 128 parts, the draft and
+// What a row's decision reads, all of it under way at once: 64 parts, the draft and
 // what depends on it.
 struct RowIn {
-  VerifyStat first[2];
+  VerifyStat first;
   long draft;
   float x, q, u;
   bool some;
 };
 template <typename T>
-__device__ __forceinline__ RowIn read_row(const VerifyArgs& a, const T* logits, const VerifyStat* stat, int b, int i) {
+__device__ __forceinline__ RowIn read_row(const VerifyArgs& a, const T* logits, const VerifyStat* s, int b, int i) {
   const int lane = threadIdx.x & 63;
-  const long at = (long)b * (a.N + 1) + i;
   RowIn r;
   r.draft = i < a.N ? a.drafts[(long)b * a.N + i] : -1;
-#pragma unroll
-  for (int v = 0; v < 2; ++v) r.first[v] = stat[at * a.parts + min(lane + 64 * v, a.parts - 1)];
-  r.u = a.uniforms[at];
+  r.first = s[(long)i * a.parts + min(lane, a.parts - 1)];
+  r.u = a.uniforms[(long)b * (a.N + 1) + i];
   r.some = r.draft >= 0 && r.draft < a.V;
   r.x = r.some ? load1(logits + b * a.ldb + i * a.ldt + r.draft) : -INFINITY;
   r.q = 1.f;
@@ -311,18 +336,16 @@ __device__ __forceinline__ RowIn read_row(const VerifyArgs& a, const T* logits, 
 __device__ __forceinline__ RowStat join_row(const VerifyArgs& a, const VerifyStat* s, const RowIn& r, double scale,
                                             bool drafted) {
   const int lane = threadIdx.x & 63;
-  float top = fmaxf(r.first[0].top, r.first[1].top);  // (a part twice where there are few)
-  for (int p = lane + 128; p < a.parts; p += 64) top = fmaxf(top, s[p].top);
+  float top = r.first.top;  // (a part twice where there are few)
+  for (int p = lane + 64; p < a.parts; p += 64) top = fmaxf(top, s[p].top);
   top = wave_allmax(top);
   int at = 0x7fffffff;
   double sum = 0.0;
-  const auto add = [&](const VerifyStat& v) {
+  for (int p = lane; p < a.parts; p += 64) {
+    const VerifyStat v = p < 64 ? r.first : s[p];
     if (v.top == top) at = min(at, v.at);
     sum += v.sum * weight(v.top, top, scale);  // (0 for a part of -inf)
-  };
-  if (lane < a.parts) add(r.first[0]);
-  if (lane + 64 < a.parts) add(r.first[1]);
-  for (int p = lane + 128; p < a.parts; p += 64) add(s[p]);
+  }
   const double d = drafted && r.x > -INFINITY ? weight(r.x, top, scale) : 0.0;
   return RowStat{top, wave_allmin_i32(at), wave_sum(sum) + d, d};
 }
@@ -335,42 +358,44 @@ struct Decision {
   RowStat row;
 };
 
-// By a whole workgroup: rows 0 .. n, two for each wave at a time.
-template <typename T>
-__device__ __forceinline__ Decision decide(const VerifyArgs& a, const T* logits, const VerifyStat* stat, int b) {
-  __shared__ int first;
-  __shared__ RowStat rows[kRows];
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+// By a workgroup of WAVES, each of which takes every WAVES-th row up to the first
+// that keeps no draft.  s: the sequence's parts.
+template <int WAVES, typename T>
+__device__ __forceinline__ Decision decide(const VerifyArgs& a, const T* logits, const VerifyStat* s, int b) {
+  __shared__ int ends[WAVES];
+  __shared__ RowStat rows[WAVES];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // (rows behind the drafts are read here too, and do not count)
-  RowIn in[2];
-#pragma unroll
-  for (int v = 0; v < 2; ++v) in[v] = read_row(a, logits, stat, b, min(wave + kWaves * v, a.N));
+  RowIn r = read_row(a, logits, s, b, min(wave, a.N));
   const int n = verify_drafts_of(a, b);
   const float t = verify_temperature(a, b);
   const double scale = scale_of(t);
-  if (tid == 0) first = n;
-  __syncthreads();
-  const auto stat_of = [&](int i) { return stat + ((long)b * (a.N + 1) + i) * a.parts; };
-  const auto judge = [&](int i, const RowIn& r) {
-    if (i > n) return;
-    const RowStat s = join_row(a, stat_of(i), r, scale, i < n);
-    const double p = t > 0.f ? s.draft / s.sum : s.sum > 0.0 && s.at == r.draft ? 1.0 : 0.0;
-    if (lane == 0) {
-      if (i < n && !(r.some && (double)r.u * (double)r.q < p)) atomicMin(&first, i);
-      if (i < kRows) rows[i] = s;
+  int end = 0x7fffffff;
+  RowStat row = {};
+#pragma unroll 1
+  for (int i = wave; i <= n; i += WAVES) {
+    const RowIn next = read_row(a, logits, s, b, min(i + WAVES, a.N));
+    row = join_row(a, s + (long)i * a.parts, r, scale, i < n);
+    const bool likely = t > 0.f ? (double)r.u * (double)r.q * row.sum < row.draft
+                                : row.sum > 0.0 && row.at == r.draft && (double)r.u * (double)r.q < 1.0;
+    if (!(i < n && r.some && likely)) {
+      end = i;
+      break;
     }
-  };
-  judge(wave, in[0]);
-  judge(wave + kWaves, in[1]);
-  for (int i = wave + 2 * kWaves; i <= n; i += kWaves) judge(i, read_row(a, logits, stat, b, i));
+    r = next;
+  }
+  if ((threadIdx.x & 63) == 0) {
+    ends[wave] = end;
+    rows[wave] = row;
+  }
   __syncthreads();
-  const int kept = first;
-  RowStat row;
-  if (kept < kRows)
-    row = rows[kept];
-  else
-    row = join_row(a, stat_of(kept), read_row(a, logits, stat, b, kept), scale, kept < n);
-  return Decision{kept, n, t, kept < n ? a.drafts[(long)b * a.N + kept] : -1, row};
+  int kept = ends[0], of = 0;
+#pragma unroll
+  for (int v = 1; v < WAVES; ++v) {
+    of = ends[v] < kept ? v : of;
+    kept = min(kept, ends[v]);
+  }
+  return Decision{kept, n, t, kept < n ? a.drafts[(long)b * a.N + kept] : -1, rows[of]};
 }
 
 // The row behind the kept drafts, and what is taken from its weights.
@@ -394,150 +419,117 @@ struct Behind {
   __device__ __forceinline__ double operator()(float x) const { return weight(x, top, scale); }
 };
 
-}  // namespace
-
-// grid (parts / 4, B): the drafts kept, and the fp64 sums over the row behind them.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void verify_left_kernel(VerifyArgs a, const T* __restrict__ logits,
-                                                               const VerifyStat* __restrict__ stat,
-                                                               VerifyLeft* __restrict__ left,
-                                                               Decision* __restrict__ decisions) {
-  const int b = blockIdx.y, lane = threadIdx.x & 63;
-  const int part = blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const Decision d = decide(a, logits, stat, b);
-  if (part == 0 && lane == 0) decisions[b] = d;
-  if (!(d.t > 0.f) || !(d.row.sum > 0.0) || part >= a.parts) return;
+// The fp64 sums over a part of the row behind the kept drafts, by a wave.
+template <int PIECES, typename T>
+__device__ __forceinline__ VerifyLeft left_part(const VerifyArgs& a, const T* logits, int b, const Decision& d,
+                                                int part) {
+  const int lane = threadIdx.x & 63;
   const Behind<T> r(a, logits, b, d);
-  const int first = part * kPart - shift_of(r.row), j0 = first + 8 * lane;
+  const int j0 = part * PIECES * kPiece - shift_of(r.row) + 8 * lane;
   double sum = 0.0, over = 0.0;
   float qs = 0.f;
-  Raw8<T> x[kPieces];
-  load_part(r.row, first, a.V, x);
-  const auto with = [&](const auto* probs) {
-    Raw8<std::remove_const_t<std::remove_reference_t<decltype(*probs)>>> q[kPieces];
-    if (first >= 0 && first + kPart <= a.V) {
+  Raw8<T> x = r.logits(j0);
+  Q8 q(r.probs, a.probs_bf16, j0, a.V);
+#pragma unroll 1
+  for (int c = 0; c < PIECES; ++c) {
+    const int j = j0 + kPiece * c;
+    const bool more = c + 1 < PIECES;
+    const Raw8<T> nx = more ? r.logits(j + kPiece) : x;
+    const Q8 nq = more ? Q8(r.probs, a.probs_bf16, j + kPiece, a.V) : q;
+    if (!r.probs && r.gone >= j && r.gone < j + 8)
 #pragma unroll
-      for (int c = 0; c < kPieces; ++c) q[c] = any8(probs + j0 + 512 * c);
-    } else {
+      for (int e = 0; e < 8; ++e)
+        if (j + e == (int)r.gone) x.set(e, -INFINITY);
+    q.widen();
 #pragma unroll
-      for (int c = 0; c < kPieces; ++c) q[c] = load_any8(probs, j0 + 512 * c, a.V);
+    for (int e = 0; e < 8; ++e) {
+      const double w = r(x[e]), m = __builtin_fma(-d.row.sum, (double)q.f[e], w);
+      sum += w;
+      over += fmax(m, 0.0);
+      qs += m > 0.0 ? q.f[e] : 0.f;
     }
-#pragma unroll
-    for (int c = 0; c < kPieces; ++c)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const double w = r(x[c][e]), m = __builtin_fma(-d.row.sum, (double)q[c][e], w);
-        sum += w;
-        over += fmax(m, 0.0);
-        qs += m > 0.0 ? q[c][e] : 0.f;
-      }
-  };
-  if (!r.probs) {
-#pragma unroll
-    for (int c = 0; c < kPieces; ++c)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) sum += j0 + 512 * c + e == r.gone ? 0.0 : r(x[c][e]);
-  } else if (a.probs_bf16) {
-    with((const bf16_t*)r.probs);
-  } else {
-    with((const float*)r.probs);
+    x = nx;
+    q = nq;
   }
-  sum = wave_sum(sum);
-  if (r.probs) {
-    over = wave_sum(over);
-    qs = wave_allsum(qs);
-  }
-  if (lane == 0) left[(long)b * a.parts + part] = VerifyLeft{sum, over, qs};
+  return VerifyLeft{wave_sum(sum), wave_sum(over), wave_allsum(qs)};
 }
 
-// grid (B), eight logits of a part for each thread: the part that the random
-// number falls in, the token in it, and the sequence's results.  DECIDED: from the
-// second launch's sums, else from the first's.
-template <typename T, bool DECIDED>
-__global__ __launch_bounds__(kThreads) void verify_pick_kernel(VerifyArgs a, const T* __restrict__ logits,
-                                                               const VerifyStat* __restrict__ stat,
-                                                               const VerifyLeft* __restrict__ left,
-                                                               const Decision* __restrict__ decisions) {
-  static_assert(kPart == 8 * kThreads, "a piece a thread");
-  __shared__ int found[kWaves], last[kWaves];
-  __shared__ double sums[kWaves];
-  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+// The token behind the kept drafts of a row with a distribution, by a workgroup:
+// the part that the random number falls in, and the token in it, a piece for each of
+// the first PIECES waves.  LEFT: from the fp64 sums of left_part (l), else
+// from those of the first launch (s).
+template <bool LEFT, int PIECES, typename T>
+__device__ __forceinline__ long pick(const VerifyArgs& a, const T* logits, int b, const Decision& d,
+                                     const VerifyStat* s, const VerifyLeft* l) {
+  __shared__ int found[PIECES], last[PIECES];
+  __shared__ double sums[PIECES];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const double u = a.uniforms[(long)b * (a.N + 1) + a.N];
-  Decision d;
-  if constexpr (DECIDED)
-    d = decisions[b];
-  else
-    d = decide(a, logits, stat, b);
-  const bool some = d.row.sum > 0.0;  // (not NaN)
-  long token = -1;
-  if (!(d.t > 0.f)) {
-    // what is left of a weight that is all on one token is on it too
-    if (some) token = d.row.at;
-  } else if (some) {
-    const VerifyStat* s = stat + ((long)b * (a.N + 1) + d.kept) * a.parts;
-    const VerifyLeft* l = left + (long)b * a.parts;
-    const Behind<T> r(a, logits, b, d);
-    const int shift = shift_of(r.row), gone_part = r.gone >= 0 && r.gone < a.V ? (int)((r.gone + shift) / kPart) : -1;
-    double S = 0.0;  // over the whole row, of the e that q is taken from
-    if (r.probs) {
-      for (int p = lane; p < a.parts; p += 64) S += l[p].sum;
-      S = wave_sum(S);
+  const Behind<T> r(a, logits, b, d);
+  const int shift = shift_of(r.row), gone_part = r.gone >= 0 && r.gone < a.V ? (int)((r.gone + shift) / (PIECES * kPiece)) : -1;
+  double S = 0.0;  // over the whole row, of the e that q is taken from
+  if (r.probs) {
+    for (int p = lane; p < a.parts; p += 64) S += l[p].sum;
+    S = wave_sum(S);
+  }
+  // weight of a part: of what is left of p (less), or of p where that is nothing
+  const auto part_weight = [&](int p, bool less) {
+    if (less && r.probs) return fmax(l[p].over + (d.row.sum - S) * l[p].q, 0.0);
+    double w;
+    if constexpr (LEFT)
+      w = l[p].sum;
+    else
+      w = s[p].sum * weight(s[p].top, d.row.top, r.scale);
+    return !less && !r.probs && p == gone_part ? w + d.row.draft : w;
+  };
+  const auto sum_of = [&](bool less) {
+    double w = 0.0;
+    for (int p = lane; p < a.parts; p += 64) w += part_weight(p, less);
+    return wave_sum(w);
+  };
+  bool less = d.kept < d.n;
+  double total = sum_of(less);
+  if (less && !(total > kNothing)) {
+    less = false;
+    total = sum_of(less);
+  }
+  const double target = u * total;
+  // the first part whose cumulative weight passes the target, else the last with
+  // any; every wave finds it by itself
+  int part = -1;
+  double base = 0.0, start = 0.0;
+  for (int p0 = 0, done = 0; p0 < a.parts && !done; p0 += 64) {
+    const int p = p0 + lane;
+    const double own = p < a.parts ? part_weight(p, less) : 0.0, sum = wave_scan(own);
+    const unsigned long long past = __ballot(own > kNothing && base + sum > target), any = __ballot(own > kNothing);
+    const unsigned long long from = past ? past & -past : any ? 1ull << (63 - __clzll(any)) : 0;
+    if (from) {
+      const int at = __ffsll(from) - 1;
+      part = p0 + at;
+      start = base + lane_of(sum - own, at);
     }
-    // weight of a part: of what is left of p (less), or of p where that is nothing
-    const auto part_weight = [&](int p, bool less) {
-      if (less && r.probs) return fmax(l[p].over + (d.row.sum - S) * l[p].q, 0.0);
-      double w;
-      if constexpr (DECIDED)
-        w = l[p].sum;
-      else
-        w = s[p].sum * weight(s[p].top, d.row.top, r.scale);
-      return !less && !r.probs && p == gone_part ? w + d.row.draft : w;
-    };
-    const auto sum_of = [&](bool less) {
-      double w = 0.0;
-      for (int p = lane; p < a.parts; p += 64) w += part_weight(p, less);
-      return wave_sum(w);
-    };
-    bool less = d.kept < d.n;
-    double total = sum_of(less);
-    if (less && !(total > kNothing)) {
-      less = false;
-      total = sum_of(less);
-    }
-    const double target = u * total;
-    // the first part whose cumulative weight passes the target, else the last with
-    // any; every wave finds it by itself
-    int part = -1;
-    double base = 0.0, start = 0.0;
-    for (int p0 = 0, done = 0; p0 < a.parts && !done; p0 += 64) {
-      const int p = p0 + lane;
-      const double own = p < a.parts ? part_weight(p, less) : 0.0, sum = wave_scan(own);
-      const unsigned long long past = __ballot(own > kNothing && base + sum > target), any = __ballot(own > kNothing);
-      const unsigned long long from = past ? past & -past : any ? 1ull << (63 - __clzll(any)) : 0;
-      if (from) {
-        const int at = __ffsll(from) - 1;
-        part = p0 + at;
-        start = base + lane_of(sum - own, at);
-      }
-      done = past != 0;
-      base += lane_of(sum, 63);
-    }
-    const int j0 = part * kPart - shift + 8 * tid;
+    done = past != 0;
+    base += lane_of(sum, 63);
+  }
+  double w[8], own = 0.0, sum = 0.0;
+  const int j0 = part * PIECES * kPiece - shift + 8 * tid;
+  if (wave < PIECES) {
     const Raw8<T> x = r.logits(j0);
-    double w[8], own = 0.0;
+    Q8 q(less ? r.probs : nullptr, a.probs_bf16, j0, a.V);
 #pragma unroll
     for (int e = 0; e < 8; ++e) w[e] = less && j0 + e == r.gone && !r.probs ? 0.0 : r(x[e]);
-    const auto minus = [&](const auto* probs) {
-      const auto q = load_any8(probs, j0, a.V);
+    if (less && r.probs) {
+      q.widen();
 #pragma unroll
-      for (int e = 0; e < 8; ++e) w[e] = fmax(__builtin_fma(-S, (double)q[e], w[e]), 0.0);
-    };
-    if (less && r.probs) a.probs_bf16 ? minus((const bf16_t*)r.probs) : minus((const float*)r.probs);
+      for (int e = 0; e < 8; ++e) w[e] = fmax(__builtin_fma(-S, (double)q.f[e], w[e]), 0.0);
+    }
 #pragma unroll
     for (int e = 0; e < 8; ++e) own += w[e];
-    const double sum = wave_scan(own);
+    sum = wave_scan(own);
     if (lane == 63) sums[wave] = sum;
-    __syncthreads();
+  }
+  __syncthreads();
+  if (wave < PIECES) {
     double at = start + (sum - own);
     for (int v = 0; v < wave; ++v) at += sums[v];
     int hit = 0x7fffffff, mine = -1;
@@ -549,69 +541,171 @@ __global__ __launch_bounds__(kThreads) void verify_pick_kernel(VerifyArgs a, con
         if (at > target && hit == 0x7fffffff) hit = j0 + e;
       }
     }
-    const unsigned long long hits = __ballot(hit != 0x7fffffff), some_here = __ballot(mine >= 0);
+    const unsigned long long hits = __ballot(hit != 0x7fffffff), any = __ballot(mine >= 0);
+    const int to = any ? __builtin_amdgcn_readlane(mine, 63 - __clzll(any)) : -1;
+    const int from = hits ? __builtin_amdgcn_readlane(hit, __ffsll(hits) - 1) : 0x7fffffff;
     if (lane == 0) {
-      found[wave] = 0x7fffffff;
-      last[wave] = -1;
+      found[wave] = from;
+      last[wave] = to;
     }
-    if (hits && lane == __ffsll(hits) - 1) found[wave] = hit;
-    if (some_here && lane == 63 - __clzll(some_here)) last[wave] = mine;
-    __syncthreads();
-    int from = 0x7fffffff, to = -1;
-#pragma unroll
-    for (int v = 0; v < kWaves; ++v) {
-      from = min(from, found[v]);
-      to = max(to, last[v]);
-    }
-    token = from != 0x7fffffff ? from : to;
   }
-  for (int i = tid; i <= a.N; i += kThreads)
+  __syncthreads();
+  int from = 0x7fffffff, to = -1;
+#pragma unroll
+  for (int v = 0; v < PIECES; ++v) {
+    from = min(from, found[v]);
+    to = max(to, last[v]);
+  }
+  return from != 0x7fffffff ? from : to;
+}
+
+// a row without a distribution, or greedy: no token, or the largest logit (what is
+// left of a weight that is all on one token is on it too)
+__device__ __forceinline__ bool drawn(const Decision& d) { return d.t > 0.f && d.row.sum > 0.0; }
+__device__ __forceinline__ long undrawn(const Decision& d) { return d.row.sum > 0.0 ? d.row.at : -1; }
+
+// a sequence's results, by a workgroup
+__device__ __forceinline__ void answer(const VerifyArgs& a, int b, const Decision& d, long token) {
+  for (int i = threadIdx.x; i <= a.N; i += blockDim.x)
     a.tokens[(long)b * (a.N + 1) + i] = i < d.kept ? a.drafts[(long)b * a.N + i] : i == d.kept ? token : -1;
-  if (tid == 0) a.accepted[b] = d.kept;
+  if (threadIdx.x == 0) a.accepted[b] = d.kept;
+}
+
+}  // namespace
+
+// grid (parts / 4, N + 1, B), a part for each wave.
+template <typename T, bool EXACT>
+__global__ __launch_bounds__(kThreads, EXACT || sizeof(T) == 4 ? 1 : 8) void verify_stat_kernel(
+    VerifyArgs a, const T* __restrict__ logits, VerifyStat* __restrict__ stat) {
+  const int i = blockIdx.y, b = blockIdx.z;
+  const int part = blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n = verify_drafts_of(a, b);
+  if (i > n || part >= a.parts) return;
+  const VerifyStat s = stat_part<kPieces, EXACT>(a, logits, b, i, n, part);
+  if ((threadIdx.x & 63) == 0) stat[((long)b * (a.N + 1) + i) * a.parts + part] = s;
+}
+
+// grid (parts / 4, B): the drafts kept, and the fp64 sums over the row behind them.
+// (The last workgroup of a sequence finding the token here, behind a fence of the
+// device, takes 6 us more than a launch of its own.)
+template <typename T>
+__global__ __launch_bounds__(kThreads) void verify_left_kernel(VerifyArgs a, const T* __restrict__ logits,
+                                                               const VerifyStat* __restrict__ stat,
+                                                               VerifyLeft* __restrict__ left,
+                                                               Decision* __restrict__ decisions) {
+  const int b = blockIdx.y;
+  const int part = blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const Decision d = decide<kWaves>(a, logits, stat + (long)b * (a.N + 1) * a.parts, b);
+  if (blockIdx.x == 0 && threadIdx.x == 0) decisions[b] = d;
+  if (!drawn(d) || part >= a.parts) return;
+  const VerifyLeft l = left_part<kPieces>(a, logits, b, d, part);
+  if ((threadIdx.x & 63) == 0) left[(long)b * a.parts + part] = l;
+}
+
+// grid (B): the token, from the fp64 sums of the second launch (LEFT) or the first.
+template <typename T, bool LEFT>
+__global__ __launch_bounds__(kThreads) void verify_pick_kernel(VerifyArgs a, const T* __restrict__ logits,
+                                                               const VerifyStat* __restrict__ stat,
+                                                               const VerifyLeft* __restrict__ left,
+                                                               const Decision* __restrict__ decisions) {
+  const int b = blockIdx.x;
+  Decision d;
+  if constexpr (LEFT)
+    d = decisions[b];
+  else
+    d = decide<kWaves>(a, logits, stat + (long)b * (a.N + 1) * a.parts, b);
+  const VerifyStat* s = stat + ((long)b * (a.N + 1) + d.kept) * a.parts;
+  answer(a, b, d, drawn(d) ? pick<LEFT, kPieces>(a, logits, b, d, s, left + (long)b * a.parts) : undrawn(d));
+}
+
+// grid (B): all of it by one workgroup, where a sequence has few logits.
+template <typename T>
+__global__ __launch_bounds__(64 * kSmallWaves) void verify_small_kernel(VerifyArgs a, const T* __restrict__ logits) {
+  __shared__ VerifyStat stat[kSmallParts];
+  __shared__ VerifyLeft left[kSmallParts];
+  const int b = blockIdx.x, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int n = verify_drafts_of(a, b);
+  for (int k = wave; k < (n + 1) * a.parts; k += kSmallWaves) {
+    const VerifyStat s = stat_part<1, false>(a, logits, b, k / a.parts, n, k % a.parts);
+    if (lane == 0) stat[k] = s;
+  }
+  __syncthreads();
+  const Decision d = decide<kSmallWaves>(a, logits, stat, b);
+  if (!drawn(d)) {
+    answer(a, b, d, undrawn(d));
+    return;
+  }
+  for (int p = wave; p < a.parts; p += kSmallWaves) {
+    const VerifyLeft l = left_part<1>(a, logits, b, d, p);
+    if (lane == 0) left[p] = l;
+  }
+  __syncthreads();
+  answer(a, b, d, pick<true, 1>(a, logits, b, d, (const VerifyStat*)nullptr, left));
 }
 
 namespace {
 
 // (a row that begins between two 16-byte boundaries may need one more)
-int verify_parts(const VerifyArgs& a) { return (int)(((long)a.V + 7 + kPart - 1) / kPart); }
+int verify_parts(const VerifyArgs& a, int pieces) {
+  return (int)(((long)a.V + 7 + pieces * kPiece - 1) / (pieces * kPiece));
+}
+
+// One launch for sequences of few logits (100 sequences with three drafts at 8000
+// logits and q 16.8 us, in three launches 18.9 and their gaps; 64 with seven at 2000
+// without q 12.6, in two 12.8; beyond that a workgroup's CU is slower than launches: four
+// sequences with three at 15000 19.9 without q, 11.0 in two).  Two, the first in fp64,
+// where q is not given and the logits are few; else three.
+enum VerifyForm { kSmall, kBrief, kFull };
+VerifyForm verify_form(const VerifyArgs& a) {
+  if ((long)verify_parts(a, 1) * (a.N + 1) <= (a.probs ? 96 : 48)) return kSmall;
+  return !a.probs && (long)a.B * (a.N + 1) * a.V <= (1l << 24) ? kBrief : kFull;
+}
 
 }  // namespace
 
-// Two launches, the first in fp64, where q is not given and the rows are few.
-bool verify_brief(const VerifyArgs& a) {
-  return !a.probs && (long)a.B * (a.N + 1) * a.V <= (1l << 24);
-}
-
 size_t verify_ws_bytes(const VerifyArgs& a) {
-  const size_t parts = verify_parts(a);
+  const size_t parts = verify_parts(a, kPieces);
   const size_t stat = parts * a.B * (a.N + 1) * sizeof(VerifyStat);
-  return verify_brief(a) ? stat : stat + a.B * (parts * sizeof(VerifyLeft) + sizeof(Decision));
+  const VerifyForm form = verify_form(a);
+  return form == kSmall ? 0 : form == kBrief ? stat : stat + a.B * (parts * sizeof(VerifyLeft) + sizeof(Decision));
 }
 
 hipError_t launch_verify(VerifyArgs a, const void* logits, bool bf16, void* ws, hipStream_t st) {
-  a.parts = verify_parts(a);
+  const VerifyForm form = verify_form(a);
+  a.parts = verify_parts(a, form == kSmall ? 1 : kPieces);
   VerifyStat* stat = (VerifyStat*)ws;
   VerifyLeft* left = (VerifyLeft*)(stat + (size_t)a.parts * a.B * (a.N + 1));
   Decision* decisions = (Decision*)(left + (size_t)a.parts * a.B);
   const unsigned groups = (a.parts + kWaves - 1) / kWaves;
-  auto run = [&](auto type, auto brief) {
+  auto run = [&](auto type) {
     using T = decltype(type);
-    constexpr bool BRIEF = decltype(brief)::value;
     const T* x = (const T*)logits;
-    NAYLIS_TIMED("verify_stat", st,
-                 hipLaunchKernelGGL((verify_stat_kernel<T, BRIEF>), dim3(groups, a.N + 1, a.B), dim3(kThreads), 0, st,
-                                    a, x, stat));
-    if constexpr (!BRIEF) {
+    auto first = [&](auto exact) {
+      NAYLIS_TIMED("verify_stat", st,
+                   hipLaunchKernelGGL((verify_stat_kernel<T, decltype(exact)::value>), dim3(groups, a.N + 1, a.B),
+                                      dim3(kThreads), 0, st, a, x, stat));
+    };
+    auto last = [&](auto from_left) {
+      NAYLIS_TIMED("verify_pick", st,
+                   hipLaunchKernelGGL((verify_pick_kernel<T, decltype(from_left)::value>), dim3(a.B), dim3(kThreads),
+                                      0, st, a, x, (const VerifyStat*)stat, (const VerifyLeft*)left,
+                                      (const Decision*)decisions));
+    };
+    if (form == kSmall) {
+      NAYLIS_TIMED("verify_small", st,
+                   hipLaunchKernelGGL((verify_small_kernel<T>), dim3(a.B), dim3(64 * kSmallWaves), 0, st, a, x));
+    } else if (form == kBrief) {
+      first(std::true_type{});
+      last(std::false_type{});
+    } else {
+      first(std::false_type{});
       NAYLIS_TIMED("verify_left", st,
                    hipLaunchKernelGGL((verify_left_kernel<T>), dim3(groups, a.B), dim3(kThreads), 0, st, a, x,
                                       (const VerifyStat*)stat, left, decisions));
+      last(std::true_type{});
     }
-    NAYLIS_TIMED("verify_pick", st,
-                 hipLaunchKernelGGL((verify_pick_kernel<T, !BRIEF>), dim3(a.B), dim3(kThreads), 0, st, a, x,
-                                    (const VerifyStat*)stat, (const VerifyLeft*)left, (const Decision*)decisions));
   };
-  auto pick = [&](auto type) { verify_brief(a) ? run(type, std::true_type{}) : run(type, std::false_type{}); };
-  bf16 ? pick(bf16_t{}) : pick(float{});
+  bf16 ? run(bf16_t{}) : run(float{});
   return hipGetLastError();
 }
 

@@ -112,8 +112,8 @@ def test_verify_refusals(lib, bad, text):
 
 def test_verify_workspace(lib):
     need = lambda B, N, V, q: lib.naylis_mom_verify_drafts_workspace_bytes(B, N, V, q)  # noqa: E731
-    assert need(3, 2, 100, 1) > need(3, 2, 100, 0) > 0 and need(3, 2, 0, 0) == 0 and need(0, 0, 1, 0) > 0
-    assert _verify(lib, ws_bytes=need(3, 2, 100, 1) - 1) == _lib.NAYLIS_ERR_WORKSPACE
+    assert need(3, 2, 100000, 1) > need(3, 2, 100000, 0) > 0 and need(3, 2, 0, 0) == 0 and need(0, 0, 1, 0) > 0
+    assert _verify(lib, V=100000, ws_bytes=need(3, 2, 100000, 1) - 1) == _lib.NAYLIS_ERR_WORKSPACE
     assert _verify(lib, B=0) == _lib.NAYLIS_OK
 
 

@@ -96,7 +96,8 @@ def _check(c, dev, **kw):
 
 
 SHAPES = [(1, 0, 1), (1, 1, 2), (3, 2, 7), (5, 3, 8), (2, 8, 1000), (70, 4, 2047), (3, 1, 2048), (3, 2, 2049), (2, 3, 4096),
-          (9, 5, 8191), (4, 2, 50001), (2, 1, 151999), (1, 12, 32768)]
+          (9, 5, 8191), (4, 2, 50001), (2, 1, 151999), (1, 12, 32768), (2, 40, 513), (3, 95, 500), (2, 100, 9001), (5, 0, 24000),
+          (5, 0, 24700), (4, 3, 12281), (4, 3, 12282)]
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
@@ -191,11 +192,10 @@ def test_verify_rows_without_a_distribution(t, probs, bad, dev):
         assert torch.equal(got.tokens[b], fine.tokens[b])
 
 
-@pytest.mark.parametrize("B", [2, 600])  # sums in fp64, and in fp32
-def test_verify_signalling_nans(B, dev):
+@pytest.mark.parametrize("B,V", [(2, 10000), (2, 40000), (600, 20000)])  # one launch, sums in fp64, and in fp32
+def test_verify_signalling_nans(B, V, dev):
     """NaNs of every bit pattern, one and a whole part of them."""
     from naylis_amd.mom_kernels import verify_drafts
-    V = 20000
     x = torch.zeros(B, 2, V, dtype=torch.bfloat16, device=dev)
     drafts, u = torch.full((B, 1), 17, device=dev), torch.zeros(B, 2, device=dev)
     for bits in (0x7f81, 0x7fc0, 0xff81 - 65536, 0xffff - 65536):
