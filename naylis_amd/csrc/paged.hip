@@ -783,9 +783,12 @@ PagedSplit paged_split(const PagedCacheDims& c, PagedFormat fmt) {
   return p;
 }
 
-// Several tokens of sequences that have eight partials each or so at most: a launch of
-// a thousand workgroups less takes a microsecond less.
-bool paged_join_few(const PagedCacheDims& c, const PagedSplit& p) { return c.N > 1 && p.wgs <= 8 * c.B; }
+// Several tokens, or pages of 4 bits, of sequences that have eight partials each or so
+// at most: a launch of a thousand workgroups less takes a microsecond less.  (One token
+// over other pages keeps the order of its sums.)
+bool paged_join_few(const PagedCacheDims& c, const PagedSplit& p, PagedFormat fmt) {
+  return (c.N > 1 || fmt == kPagedE2m1) && p.wgs <= 8 * c.B;
+}
 
 size_t paged_part_floats(const PagedCacheDims& c, const PagedSplit& p, int hd) {
   return p.whole ? 0 : (size_t)c.Hkv * p.head_tiles * p.wgs * 2 * p.rows * hd;
@@ -868,7 +871,7 @@ hipError_t launch_paged_attn(const PagedCacheDims& c, int hd, PagedFormat fmt, c
                  hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, c, q.live, lens, (bf16_t*)out, (const float*)part,
                                     (const float2*)stat, (const int*)starts, p));
   };
-  if (paged_join_few(c, p)) {
+  if (paged_join_few(c, p, fmt)) {
     const dim3 grid((c.G * c.N * hd + 1023) / 1024, c.Hkv, c.B);
     hd == 64 ? join(paged_join_few_kernel<64>, grid) : join(paged_join_few_kernel<128>, grid);
   } else {

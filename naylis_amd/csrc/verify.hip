@@ -39,6 +39,7 @@ namespace {
 constexpr int kThreads = 256, kWaves = kThreads / 64;
 constexpr int kPiece = 512;          // logits of a wave at a time, eight a lane
 constexpr int kPieces = 4;           // pieces of a part: PIECES 4, or 1 where one workgroup does it all
+constexpr int kLeftWaves = 8;         // of the second launch, which decides in each workgroup
 constexpr int kSmallParts = 128, kSmallWaves = 16;  // the workgroup that does it all
 constexpr double kNothing = 0x1p-900;  // weights up to this are none: those of -inf count as 2^-1000
 
@@ -585,17 +586,17 @@ __global__ __launch_bounds__(kThreads, EXACT || sizeof(T) == 4 ? 1 : 8) void ver
   if ((threadIdx.x & 63) == 0) stat[((long)b * (a.N + 1) + i) * a.parts + part] = s;
 }
 
-// grid (parts / 4, B): the drafts kept, and the fp64 sums over the row behind them.
+// grid (parts / 8, B): the drafts kept, and the fp64 sums over the row behind them.
 // (The last workgroup of a sequence finding the token here, behind a fence of the
 // device, takes 6 us more than a launch of its own.)
 template <typename T>
-__global__ __launch_bounds__(kThreads) void verify_left_kernel(VerifyArgs a, const T* __restrict__ logits,
+__global__ __launch_bounds__(64 * kLeftWaves) void verify_left_kernel(VerifyArgs a, const T* __restrict__ logits,
                                                                const VerifyStat* __restrict__ stat,
                                                                VerifyLeft* __restrict__ left,
                                                                Decision* __restrict__ decisions) {
   const int b = blockIdx.y;
-  const int part = blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const Decision d = decide<kWaves>(a, logits, stat + (long)b * (a.N + 1) * a.parts, b);
+  const int part = blockIdx.x * kLeftWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const Decision d = decide<kLeftWaves>(a, logits, stat + (long)b * (a.N + 1) * a.parts, b);
   if (blockIdx.x == 0 && threadIdx.x == 0) decisions[b] = d;
   if (!drawn(d) || part >= a.parts) return;
   const VerifyLeft l = left_part<kPieces>(a, logits, b, d, part);
@@ -700,7 +701,8 @@ hipError_t launch_verify(VerifyArgs a, const void* logits, bool bf16, void* ws, 
     } else {
       first(std::false_type{});
       NAYLIS_TIMED("verify_left", st,
-                   hipLaunchKernelGGL((verify_left_kernel<T>), dim3(groups, a.B), dim3(kThreads), 0, st, a, x,
+                   hipLaunchKernelGGL((verify_left_kernel<T>), dim3((a.parts + kLeftWaves - 1) / kLeftWaves, a.B),
+                                      dim3(64 * kLeftWaves), 0, st, a, x,
                                       (const VerifyStat*)stat, left, decisions));
       last(std::true_type{});
     }
