@@ -193,8 +193,13 @@ __device__ __forceinline__ int v_slot(int row, int chunk) {  // byte of a 16-byt
   return row * 2 * HD + ((chunk ^ f) << 4);
 }
 
+// Loads past the caches, unless another slice reads the same.
+template <bool AGAIN>
 __device__ __forceinline__ uint4 load_once16(const uint8_t* p) {
-  return __builtin_bit_cast(uint4, __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(p)));
+  if constexpr (AGAIN)
+    return *reinterpret_cast<const uint4*>(p);
+  else
+    return __builtin_bit_cast(uint4, __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(p)));
 }
 template <int N>
 struct Words {
@@ -202,11 +207,14 @@ struct Words {
 };
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-template <int N>
+template <int N, bool AGAIN>
 __device__ __forceinline__ Words<N> load_once(const uint8_t* p) {
   using V = std::conditional_t<N == 4, u32x4, u32x2>;
   static_assert(N == 2 || N == 4, "8 or 16 bytes");
-  return __builtin_bit_cast(Words<N>, __builtin_nontemporal_load(reinterpret_cast<const V*>(p)));
+  if constexpr (AGAIN)
+    return __builtin_bit_cast(Words<N>, *reinterpret_cast<const V*>(p));
+  else
+    return __builtin_bit_cast(Words<N>, __builtin_nontemporal_load(reinterpret_cast<const V*>(p)));
 }
 
 // A query row of a key head is (new token, query head): token-major, so that one
@@ -236,8 +244,11 @@ __device__ __forceinline__ long part_row(const PagedSplit& p, int slice, int wg,
 // number, its waves an equal share each.
 // ROWS: partials' rows, at least the query rows of a slice; a product's 16 or, of 32,
 // two products' for each read of the cache.  MANY: more than one
-// new token, or a number of them that each sequence has of its own.
-template <int HD, PagedFormat FMT, int ROWS, bool MANY>
+// new token, or a number of them that each sequence has of its own.  AGAIN: a key head
+// has more than one slice, which read the same keys and values at about the same time
+// (seven sequences of up to 5775 tokens, 40 rows for each of 4 key heads, bf16: 31 us;
+// past the caches 38, and with the choice made in the loop a single slice loses a tenth).
+template <int HD, PagedFormat FMT, int ROWS, bool MANY, bool AGAIN = false>
 __global__ __launch_bounds__(256, FMT == kPagedE2m1 && ROWS <= kRowsMfma ? 3 : 2) void paged_attn_kernel(PagedCacheDims c, PagedQueries q,
                                                             const int32_t* __restrict__ table,
                                                             const int32_t* __restrict__ lens,
@@ -376,11 +387,11 @@ __global__ __launch_bounds__(256, FMT == kPagedE2m1 && ROWS <= kRowsMfma ? 3 : 2
 #pragma unroll
       for (int i = 0; i < NS; ++i) {
         if constexpr (FP4) {
-          kw[i] = load_once<NW>((const uint8_t*)c.k + row16[i] * RB + off);
+          kw[i] = load_once<NW, AGAIN>((const uint8_t*)c.k + row16[i] * RB + off);
           ke[i] = __builtin_nontemporal_load((const uint8_t*)c.k_scale + row16[i] * NW + eoff);
         } else {
 #pragma unroll
-          for (int j = 0; j < KL; ++j) kx[i][j] = load_once16((const uint8_t*)c.k + row16[i] * RB + 64 * j + off);
+          for (int j = 0; j < KL; ++j) kx[i][j] = load_once16<AGAIN>((const uint8_t*)c.k + row16[i] * RB + 64 * j + off);
         }
         if constexpr (FP8) {
           ksc[i] = *reinterpret_cast<const f32x4*>((const float*)c.k_scale + row16[i] + 4 * g);
@@ -393,12 +404,12 @@ __global__ __launch_bounds__(256, FMT == kPagedE2m1 && ROWS <= kRowsMfma ? 3 : 2
 #pragma unroll
       for (int i = 0; i < NS; ++i) {
         if constexpr (FP4) {
-          vw[i] = load_once<NW>((const uint8_t*)c.v + row16[i] * RB + off);
+          vw[i] = load_once<NW, AGAIN>((const uint8_t*)c.v + row16[i] * RB + off);
           ve[i] = __builtin_nontemporal_load((const uint8_t*)c.v_scale + row16[i] * NW + eoff);
         } else {
 #pragma unroll
           for (int j = 0; j < VL / NS; ++j)
-            vx[i * (VL / NS) + j] = load_once16((const uint8_t*)c.v + row16[i] * RB + 1024 * j + off);
+            vx[i * (VL / NS) + j] = load_once16<AGAIN>((const uint8_t*)c.v + row16[i] * RB + 1024 * j + off);
         }
       }
     };
@@ -860,7 +871,8 @@ hipError_t launch_paged_attn(const PagedCacheDims& c, int hd, PagedFormat fmt, c
     if (c.N > 1 || q.live)
       p.rows == 4    ? run(paged_attn_kernel<HD, F, 4, true>)
       : p.rows == 16 ? run(paged_attn_kernel<HD, F, 16, true>)
-                     : run(paged_attn_kernel<HD, F, 32, true>);
+      : p.head_tiles == 1 ? run(paged_attn_kernel<HD, F, 32, true>)
+                          : run(paged_attn_kernel<HD, F, 32, true, true>);
     else
       p.rows == 4 ? run(paged_attn_kernel<HD, F, 4, false>) : run(paged_attn_kernel<HD, F, 16, false>);
   });
