@@ -187,9 +187,15 @@ __device__ __forceinline__ int part_offset(int slot) {
   return slot == 0 ? 32 * 2 * HD : 0;
 }
 
-template <int HD>
-__device__ __forceinline__ int v_slot(int row, int chunk) {  // byte of a 16-byte chunk in the V tile
-  const int f = HD == 128 ? 2 * (row & 7) : 2 * ((row >> 1) & 3);
+// Byte of a 16-byte chunk in the V tile: dealt so that the 128 bytes that LDS serves
+// at a time lie in its 32 banks once.  A transposing read takes a pair of chunks from
+// each of four rows; of widened codes a write takes every second chunk of a row, or of
+// e2m1 every fourth one of two (in the halves of a row the chunks of a pair change
+// places).
+template <int HD, PagedFormat FMT>
+__device__ __forceinline__ int v_slot(int row, int chunk) {
+  constexpr bool CODES = FMT != kPagedBf16;
+  const int f = HD == 128 ? (2 * (row & 7)) ^ (CODES ? chunk >> 3 : 0) : 2 * (row & 3) + (CODES ? row & 1 : 0);
   return row * 2 * HD + ((chunk ^ f) << 4);
 }
 
@@ -454,7 +460,7 @@ __global__ __launch_bounds__(256, FMT == kPagedE2m1 && ROWS <= kRowsMfma ? 3 : 2
             }
 #pragma unroll
             for (int w = 0; w < NW; ++w)
-              *reinterpret_cast<bf16x8*>(vt + v_slot<HD>(row, NW * vpc + w)) = widen8_e2m1(vw[i].w[w], ve[i]);
+              *reinterpret_cast<bf16x8*>(vt + v_slot<HD, FMT>(row, NW * vpc + w)) = widen8_e2m1(vw[i].w[w], ve[i]);
           }
           lds_order();
           return;
@@ -465,10 +471,10 @@ __global__ __launch_bounds__(256, FMT == kPagedE2m1 && ROWS <= kRowsMfma ? 3 : 2
           if (tail && tok0 + row >= n) vx[j] = make_uint4(0, 0, 0, 0);
           const uint4 u = vx[j];
           if constexpr (FP8) {
-            *reinterpret_cast<bf16x8*>(vt + v_slot<HD>(row, 2 * vpc)) = widen8(u.x, u.y);
-            *reinterpret_cast<bf16x8*>(vt + v_slot<HD>(row, 2 * vpc + 1)) = widen8(u.z, u.w);
+            *reinterpret_cast<bf16x8*>(vt + v_slot<HD, FMT>(row, 2 * vpc)) = widen8(u.x, u.y);
+            *reinterpret_cast<bf16x8*>(vt + v_slot<HD, FMT>(row, 2 * vpc + 1)) = widen8(u.z, u.w);
           } else {
-            *reinterpret_cast<uint4*>(vt + v_slot<HD>(row, vpc)) = u;
+            *reinterpret_cast<uint4*>(vt + v_slot<HD, FMT>(row, vpc)) = u;
           }
         }
         lds_order();
@@ -545,8 +551,8 @@ __global__ __launch_bounds__(256, FMT == kPagedE2m1 && ROWS <= kRowsMfma ? 3 : 2
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         const int ch = 2 * t + ((r16 & 3) >> 1), b8 = 8 * (r16 & 1);
-        const v4i16 lo = lds_read_tr16(reinterpret_cast<const bf16_t*>(vt + v_slot<HD>(rlo, ch) + b8));
-        const v4i16 hi = lds_read_tr16(reinterpret_cast<const bf16_t*>(vt + v_slot<HD>(rhi, ch) + b8));
+        const v4i16 lo = lds_read_tr16(reinterpret_cast<const bf16_t*>(vt + v_slot<HD, FMT>(rlo, ch) + b8));
+        const v4i16 hi = lds_read_tr16(reinterpret_cast<const bf16_t*>(vt + v_slot<HD, FMT>(rhi, ch) + b8));
         typedef short v8i16 __attribute__((ext_vector_type(8)));
         const v8i16 vf = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 #pragma unroll

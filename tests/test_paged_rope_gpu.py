@@ -236,6 +236,46 @@ def test_gather_bad_pages(fmt, dev):
     assert paged_gather(cache, bad, cu, 0)[0].shape == (0, 2, 64)
 
 
+def test_chunk_in_a_graph(dev):
+    """A chunk's append, its gather and the packed attention over it in one captured
+    graph, replayed with new tokens, places and lengths."""
+    from naylis_amd.mom_kernels import new_paged_cache, packed_attention, paged_append_rope, paged_gather
+    B, W, T, Hkv, hd = 3, 6, 40, 2, 64
+    caches = [new_paged_cache(B * W, Hkv, 16, hd, dev, fp4=True) for _ in range(2)]
+    table = torch.randperm(B * W, generator=torch.Generator().manual_seed(0)).view(B, W).int().to(dev)
+    q, k, v = _new(T, 4, Hkv, hd, dev)
+    freq = _freq(32, dev)
+    rows, pos = torch.zeros(T, dtype=torch.int32, device=dev), torch.arange(T, dtype=torch.int32, device=dev)
+    cu_q, cu_k = (torch.tensor([0, T, T, T], dtype=torch.int32, device=dev) for _ in range(2))
+
+    def chunk(cache):
+        r = paged_append_rope(cache, q, k, v, freq, table, pos, rows)
+        kd, vd = paged_gather(cache, table, cu_k, 150)
+        return packed_attention(r, kd, vd, cu_q, cu_k)
+    chunk(caches[0])
+    for t in caches[0]:
+        t.zero_()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=torch.cuda.Stream()):
+        out = chunk(caches[0])
+    start = [0, 0, 0]
+    for i in range(5):
+        for t, new in zip((q, k, v), _new(T, 4, Hkv, hd, dev, seed=i + 1)):
+            t.copy_(new)
+        add = [(10, 15, 15), (1, 38, 1), (20, 0, 20), (13, 13, 14), (0, 1, 39)][i]
+        rows.copy_(torch.repeat_interleave(torch.arange(B), torch.tensor(add)))
+        pos.copy_(torch.cat([torch.arange(a, a + n) for a, n in zip(start, add)]))
+        start = [(a + n) % 50 for a, n in zip(start, add)]
+        ends = [int(pos[rows == b].max()) + 1 if n else 0 for b, n in enumerate(add)]
+        cu_q.copy_(torch.tensor([0, *torch.tensor(add).cumsum(0).tolist()]))
+        cu_k.copy_(torch.tensor([0, *torch.tensor(ends).cumsum(0).tolist()]))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, chunk(caches[1]))
+        assert all(torch.equal(x, y) for x, y in zip(*(c[:2] for c in caches)))
+
+
 def test_chunk_refusals(dev):
     from naylis_amd.mom_kernels import PagedCache, new_paged_cache, paged_append_rope, paged_gather
     cache = new_paged_cache(4, 2, 16, 64, dev)

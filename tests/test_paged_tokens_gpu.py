@@ -413,3 +413,69 @@ def test_e2m1_large_cache(dev):
     from naylis_amd.mom_kernels import paged_attention
     got = paged_attention(c["q"], cache, table, c["lens"])
     assert bool(((got.double() - want).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("width", [None, 100])  # a table of one launch, and of two
+def test_tokens_that_hold_no_numbers(width, fmt, dev):
+    """A new token's keys of NaN reach the rows that see it alone; of its values they
+    reach the earlier new tokens of its sequence too (a weight of 0 times what it
+    stands for), and no other sequence.  A token behind the sequence reaches none."""
+    from naylis_amd.mom_kernels import paged_append, paged_attention
+    c = _case([70, 45, 33], 4, 2, 64, 16, fmt, dev, N=4, q_lens=[4, 4, 2], width=width)
+    run = lambda: paged_attention(c["q"], c["cache"], c["table"], c["lens"], q_lens=c["q_lens"])  # noqa: E731
+    good = run()
+    last = (c["rows"] == 1) & (c["pos"] == 43)  # seen by the last two of four
+    k, v = c["k"].clone(), c["v"].clone()
+    k[last] = math.nan
+    paged_append(c["cache"], k, c["v"], c["table"], c["pos"], c["rows"])
+    got = run()
+    assert bool(got[1, 2:].isnan().all()) and torch.equal(got[1, :2], good[1, :2])
+    assert torch.equal(got[0], good[0]) and torch.equal(got[2], good[2])
+    v[last] = math.nan
+    paged_append(c["cache"], c["k"], v, c["table"], c["pos"], c["rows"])
+    got = run()
+    assert bool(got[1, 2:].isnan().all()) and torch.equal(got[0], good[0]) and torch.equal(got[2], good[2])
+    c["lens"][1], c["q_lens"][1] = 43, 2  # the token is behind the sequence now
+    got = run()
+    assert torch.equal(got[1, :2], good[1, :2])
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_tokens_one_sequence_among_many(fmt, dev):
+    """Sequences that end and begin within a wave's range, 32 rows and two tiles of
+    them: the same as each sequence alone, up to where its tokens are cut."""
+    from naylis_amd.mom_kernels import paged_attention
+    lens = [(i * 37) % 90 + 1 for i in range(150)] + [3000] + [(i * 53) % 70 for i in range(100)]
+    for H, N in ((8, 5), (16, 5)):  # 20 rows a key head, 40
+        c = _case(lens, H, 2, 128, 16, fmt, dev, N=N, q_lens=[i % (N + 1) for i in range(len(lens))])
+        _check(c, 16)
+
+
+def test_formats_under_trace(dev):
+    """A traced attention of several tokens and a traced gather run again on new inputs."""
+    from naylis_amd.mom_kernels import paged_attention, paged_gather
+    c = _case([70, 45], 4, 2, 64, 16, "e2m1", dev, N=3)
+    cu = torch.tensor([0, 70, 115], dtype=torch.int32, device=dev)
+
+    def call(q, lens):
+        return paged_attention(q, c["cache"], c["table"], lens, q_lens=lens - 40), *paged_gather(c["cache"], c["table"], cu, 115)
+    traced = torch.jit.trace(call, (c["q"], c["lens"]), check_trace=False)
+    for q, lens in ((c["q"], c["lens"]), (c["q"].flip(0).contiguous(), c["lens"] - 2)):
+        for x, y in zip(traced(q, lens), call(q, lens)):
+            assert torch.equal(x, y)
+
+
+def test_tokens_forward_mode_derivatives_raise(dev):
+    import torch.autograd.forward_ad as fwAD
+    from naylis_amd.mom_kernels import paged_append_rope, paged_attention, verify_drafts
+    c = _case([20, 30], 4, 2, 64, 16, "bf16", dev, N=2)
+    x = torch.zeros(2, 3, 50, device=dev)
+    with fwAD.dual_level():
+        q = fwAD.make_dual(c["q"], torch.ones_like(c["q"]))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            paged_attention(q, c["cache"], c["table"], c["lens"])
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            paged_append_rope(c["cache"], q[:, 0], c["k"][:2], c["v"][:2], torch.ones(32, device=dev), c["table"], c["pos"][:2])
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            verify_drafts(fwAD.make_dual(x, x), torch.zeros(2, 2, dtype=torch.long, device=dev), x[:, :, 0].contiguous())
