@@ -25,6 +25,13 @@
 // for S is so near to S' that only tokens that weigh nothing change sides;
 // (3) a workgroup for each sequence finds the part and the token in it.  Few logits
 // and no q: (1) in fp64, and no (2).
+//
+// One sequence, three drafts of a rule, 32768 logits: 10 us, two launches whose waves
+// wait for chains of loads (parts, draft, logit; part, token).  64 sequences, four
+// drafts, 50001 logits, q fp32: 23 us, of which (1) 9.4 (32 MB), (2) 9.2 and (3) 5.4,
+// each of them mostly a launch's start and end.  48, seven, 151999, q bf16: 40 us, (1)
+// 19.7 (117 MB, 5.9 TB/s), (2) 14: the decisions' chains before the first byte, then 29
+// MB from the caches and twelve fp64 products each, (3) 5.6.
 #include "common.h"
 #include "launch.h"
 #include "timing.h"
@@ -41,7 +48,9 @@ constexpr int kPiece = 512;          // logits of a wave at a time, eight a lane
 constexpr int kPieces = 4;           // pieces of a part: PIECES 4, or 1 where one workgroup does it all
 constexpr int kLeftWaves = 8;         // of the second launch, which decides in each workgroup
 constexpr int kSmallParts = 128, kSmallWaves = 16;  // the workgroup that does it all
-constexpr double kNothing = 0x1p-900;  // weights up to this are none: those of -inf count as 2^-1000
+// Weights up to these are none, those of -inf count as 2^-1000: of a part, and of a
+// token, so much less that a part with a weight has a token with one.
+constexpr double kNothing = 0x1p-900, kNoToken = 0x1p-920;
 
 // what the first launch leaves of a part of a row
 struct VerifyStat {
@@ -214,14 +223,19 @@ __device__ __forceinline__ double wave_scan(double x) {
 }
 __device__ __forceinline__ double wave_sum(double x) { return lane_of(wave_scan(x), 63); }
 
-__device__ __forceinline__ double scale_of(float t) { return 1.4426950408889634074 / (t > 0.f ? (double)t : 1.0); }
+// (within what fp32 holds, so that 0 and -inf times it stay what they are)
+__device__ __forceinline__ double scale_of(float t) {
+  return 1.4426950408889634074 / (t > 0.f ? (double)fminf(fmaxf(t, 0x1p-120f), 0x1p120f) : 1.0);
+}
 
 }  // namespace
 
 __device__ __forceinline__ int verify_drafts_of(const VerifyArgs& a, int b) {
   return a.lens ? min(max(a.lens[b], 0), a.N) : a.N;
 }
-__device__ __forceinline__ float verify_temperature(const VerifyArgs& a, int b) { return a.temps ? a.temps[b] : a.temp; }
+__device__ __forceinline__ float verify_temperature(const VerifyArgs& a, int b) {
+  return a.temps ? a.temps[b] : a.temp;
+}
 
 namespace {
 
@@ -410,7 +424,8 @@ struct Behind {
   double scale;
 
   __device__ __forceinline__ Behind(const VerifyArgs& a, const T* logits, int b, const Decision& d)
-      : a(a), row(logits + b * a.ldb + d.kept * a.ldt), probs(nullptr), gone(d.gone), top(d.row.top), scale(scale_of(d.t)) {
+      : a(a), row(logits + b * a.ldb + d.kept * a.ldt), probs(nullptr), gone(d.gone), top(d.row.top),
+        scale(scale_of(d.t)) {
     if (d.kept == d.n || !a.probs) return;
     const long at = b * a.lqb + d.kept * a.lqt;
     probs = a.probs_bf16 ? (const void*)((const bf16_t*)a.probs + at) : (const void*)((const float*)a.probs + at);
@@ -467,7 +482,8 @@ __device__ __forceinline__ long pick(const VerifyArgs& a, const T* logits, int b
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const double u = a.uniforms[(long)b * (a.N + 1) + a.N];
   const Behind<T> r(a, logits, b, d);
-  const int shift = shift_of(r.row), gone_part = r.gone >= 0 && r.gone < a.V ? (int)((r.gone + shift) / (PIECES * kPiece)) : -1;
+  const int shift = shift_of(r.row);
+  const int gone_part = r.gone >= 0 && r.gone < a.V ? (int)((r.gone + shift) / (PIECES * kPiece)) : -1;
   double S = 0.0;  // over the whole row, of the e that q is taken from
   if (r.probs) {
     for (int p = lane; p < a.parts; p += 64) S += l[p].sum;
@@ -489,75 +505,82 @@ __device__ __forceinline__ long pick(const VerifyArgs& a, const T* logits, int b
     return wave_sum(w);
   };
   bool less = d.kept < d.n;
-  double total = sum_of(less);
-  if (less && !(total > kNothing)) {
-    less = false;
-    total = sum_of(less);
-  }
-  const double target = u * total;
-  // the first part whose cumulative weight passes the target, else the last with
-  // any; every wave finds it by itself
-  int part = -1;
-  double base = 0.0, start = 0.0;
-  for (int p0 = 0, done = 0; p0 < a.parts && !done; p0 += 64) {
-    const int p = p0 + lane;
-    const double own = p < a.parts ? part_weight(p, less) : 0.0, sum = wave_scan(own);
-    const unsigned long long past = __ballot(own > kNothing && base + sum > target), any = __ballot(own > kNothing);
-    const unsigned long long from = past ? past & -past : any ? 1ull << (63 - __clzll(any)) : 0;
-    if (from) {
-      const int at = __ffsll(from) - 1;
-      part = p0 + at;
-      start = base + lane_of(sum - own, at);
+  // (again from all of p where less is none of it, or only what rounding left: a part
+  // then has a weight of 1e-14 of p that none of its tokens has)
+#pragma unroll 1
+  for (;;) {
+    const double total = sum_of(less);
+    if (less && !(total > kNothing)) {
+      less = false;
+      continue;
     }
-    done = past != 0;
-    base += lane_of(sum, 63);
-  }
-  double w[8], own = 0.0, sum = 0.0;
-  const int j0 = part * PIECES * kPiece - shift + 8 * tid;
-  if (wave < PIECES) {
-    const Raw8<T> x = r.logits(j0);
-    Q8 q(less ? r.probs : nullptr, a.probs_bf16, j0, a.V);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) w[e] = less && j0 + e == r.gone && !r.probs ? 0.0 : r(x[e]);
-    if (less && r.probs) {
-      q.widen();
-#pragma unroll
-      for (int e = 0; e < 8; ++e) w[e] = fmax(__builtin_fma(-S, (double)q.f[e], w[e]), 0.0);
+    const double target = u * total;
+    // the first part whose cumulative weight passes the target, else the last with
+    // any; every wave finds it by itself
+    int part = -1;
+    double base = 0.0, start = 0.0;
+    for (int p0 = 0, done = 0; p0 < a.parts && !done; p0 += 64) {
+      const int p = p0 + lane;
+      const double own = p < a.parts ? part_weight(p, less) : 0.0, sum = wave_scan(own);
+      const unsigned long long past = __ballot(own > kNothing && base + sum > target), any = __ballot(own > kNothing);
+      const unsigned long long from = past ? past & -past : any ? 1ull << (63 - __clzll(any)) : 0;
+      if (from) {
+        const int at = __ffsll(from) - 1;
+        part = p0 + at;
+        start = base + lane_of(sum - own, at);
+      }
+      done = past != 0;
+      base += lane_of(sum, 63);
     }
+    double w[8], own = 0.0, sum = 0.0;
+    const int j0 = part * PIECES * kPiece - shift + 8 * tid;
+    if (wave < PIECES) {
+      const Raw8<T> x = r.logits(j0);
+      Q8 q(less ? r.probs : nullptr, a.probs_bf16, j0, a.V);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) own += w[e];
-    sum = wave_scan(own);
-    if (lane == 63) sums[wave] = sum;
-  }
-  __syncthreads();
-  if (wave < PIECES) {
-    double at = start + (sum - own);
-    for (int v = 0; v < wave; ++v) at += sums[v];
-    int hit = 0x7fffffff, mine = -1;
+      for (int e = 0; e < 8; ++e) w[e] = less && j0 + e == r.gone && !r.probs ? 0.0 : r(x[e]);
+      if (less && r.probs) {
+        q.widen();
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      at += w[e];
-      if (w[e] > kNothing) {
-        mine = j0 + e;
-        if (at > target && hit == 0x7fffffff) hit = j0 + e;
+        for (int e = 0; e < 8; ++e) w[e] = fmax(__builtin_fma(-S, (double)q.f[e], w[e]), 0.0);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) own += w[e];
+      sum = wave_scan(own);
+      if (lane == 63) sums[wave] = sum;
+    }
+    __syncthreads();
+    if (wave < PIECES) {
+      double at = start + (sum - own);
+      for (int v = 0; v < wave; ++v) at += sums[v];
+      int hit = 0x7fffffff, mine = -1;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        at += w[e];
+        if (w[e] > kNoToken) {
+          mine = j0 + e;
+          if (at > target && hit == 0x7fffffff) hit = j0 + e;
+        }
+      }
+      const unsigned long long hits = __ballot(hit != 0x7fffffff), any = __ballot(mine >= 0);
+      const int to = any ? __builtin_amdgcn_readlane(mine, 63 - __clzll(any)) : -1;
+      const int from = hits ? __builtin_amdgcn_readlane(hit, __ffsll(hits) - 1) : 0x7fffffff;
+      if (lane == 0) {
+        found[wave] = from;
+        last[wave] = to;
       }
     }
-    const unsigned long long hits = __ballot(hit != 0x7fffffff), any = __ballot(mine >= 0);
-    const int to = any ? __builtin_amdgcn_readlane(mine, 63 - __clzll(any)) : -1;
-    const int from = hits ? __builtin_amdgcn_readlane(hit, __ffsll(hits) - 1) : 0x7fffffff;
-    if (lane == 0) {
-      found[wave] = from;
-      last[wave] = to;
-    }
-  }
-  __syncthreads();
-  int from = 0x7fffffff, to = -1;
+    __syncthreads();
+    int from = 0x7fffffff, to = -1;
 #pragma unroll
-  for (int v = 0; v < PIECES; ++v) {
-    from = min(from, found[v]);
-    to = max(to, last[v]);
+    for (int v = 0; v < PIECES; ++v) {
+      from = min(from, found[v]);
+      to = max(to, last[v]);
+    }
+    const int token = from != 0x7fffffff ? from : to;
+    if (token >= 0 || !less) return token;
+    less = false;
   }
-  return from != 0x7fffffff ? from : to;
 }
 
 // a row without a distribution, or greedy: no token, or the largest logit (what is

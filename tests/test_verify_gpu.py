@@ -127,6 +127,17 @@ def test_verify_temperatures(dtype, temperature, dev):
     _check(_case(20, 3, 3001, dtype, torch.float32, dev), dev, temperature=temperature)
 
 
+@pytest.mark.parametrize("probs", [None, torch.float32], ids=["rule", "q32"])
+@pytest.mark.parametrize("B,V", [(4, 3001), (4, 50001), (150, 33001)])  # one launch; in two or three; in three
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
+def test_verify_temperatures_at_the_ends(dtype, B, V, probs, dev):
+    """The least that fp32 holds takes the largest logit, infinity all columns alike."""
+    c = _case(B, 3, V, dtype, probs, dev)
+    c["logits"][..., 77] = 60.0  # the one largest
+    ends = torch.tensor([2.0 ** -149, 2.0 ** -130, 3e38, math.inf], device=dev)
+    _check(c, dev, temperature=ends[torch.arange(B, device=dev) % 4])
+
+
 def test_verify_greedy(dev):
     """Temperature 0: drafts are kept while they are the first largest logit, and
     that one follows, with and without probabilities of the drafts."""
@@ -241,6 +252,22 @@ def test_verify_random_numbers_at_the_ends(dev):
     for last in (1 - 2.0 ** -24, 1.0):
         u[:, 1] = last
         assert verify_drafts(x, drafts, u).tokens.tolist() == [[7, V - 4], [V - 4, -1]]
+
+
+@pytest.mark.parametrize("probs", [False, True], ids=["rule", "q32"])
+@pytest.mark.parametrize("B,V", [(2, 12000), (2, 50001), (130, 66001)])  # one launch; in two or three; in three
+def test_verify_parts_of_next_to_nothing(B, V, probs, dev):
+    """A random number of 0 takes the first column with a weight, where the weights of
+    many columns together pass what counts as one and each by itself does not."""
+    from naylis_amd.mom_kernels import verify_drafts
+    x = torch.zeros(B, 2, V, device=dev)
+    x[..., :4096] = -905 * math.log(2)  # a weight of 2^-905, of 512 of them 2^-896
+    drafts, u = torch.full((B, 1), V - 1, device=dev), torch.zeros(B, 2, device=dev)
+    got = verify_drafts(x, drafts, u, draft_probs=torch.full((B, 1, V), 1 / V, device=dev) if probs else None)
+    assert got.accepted.tolist() == [1] * B and got.tokens[:, 1].tolist() == [0] * B
+    x[..., :4096] = -2000.0  # no weight at all
+    got = verify_drafts(x, drafts, u)
+    assert got.tokens[:, 1].tolist() == [4096] * B
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
