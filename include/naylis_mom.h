@@ -547,7 +547,7 @@ int naylis_mom_packed_attn_bwd(const void* q, const void* k, const void* v, cons
  * first cu_seqlens[b + 1] - cu_seqlens[b] tokens of each sequence b, in rows
  * cu_seqlens[b] .. (int32, B + 1, not descending; rows outside all sequences are
  * 0), NaN where the page lies outside the cache or the token past the table's
- * row.  T < 2^28.
+ * row.  T <= 2^28 - 16.
  *
  * naylis_mom_paged_attn: out (B, H, head_dim) bf16 dense = softmax_n(scale
  * q . k_n) v_n over the tokens n < lens[b] (int32); 0 where lens[b] <= 0; NaN
@@ -560,7 +560,9 @@ int naylis_mom_packed_attn_bwd(const void* q, const void* k, const void* v, cons
  * H, head_dim), q_strides its batch, token and head strides.  The last of them
  * sees all lens[b] tokens, each earlier one a token less.  q_lens (B) int32:
  * new tokens of each sequence, clamped to [0, N], the first ones of its N rows
- * (NULL: N); rows behind them, and rows that see no token, are 0.
+ * (NULL: N); rows behind them, and rows that see no token, are 0.  The weight of
+ * a new token that a row does not see is 0, but a NaN or an infinity in that
+ * token's v times 0 is NaN there (in its k it reaches only rows that see it).
  * Constraints: head_dim 64 or 128, page_size a power of two in [16, 256], H a
  * multiple of Hkv, N H / Hkv <= 4096, Hkv ceil(N H / Hkv / 16) and B <= 65535, W
  * page_size <= 2^31 - 2048, B ceil(W page_size / 32) < 2^30, scale > 0, pointers
@@ -603,7 +605,9 @@ int naylis_mom_paged_attn_tokens(const void* q, const void* k_pages, const void*
  *   turned away (from p_a where that is 0 everywhere), from p_n where none was:
  *   the first j whose cumulative weight exceeds u[N] of the whole
  *   tokens[b] (N + 1) int64: the kept drafts, that token, -1 behind it
- * so the tokens are distributed as p's own.  Weights and sums are fp64.
+ * so the tokens are distributed as p's own.  The weights that the last token is
+ * drawn by and their sums are fp64, those that keep or turn away a draft fp32 where
+ * there are many rows; one under 2^-900 of the largest counts as none.
  *   logits (B, N + 1, V) in dtype (bf16 or fp32), draft_probs (B, N, V) bf16 or
  *   fp32, both with host arrays of their batch and token strides, last
  *   dimension dense, any address that their elements allow; draft_probs NULL:
@@ -612,9 +616,11 @@ int naylis_mom_paged_attn_tokens(const void* q, const void* k_pages, const void*
  *   fp32 in [0, 1), the last one for the token behind; draft_lens (B) int32, the
  *   drafts of each sequence, clamped to [0, N] (NULL: N)
  *   temperatures (B) fp32, or NULL for one temperature; 0 (or less, or NaN):
- *   all of p on the largest logit, the first of equal ones
+ *   all of p on the largest logit, the first of equal ones; infinity: all of
+ *   them but -inf alike
  * A row that has no distribution (a NaN, +inf, or nothing but -inf) keeps no
- * draft and gives token -1.  Rows behind a sequence's drafts are not read.
+ * draft and gives token -1.  Rows behind a sequence's kept drafts, and behind its
+ * drafts, change nothing, whatever they hold.
  * B <= 65535, N <= 1023, V <= 2^28; workspace 16-byte aligned. */
 size_t naylis_mom_verify_drafts_workspace_bytes(int64_t B, int64_t N, int64_t V, int draft_probs);
 int naylis_mom_verify_drafts(const void* logits, int dtype, const int64_t* logits_strides, const int64_t* drafts,

@@ -1282,7 +1282,7 @@ int naylis_mom_paged_gather(const void* k_pages, const void* v_pages, const void
   int rc = check_paged(pages, Hkv, page_size, B, W, 1, head_dim, cache_dtype, who);
   if (rc || (rc = check_cache(c, cache_dtype, who))) return rc;
   if (B < 1) return fail(NAYLIS_ERR_ARG, "%s: bad shape B=%lld", who, (long long)B);
-  if (T < 0 || T >= (1 << 28))  // a workgroup of 256 threads for 16 tokens
+  if (T < 0 || T > (1 << 28) - 16)  // a workgroup of 256 threads for 16 tokens
     return fail(NAYLIS_ERR_ARG, "%s: bad token count %lld", who, (long long)T);
   if (T == 0) return NAYLIS_OK;
   if (!table || !cu_seqlens) return fail(NAYLIS_ERR_ARG, "%s: null pointer argument", who);

@@ -1,13 +1,16 @@
-// Key / value cache in pages, and the attention of one new token over it.
+// Key / value cache in pages, and the attention of a sequence's new tokens over it.
 //
 // Pages (P, Hkv, page, hd) hold `page` consecutive tokens of one sequence, a
 // head's rows together; table (B, W) names each sequence's pages in order.
 // Rows are bf16, or e4m3 codes with one fp32 scale per row (the bank's form:
-// scale = max|row| / 448, 1 for a row of zeros; code = e4m3(x / scale)).
+// scale = max|row| / 448, 1 for a row of zeros; code = e4m3(x / scale)), or pairs of
+// e2m1 codes with a power of two for 32 features, its exponent in a byte.
 //
-// Attention: o[b, h] = softmax_n(scale q[b, h] . k[n]) v[n] over the sequence's
-// tokens n < lens[b].  Bound by memory: every live K and V byte is read once
-// (again for each further 16 query heads of a key head), past the caches.
+// Attention: o[b, i, h] = softmax_n(scale q[b, i, h] . k[n]) v[n] over the tokens
+// n < lens[b] - (N - 1 - i): the last of N new tokens sees all of its sequence, each one
+// before it a token less.  Bound by memory: every live K and V byte is read once
+// (again for each further 16 query heads of a key head, or 32 rows of several new
+// tokens), past the caches.
 //
 // Work is dealt in steps of 32 tokens: each slice's (key head's) steps of all
 // sequences form one list, cut into equal ranges for its workgroups and those
@@ -30,6 +33,20 @@
 // launch).  Three contexts of 65537 .. 131072 tokens, e4m3, 747 MB: 123 us (6.1 TB/s);
 // in steps of 64 tokens 134 (256 registers).  One sequence of 500 tokens, 16 heads of
 // 64: 7.0 us, a chain of dependent loads (length, page, rows) that fill nothing.
+//
+// Several new tokens make more rows of the same products: a row is (token, head), and a
+// token's end masks its scores in the steps that reach it.  32 sequences of up to 8191
+// tokens, five new ones each, 8 key heads of 128 with four query heads, bf16, 551 MB:
+// 105 us (5.2 TB/s; the attention 100, vector units in use 19 % of the time), where one
+// call a token would read the cache five times.
+//
+// Pages of 4 bits: a lane's 16 bytes are 32 features of K, the scale's reach, and widen
+// to bf16 by the conversions that take the scale (exact: two bits of a bf16's seven), so
+// that products and sums are those of bf16 pages.  64 sequences of up to 4096 tokens,
+// one new each, 157 MB: 34.6 us with the join's 4 (5.1 TB/s in the attention); three of
+// up to 131072, four new ones each, 385 MB: 76 (5.3 TB/s).  Not the memory alone: a byte
+// brings four times the work that it does in bf16, the vector units are in use for half
+// the time and LDS for a quarter, and the first loads wait for length and page.
 #include "common.h"
 #include "launch.h"
 #include "packed_tiles.h"
@@ -255,12 +272,10 @@ __device__ __forceinline__ long part_row(const PagedSplit& p, int slice, int wg,
 // (seven sequences of up to 5775 tokens, 40 rows for each of 4 key heads, bf16: 31 us;
 // past the caches 38, and with the choice made in the loop a single slice loses a tenth).
 template <int HD, PagedFormat FMT, int ROWS, bool MANY, bool AGAIN = false>
-__global__ __launch_bounds__(256, FMT == kPagedE2m1 && ROWS <= kRowsMfma ? 3 : 2) void paged_attn_kernel(PagedCacheDims c, PagedQueries q,
-                                                            const int32_t* __restrict__ table,
-                                                            const int32_t* __restrict__ lens,
-                                                            bf16_t* __restrict__ out, float* __restrict__ part,
-                                                            float2* __restrict__ stat, int* __restrict__ starts,
-                                                            float* __restrict__ ended, PagedSplit p, float sc) {
+__global__ __launch_bounds__(256, FMT == kPagedE2m1 && ROWS <= kRowsMfma ? 3 : 2) void paged_attn_kernel(
+    PagedCacheDims c, PagedQueries q, const int32_t* __restrict__ table, const int32_t* __restrict__ lens,
+    bf16_t* __restrict__ out, float* __restrict__ part, float2* __restrict__ stat, int* __restrict__ starts,
+    float* __restrict__ ended, PagedSplit p, float sc) {
   constexpr int QT = ROWS > kRowsMfma ? 2 : 1;  // 16-row tiles
   constexpr bool FP8 = FMT == kPagedE4m3, FP4 = FMT == kPagedE2m1;
   constexpr int TOK = kPagedStep;        // tokens of a step
@@ -282,7 +297,8 @@ __global__ __launch_bounds__(256, FMT == kPagedE2m1 && ROWS <= kRowsMfma ? 3 : 2
   const int kvh = slice / p.head_tiles, h0 = QT * kRowsMfma * (slice % p.head_tiles);
   const int nh = min(QT * kRowsMfma, (MANY ? c.G * c.N : c.G) - h0);  // live query rows of the slice
   constexpr bool OUTSIDE = ends_outside(FMT, ROWS);
-  if constexpr (OUTSIDE) ended += (((long)slice * p.wgs + wg) * 4) * ROWS * HD;  // a wave's partial that ends within its range
+  // the partial that ends within a wave's range
+  if constexpr (OUTSIDE) ended += ((long)slice * p.wgs + wg) * 4 * ROWS * HD;
   const int H = c.Hkv * c.G, hbase = kvh * c.G + h0;
   const Rows rows{c.G, c.N, H};
   // the slice's row r of sequence b in out
@@ -397,7 +413,8 @@ __global__ __launch_bounds__(256, FMT == kPagedE2m1 && ROWS <= kRowsMfma ? 3 : 2
           ke[i] = __builtin_nontemporal_load((const uint8_t*)c.k_scale + row16[i] * NW + eoff);
         } else {
 #pragma unroll
-          for (int j = 0; j < KL; ++j) kx[i][j] = load_once16<AGAIN>((const uint8_t*)c.k + row16[i] * RB + 64 * j + off);
+          for (int j = 0; j < KL; ++j)
+            kx[i][j] = load_once16<AGAIN>((const uint8_t*)c.k + row16[i] * RB + 64 * j + off);
         }
         if constexpr (FP8) {
           ksc[i] = *reinterpret_cast<const f32x4*>((const float*)c.k_scale + row16[i] + 4 * g);

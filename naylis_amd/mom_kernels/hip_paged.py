@@ -125,5 +125,7 @@ def paged_attention(q, cache: PagedCache, block_table, seq_lens, scale=None, q_l
     token), all appended first; the last sees seq_lens[b] tokens, each earlier one
     a token less.  With q_lens (B,) int32 sequence b has the first q_lens[b] of
     its N rows (clamped to [0, N]), the last of those seeing all.  Rows behind
-    them, and rows that see no token, are 0.  No backward."""
+    them, and rows that see no token, are 0.  A new token weighs 0 in the rows
+    that do not see it, so a NaN or an infinity in its v makes them NaN (one in
+    its k does not).  No backward."""
     return _torch_ext.load().paged_attention(q, *cache, block_table, seq_lens, scale, q_lens, 0)
