@@ -30,8 +30,9 @@
 // wait for chains of loads (parts, draft, logit; part, token).  64 sequences, four
 // drafts, 50001 logits, q fp32: 23 us, of which (1) 9.4 (32 MB), (2) 9.2 and (3) 5.4,
 // each of them mostly a launch's start and end.  48, seven, 151999, q bf16: 40 us, (1)
-// 19.7 (117 MB, 5.9 TB/s), (2) 14: the decisions' chains before the first byte, then 29
-// MB from the caches and twelve fp64 products each, (3) 5.6.
+// 19.7 (117 MB, 5.9 TB/s, and the vector units in use all the time: the weights by one
+// multiply-add each take as long), (2) 14: the decisions' chains of loads, then some
+// thirty fp64 operations a logit (vector units 69 %), (3) 5.6.
 #include "common.h"
 #include "launch.h"
 #include "timing.h"
