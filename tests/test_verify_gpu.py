@@ -365,6 +365,44 @@ def test_verify_large_logits(dev):
     assert got.accepted.tolist() == [9] * B and torch.equal(got.tokens[:, :10], want[:, :10])
 
 
+@pytest.mark.parametrize("probs", [False, True], ids=["rule", "q32"])
+@pytest.mark.parametrize("V", [700, 26001])  # one launch, three
+def test_verify_most_sequences(V, probs, dev):
+    """65535 sequences with a draft each (the most of a call), one row of logits for all."""
+    from naylis_amd.mom_kernels import verify_drafts
+    B = 65535
+    g = torch.Generator(device=dev).manual_seed(V)
+    x = torch.randn(1, 1, V, generator=g, device=dev) * 2
+    p = torch.softmax(x[0, 0].double(), 0)
+    q = torch.softmax(torch.randn(V, generator=g, device=dev) * 2, 0)
+    d = torch.multinomial(q, B, replacement=True, generator=g)
+    u = torch.rand(B, 2, generator=g, device=dev)
+    got = verify_drafts(x.expand(B, 2, V), d[:, None], u, draft_probs=q.expand(B, 1, V) if probs else None)
+    left = u[:, 0].double() * (q[d].double() if probs else 1.0) - p[d]
+    kept = left < 0
+    # p and p behind kept drafts; what is left of p, or p without the draft, behind others
+    place = lambda cum, target: torch.searchsorted(cum, target[:, None], right=True).clamp(max=V - 1)[:, 0]  # noqa: E731
+    cum, t = p.cumsum(0), u[:, 1].double()
+    want = place(cum, t * cum[-1])
+    near = (left.abs() < 2.0 ** -20 * p[d]) | ((cum[want] - t).abs() < 2.0 ** -38)
+    if probs:
+        rest = (p - q.double()).clamp(min=0).cumsum(0)
+        other = place(rest, t * rest[-1])
+        edge = (rest[other] / rest[-1] - t).abs().minimum((rest[(other - 1).clamp(min=0)] / rest[-1] - t).abs())
+    else:
+        # tokens below the draft have their cumulative weight, those above it p[d] less
+        target = t * (cum[-1] - p[d])
+        before = place(cum, target)
+        other = torch.where(before < d, before, place(cum, target + p[d]))
+        edge = (cum[other] - target - torch.where(before < d, 0.0, p[d])).abs()
+    near |= (cum[(want - 1).clamp(min=0)] - t).abs() < 2.0 ** -38
+    near |= edge < 2.0 ** -38
+    assert int(near.sum()) < 100, "the inputs put random numbers next to borders"
+    assert torch.equal(got.accepted.bool()[~near], kept[~near])
+    first, second = torch.where(kept, d, other), torch.where(kept, want, -1)
+    assert torch.equal(got.tokens[~near], torch.stack((first, second), 1)[~near])
+
+
 def test_verify_refusals(dev):
     from naylis_amd.mom_kernels import verify_drafts
     c = _case(3, 2, 50, torch.float32, torch.float32, dev)
