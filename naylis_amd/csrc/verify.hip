@@ -474,10 +474,11 @@ __device__ __forceinline__ VerifyLeft left_part(const VerifyArgs& a, const T* lo
 // The token behind the kept drafts of a row with a distribution, by a workgroup:
 // the part that the random number falls in, and the token in it, a piece for each of
 // the first PIECES waves.  LEFT: from the fp64 sums of left_part (l), else
-// from those of the first launch (s).
+// from those of the first launch (s).  first: the lane's of the first 64 parts, read
+// beside the decision.
 template <bool LEFT, int PIECES, typename T>
 __device__ __forceinline__ long pick(const VerifyArgs& a, const T* logits, int b, const Decision& d,
-                                     const VerifyStat* s, const VerifyLeft* l) {
+                                     const VerifyStat* s, const VerifyLeft* l, const VerifyLeft& first) {
   __shared__ int found[PIECES], last[PIECES];
   __shared__ double sums[PIECES];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -485,17 +486,21 @@ __device__ __forceinline__ long pick(const VerifyArgs& a, const T* logits, int b
   const Behind<T> r(a, logits, b, d);
   const int shift = shift_of(r.row);
   const int gone_part = r.gone >= 0 && r.gone < a.V ? (int)((r.gone + shift) / (PIECES * kPiece)) : -1;
+  const auto left_of = [&](int p) { return p < 64 ? first : l[p]; };  // of the lane's parts
   double S = 0.0;  // over the whole row, of the e that q is taken from
   if (r.probs) {
-    for (int p = lane; p < a.parts; p += 64) S += l[p].sum;
+    for (int p = lane; p < a.parts; p += 64) S += left_of(p).sum;
     S = wave_sum(S);
   }
   // weight of a part: of what is left of p (less), or of p where that is nothing
   const auto part_weight = [&](int p, bool less) {
-    if (less && r.probs) return fmax(l[p].over + (d.row.sum - S) * l[p].q, 0.0);
+    if (less && r.probs) {
+      const VerifyLeft v = left_of(p);
+      return fmax(v.over + (d.row.sum - S) * v.q, 0.0);
+    }
     double w;
     if constexpr (LEFT)
-      w = l[p].sum;
+      w = left_of(p).sum;
     else
       w = s[p].sum * weight(s[p].top, d.row.top, r.scale);
     return !less && !r.probs && p == gone_part ? w + d.row.draft : w;
@@ -635,12 +640,16 @@ __global__ __launch_bounds__(kThreads) void verify_pick_kernel(VerifyArgs a, con
                                                                const Decision* __restrict__ decisions) {
   const int b = blockIdx.x;
   Decision d;
-  if constexpr (LEFT)
+  VerifyLeft first = {};
+  left += (long)b * a.parts;
+  if constexpr (LEFT) {
+    first = left[min((int)threadIdx.x & 63, a.parts - 1)];
     d = decisions[b];
-  else
+  } else {
     d = decide<kWaves>(a, logits, stat + (long)b * (a.N + 1) * a.parts, b);
+  }
   const VerifyStat* s = stat + ((long)b * (a.N + 1) + d.kept) * a.parts;
-  answer(a, b, d, drawn(d) ? pick<LEFT, kPieces>(a, logits, b, d, s, left + (long)b * a.parts) : undrawn(d));
+  answer(a, b, d, drawn(d) ? pick<LEFT, kPieces>(a, logits, b, d, s, left, first) : undrawn(d));
 }
 
 // grid (B): all of it by one workgroup, where a sequence has few logits.
@@ -665,7 +674,7 @@ __global__ __launch_bounds__(64 * kSmallWaves) void verify_small_kernel(VerifyAr
     if (lane == 0) left[p] = l;
   }
   __syncthreads();
-  answer(a, b, d, pick<true, 1>(a, logits, b, d, (const VerifyStat*)nullptr, left));
+  answer(a, b, d, pick<true, 1>(a, logits, b, d, (const VerifyStat*)nullptr, left, left[min(lane, a.parts - 1)]));
 }
 
 namespace {
