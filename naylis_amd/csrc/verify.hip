@@ -684,14 +684,16 @@ int verify_parts(const VerifyArgs& a, int pieces) {
   return (int)(((long)a.V + 7 + pieces * kPiece - 1) / (pieces * kPiece));
 }
 
-// One launch for sequences of few logits (100 sequences with three drafts at 8000
-// logits and q 16.8 us, in three launches 18.9 and their gaps; 64 with seven at 2000
-// without q 12.6, in two 12.8; beyond that a workgroup's CU is slower than launches: four
-// sequences with three at 15000 19.9 without q, 11.0 in two).  Two, the first in fp64,
-// where q is not given and the logits are few; else three.
+// One launch for sequences of few logits: its 16 waves pass N + 1 rows' parts and, in
+// fp64, one row's, which takes twice as long a part.  Beyond the limits a workgroup's CU
+// is slower than launches over the chip (16 sequences, us in one launch and in more:
+// without q, no drafts, 7000 logits 10.1 and 10.3, 18000 13.7 and 9.7; three drafts, 3500
+// 10.1 and 11.0, 5000 11.7 and 11.1; with q, one draft, 14000 14.6 and 16.1, 23000 20.0
+// and 15.8; seven, 3500 13.1 and 15.4, 5000 15.9 and 15.9).  Two launches, the first in
+// fp64, where q is not given and the logits are few; else three.
 enum VerifyForm { kSmall, kBrief, kFull };
 VerifyForm verify_form(const VerifyArgs& a) {
-  if ((long)verify_parts(a, 1) * (a.N + 1) <= (a.probs ? 96 : 48)) return kSmall;
+  if ((long)verify_parts(a, 1) * (a.N + 3) <= (a.probs ? 112 : 50)) return kSmall;
   return !a.probs && (long)a.B * (a.N + 1) * a.V <= (1l << 24) ? kBrief : kFull;
 }
 
