@@ -795,8 +795,13 @@ __global__ __launch_bounds__(256) void paged_join_few_kernel(PagedCacheDims c, c
 
 // A workgroup for each sequence where tables hold at most 16 steps, four for each
 // wave, and no second launch (128 sequences of up to 500 tokens, 8 key heads of
-// 128: 38 us against 50).  Else the list is cut for two workgroups a CU over all
-// slices, and no finer than a step a wave.
+// 128: 38 us against 50), and in the forms with several tokens or 4 bits, whose
+// partials are more of the work, at most 32 steps where these workgroups are one round
+// of the chip or a good part of one (32 sequences of up to 1000 tokens, four new ones, 8
+// key heads of 128 with four query heads, us whole and cut: bf16 21 and 25, e4m3 18 and
+// 22, 4 bits 14 and 20; of 8 sequences 17.4 and 17.0, 15.9 and 16.5, 14 and 16, of one 15
+// and 12, 18 and 12, 14 and 12; of 128 69 and 58, 46 and 40, 34 and 34).  Else the list is
+// cut for two workgroups a CU over all slices, and no finer than a step a wave.
 // Three or four a CU take longer (three contexts of 65537 .. 131072 tokens, e4m3:
 // 124 us with 512 workgroups, 147 with 768, 130 with 1024); pages of 4 bits, with
 // half the loads of a step, leave registers for three and gain by them (three
@@ -810,8 +815,8 @@ PagedSplit paged_split(const PagedCacheDims& c, PagedFormat fmt) {
   p.rows = rows <= 4 ? 4 : p.tile;
   const long slices = (long)c.Hkv * p.head_tiles;
   const long cap = ((long)c.W * c.page + kPagedStep - 1) / kPagedStep;
-  p.whole = cap <= 16;
   const long most = fmt == kPagedE2m1 && p.tile == kRowsMfma ? 768 : 512;
+  p.whole = cap <= 16 || ((c.N > 1 || fmt == kPagedE2m1) && cap <= 32 && c.B * slices >= 64 && c.B * slices <= most);
   p.wgs = (int)(p.whole ? std::max(c.B, 1)
                         : std::max(1L, std::min({most / slices, (c.B * cap + 3) / 4, (long)kPagedMaxWgs})));
   return p;

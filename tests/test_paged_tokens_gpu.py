@@ -96,6 +96,7 @@ ONE = [
     ([(37 * i) % 400 for i in range(130)], 6, 2, 64, 32),
     ([70001], 4, 2, 128, 64),
     ([(53 * i) % 1900 for i in range(65)], 32, 8, 128, 16),
+    ([(53 * i) % 1020 for i in range(65)], 8, 2, 128, 16),  # a workgroup for each, of more than 16 steps
     ([0] * 70 + [1600] + [0] * 200 + [(29 * i) % 90 for i in range(100)] + [0], 2, 1, 64, 16),
     ([0 if i % 3 else (i * i) % 23 for i in range(4200)] + [1530], 2, 1, 64, 16),  # chunks of 66 sequences
 ]
@@ -119,6 +120,8 @@ MANY = [
     ([2600, 1, 900], 4, 4, 64, 16, 8, [8, 8, 5]),
     ([40], 34, 2, 128, 128, 3, None),                                 # 51 rows, three products
     ([(53 * i) % 900 for i in range(65)], 8, 2, 64, 16, 4, [i % 5 for i in range(65)]),
+    ([(53 * i) % 1900 for i in range(65)], 8, 2, 128, 16, 4, [i % 5 for i in range(65)]),
+    ([(53 * i) % 1020 for i in range(35)], 16, 2, 128, 32, 5, [i % 6 for i in range(35)]),  # 40 rows, two slices
     ([600], 1, 1, 64, 16, 1, [1]),
     ([600, 20], 2, 1, 64, 16, 1, [0, 1]),
 ]
