@@ -621,7 +621,8 @@ int naylis_mom_paged_attn_tokens(const void* q, const void* k_pages, const void*
  * A row that has no distribution (a NaN, +inf, or nothing but -inf) keeps no
  * draft and gives token -1.  Rows behind a sequence's kept drafts, and behind its
  * drafts, change nothing, whatever they hold.
- * B <= 65535, N <= 1023, V <= 2^28; workspace 16-byte aligned. */
+ * B <= 65535, N <= 1023, V <= 2^28; workspace 16-byte aligned (0 bytes for
+ * sequences of few logits). */
 size_t naylis_mom_verify_drafts_workspace_bytes(int64_t B, int64_t N, int64_t V, int draft_probs);
 int naylis_mom_verify_drafts(const void* logits, int dtype, const int64_t* logits_strides, const int64_t* drafts,
                              const float* uniforms, const void* draft_probs, int probs_dtype,

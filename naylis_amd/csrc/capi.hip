@@ -1378,7 +1378,7 @@ static int check_verify(VerifyArgs* a, int64_t B, int64_t N, int64_t V, bool pro
 size_t naylis_mom_verify_drafts_workspace_bytes(int64_t B, int64_t N, int64_t V, int draft_probs) {
   VerifyArgs a;
   if (check_verify(&a, B, N, V, draft_probs != 0, "mom_verify_drafts")) return 0;
-  return std::max<size_t>(verify_ws_bytes(a), 16);
+  return verify_ws_bytes(a);
 }
 
 int naylis_mom_verify_drafts(const void* logits, int dtype, const int64_t* logits_strides, const int64_t* drafts,
@@ -1405,10 +1405,10 @@ int naylis_mom_verify_drafts(const void* logits, int dtype, const int64_t* logit
   if ((uintptr_t)logits % (dtype == NAYLIS_DTYPE_BF16 ? 2 : 4) != 0 ||
       (uintptr_t)draft_probs % (probs_dtype == NAYLIS_DTYPE_BF16 ? 2 : 4) != 0)
     return fail(NAYLIS_ERR_ARG, "%s: logits and draft_probs must be aligned to their elements", who);
-  if (workspace_bytes < verify_ws_bytes(a))
-    return fail(NAYLIS_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", who, workspace_bytes,
-                verify_ws_bytes(a));
-  if ((rc = check_pointers({workspace}, who))) return rc;
+  const size_t needed = verify_ws_bytes(a);
+  if (workspace_bytes < needed)
+    return fail(NAYLIS_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", who, workspace_bytes, needed);
+  if (needed > 0 && (rc = check_pointers({workspace}, who))) return rc;
   a.drafts = drafts;
   a.uniforms = uniforms;
   a.probs = draft_probs;

@@ -562,13 +562,13 @@ variable_list verify_drafts(const at::Tensor& logits_in, const at::Tensor& draft
   }
   at::Tensor tokens = at::empty({B, N + 1}, logits.options().dtype(at::kLong));
   at::Tensor accepted = at::empty({B}, logits.options().dtype(at::kInt));
-  const size_t bytes = need(naylis_mom_verify_drafts_workspace_bytes(B, N, V, probs.defined()));
-  const at::Tensor ws = workspace(bytes, logits);
+  const size_t bytes = naylis_mom_verify_drafts_workspace_bytes(B, N, V, probs.defined());
+  const at::Tensor ws = bytes ? workspace(bytes, logits) : at::Tensor();
   check(naylis_mom_verify_drafts(logits.data_ptr(), dtype_code(logits), strides, drafts.data_ptr<int64_t>(),
                                  uniforms.data_ptr<float>(), ptr(probs), probs.defined() ? dtype_code(probs) : kF32,
                                  probs_strides, lens.defined() ? lens.data_ptr<int32_t>() : nullptr,
                                  temps.defined() ? temps.data_ptr<float>() : nullptr, (float)temperature,
-                                 tokens.data_ptr<int64_t>(), accepted.data_ptr<int32_t>(), ws.data_ptr(), bytes, B, N,
+                                 tokens.data_ptr<int64_t>(), accepted.data_ptr<int32_t>(), ptr(ws), bytes, B, N,
                                  V, stream_of(st, logits)));
   return {tokens, accepted};
 }

@@ -102,7 +102,7 @@ def _verify(lib, dtype=1, strides=(300, 100), logits=P, drafts=P, uniforms=P, pr
     (dict(dtype=2), "dtype"), (dict(probs_dtype=3), "dtype"), (dict(B=-1), "bad shape"), (dict(B=1 << 16), "bad shape"),
     (dict(N=-1), "bad shape"), (dict(N=1024), "bad shape"), (dict(V=0), "bad shape"), (dict(V=(1 << 28) + 1), "bad shape"),
     (dict(logits=None), "null"), (dict(strides=None), "null"), (dict(drafts=None), "null"), (dict(uniforms=None), "null"),
-    (dict(probs_strides=None), "null"), (dict(tokens=None), "null"), (dict(ws=None), "null"), (dict(ws=ODD), "aligned"),
+    (dict(probs_strides=None), "null"), (dict(tokens=None), "null"), (dict(V=100000, ws=None), "null"), (dict(V=100000, ws=ODD), "aligned"),
     (dict(strides=(-1, 100)), "strides"), (dict(probs_strides=(200, 1 << 40)), "strides"), (dict(logits=ctypes.c_void_p(4097)), "aligned"),
     (dict(probs=ODD), "aligned"), (dict(temps=None, temperature=-0.5), "temperature"),
     (dict(temps=None, temperature=math.nan), "temperature"), (dict(temps=None, temperature=math.inf), "temperature")])
@@ -112,7 +112,8 @@ def test_verify_refusals(lib, bad, text):
 
 def test_verify_workspace(lib):
     need = lambda B, N, V, q: lib.naylis_mom_verify_drafts_workspace_bytes(B, N, V, q)  # noqa: E731
-    assert need(3, 2, 100000, 1) > need(3, 2, 100000, 0) > 0 and need(3, 2, 0, 0) == 0 and need(0, 0, 1, 0) > 0
+    assert need(3, 2, 100000, 1) > need(3, 2, 100000, 0) > 0 and need(3, 2, 0, 0) == 0
+    assert need(3, 2, 500, 1) == need(0, 0, 1, 0) == 0  # one launch
     assert _verify(lib, V=100000, ws_bytes=need(3, 2, 100000, 1) - 1) == _lib.NAYLIS_ERR_WORKSPACE
     assert _verify(lib, B=0) == _lib.NAYLIS_OK
 
