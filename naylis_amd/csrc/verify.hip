@@ -652,15 +652,16 @@ __global__ __launch_bounds__(kThreads) void verify_pick_kernel(VerifyArgs a, con
   answer(a, b, d, drawn(d) ? pick<LEFT, kPieces>(a, logits, b, d, s, left, first) : undrawn(d));
 }
 
-// grid (B): all of it by one workgroup, where a sequence has few logits.
-template <typename T>
+// grid (B): all of it by one workgroup, where a sequence has few logits.  EXACT: without
+// q, the rows' sums in fp64, so that there are no others to form.
+template <typename T, bool EXACT>
 __global__ __launch_bounds__(64 * kSmallWaves) void verify_small_kernel(VerifyArgs a, const T* __restrict__ logits) {
   __shared__ VerifyStat stat[kSmallParts];
-  __shared__ VerifyLeft left[kSmallParts];
+  __shared__ VerifyLeft left[EXACT ? 1 : kSmallParts];
   const int b = blockIdx.x, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int n = verify_drafts_of(a, b);
   for (int k = wave; k < (n + 1) * a.parts; k += kSmallWaves) {
-    const VerifyStat s = stat_part<1, false>(a, logits, b, k / a.parts, n, k % a.parts);
+    const VerifyStat s = stat_part<1, EXACT>(a, logits, b, k / a.parts, n, k % a.parts);
     if (lane == 0) stat[k] = s;
   }
   __syncthreads();
@@ -669,12 +670,16 @@ __global__ __launch_bounds__(64 * kSmallWaves) void verify_small_kernel(VerifyAr
     answer(a, b, d, undrawn(d));
     return;
   }
-  for (int p = wave; p < a.parts; p += kSmallWaves) {
-    const VerifyLeft l = left_part<1>(a, logits, b, d, p);
-    if (lane == 0) left[p] = l;
+  if constexpr (EXACT) {
+    answer(a, b, d, pick<false, 1>(a, logits, b, d, stat + d.kept * a.parts, left, VerifyLeft{}));
+  } else {
+    for (int p = wave; p < a.parts; p += kSmallWaves) {
+      const VerifyLeft l = left_part<1>(a, logits, b, d, p);
+      if (lane == 0) left[p] = l;
+    }
+    __syncthreads();
+    answer(a, b, d, pick<true, 1>(a, logits, b, d, stat, left, left[min(lane, a.parts - 1)]));
   }
-  __syncthreads();
-  answer(a, b, d, pick<true, 1>(a, logits, b, d, (const VerifyStat*)nullptr, left, left[min(lane, a.parts - 1)]));
 }
 
 namespace {
@@ -685,15 +690,16 @@ int verify_parts(const VerifyArgs& a, int pieces) {
 }
 
 // One launch for sequences of few logits: its 16 waves pass N + 1 rows' parts and, in
-// fp64, one row's, which takes twice as long a part.  Beyond the limits a workgroup's CU
-// is slower than launches over the chip (16 sequences, us in one launch and in more:
-// without q, no drafts, 7000 logits 10.1 and 10.3, 18000 13.7 and 9.7; three drafts, 3500
-// 10.1 and 11.0, 5000 11.7 and 11.1; with q, one draft, 14000 14.6 and 16.1, 23000 20.0
-// and 15.8; seven, 3500 13.1 and 15.4, 5000 15.9 and 15.9).  Two launches, the first in
-// fp64, where q is not given and the logits are few; else three.
+// fp64, one row's, which takes twice as long a part (or both at once, up to one draft
+// without q).  Beyond the limits a workgroup's CU is slower than launches over the chip
+// (16 sequences, us in one launch and in more: without q, no drafts, 10000 logits 9.1 and
+// 9.7; one, 7000 10.5 and 11.2, 8500 11.8 and 10.7; three, 3500 10.1 and 11.0, 5000 11.7
+// and 11.1; with q, one draft, 14000 14.6 and 16.1, 23000 20.0 and 15.8; seven, 3500 13.1
+// and 15.4, 5000 15.9 and 15.9).  Two launches, the first in fp64, where q is not given
+// and the logits are few; else three.
 enum VerifyForm { kSmall, kBrief, kFull };
 VerifyForm verify_form(const VerifyArgs& a) {
-  if ((long)verify_parts(a, 1) * (a.N + 3) <= (a.probs ? 112 : 50)) return kSmall;
+  if ((long)verify_parts(a, 1) * (a.N + 3) <= (a.probs ? 112 : a.N <= 1 ? 60 : 50)) return kSmall;
   return !a.probs && (long)a.B * (a.N + 1) * a.V <= (1l << 24) ? kBrief : kFull;
 }
 
@@ -728,8 +734,13 @@ hipError_t launch_verify(VerifyArgs a, const void* logits, bool bf16, void* ws, 
                                       (const Decision*)decisions));
     };
     if (form == kSmall) {
-      NAYLIS_TIMED("verify_small", st,
-                   hipLaunchKernelGGL((verify_small_kernel<T>), dim3(a.B), dim3(64 * kSmallWaves), 0, st, a, x));
+      auto all = [&](auto kernel) {
+        NAYLIS_TIMED("verify_small", st,
+                     hipLaunchKernelGGL(kernel, dim3(a.B), dim3(64 * kSmallWaves), 0, st, a, x));
+      };
+      // (an fp64 sum over two rows costs less than one more pass over one: without drafts,
+      // 16 sequences of 5000 logits 8.4 us and 9.3, with one 9.4 and 9.8, with two level)
+      !a.probs && a.N <= 1 ? all(verify_small_kernel<T, true>) : all(verify_small_kernel<T, false>);
     } else if (form == kBrief) {
       first(std::true_type{});
       last(std::false_type{});

@@ -98,7 +98,8 @@ def _check(c, dev, **kw):
 SHAPES = [(1, 0, 1), (1, 1, 2), (3, 2, 7), (5, 3, 8), (2, 8, 1000), (70, 4, 2047), (3, 1, 2048), (3, 2, 2049), (2, 3, 4096),
           (9, 5, 8191), (4, 2, 50001), (2, 1, 151999), (1, 12, 32768), (2, 40, 513), (3, 95, 500), (2, 100, 9001), (5, 0, 24000),
           (5, 0, 24700), (4, 3, 12281), (4, 3, 12282), (5, 0, 8185), (5, 0, 8186), (4, 3, 4089), (4, 3, 4090), (4, 3, 9209),
-          (4, 3, 9210), (3, 47, 500), (3, 48, 500), (2, 109, 500), (2, 110, 500)]
+          (4, 3, 9210), (3, 47, 500), (3, 48, 500), (2, 109, 500), (2, 110, 500),
+          (5, 0, 10233), (5, 0, 10234), (5, 1, 7673), (5, 1, 7674)]
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
