@@ -204,6 +204,13 @@ __device__ __forceinline__ int part_offset(int slot) {
   return slot == 0 ? 32 * 2 * HD : 0;
 }
 
+// Place of features f .. f + 3 of row r in a wave's partial: a write takes the same
+// chunk of sixteen rows, which lie in eight places of the banks.
+template <int HD>
+__device__ __forceinline__ int part_at(int r, int f) {
+  return r * HD + (f ^ (4 * (r & 7)));
+}
+
 // Byte of a 16-byte chunk in the V tile: dealt so that the 128 bytes that LDS serves
 // at a time lie in its 32 banks once.  A transposing read takes a pair of chunks from
 // each of four rows; of widened codes a write takes every second chunk of a row, or of
@@ -565,24 +572,39 @@ __global__ __launch_bounds__(256, FMT == kPagedE2m1 && ROWS <= kRowsMfma ? 3 : 2
           pf[u][4 + e] = (__bf16)x[u][1][e];
         }
       const int rlo = 4 * g + (r16 >> 2), rhi = rlo + 16;
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
+      typedef short v8i16 __attribute__((ext_vector_type(8)));
+      v8i16 vf[NT];
+      const auto read_v = [&](int t) {
         const int ch = 2 * t + ((r16 & 3) >> 1), b8 = 8 * (r16 & 1);
         const v4i16 lo = lds_read_tr16(reinterpret_cast<const bf16_t*>(vt + v_slot<HD, FMT>(rlo, ch) + b8));
         const v4i16 hi = lds_read_tr16(reinterpret_cast<const bf16_t*>(vt + v_slot<HD, FMT>(rhi, ch) + b8));
-        typedef short v8i16 __attribute__((ext_vector_type(8)));
-        const v8i16 vf = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        vf[t] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+      };
+      // (of two tiles of rows the reads are kept AHEAD products in front, where the
+      // compiler, short of registers, waits for each: with the partials' places 56 -> 53.5
+      // us for 32 sequences of up to 8191 tokens in 4 bits, eight new ones each)
+      constexpr int AHEAD = QT > 1 ? 2 : 0;
 #pragma unroll
-        for (int u = 0; u < QT; ++u) acc[u][t] = mfma16(__builtin_bit_cast(bf16x8, vf), pf[u], acc[u][t]);
+      for (int t = 0; t < AHEAD; ++t) read_v(t);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        if (t + AHEAD < NT) read_v(t + AHEAD);
+        if constexpr (AHEAD > 0) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int u = 0; u < QT; ++u) acc[u][t] = mfma16(__builtin_bit_cast(bf16x8, vf[t]), pf[u], acc[u][t]);
+        if constexpr (AHEAD > 0) __builtin_amdgcn_sched_barrier(0);
       }
       lds_order();
     }
     const auto add = [](float a, float b2) { return a + b2; };
     const bool whole = s0 == 0 && s1 == nsteps;
     const int slot = first + s1 < end ? 0 : 1;  // ends within the range, or with it
+    // (new to the compiler here, so that the places keep no registers through the steps)
+    int lane_p = lane;
+    asm volatile("" : "+v"(lane_p));
 #pragma unroll
     for (int u = 0; u < QT; ++u) {
-      const int r = 16 * u + r16;
+      const int r = 16 * u + r16, rp = 16 * u + (lane_p & 15), gp = lane_p >> 4;
       l[u] = xor32_f32(xor16_f32(l[u], add), add);
       if (bad) l[u] = __builtin_nanf("");  // a page that is none: the sequence's result is NaN
       if (r >= nh) continue;
@@ -601,7 +623,7 @@ __global__ __launch_bounds__(256, FMT == kPagedE2m1 && ROWS <= kRowsMfma ? 3 : 2
         float* to = OUTSIDE && slot == 0 ? ended + (long)wave * ROWS * HD
                                          : reinterpret_cast<float*>(vt + part_offset<HD>(slot));
 #pragma unroll
-        for (int t = 0; t < NT; ++t) *reinterpret_cast<f32x4*>(to + r * HD + 16 * t + 4 * g) = acc[u][t];
+        for (int t = 0; t < NT; ++t) *reinterpret_cast<f32x4*>(to + part_at<HD>(rp, 16 * t + 4 * gp)) = acc[u][t];
         if (g == 0) stats[2 * wave + slot][r] = make_float2(m[u], l[u]);
       }
     }
@@ -634,10 +656,11 @@ __global__ __launch_bounds__(256, FMT == kPagedE2m1 && ROWS <= kRowsMfma ? 3 : 2
     for (int e = 0; e < 8; ++e) {
       st[e] = stats[e][r];
       if (OUTSIDE && e % 2 == 0) {
-        if (ps[e].b >= 0) px[e] = *reinterpret_cast<const f32x4*>(ended + ((e >> 1) * ROWS + r) * HD + f);
+        if (ps[e].b >= 0) px[e] = *reinterpret_cast<const f32x4*>(ended + (e >> 1) * ROWS * HD + part_at<HD>(r, f));
       } else {
         px[e] = *reinterpret_cast<const f32x4*>(
-            reinterpret_cast<const float*>(lds + (e >> 1) * kWaveLds<HD, FMT, ROWS> + part_offset<HD>(e & 1)) + r * HD + f);
+            reinterpret_cast<const float*>(lds + (e >> 1) * kWaveLds<HD, FMT, ROWS> + part_offset<HD>(e & 1)) +
+            part_at<HD>(r, f));
       }
     }
     float m = kLowest, l = 0.f;
