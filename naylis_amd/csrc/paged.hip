@@ -37,7 +37,7 @@
 // Several new tokens make more rows of the same products: a row is (token, head), and a
 // token's end masks its scores in the steps that reach it.  32 sequences of up to 8191
 // tokens, five new ones each, 8 key heads of 128 with four query heads, bf16, 551 MB:
-// 105 us (5.2 TB/s; the attention 100, vector units in use 19 % of the time), where one
+// 99 us (5.5 TB/s; the attention 95, vector units in use 19 % of the time), where one
 // call a token would read the cache five times.
 //
 // Pages of 4 bits: a lane's 16 bytes are 32 features of K, the scale's reach, and widen
@@ -828,7 +828,10 @@ __global__ __launch_bounds__(256) void paged_join_few_kernel(PagedCacheDims c, c
 // Three or four a CU take longer (three contexts of 65537 .. 131072 tokens, e4m3:
 // 124 us with 512 workgroups, 147 with 768, 130 with 1024); pages of 4 bits, with
 // half the loads of a step, leave registers for three and gain by them (three
-// contexts of 99396 .. 131072 tokens, four new ones each: 71 us against 76).
+// contexts of 99396 .. 131072 tokens, four new ones each: 71 us against 76).  Several
+// tokens over bf16 pages take one workgroup a CU, whose waves have 64 KB under way, for
+// half the partials (32 sequences of up to 8191 tokens, five new ones each: 99 us against
+// 105; two 101 against 104; e4m3 in turn 77 against 70).
 PagedSplit paged_split(const PagedCacheDims& c, PagedFormat fmt) {
   PagedSplit p;
   const int rows = c.G * c.N;
@@ -840,8 +843,9 @@ PagedSplit paged_split(const PagedCacheDims& c, PagedFormat fmt) {
   const long cap = ((long)c.W * c.page + kPagedStep - 1) / kPagedStep;
   const long most = fmt == kPagedE2m1 && p.tile == kRowsMfma ? 768 : 512;
   p.whole = cap <= 16 || ((c.N > 1 || fmt == kPagedE2m1) && cap <= 32 && c.B * slices >= 64 && c.B * slices <= most);
+  const long cut = fmt == kPagedBf16 && c.N > 1 ? 256 : most;
   p.wgs = (int)(p.whole ? std::max(c.B, 1)
-                        : std::max(1L, std::min({most / slices, (c.B * cap + 3) / 4, (long)kPagedMaxWgs})));
+                        : std::max(1L, std::min({cut / slices, (c.B * cap + 3) / 4, (long)kPagedMaxWgs})));
   return p;
 }
 
