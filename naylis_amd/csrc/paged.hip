@@ -37,14 +37,14 @@
 // Several new tokens make more rows of the same products: a row is (token, head), and a
 // token's end masks its scores in the steps that reach it.  32 sequences of up to 8191
 // tokens, five new ones each, 8 key heads of 128 with four query heads, bf16, 551 MB:
-// 99 us (5.5 TB/s; the attention 95, vector units in use 19 % of the time), where one
+// 99 us (5.6 TB/s; the attention 95, vector units in use 19 % of the time), where one
 // call a token would read the cache five times.
 //
 // Pages of 4 bits: a lane's 16 bytes are 32 features of K, the scale's reach, and widen
 // to bf16 by the conversions that take the scale (exact: two bits of a bf16's seven), so
 // that products and sums are those of bf16 pages.  64 sequences of up to 4096 tokens,
 // one new each, 157 MB: 34.6 us with the join's 4 (5.1 TB/s in the attention); three of
-// up to 131072, four new ones each, 385 MB: 76 (5.3 TB/s).  Not the memory alone: a byte
+// up to 131072, four new ones each, 385 MB: 76 (5.4 TB/s).  Not the memory alone: a byte
 // brings four times the work that it does in bf16, the vector units are in use for half
 // the time and LDS for a quarter, and the first loads wait for length and page.
 #include "common.h"
