@@ -566,8 +566,8 @@ int naylis_mom_packed_attn_bwd(const void* q, const void* k, const void* v, cons
  * Constraints: head_dim 64 or 128, page_size a power of two in [16, 256], H a
  * multiple of Hkv, N H / Hkv <= 4096, Hkv ceil(N H / Hkv / 16) and B <= 65535, W
  * page_size <= 2^31 - 2048, B ceil(W page_size / 32) < 2^30, scale > 0, pointers
- * (tables and lengths apart) 16-byte aligned, strides multiples of 8, all but the
- * last under 2^23. */
+ * (tables and lengths apart) 16-byte aligned, strides multiples of 8, from
+ * token to token under 2^23. */
 int naylis_mom_paged_append(void* k_pages, void* v_pages, void* k_scale, void* v_scale, int cache_dtype,
                             const void* k, const void* v, const int64_t* strides, const int32_t* table,
                             const int32_t* positions, const int32_t* rows, int64_t T, int64_t pages, int64_t Hkv,

@@ -1349,7 +1349,7 @@ int naylis_mom_paged_attn_tokens(const void* q, const void* k_pages, const void*
   c.v_scale = const_cast<void*>(v_scale);
   if ((rc = check_cache(c, cache_dtype, who))) return rc;
   if (!table || !lens || !q_strides) return fail(NAYLIS_ERR_ARG, "%s: null pointer argument", who);
-  const int64_t outer[2] = {q_strides[0], q_strides[2]}, inner[2] = {q_strides[1], q_strides[2]};
+  const int64_t outer[2] = {0, q_strides[0]}, inner[2] = {q_strides[1], q_strides[2]};
   if ((rc = check_pointers({q, out}, who)) || (rc = check_strides(outer, "q", who)) ||
       (rc = check_strides(inner, "q", who)))
     return rc;

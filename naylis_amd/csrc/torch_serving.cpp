@@ -330,19 +330,13 @@ variable_list paged_gather(const at::Tensor& kp, const at::Tensor& vp, const c10
   return {k, v};
 }
 
-// A (B, N, H, hd) operand as the kernels read it; dimensions of one keep no stride.
+// A (B, N, H, hd) operand as the kernels read it; a dimension of one is not stepped over.
 at::Tensor tokens_of(const at::Tensor& t, int64_t (&strides)[3]) {
-  const auto stride = [&](const at::Tensor& x, int d) {
-    if (x.size(d) > 1) return x.stride(d);
-    int64_t dense = 1;
-    for (int64_t i = d + 1; i < x.dim(); ++i) dense *= x.size(i);
-    return dense;
-  };
   const auto fits = [&](const at::Tensor& x) {
     bool ok = x.stride(3) == 1 && (uintptr_t)x.data_ptr() % 16 == 0;
     for (int d = 0; d < 3; ++d) {
-      strides[d] = stride(x, d);
-      ok = ok && strides[d] % 8 == 0 && (d == 2 || strides[d] < (1 << 23));
+      strides[d] = x.size(d) > 1 ? x.stride(d) : 0;
+      ok = ok && strides[d] % 8 == 0 && (d != 1 || strides[d] < (1 << 23));
     }
     return ok;
   };

@@ -482,3 +482,26 @@ def test_tokens_forward_mode_derivatives_raise(dev):
             paged_append_rope(c["cache"], q[:, 0], c["k"][:2], c["v"][:2], torch.ones(32, device=dev), c["table"], c["pos"][:2])
         with pytest.raises(RuntimeError, match="forward-mode"):
             verify_drafts(fwAD.make_dual(x, x), torch.zeros(2, 2, dtype=torch.long, device=dev), x[:, :, 0].contiguous())
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("B", [1, 2])
+def test_tokens_of_the_most_rows(B, fmt, dev):
+    """1024 new tokens of 64 heads over 16 key heads, the most rows of a call: q's dense
+    stride from sequence to sequence is 2^23."""
+    from naylis_amd.mom_kernels import paged_attention
+    N, H, Hkv, hd = 1024, 64, 16, 128
+    c = _case([1040, 700][:B], H, Hkv, hd, 16, fmt, dev, N=N)
+    got = paged_attention(c["q"], c["cache"], c["table"], c["lens"])
+    k, v = _stored(c, 16)
+    at = 0
+    for b, n in enumerate(c["lens"].tolist()):
+        seen = torch.arange(n, device=dev) <= torch.arange(N, device=dev)[:, None] + n - N  # (N, n)
+        for h in range(H):
+            x, y = k[at:at + n, h // 4], v[at:at + n, h // 4]
+            s = (c["q"][b, :, h].double() @ x.T * hd ** -0.5).masked_fill(~seen, -math.inf)
+            p = torch.softmax(s, -1).nan_to_num(0.0)  # (rows that see nothing)
+            far = (got[b, :, h].double() - p @ y).abs()
+            # (as in _attention: the weights and the result are rounded to bf16 once each)
+            assert bool((far <= p @ y.abs() * (2.0 ** -7 + 2.0 ** -10) + 1e-30).all())
+        at += n

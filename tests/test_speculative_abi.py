@@ -91,6 +91,14 @@ def test_attention_of_tokens_workspace(lib):
     assert _tokens(lib, B=0) == _lib.NAYLIS_OK
 
 
+def test_attention_of_tokens_batch_strides(lib):
+    """From sequence to sequence q may step as far as memory goes."""
+    for far in (1 << 23, (1 << 40) - 8):
+        assert _tokens(lib, W=100, ws_bytes=0, strides=(far, 256, 64)) == _lib.NAYLIS_ERR_WORKSPACE
+    for bad in (1 << 40, (1 << 23) + 4):
+        _refused(lib, _tokens(lib, W=100, ws_bytes=0, strides=(bad, 256, 64)), "strides")
+
+
 def _verify(lib, dtype=1, strides=(300, 100), logits=P, drafts=P, uniforms=P, probs=P, probs_dtype=0, probs_strides=(200, 100), temps=P,
             temperature=1.0, tokens=P, ws=P, ws_bytes=1 << 40, B=3, N=2, V=100):
     return lib.naylis_mom_verify_drafts(logits, dtype, strides and _i64(*strides), drafts, uniforms, probs, probs_dtype,
