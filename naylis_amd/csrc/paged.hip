@@ -63,6 +63,7 @@ namespace {
 constexpr int kRowsMfma = 16;       // query rows of a product
 constexpr int kPagedStep = 32;      // tokens of a step
 constexpr int kPagedMaxWgs = 512;   // workgroups that share a slice's steps
+constexpr int kJoinFew = 128;       // of them, the most whose partials rows' own threads join
 
 __device__ __forceinline__ f32x4 mfma16(const bf16x8& a, const bf16x8& b, const f32x4& c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
@@ -778,15 +779,19 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedCacheDims c, const
   *reinterpret_cast<bf16x4*>(out + (((long)b * c.N + token) * H + h) * HD + 4 * f) = o;
 }
 
-// The same with HD / 4 threads a row, one partial after another: for a few partials
-// of many rows.  Grid (1024 / HD rows of a key head, key heads, B).
+// The same with HD / 4 threads a row, for few partials of many rows: one after another,
+// or for a long sequence among short ones (its length stays on the device) the weights
+// first, a partial a thread, and then kRun rows at a time.  Grid (1024 / HD rows of a key
+// head, key heads, B).
 template <int HD>
 __global__ __launch_bounds__(256) void paged_join_few_kernel(PagedCacheDims c, const int32_t* __restrict__ live,
                                                              const int32_t* __restrict__ lens, bf16_t* __restrict__ out,
                                                              const float* __restrict__ part,
                                                              const float2* __restrict__ stat,
                                                              const int* __restrict__ starts, PagedSplit p) {
-  constexpr int TR = HD / 4, NG = 256 / TR;
+  constexpr int TR = HD / 4, NG = 256 / TR, kRun = 16;
+  static_assert(kJoinFew % TR == 0 && kJoinFew % kRun == 0, "whole rounds");
+  __shared__ float weights[NG][kJoinFew];
   const int hr = blockIdx.x * NG + threadIdx.x / TR, f = threadIdx.x % TR, kvh = blockIdx.y, b = blockIdx.z;
   const StepList list{lens, c.B, c.W * c.page};
   const int n = list.steps(b);
@@ -794,18 +799,50 @@ __global__ __launch_bounds__(256) void paged_join_few_kernel(PagedCacheDims c, c
   const int total = starts[c.B], range = max((total + p.wgs - 1) / p.wgs, 1);
   const int first = starts[b], w0 = first / range, w1 = (first + n - 1) / range;
   if (w0 == w1) return;
-  const int slice = kvh * p.head_tiles + hr / p.tile;
+  const int slice = kvh * p.head_tiles + hr / p.tile, count = w1 - w0 + 1;
   const auto row = [&](int w) { return part_row(p, slice, w, w * range >= first ? 0 : 1) + hr % p.tile; };
+  const auto piece = [&](int w) { return *reinterpret_cast<const f32x4*>(part + row(w) * HD + 4 * f); };
   float m = kLowest, l = 0.f;
   f32x4 a = f32x4{};
+  if (count <= kRun) {
 #pragma unroll 4
-  for (int w = w0; w <= w1; ++w) {
-    const float2 s = stat[row(w)];
-    const f32x4 x = *reinterpret_cast<const f32x4*>(part + row(w) * HD + 4 * f);
-    const float mn = fmaxf(m, s.x), wa = __builtin_amdgcn_exp2f(m - mn), wb = __builtin_amdgcn_exp2f(s.x - mn);
-    a = a * wa + x * wb;
-    l = l * wa + s.y * wb;
-    m = mn;
+    for (int w = w0; w <= w1; ++w) {
+      const float2 s = stat[row(w)];
+      const f32x4 x = piece(w);
+      const float mn = fmaxf(m, s.x), wa = __builtin_amdgcn_exp2f(m - mn), wb = __builtin_amdgcn_exp2f(s.x - mn);
+      a = a * wa + x * wb;
+      l = l * wa + s.y * wb;
+      m = mn;
+    }
+  } else {
+    // (of a row's own threads, which lie in one wave)
+    float* weight = weights[threadIdx.x / TR];
+    float2 st[kJoinFew / TR];
+#pragma unroll
+    for (int u = 0; u < kJoinFew / TR; ++u) {
+      const int i = f + TR * u;
+      st[u] = i < count ? stat[row(w0 + i)] : float2{kLowest, 0.f};
+      m = fmaxf(m, st[u].x);
+    }
+#pragma unroll
+    for (int o = 1; o < TR; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+#pragma unroll
+    for (int u = 0; u < kJoinFew / TR; ++u) {
+      const int i = f + TR * u;
+      const float w = i < count ? __builtin_amdgcn_exp2f(st[u].x - m) : 0.f;
+      weight[i] = w;
+      l += w * st[u].y;
+    }
+#pragma unroll
+    for (int o = 1; o < TR; o <<= 1) l += __shfl_xor(l, o, 64);
+    lds_order();
+    for (int i0 = 0; i0 < count; i0 += kRun) {
+      f32x4 x[kRun];
+#pragma unroll
+      for (int i = 0; i < kRun; ++i) x[i] = piece(w0 + min(i0 + i, count - 1));
+#pragma unroll
+      for (int i = 0; i < kRun; ++i) a += x[i] * weight[i0 + i];
+    }
   }
   const int token = hr / c.G;
   const bool none = seen(lens[b], live ? min(max(live[b], 0), c.N) : c.N, token) == 0;
@@ -850,10 +887,16 @@ PagedSplit paged_split(const PagedCacheDims& c, PagedFormat fmt) {
 }
 
 // Several tokens, or pages of 4 bits, of sequences that have eight partials each or so
-// at most: a launch of a thousand workgroups less takes a microsecond less.  (One token
-// over other pages keeps the order of its sums.)
+// on average: a launch of a thousand workgroups less takes a microsecond less, of several
+// thousand more (64 sequences of up to 4096 tokens, four query heads of 128 a key head, us
+// with it and with the other join: eight key heads, five tokens, bf16 112 and 121, e4m3 82
+// and 91; one token, 4 bits 37 and 39).  One of them may have all there are, which the
+// other join reads by more threads (100000 tokens among 63 sequences of up to 120: 101 and
+// 103, 93 and 93, 40 and 35; two key heads, bf16, 128 partials, 45 and 39, where even
+// sequences take 38 and 40; four, 4 bits, 192 partials, 35 and 25, even ones 25 and 25).
+// (One token over other pages keeps the order of its sums.)
 bool paged_join_few(const PagedCacheDims& c, const PagedSplit& p, PagedFormat fmt) {
-  return (c.N > 1 || fmt == kPagedE2m1) && p.wgs <= 8 * c.B;
+  return (c.N > 1 || fmt == kPagedE2m1) && p.wgs <= std::min(8 * c.B, kJoinFew);
 }
 
 size_t paged_part_floats(const PagedCacheDims& c, const PagedSplit& p, int hd) {

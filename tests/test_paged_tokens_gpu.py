@@ -505,3 +505,16 @@ def test_tokens_of_the_most_rows(B, fmt, dev):
             # (as in _attention: the weights and the result are rounded to bf16 once each)
             assert bool((far <= p @ y.abs() * (2.0 ** -7 + 2.0 ** -10) + 1e-30).all())
         at += n
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("Hkv", [1, 4, 8])
+def test_tokens_of_a_long_sequence_among_short_ones(Hkv, hd, fmt, dev):
+    """A batch whose sequences have few partials on average, and one of which has
+    nearly all there are: any number of them is joined."""
+    for far in (3001, 6007, 9100):
+        lens = [(i * 37) % 90 for i in range(40)] + [far] + [(i * 53) % 70 for i in range(30)]
+        c = _case(lens, Hkv, Hkv, hd, 16, fmt, dev, N=3, q_lens=[i % 4 for i in range(len(lens))])
+        c["q_lens"][40] = 3
+        _check(c, 16)
