@@ -868,7 +868,12 @@ __global__ __launch_bounds__(256) void paged_join_few_kernel(PagedCacheDims c, c
 // contexts of 99396 .. 131072 tokens, four new ones each: 71 us against 76).  Several
 // tokens over bf16 pages take one workgroup a CU, whose waves have 64 KB under way, for
 // half the partials (32 sequences of up to 8191 tokens, five new ones each: 99 us against
-// 105; two 101 against 104; e4m3 in turn 77 against 70).
+// 105; two 101 against 104; e4m3 in turn 77 against 70).  Heads of 64 have half of that
+// under way but gain alike where a key head has more rows than four (five tokens of four
+// query heads, the same sequences 62.4 and 62.5, 64 of up to 2048 tokens and two key heads
+// 19.0 and 21.5, one of 30000 20.6 and 22.1); of up to four rows they lose a little (the
+// same 58.0 and 57.2, 15.3 and 14.8, 18.1 and 18.4), where heads of 128 do not (103 and
+// 106, 21.3 and 20.8, 31 and 33).
 PagedSplit paged_split(const PagedCacheDims& c, PagedFormat fmt) {
   PagedSplit p;
   const int rows = c.G * c.N;
