@@ -224,10 +224,10 @@ __device__ __forceinline__ double wave_scan(double x) {
 }
 __device__ __forceinline__ double wave_sum(double x) { return lane_of(wave_scan(x), 63); }
 
-// (within what fp32 holds, so that 0 and -inf times it stay what they are)
-__device__ __forceinline__ double scale_of(float t) {
-  return 1.4426950408889634074 / (t > 0.f ? (double)fminf(fmaxf(t, 0x1p-120f), 0x1p120f) : 1.0);
-}
+// (0 at infinity: -inf times it is NaN, which weighs next to nothing as -inf does)
+__device__ __forceinline__ double scale_of(float t) { return 1.4426950408889634074 / (t > 0.f ? (double)t : 1.0); }
+// whether fp32 holds differences of logits that matter, and log2(e) / T
+__device__ __forceinline__ bool ordinary(float t) { return !(t > 0.f) || (t > 0x1p-100f && t < 0x1p100f); }
 
 }  // namespace
 
@@ -295,12 +295,23 @@ __device__ __forceinline__ VerifyStat stat_part(const VerifyArgs& a, const T* lo
         for (int k = 1; k < PIECES; ++k) x[k - 1] = x[k];
       }
     } else {
-      const float fs = (float)scale;
       float sums[PIECES] = {};
+      const auto sum = [&](auto exponent) {
 #pragma unroll
-      for (int c = 0; c < PIECES; ++c)
+        for (int c = 0; c < PIECES; ++c)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) sums[c] += __builtin_amdgcn_exp2f((x[c][e] - top) * fs);
+          for (int e = 0; e < 8; ++e) sums[c] += __builtin_amdgcn_exp2f(exponent(x[c][e]));
+      };
+      const float fs = (float)scale;
+      if (ordinary(t)) {
+        sum([&](float y) { return (y - top) * fs; });
+      } else {
+        // differences beyond fp32's largest number, or a scale beyond it (above 0 at
+        // infinity, so that -inf stays what it is)
+        const float before = t > 1.f ? 0x1p-4f : 1.f, after = t > 1.f ? 1.f : 0x1p64f, low = top * before;
+        const float rest = (float)fmax(scale / ((double)before * after), 0x1p-149);
+        sum([&](float y) { return (mul_rn(y, before) - low) * after * rest; });
+      }
 #pragma unroll
       for (int c = 0; c < PIECES; ++c) s += sums[c];
     }

@@ -140,6 +140,31 @@ def test_verify_temperatures_at_the_ends(dtype, B, V, probs, dev):
     _check(c, dev, temperature=ends[torch.arange(B, device=dev) % 4])
 
 
+@pytest.mark.parametrize("probs", [None, torch.float32], ids=["rule", "q32"])
+@pytest.mark.parametrize("B,V", [(4, 3001), (4, 50001), (150, 33001)])  # one launch; in two or three; in three
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
+def test_verify_temperatures_of_any_size(dtype, B, V, probs, dev):
+    """Logits up to the largest numbers and down to the smallest with temperatures of their
+    size: differences beyond fp32's largest number, scales beyond it."""
+    g = torch.Generator(device=dev).manual_seed(V)
+    for size, t in ((2.0 ** 127, 2.0 ** 126), (2.0 ** 127, 2.0 ** 127 * 1.9), (2.0 ** 127, math.inf), (2.0 ** 110, 2.0 ** 109),
+                    (2.0 ** -95, 2.0 ** -96), (2.0 ** -110, 2.0 ** -111), (2.0 ** -125, 2.0 ** -126)):
+        x = ((torch.rand(B, 4, V, generator=g, device=dev, dtype=torch.float64) * 2 - 1) * size).to(dtype)
+        drafts = x[:, :3].float().argmax(-1)
+        drafts[::2] = torch.randint(0, V, drafts[::2].shape, generator=g, device=dev)
+        u = torch.rand(B, 4, generator=g, device=dev)
+        u[:, :3] /= V  # near the probabilities of a row that is nearly flat
+        q = None
+        if probs is not None:
+            q = torch.rand(B, 3, V, generator=g, device=dev)
+            u[:, :3] *= V
+            q /= q.sum(-1, keepdim=True)
+        got = _check(dict(logits=x, drafts=drafts, uniforms=u, draft_probs=q), dev, temperature=torch.full((B,), t, device=dev))
+        # (at infinity every p is 1 / V, and every u / V below it)
+        all_kept = t == math.inf and probs is None
+        assert B < 150 or (int(got.accepted.sum()) == 3 * B if all_kept else 0 < int(got.accepted.sum()) < 3 * B)
+
+
 def test_verify_greedy(dev):
     """Temperature 0: drafts are kept while they are the first largest logit, and
     that one follows, with and without probabilities of the drafts."""
