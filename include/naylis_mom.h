@@ -606,8 +606,10 @@ int naylis_mom_paged_attn_tokens(const void* q, const void* k_pages, const void*
  *   the first j whose cumulative weight exceeds u[N] of the whole
  *   tokens[b] (N + 1) int64: the kept drafts, that token, -1 behind it
  * so the tokens are distributed as p's own.  The weights that the last token is
- * drawn by and their sums are fp64, those that keep or turn away a draft fp32 where
- * there are many rows; one under 2^-900 of the largest counts as none.
+ * drawn by and their sums are fp64; one under 2^-900 of the largest counts as none.
+ * The sums that keep or turn away a draft are fp64 in calls without draft_probs of
+ * up to 2^24 logits that have N <= 1 drafts or more logits than one launch takes;
+ * else fp32, off by less than 2^-19.
  *   logits (B, N + 1, V) in dtype (bf16 or fp32), draft_probs (B, N, V) bf16 or
  *   fp32, both with host arrays of their batch and token strides, last
  *   dimension dense, any address that their elements allow; draft_probs NULL:

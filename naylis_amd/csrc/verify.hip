@@ -14,15 +14,21 @@
 // would move the border between two tokens of the tail past u once in a hundred
 // draws.  fp64 runs at fp32's rate here, and 2^x costs ten products (a polynomial of
 // degree 10 fitted at the Chebyshev nodes of [-1/2, 1/2], off by 3e-16).  The sums
-// that only decide which drafts are kept are fp32 where there are many rows: u falls
-// between p and p (1 + 2^-20) once in a million draws.
+// that only decide which drafts are kept are fp32 wherever that token's row is summed
+// again: with q, in three launches, and in one with two drafts or more.  They are off by
+// less than 2^-19: a weight 2^-a of a part by three roundings of a (over 2048 logits 11 on
+// average at most) and two of itself, a lane's sum of eight by seven.  u falls that near
+// to p a few times in a million draws.
 //
 // Launches: (1) a wave for each 2048 logits of each row leaves (largest logit, its
 // place, sum of 2^z against it) -- all that the rows' bytes are read for; (2) for
 // each sequence the drafts kept, and over the row behind them the parts' fp64 sums
 //   S = sum e,  and with q  R = sum max(0, e - S' q),  Q = sum of q where that is not 0,
 // e = e^((x - top) / T) and S' the fp32 sum: what is left of p weighs R + (S' - S) Q,
-// for S is so near to S' that only tokens that weigh nothing change sides;
+// for S is so near to S' that only tokens that weigh next to nothing change sides.  Where
+// p and q differ by no more than fp32's rounding (q the softmax of the same logits) these
+// are all that is left: the part is then found among other tokens than the token in it, or
+// the token in p where the part has none.  There a draft is turned away once in a million;
 // (3) a workgroup for each sequence finds the part and the token in it.  Few logits
 // and no q: (1) in fp64, and no (2).
 //

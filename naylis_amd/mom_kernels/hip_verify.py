@@ -38,9 +38,10 @@ def verify_drafts(logits, drafts, uniforms, draft_probs=None, draft_lens=None, t
 
     draft_lens (B,) int32: drafts of each sequence (default N; clamped to [0, N]);
     the row behind them gives the token, later rows change nothing.  temperature: a
-    number or (B,) fp32; 0 takes the largest logit, the first of equal ones.  A
-    column under 2 ** -900 of the likeliest one has no probability.
-    Columns of -inf have no probability; a row with a NaN, with +inf or with
+    number, finite and not negative, or (B,) fp32, where what is not above 0 counts as
+    0 and infinity makes all columns but those of -inf alike; 0 takes the largest
+    logit, the first of equal ones.  A column under 2 ** -900 of the likeliest one has
+    no probability.  Columns of -inf have no probability; a row with a NaN, with +inf or with
     nothing else keeps no draft and gives token -1.  No backward."""
     temps = temperature if isinstance(temperature, torch.Tensor) else None
     tokens, accepted = _torch_ext.load().verify_drafts(logits, drafts, uniforms, draft_probs, draft_lens, temps,

@@ -184,6 +184,39 @@ def test_verify_greedy(dev):
             assert torch.equal(r.tokens, torch.where(i <= same[:, None], best, -1))
 
 
+# the first of drafts of a rule, or with probabilities; whether its decision's sums are fp64
+DECISIONS = [(40, 1, 7000, False, True), (20, 3, 50001, False, True),
+             (40, 3, 2000, False, False), (40, 2, 3000, True, False), (40, 3, 50001, True, False), (150, 3, 33001, False, False)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("B,N,V,probs,exact", DECISIONS)
+def test_verify_decisions_next_to_their_border(B, N, V, probs, exact, dtype, dev):
+    """Random numbers beside p / q: the neighbouring fp32 number on either side where the
+    sums are fp64, 2^-18 away where they are fp32 (off by less than 2^-19)."""
+    from naylis_amd.mom_kernels import verify_drafts
+    c = _case(B, N, V, dtype, torch.float32 if probs else None, dev)
+    T, row = 0.83, torch.arange(B, device=dev)
+    x, d, q = c["logits"], c["drafts"], c["draft_probs"]
+    d[::3, 0] = torch.randint(0, V, (len(d[::3]),), device=dev, generator=torch.Generator(device=dev).manual_seed(1))
+    t = torch.full((B,), T, device=dev)
+    # (on the CPU: on this GPU torch's fp64 softmax is off by up to 1e-6)
+    p = torch.softmax(x[:, 0].cpu().double() / t.cpu().double()[:, None], -1).to(dev)[row, d[:, 0]]
+    if probs:
+        q[row, 0, d[:, 0]] = (1.5 * p).float()
+        p = p / q[row, 0, d[:, 0]].double()
+    for kept in (True, False):
+        if exact:
+            u = p.float()
+            off = u.double() >= p if kept else u.double() < p  # on the wrong side of p
+            u = torch.where(off, torch.nextafter(u, torch.tensor(0.0 if kept else 2.0, device=dev)), u)
+        else:
+            u = (p * (1 + (-1 if kept else 1) * 2.0 ** -18)).float()
+        c["uniforms"][:, 0] = u
+        got = verify_drafts(x, d, c["uniforms"], draft_probs=q, temperature=t)
+        assert torch.equal(got.accepted > 0, torch.full((B,), kept, device=dev))
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
 def test_verify_masked_columns(dtype, dev):
     """Columns of -inf are never drawn, the type's lowest value is an ordinary
