@@ -920,27 +920,6 @@ size_t paged_ws_bytes(const PagedCacheDims& c, int hd, PagedFormat fmt) {
   return paged_joined_bytes(c, p, hd) + (ends_outside(fmt, p.rows) ? paged_part_floats(c, p, hd) * 2 * 4 : 0);
 }
 
-namespace {
-
-template <PagedFormat F>
-using Format = std::integral_constant<PagedFormat, F>;
-
-// f(head dim, format) as compile-time constants
-template <typename F>
-void with_format(int hd, PagedFormat fmt, F f) {
-  auto go = [&](auto d) {
-    if (fmt == kPagedBf16)
-      f(d, Format<kPagedBf16>{});
-    else if (fmt == kPagedE4m3)
-      f(d, Format<kPagedE4m3>{});
-    else
-      f(d, Format<kPagedE2m1>{});
-  };
-  hd == 64 ? go(std::integral_constant<int, 64>{}) : go(std::integral_constant<int, 128>{});
-}
-
-}  // namespace
-
 hipError_t launch_paged_append(const PagedCacheDims& c, int hd, PagedFormat fmt, const void* k, const void* v,
                                const int32_t* table, const int32_t* positions, const int32_t* rows,
                                const PagedNew& src, hipStream_t st) {

@@ -20,7 +20,6 @@
 #include "timing.h"
 
 #include <algorithm>
-#include <type_traits>
 
 namespace naylis {
 
@@ -29,7 +28,8 @@ namespace {
 constexpr int kChunkThreads = 256;
 
 // sin and cos of x: x less a multiple of pi / 2 in two parts (Cody and Waite), then
-// the Taylor series up to r^17 / r^16 on |r| <= pi / 4, off by 5e-17 and 2e-18.
+// the Taylor series up to r^17 / r^16 on |r| <= pi / 4: what they leave out is 8e-20
+// and 2e-18, fp64's roundings some 1e-16.
 __device__ __forceinline__ void sincos64(double x, float& sine, float& cosine) {
   const double n = rint(x * 0.63661977236758134308);
   double r = __builtin_fma(-n, 1.57079632679489661923, x);
@@ -210,22 +210,6 @@ __global__ __launch_bounds__(kChunkThreads) void paged_gather_kernel(PagedCacheD
 
 namespace {
 
-template <PagedFormat F>
-using ChunkFormat = std::integral_constant<PagedFormat, F>;
-
-template <typename F>
-void with_chunk_format(int hd, PagedFormat fmt, F f) {
-  auto go = [&](auto d) {
-    if (fmt == kPagedBf16)
-      f(d, ChunkFormat<kPagedBf16>{});
-    else if (fmt == kPagedE4m3)
-      f(d, ChunkFormat<kPagedE4m3>{});
-    else
-      f(d, ChunkFormat<kPagedE2m1>{});
-  };
-  hd == 64 ? go(std::integral_constant<int, 64>{}) : go(std::integral_constant<int, 128>{});
-}
-
 // Workgroups that share the rows of one of n: as many as fill the chip.
 unsigned shares(long n, int rows, int at_a_time) {
   const long passes = (rows + at_a_time - 1) / at_a_time;
@@ -238,7 +222,7 @@ hipError_t launch_paged_append_rope(const PagedCacheDims& c, int hd, PagedFormat
                                     const int32_t* table, const int32_t* positions, const int32_t* rows,
                                     hipStream_t st) {
   const dim3 grid((unsigned)r.T, shares(r.T, r.H + 2 * c.Hkv, kChunkThreads / (hd / 8)));
-  with_chunk_format(hd, fmt, [&](auto d, auto f) {
+  with_format(hd, fmt, [&](auto d, auto f) {
     NAYLIS_TIMED("paged_append_rope", st,
                  hipLaunchKernelGGL((paged_rope_kernel<decltype(d)::value, decltype(f)::value>), grid,
                                     dim3(kChunkThreads), 0, st, c, r, table, positions, rows));
@@ -250,7 +234,7 @@ hipError_t launch_paged_gather(const PagedCacheDims& c, int hd, PagedFormat fmt,
                                const int32_t* cu, void* k_out, void* v_out, long T, hipStream_t st) {
   const long tiles = (T + kGatherTokens - 1) / kGatherTokens;
   const dim3 grid((unsigned)tiles, shares(tiles, 2 * c.Hkv * kGatherTokens, kChunkThreads / (hd / 8)));
-  with_chunk_format(hd, fmt, [&](auto d, auto f) {
+  with_format(hd, fmt, [&](auto d, auto f) {
     NAYLIS_TIMED("paged_gather", st,
                  hipLaunchKernelGGL((paged_gather_kernel<decltype(d)::value, decltype(f)::value>), grid,
                                     dim3(kChunkThreads), 0, st, c, table, cu, (bf16_t*)k_out, (bf16_t*)v_out, T));

@@ -1,5 +1,7 @@
 // Device code shared by the kernels that read and write the paged cache.
 #pragma once
+#include <type_traits>
+
 #include "common.h"
 #include "launch.h"
 
@@ -79,6 +81,23 @@ __device__ __forceinline__ void store_codes(const PagedCacheDims& c, bool is_v, 
     if (piece % 4 == 0)
       reinterpret_cast<uint8_t*>(is_v ? c.v_scale : c.k_scale)[row * (HD / 32) + piece / 4] = (uint8_t)byte;
   }
+}
+
+template <PagedFormat F>
+using Format = std::integral_constant<PagedFormat, F>;
+
+// f(head dim, format) as compile-time constants
+template <typename F>
+void with_format(int hd, PagedFormat fmt, F f) {
+  auto go = [&](auto d) {
+    if (fmt == kPagedBf16)
+      f(d, Format<kPagedBf16>{});
+    else if (fmt == kPagedE4m3)
+      f(d, Format<kPagedE4m3>{});
+    else
+      f(d, Format<kPagedE2m1>{});
+  };
+  hd == 64 ? go(std::integral_constant<int, 64>{}) : go(std::integral_constant<int, 128>{});
 }
 
 }  // namespace naylis
