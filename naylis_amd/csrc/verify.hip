@@ -38,7 +38,8 @@
 // each of them mostly a launch's start and end.  48, seven, 151999, q bf16: 40 us, (1)
 // 19.7 (117 MB, 5.9 TB/s, and the vector units in use all the time: the weights by one
 // multiply-add each take as long), (2) 14: the decisions' chains of loads, then some
-// thirty fp64 operations a logit (vector units 69 %), (3) 5.6.
+// thirty fp64 operations a logit (vector units 69 %), (3) 5.6.  The two with fp32 logits:
+// 27 and 61, (1) 11.7 and 41 (233 MB, 5.7 TB/s).
 #include "common.h"
 #include "launch.h"
 #include "timing.h"
@@ -620,7 +621,9 @@ __device__ __forceinline__ void answer(const VerifyArgs& a, int b, const Decisio
 
 }  // namespace
 
-// grid (parts / 4, N + 1, B), a part for each wave.
+// grid (parts / 4, N + 1, B), a part for each wave.  (Eight waves a SIMD have registers
+// for a part of bf16 logits; the sums in fp64, and fp32 logits, which wait for memory, are
+// left what they take: 74 and 50.)
 template <typename T, bool EXACT>
 __global__ __launch_bounds__(kThreads, EXACT || sizeof(T) == 4 ? 1 : 8) void verify_stat_kernel(
     VerifyArgs a, const T* __restrict__ logits, VerifyStat* __restrict__ stat) {
